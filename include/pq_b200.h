@@ -284,6 +284,40 @@ int pq_int8_linear_g32(const void* x, int dtype, int64_t ldx, const int8_t* w, i
  * ldo % 16 == 0, 16-byte aligned bases.  No counterpart in the reference. */
 int pq_unpack_int4(const uint8_t* packed, int64_t ldp, int8_t* out, int64_t ldo, int64_t N, int64_t K, void* stream);
 
+/* 4-bit floating-point rows (no counterpart in the reference, whose 4-bit weights are integers kept for storage only).
+ * A row of K elements is K / 2 bytes of E2M1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign bit), element 2b in the low
+ * nibble of byte b, element 2b + 1 in the high one.  Two formats of the scales:
+ *   PQ_FP4_MX  one E8M0 scale per 32 elements, s = 2^(floor(log2 max|x|) - 2), not below 2^-127;
+ *   PQ_FP4_NV  one E4M3 scale per 16 elements, s = e4m3(max|x| / (6 s_row)), under a power of two per row, s_row = the
+ *              smallest not below 2^-100 with max|x over the row| <= 2688 s_row (1 for a row of zeros).
+ * code = e2m1(x / s) or e2m1(x / (s s_row)), round half to even, magnitudes beyond 6 to 6 (codes 0 where s is 0).
+ * Infinities and NaN: an mx block that holds one gets scale NaN (byte 255), an nv row s_row = NaN; codes 0.
+ * Scale bytes stand in tiles of 128 rows x 4 scales, 512 bytes each: byte (r % 32) * 16 + (r / 32 % 4) * 4 + k of tile
+ * (r / 128) * tiles_k + t is scale 4 t + k of row r, tiles_k = ceil(K / 128) (mx) or ceil(K / 64) (nv).  Scales past the
+ * end of a row are 0; those of rows past the last one in its tile are not written. */
+#define PQ_FP4_MX 0
+#define PQ_FP4_NV 1
+/* Bytes of the scale array of M rows; 0 for bad arguments. */
+int64_t pq_fp4_scale_bytes(int64_t M, int64_t K, int fmt);
+/* x [M,K] 16-bit, row stride ldx -> codes [M, K/2] contiguous, scales (pq_fp4_scale_bytes), row_scale [M] (nv; NULL for
+ * mx).  K % 32 == 0, ldx % 16 == 0, x 32-byte aligned, codes and scales 16-byte aligned. */
+int pq_quant_rows_fp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fmt, uint8_t* codes,
+                      uint8_t* scales, float* row_scale, void* stream);
+/* The values that packed rows stand for, rounded to `dtype` (fp16: clipped to +-65504): codes with row stride ldc bytes
+ * (% 16 == 0) -> out [M,K], row stride ldo (% 16 == 0), 32-byte aligned. */
+int pq_dequant_rows_fp4(const uint8_t* codes, int64_t ldc, const uint8_t* scales, const float* row_scale, int fmt,
+                        void* out, int dtype, int64_t ldo, int64_t M, int64_t K, void* stream);
+/* Product of packed rows: out[m,n] = (sum_k x[m,k] w[n,k]) (s_row[m] s_col[n]) (+ bias[n]) rounded to out_dtype, x and w
+ * the values of codes and block scales (applied by the tensor cores, fp32 accumulation).  Both operands in one format;
+ * x [M, K/2] and w [N, K/2] with row strides ldx, ldw bytes (% 16 == 0), 16-byte aligned codes and scales; s_row [M] and
+ * s_col [N] are the operands' row scales (required for nv, NULL means 1 for mx); bias fp32 [N] or NULL; K % 32 == 0;
+ * any M and N; out [M,N] row stride ldo (16-byte stores when ldo % 8 == 0 and out is 16-byte aligned).  workspace as for
+ * pq_int8_gemm.  M == 0 is a no-op. */
+int pq_fp4_gemm(const uint8_t* xq, int64_t ldx, const uint8_t* x_scales, const float* s_row,
+                const uint8_t* w, int64_t ldw, const uint8_t* w_scales, const float* s_col, const float* bias, int fmt,
+                void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                void* workspace, size_t ws_bytes, void* stream);
+
 /* Feathered scatter of routed rows back over the cached canvas, in place: the pull form of
  * fuse_patch_predictions (flux/routing.py:328-379).  For canvas token j with contributor list
  * e in [ptr[j], ptr[j+1]):  local = sum_e beta[e] * y[src[e], :], bsum = sum_e beta[e] (both

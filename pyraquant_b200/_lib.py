@@ -16,6 +16,8 @@ PQ_OK = 0
 PQ_ERR_TIMEOUT = 6
 DTYPE_BF16 = 0
 DTYPE_FP16 = 1
+FP4_MX = 0
+FP4_NV = 1
 GEMM_WORKSPACE_BYTES = 256
 
 _lib: Optional[ctypes.CDLL] = None
@@ -66,6 +68,12 @@ SIGNATURES = {
     "pq_lowrank_down": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_int64,
                                 c_void_p, c_size_t, c_void_p]),
     "pq_unpack_int4": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
+    "pq_fp4_scale_bytes": (c_int64, [c_int64, c_int64, c_int]),
+    "pq_quant_rows_fp4": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pq_dequant_rows_fp4": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int64,
+                                    c_void_p]),
+    "pq_fp4_gemm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int,
+                            c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
     "pq_int8_gemm_g32": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
                                  c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
     "pq_int8_linear_scratch_bytes": (c_int64, [c_int64, c_int64, c_int]),

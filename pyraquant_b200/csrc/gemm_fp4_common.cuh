@@ -1,0 +1,111 @@
+// Pieces shared by the block-scaled 4-bit GEMM kernels: parameters, the tcgen05 wrappers and descriptors of
+// kind::mxf4 / kind::mxf4nvf4, and the output stores.
+//
+// Operands.  A row of K E2M1 codes is K / 2 bytes, so a tile of 128-byte rows with the 128-byte swizzle holds 256
+// elements per row and one MMA (K = 64) takes 32 bytes of it: the same bytes as an INT8 MMA of K = 32.
+// Scales.  A scale tile (fp4_common.cuh) is exactly what tcgen05.cp.32x128b.warpx4 turns into four tensor-memory columns:
+// 16 bytes per lane, word j of lane r = the four scales of row 32 j + r, replicated over the four lane quarters.  nv: a
+// tile holds the scales of one MMA (4 x 16 elements).  mx: of two (2 x 32 elements each); the instruction descriptor's
+// scale ids 0 and 2 pick the half.
+#pragma once
+
+#include "fp4_common.cuh"
+#include "gemm_common.cuh"
+
+namespace pq {
+
+struct Fp4GemmParams {
+  const uint8_t* sfa;      // scale tiles of the activations
+  const uint8_t* sfb;      // and of the weights
+  const float* s_row;      // [M] or NULL (1)
+  const float* s_col;      // [N] or NULL (1)
+  const float* bias;       // [N] or NULL
+  void* out;
+  int32_t* status;
+  int64_t ldo;
+  int M, N, K;
+  int tiles_k;             // scale tiles per row group
+  int mt, nt;              // row and column tiles
+  int bf16;                // output type
+  int vec;                 // rows may be stored 16 bytes at a time
+};
+
+namespace {
+
+constexpr int kFp4StageK = 256;                                   // elements per stage = 128 bytes
+
+template <int FMT>
+struct Fp4Fmt {
+  static constexpr int kTilesPerStage = FMT == PQ_FP4_MX ? 2 : 4;       // scale tiles per stage and row group
+  static constexpr int kTileK = kFp4StageK / kTilesPerStage;            // elements per scale tile
+  static constexpr int kScaleBytes = kTilesPerStage * 512;
+};
+
+// Instruction descriptor of kind::mxf4 / kind::mxf4nvf4: E2M1 operands, K-major, shape M x N, scales E8M0 or E4M3.
+__host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, bool mx, int scale_id) {
+  return (static_cast<uint32_t>(scale_id) << 4)                   // B scale id
+         | (1u << 7)                                              // A format: E2M1
+         | (1u << 10)                                             // B format: E2M1
+         | (static_cast<uint32_t>(N >> 3) << 17)
+         | ((mx ? 1u : 0u) << 23)                                 // scale format: E8M0 (else E4M3)
+         | (static_cast<uint32_t>(M >> 4) << 24)
+         | (static_cast<uint32_t>(scale_id) << 29);               // A scale id
+}
+
+template <int FMT>
+__device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa_tmem,
+                                           uint32_t sfb_tmem, uint32_t acc) {
+  if constexpr (FMT == PQ_FP4_MX)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(acc)
+        : "memory");
+}
+
+// Shared-memory descriptor of a scale tile: 32 rows of 16 contiguous bytes, no swizzle, eight-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_tile_desc(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+__device__ __forceinline__ void tc_cp_scale_tile(uint32_t tmem_addr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem_addr), "l"(desc) : "memory");
+}
+
+// contiguous copy global -> shared, completion bytes on a barrier of this CTA; 16-byte aligned, size % 16 == 0
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack2_any(float a, float b, int bf16) {
+  return bf16 ? pack2(a, b, __nv_bfloat16{}) : pack2(a, b, __half{});
+}
+// eight consecutive outputs of one row, columns [col, col + 8)
+__device__ __forceinline__ void store8(const Fp4GemmParams& p, int row, int col, const float (&y)[8]) {
+  unsigned short* o = static_cast<unsigned short*>(p.out) + static_cast<int64_t>(row) * p.ldo + col;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack2_any(y[2 * i], y[2 * i + 1], p.bf16);
+  if (p.vec && col + 8 <= p.N) {
+    st_v4(o, make_uint4(w[0], w[1], w[2], w[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < p.N) o[i] = static_cast<unsigned short>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu);
+  }
+}
+
+}  // namespace
+}  // namespace pq

@@ -1,0 +1,199 @@
+"""Linears in microscaled 4-bit floating point: both operands as E2M1 codes with block scales that the tensor cores apply.
+
+The reference keeps 4-bit weights for storage only and expands them to INT8 (deploy/run_flux_latency.py:16-18); this module
+is the 4-bit counterpart of ``int8_exec``: ``quant_rows_fp4`` and ``fp4_gemm`` beside ``quant_rows`` and
+``int8_gemm_fused``, ``Fp4Linear`` beside ``Int8Linear``, ``convert_linears_to_fp4`` beside ``convert_linears_to_int8``.
+
+Two formats (``fmt``)
+  ``"mx"``  one power of two (E8M0) per 32 elements;
+  ``"nv"``  one E4M3 scale per 16 elements under a power of two per row: finer scales, 6 % more bytes.
+Packed rows are an ``Fp4Rows``: codes uint8 [M, K/2], scale bytes uint8 [ceil(M/128), tiles, 512] in the order the tensor cores
+read them (``include/pq_b200.h`` spells it out), and the nv format's row scales fp32 [M].
+
+CUDA tensors only; a CPU tensor raises AssertionError.  There is no gradient: the results of a quantisation are codes.
+"""
+from __future__ import annotations
+
+from typing import Callable, Dict, NamedTuple, Optional, Tuple
+
+import torch
+import torch.nn as nn
+
+from . import ops
+from .int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR, _eager, is_bf16_whitelisted
+
+FORMATS = tuple(ops.FP4_FORMATS)
+DEFAULT_FORMAT = "nv"
+
+
+class Fp4Rows(NamedTuple):
+    """Packed rows: E2M1 codes, block scales and, for the nv format, row scales."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    row_scale: Optional[torch.Tensor] = None
+
+    @property
+    def fmt(self) -> str:
+        return "mx" if self.row_scale is None else "nv"
+
+
+# --------------------------------------------------------------------------- operator wrappers
+def quant_rows_fp4(x2: torch.Tensor, fmt: str = DEFAULT_FORMAT) -> Fp4Rows:
+    """[M,K] bf16/fp16 -> packed rows; K % 32 == 0; rows may be strided (no copy when they start on 32-byte borders)."""
+    assert x2.dim() == 2 and x2.is_cuda
+    if _eager():
+        return Fp4Rows(*ops._quant_rows_fp4_impl(x2, fmt))
+    codes, scales, row = torch.ops.pq_b200.quant_rows_fp4(x2, fmt)
+    return Fp4Rows(codes, scales, row if fmt == "nv" else None)
+
+
+def dequant_rows_fp4(q: Fp4Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values packed rows stand for, [M,K] in ``dtype``.  bf16 holds them exactly; fp16 rounds what lies below its
+    normal range and clips to +-65504."""
+    if _eager():
+        return ops._dequant_rows_fp4_impl(q.codes, q.scales, q.row_scale, dtype)
+    return torch.ops.pq_b200.dequant_rows_fp4(q.codes, q.scales, q.row_scale, ops.dtype_code(dtype))
+
+
+def fp4_gemm(xq: Fp4Rows, w: Fp4Rows, bias: Optional[torch.Tensor] = None,
+             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x [M,K] times the transpose of w [N,K] (+ fp32 bias [N]) in ``out_dtype``; both operands in the same format."""
+    if _eager():
+        return ops._fp4_gemm_impl(xq.codes, xq.scales, xq.row_scale, w.codes, w.scales, w.row_scale, bias, out_dtype)
+    return torch.ops.pq_b200.fp4_gemm(xq.codes, xq.scales, xq.row_scale, w.codes, w.scales, w.row_scale, bias,
+                                      ops.dtype_code(out_dtype))
+
+
+def fp4_linear_2d(x2: torch.Tensor, w: Fp4Rows, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x2 [M,K] -> [M,N] in x2's dtype: quantisation in the weights' format, then the product."""
+    return fp4_gemm(quant_rows_fp4(x2, w.fmt), w, bias, x2.dtype)
+
+
+# --------------------------------------------------------------------------- weights
+def quantize_weight_fp4(w: torch.Tensor, fmt: str = DEFAULT_FORMAT) -> Fp4Rows:
+    """Packed rows of a weight matrix [N,K] of any floating type, K % 32 == 0.  Plain tensor arithmetic (done once per
+    layer, on any device); for 16-bit weights the bytes are those of ``quant_rows_fp4``."""
+    block = ops.FP4_BLOCK.get(fmt)
+    if block is None:
+        ops._fp4_code(fmt)
+    N, K = w.shape
+    assert K > 0 and K % 32 == 0, f"K={K} must be a multiple of 32"
+    b = w.detach().float().reshape(N, K // block, block)
+    assert bool(torch.isfinite(b).all()), "weights must be finite"
+    amax = b.abs().amax(dim=2)
+    row = None
+    if fmt == "mx":
+        scale = (torch.frexp(amax)[1] - 3).clamp(-127, 127)                     # floor(log2) - 2; frexp's m is in [1/2, 1)
+        scale = torch.where(amax > 0, scale, torch.full_like(scale, -127))
+        q = torch.ldexp(b, -scale[:, :, None])
+        byte = (scale + 127).to(torch.uint8)
+    else:
+        m, e = torch.frexp(amax.amax(dim=1))
+        e = torch.where(m > 2688 / 4096, e - 11, e - 12).clamp(min=-100)
+        row = torch.ldexp(torch.ones_like(m), torch.where(m > 0, e, torch.zeros_like(e)))
+        s8 = (amax / row[:, None] / 6).to(torch.float8_e4m3fn)
+        s = s8.float()[:, :, None]
+        q = torch.where(s > 0, b / row[:, None, None] / s.clamp_min(2.0 ** -9), torch.zeros_like(b))
+        byte = s8.view(torch.uint8)
+    a = q.abs()
+    # the borders between 0, 1/2, 1, 3/2, 2, 3, 4, 6; a value on a border goes to the even code
+    code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0))
+    code = (code | (torch.signbit(q).to(torch.uint8) << 3)).reshape(N, K)
+    codes = (code[:, 0::2] | (code[:, 1::2] << 4)).contiguous()
+    groups, tiles, _ = ops.fp4_scale_shape(N, K, fmt)
+    flat = torch.zeros((groups * 128, tiles * 4), dtype=torch.uint8, device=w.device)
+    flat[:N, : K // block] = byte
+    scales = flat.reshape(groups, 4, 32, tiles, 4).permute(0, 3, 2, 1, 4).reshape(groups, tiles, 512).contiguous()
+    return Fp4Rows(codes, scales, row)
+
+
+# --------------------------------------------------------------------------- module
+class Fp4Linear(nn.Module):
+    """4-bit stand-in for ``nn.Linear``: packed weights held as buffers, activations quantised per call in the same
+    format.  A low-rank branch (``lowrank=(A, B)`` or the ``_lowrank_A`` / ``_lowrank_B`` attributes that
+    ``Int8Linear`` reads too) is added in the activation type after the product, ``y += (x @ A) @ B``.
+    Needs in_features % 32 == 0."""
+
+    def __init__(self, lin: nn.Linear, device: Optional[torch.device] = None, fmt: str = DEFAULT_FORMAT,
+                 lowrank: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+        super().__init__()
+        w = lin.weight.detach()
+        if device is not None:
+            w = w.to(device, non_blocking=False)
+        q = quantize_weight_fp4(w, fmt)
+        self.fmt = fmt
+        self.register_buffer("weight_codes", q.codes)
+        self.register_buffer("weight_scales", q.scales)
+        self.register_buffer("weight_row_scale", q.row_scale)
+        if lin.bias is not None:
+            b = lin.bias.detach().float()
+            self.register_buffer("bias", (b.to(device) if device is not None else b).contiguous())
+        else:
+            self.bias = None
+        self.in_features = int(lin.in_features)
+        self.out_features = int(lin.out_features)
+        A, B = lowrank if lowrank is not None else (getattr(lin, LOWRANK_A_ATTR, None), getattr(lin, LOWRANK_B_ATTR, None))
+        if A is not None and B is not None:
+            if device is not None:
+                A, B = A.to(device), B.to(device)
+            self.register_buffer("lr_A", A.contiguous())
+            self.register_buffer("lr_B", B.contiguous())
+        else:
+            self.lr_A = None
+            self.lr_B = None
+
+    @property
+    def weight_rows(self) -> Fp4Rows:
+        return Fp4Rows(self.weight_codes, self.weight_scales, self.weight_row_scale)
+
+    def _apply(self, fn, recurse=True):
+        """``.half()`` / ``.to(dtype)`` convert floating buffers; row scales and bias move with them but stay the fp32 they
+        were (a row scale can lie outside fp16's range)."""
+        keep = {n: getattr(self, n) for n in ("weight_row_scale", "bias")}
+        super()._apply(fn, recurse)
+        for name, v in keep.items():
+            new = getattr(self, name)
+            if v is not None and new.dtype != v.dtype:
+                setattr(self, name, v.to(new.device))
+        return self
+
+    def _product(self, xq: Fp4Rows, x2: torch.Tensor) -> torch.Tensor:
+        y = fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype)
+        if self.lr_A is not None:
+            y.addmm_((x2.to(self.lr_A.dtype) @ self.lr_A).to(y.dtype), self.lr_B.to(y.dtype))
+        return y
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        shape = x.shape
+        assert shape[-1] == self.in_features, (tuple(shape), self.in_features)
+        x2 = x.detach().reshape(-1, shape[-1])                 # no gradient, not even through the low-rank branch alone
+        return self._product(quant_rows_fp4(x2, self.fmt), x2).reshape(*shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        return f"in={self.in_features}, out={self.out_features}, 4-bit {self.fmt} W and A, sm_100a tcgen05 kernel"
+
+
+# --------------------------------------------------------------------------- model conversion
+def convert_linears_to_fp4(model: nn.Module, device: Optional[str] = "cuda", fmt: str = DEFAULT_FORMAT,
+                           whitelist: Callable[[str], bool] = is_bf16_whitelisted) -> Dict[str, object]:
+    """Swaps every non-whitelisted ``nn.Linear`` whose in_features the format takes for ``Fp4Linear`` in place and returns
+    statistics as ``convert_linears_to_int8`` does (``n_fp4_linear``, ``params_fp4``, the kept layers)."""
+    dev = torch.device(device) if device is not None else None
+    stats = {"n_fp4_linear": 0, "n_bf16_linear_kept": 0, "params_fp4": 0, "params_bf16_linear_kept": 0, "bf16_kept_names": []}
+    for name, lin in [(n, m) for n, m in model.named_modules() if isinstance(m, nn.Linear)]:
+        if whitelist(name) or lin.in_features % 32 != 0:
+            stats["n_bf16_linear_kept"] += 1
+            stats["params_bf16_linear_kept"] += lin.weight.numel()
+            stats["bf16_kept_names"].append(name)
+            continue
+        parent_name, _, attr = name.rpartition(".")
+        parent = model.get_submodule(parent_name) if parent_name else model
+        setattr(parent, attr, Fp4Linear(lin, device=dev, fmt=fmt))
+        stats["n_fp4_linear"] += 1
+        stats["params_fp4"] += lin.weight.numel()
+    if dev is not None and dev.type == "cuda":
+        torch.cuda.synchronize()
+    per = 0.5 + 1.0 / ops.FP4_BLOCK[fmt]                                         # bytes per weight
+    stats["fp4_weight_gib"] = stats["params_fp4"] * per / 2**30
+    stats["bf16_equiv_gib"] = stats["params_fp4"] * 2 / 2**30
+    return stats

@@ -371,6 +371,100 @@ def unpack_int4(packed: Tensor, out: Optional[Tensor] = None) -> Tensor:
     return out
 
 
+# ------------------------------------------------------------------------------------------------ 4-bit floating point
+FP4_FORMATS = {"mx": _lib.FP4_MX, "nv": _lib.FP4_NV}
+FP4_BLOCK = {"mx": 32, "nv": 16}                     # elements per scale
+
+
+def fp4_scale_shape(M: int, K: int, fmt: str) -> Tuple[int, int, int]:
+    """Shape of the scale array: [row groups of 128, scale tiles, 512 bytes]."""
+    return (M + 127) // 128, (K + 4 * FP4_BLOCK[fmt] - 1) // (4 * FP4_BLOCK[fmt]), 512
+
+
+def _fp4_code(fmt: str) -> int:
+    try:
+        return FP4_FORMATS[fmt]
+    except KeyError:
+        raise ValueError(f"unknown 4-bit format {fmt!r} (expected one of {tuple(FP4_FORMATS)})") from None
+
+
+def fp4_rows_aligned(x2: Tensor) -> Tensor:
+    """The 4-bit kernels load 32 bytes at a time: rows that start elsewhere are made contiguous."""
+    assert x2.dim() == 2 and x2.is_cuda
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) % 16 != 0) or x2.data_ptr() % 32 != 0:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def _quant_rows_fp4_impl(x2: Tensor, fmt: str) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
+    code = _fp4_code(fmt)
+    dt = _dt(x2.dtype)
+    x2 = fp4_rows_aligned(x2)
+    M, K = x2.shape
+    assert K > 0 and K % 32 == 0, f"K={K} must be a multiple of 32"
+    codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x2.device)
+    scales = torch.empty(fp4_scale_shape(M, K, fmt), dtype=torch.uint8, device=x2.device)
+    row_scale = torch.empty((M,), dtype=torch.float32, device=x2.device) if fmt == "nv" else None
+    with _on_device(x2):
+        rc = _LIB().pq_quant_rows_fp4(x2.data_ptr(), dt, M, K, x2.stride(0) if M > 1 else K, code, codes.data_ptr(),
+                                      scales.data_ptr(), _ptr(row_scale), _stream(x2))
+    if rc:
+        _lib.check(rc, f"pq_quant_rows_fp4(M={M}, K={K}, {fmt})")
+    return codes, scales, row_scale
+
+
+def check_fp4_rows(codes: Tensor, scales: Tensor, row_scale: Optional[Tensor], what: str) -> Tuple[str, int, int]:
+    """(format, rows, K) of packed rows whose parts fit together (AssertionError otherwise): the C ABI receives bare
+    pointers."""
+    assert codes.is_cuda and codes.dim() == 2 and codes.dtype == torch.uint8, f"{what}: codes are a uint8 matrix on a GPU"
+    fmt = "mx" if row_scale is None else "nv"
+    M, K = codes.shape[0], codes.shape[1] * 2
+    assert K > 0 and K % 32 == 0, f"{what}: K={K} must be a positive multiple of 32"
+    assert (scales.dtype == torch.uint8 and tuple(scales.shape) == fp4_scale_shape(M, K, fmt) and scales.is_contiguous()
+            and scales.device == codes.device), f"{what}: scales {tuple(scales.shape)} do not fit [{M}, {K}] {fmt} rows"
+    assert row_scale is None or (row_scale.dtype == torch.float32 and row_scale.numel() == M and row_scale.is_contiguous()
+                                 and row_scale.device == codes.device), f"{what}: one fp32 row scale per row"
+    return fmt, M, K
+
+
+def _codes_aligned(codes: Tensor) -> Tensor:
+    if codes.stride(1) != 1 or (codes.shape[0] > 1 and codes.stride(0) % 16 != 0) or codes.data_ptr() % 16 != 0:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    return codes
+
+
+def _dequant_rows_fp4_impl(codes: Tensor, scales: Tensor, row_scale: Optional[Tensor], dtype: torch.dtype) -> Tensor:
+    fmt, M, K = check_fp4_rows(codes, scales, row_scale, "dequant_rows_fp4")
+    codes = _codes_aligned(codes)
+    out = torch.empty((M, K), dtype=dtype, device=codes.device)
+    with _on_device(codes):
+        rc = _LIB().pq_dequant_rows_fp4(codes.data_ptr(), codes.stride(0) if M > 1 else K // 2, scales.data_ptr(),
+                                        _ptr(row_scale), FP4_FORMATS[fmt], out.data_ptr(), _dt(dtype), K, M, K, _stream(codes))
+    if rc:
+        _lib.check(rc, f"pq_dequant_rows_fp4(M={M}, K={K}, {fmt})")
+    return out
+
+
+def _fp4_gemm_impl(xq: Tensor, xs: Tensor, x_row: Optional[Tensor], wq: Tensor, ws: Tensor, w_row: Optional[Tensor],
+                   bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+    fmt, M, K = check_fp4_rows(xq, xs, x_row, "fp4_gemm, activations")
+    fmt_w, N, K_w = check_fp4_rows(wq, ws, w_row, "fp4_gemm, weights")
+    assert fmt_w == fmt and K_w == K, f"{fmt} activations with K={K}, {fmt_w} weights with K={K_w}"
+    assert N > 0 and wq.device == xq.device
+    assert bias is None or (bias.dtype == torch.float32 and bias.numel() == N and bias.is_contiguous()
+                            and bias.device == xq.device), "bias is an fp32 vector with one entry per output channel"
+    xq = _codes_aligned(xq); wq = _codes_aligned(wq)
+    out = torch.empty((M, N), dtype=out_dtype, device=xq.device)
+    st = status_word(xq.device)
+    with _on_device(xq):
+        rc = _LIB().pq_fp4_gemm(xq.data_ptr(), xq.stride(0) if M > 1 else K // 2, xs.data_ptr(), _ptr(x_row), wq.data_ptr(),
+                                wq.stride(0) if N > 1 else K // 2, ws.data_ptr(), _ptr(w_row), _ptr(bias), FP4_FORMATS[fmt],
+                                out.data_ptr(), _dt(out_dtype), N, M, N, K, st.data_ptr(), st.numel() * 4, _stream(xq))
+    if rc:
+        _lib.check(rc, f"pq_fp4_gemm(M={M}, N={N}, K={K}, {fmt})")
+    return out
+
+
 # ------------------------------------------------------------------------------------------------ GEMM
 def epilogue_supported(N: int, out_stride0: int, out_ptr: int, has_lowrank: bool, rank: int = 32) -> bool:
     """Whether pq_int8_gemm_ex takes this problem (its variants live in the CTA-pair kernel's vector stores)."""
@@ -669,6 +763,42 @@ def int8_gemm_g32_op(xq: Tensor, s_a: Tensor, w_int8: Tensor, s_w_gm: Tensor, bi
 @int8_gemm_g32_op.register_fake
 def _(xq, s_a, w_int8, s_w_gm, bias, out_dtype_code):
     return xq.new_empty((xq.shape[0], w_int8.shape[0]), dtype=_CODE2DT[out_dtype_code])
+
+
+# 4-bit rows travel as (codes, scales, row scales); an operator cannot return an optional tensor, so the mx format's absent
+# row scales are an empty tensor here.
+@torch.library.custom_op("pq_b200::quant_rows_fp4", mutates_args=(), device_types="cuda")
+def quant_rows_fp4_op(x2: Tensor, fmt: str) -> Tuple[Tensor, Tensor, Tensor]:
+    codes, scales, row = _quant_rows_fp4_impl(x2, fmt)
+    return codes, scales, row if row is not None else scales.new_empty((0,), dtype=torch.float32)
+
+
+@quant_rows_fp4_op.register_fake
+def _(x2, fmt):
+    M, K = x2.shape
+    return (x2.new_empty((M, K // 2), dtype=torch.uint8), x2.new_empty(fp4_scale_shape(M, K, fmt), dtype=torch.uint8),
+            x2.new_empty((M if fmt == "nv" else 0,), dtype=torch.float32))
+
+
+@torch.library.custom_op("pq_b200::dequant_rows_fp4", mutates_args=(), device_types="cuda")
+def dequant_rows_fp4_op(codes: Tensor, scales: Tensor, row_scale: Optional[Tensor], dtype_code: int) -> Tensor:
+    return _dequant_rows_fp4_impl(codes, scales, row_scale, _CODE2DT[dtype_code])
+
+
+@dequant_rows_fp4_op.register_fake
+def _(codes, scales, row_scale, dtype_code):
+    return codes.new_empty((codes.shape[0], codes.shape[1] * 2), dtype=_CODE2DT[dtype_code])
+
+
+@torch.library.custom_op("pq_b200::fp4_gemm", mutates_args=(), device_types="cuda")
+def fp4_gemm_op(xq: Tensor, xs: Tensor, x_row: Optional[Tensor], wq: Tensor, ws: Tensor, w_row: Optional[Tensor],
+                bias: Optional[Tensor], out_dtype_code: int) -> Tensor:
+    return _fp4_gemm_impl(xq, xs, x_row, wq, ws, w_row, bias, _CODE2DT[out_dtype_code])
+
+
+@fp4_gemm_op.register_fake
+def _(xq, xs, x_row, wq, ws, w_row, bias, out_dtype_code):
+    return xq.new_empty((xq.shape[0], wq.shape[0]), dtype=_CODE2DT[out_dtype_code])
 
 
 @torch.library.custom_op("pq_b200::dequant_epilogue", mutates_args=(), device_types="cuda")

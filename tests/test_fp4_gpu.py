@@ -1,0 +1,283 @@
+"""4-bit floating-point operators on the GPU against the 64-bit restatement: codes, scales and values bit for bit, products
+within a bound derived from the formats' arithmetic.
+
+Bound of a product.  Every product of two values is exact in fp32 (at most 2 x 2 significant bits times scales of 2 x 4).
+One MMA adds 64 of them to the fp32 accumulator; with S = sum |x w| over the row of K, aligning and adding inside an MMA
+loses at most 2 units of 2^-23 S and so does adding its sum to the accumulator: 4 * 2^-23 S per 64 elements, K / 16 * 2^-23 S
+in all.  Joining up to eight partial sums of a split launch: 8 * 2^-24 S.  Row scales are powers of two (exact); the bias
+adds once more (2^-24 of the sum's size).  The rounding to 16 bits is half a step: eps / 2 of the value, or half the
+smallest subnormal.
+"""
+import pytest
+import torch
+import torch.nn as nn
+
+from oracle import fp4 as ofp4
+from pyraquant_b200 import _lib, fp4_exec, ops
+from test_fp4_host import awkward_rows
+
+pytestmark = pytest.mark.gpu
+FMTS = ["mx", "nv"]
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(autouse=True)
+def _status_clean(cuda_dev):
+    yield
+    ops.check_device_status(cuda_dev)
+
+
+def check_rows(q, x, fmt):
+    code, byte, row = ofp4.quantise(x.cpu(), fmt)
+    M, K = x.shape
+    assert q.fmt == fmt and torch.equal(ofp4.untile(q.scales.cpu(), M, K, fmt), byte)
+    if fmt == "nv":
+        assert torch.equal(q.row_scale.cpu().double(), row)
+    got = ofp4.unpack(q.codes.cpu())
+    assert torch.equal(got % 8, code % 8)
+    nz = code % 8 != 0
+    assert torch.equal(got[nz], code[nz])
+
+
+def check_product(y, xq, wq, bias, fmt):
+    """y against the 64-bit product of the packed rows."""
+    X = ofp4.packed_values(xq.codes.cpu(), xq.scales.cpu(), None if xq.row_scale is None else xq.row_scale.cpu(), fmt)
+    W = ofp4.packed_values(wq.codes.cpu(), wq.scales.cpu(), None if wq.row_scale is None else wq.row_scale.cpu(), fmt)
+    K = X.shape[1]
+    ref = X @ W.t()
+    S = X.abs() @ W.abs().t()
+    bound = (K / 16 + 4) * 2.0 ** -23 * S
+    if bias is not None:
+        ref = ref + bias.cpu().double()
+        bound = bound + 2.0 ** -24 * (S + bias.cpu().double().abs())
+    fi = torch.finfo(y.dtype)
+    bound = bound + (ref.abs() + bound) * fi.eps / 2 + fi.smallest_normal * fi.eps / 2
+    err = (y.cpu().double() - ref).abs()
+    worst = float((err / bound).max())
+    assert worst <= 1, f"error {worst:.3g} times the bound at {divmod(int((err / bound).argmax()), y.shape[1])}"
+
+
+def make_rows(M, K, fmt, dtype, seed, dev):
+    x = awkward_rows(M, K, dtype, seed).to(dev)
+    return x, fp4_exec.quant_rows_fp4(x, fmt)
+
+
+# ------------------------------------------------------------------------------------------------ quantisation
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K", [(1, 32), (3, 64), (33, 96), (127, 640), (129, 672), (300, 1280), (70, 2560), (65, 2592), (40, 5120),
+                                 (9, 10240), (5, 12288), (7, 20480), (3, 20512), (2, 40960)])
+def test_quant_rows_match_the_definition(cuda_dev, fmt, dtype, M, K):
+    x = awkward_rows(M, K, dtype, M * 7 + K)
+    check_rows(fp4_exec.quant_rows_fp4(x.to(cuda_dev), fmt), x, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quant_every_significand_against_every_block_maximum(cuda_dev, fmt, dtype):
+    """Blocks whose maximum runs over every significand of the type and whose other elements run over the binades below:
+    every border between codes that the type can hit, exactly and from both sides."""
+    one, per, step = (0x3F80, 128, 1) if dtype == torch.bfloat16 else (0x3C00, 1024, 8)
+    n = 16 if fmt == "nv" else 32
+    amax = torch.arange(one, one + per, step, dtype=torch.int32)
+    below = torch.arange(0, 5 * per, step, dtype=torch.int32)
+    below = torch.nn.functional.pad(below, (0, (-below.numel()) % (n - 1)))
+    rest = (amax[:, None] - below[None, :]).reshape(amax.numel(), -1, n - 1)
+    bits = torch.cat([amax[:, None, None].expand(-1, rest.shape[1], 1), rest], dim=2).reshape(amax.numel(), -1)
+    bits = torch.nn.functional.pad(bits, (0, (-bits.shape[1]) % 32))
+    bits[:, 1::2] |= 0x8000
+    x = torch.where(bits >= 0x8000, bits - 0x10000, bits).to(torch.int16).view(dtype)
+    check_rows(fp4_exec.quant_rows_fp4(x.to(cuda_dev), fmt), x, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quant_every_magnitude(cuda_dev, fmt, dtype):
+    """Every positive finite value of the type as the maximum of a row: row scales, block scales and codes over the whole
+    exponent range, subnormals among them."""
+    top = 0x7F80 if dtype == torch.bfloat16 else 0x7C00
+    v = torch.arange(1, top, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = torch.stack([v * f for f in (1.0, 0.75, -0.4, 0.1)], dim=1).repeat(1, 8)
+    check_rows(fp4_exec.quant_rows_fp4(x.to(cuda_dev), fmt), x, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_read_back(cuda_dev, fmt, dtype):
+    for M, K in ((1, 32), (130, 672), (37, 5120)):
+        x, q = make_rows(M, K, fmt, dtype, M + K, cuda_dev)
+        want = ofp4.packed_values(q.codes.cpu(), q.scales.cpu(), None if q.row_scale is None else q.row_scale.cpu(), fmt)
+        for t in DTYPES:
+            w = want.clamp(-65504, 65504) if t == torch.float16 else want
+            assert torch.equal(fp4_exec.dequant_rows_fp4(q, t).cpu(), w.to(t))
+    big = torch.full((1, 32), 65504.0, dtype=torch.float16, device=cuda_dev)
+    assert torch.isfinite(fp4_exec.dequant_rows_fp4(fp4_exec.quant_rows_fp4(big, fmt), torch.float16)).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_infinities_and_nan(cuda_dev, fmt):
+    x = torch.randn(6, 96, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    x[1, 40] = float("inf"); x[3, 0] = float("nan"); x[4, 95] = float("-inf")
+    q = fp4_exec.quant_rows_fp4(x.to(cuda_dev), fmt)
+    v = fp4_exec.dequant_rows_fp4(q, torch.bfloat16).cpu()
+    bad = torch.zeros(6, 96, dtype=torch.bool)
+    if fmt == "mx":
+        bad[1, 32:64] = True; bad[3, :32] = True; bad[4, 64:] = True
+    else:
+        bad[[1, 3, 4]] = True
+    assert torch.equal(torch.isnan(v), bad)
+    clean = torch.where(bad, torch.zeros_like(x), x)
+    good = ofp4.values(*ofp4.quantise(clean, fmt), fmt).to(torch.bfloat16)
+    assert torch.equal(v[~bad], good[~bad])
+    w = fp4_exec.quantize_weight_fp4(torch.randn(40, 96, generator=torch.Generator().manual_seed(4)), fmt)
+    w = fp4_exec.Fp4Rows(*(None if t is None else t.to(cuda_dev) for t in w))
+    y = fp4_exec.fp4_gemm(q, w, None, torch.bfloat16).cpu()
+    assert torch.isnan(y[[1, 3, 4]]).all() and torch.isfinite(y[[0, 2, 5]]).all()
+
+
+def test_quant_strided_and_offset_rows(cuda_dev):
+    x = awkward_rows(50, 1280, torch.bfloat16, 5).to(cuda_dev)
+    for fmt in FMTS:
+        for view in (x[:, 640:], x[::2], x[3:, :64], x[:, 8:648], x.t()[:32].t(), x[:, ::2], x[7:8, 16:48]):
+            check_rows(fp4_exec.quant_rows_fp4(view, fmt), view, fmt)
+        empty = fp4_exec.quant_rows_fp4(x[:0], fmt)
+        assert empty.codes.shape == (0, 640) and empty.scales.shape[0] == 0
+
+
+# ------------------------------------------------------------------------------------------------ product
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", [(128, 64, 256), (1, 64, 32), (1, 1, 64), (5, 7, 96), (128, 128, 64), (77, 200, 640), (16, 1288, 160),
+                                   (200, 72, 2592), (129, 130, 288), (1, 1280, 5120), (33, 650, 2048)])
+def test_product(cuda_dev, fmt, M, N, K):
+    dtype = DTYPES[(M + N) % 2]
+    _, xq = make_rows(M, K, fmt, dtype, 1, cuda_dev)
+    _, wq = make_rows(N, K, fmt, torch.bfloat16, 2, cuda_dev)
+    bias = torch.randn(N, device=cuda_dev) if N % 2 else None
+    check_product(fp4_exec.fp4_gemm(xq, wq, bias, torch.bfloat16), xq, wq, bias, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", [(2048, 2176, 640), (2500, 1990, 480), (4173, 640, 2560)])
+def test_product_many_tiles(cuda_dev, fmt, M, N, K):
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(M, K, generator=g).to(torch.float16).to(cuda_dev)
+    w = torch.randn(N, K, generator=g).to(torch.bfloat16).to(cuda_dev)
+    xq, wq = fp4_exec.quant_rows_fp4(x, fmt), fp4_exec.quant_rows_fp4(w, fmt)
+    bias = torch.randn(N, generator=g).to(cuda_dev)
+    check_product(fp4_exec.fp4_gemm(xq, wq, bias, torch.bfloat16), xq, wq, bias, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_product_leaves_its_neighbourhood_alone(cuda_dev, fmt):
+    """Rows behind the last one, columns behind the last one and the bytes around the output stay as they were."""
+    M, N, K = 70, 90, 128
+    _, xq = make_rows(M, K, fmt, torch.bfloat16, 1, cuda_dev)
+    _, wq = make_rows(N, K, fmt, torch.bfloat16, 2, cuda_dev)
+    want = fp4_exec.fp4_gemm(xq, wq, None, torch.bfloat16)
+    lib = _lib.load()
+    for ldo, off in ((96, 0), (96, 8), (91, 1)):
+        buf = torch.full((80 * 96,), 7.0, dtype=torch.bfloat16, device=cuda_dev)
+        p = lambda t: None if t is None else t.data_ptr()       # noqa: E731
+        rc = lib.pq_fp4_gemm(p(xq.codes), K // 2, p(xq.scales), p(xq.row_scale), p(wq.codes), K // 2, p(wq.scales), p(wq.row_scale),
+                             None, ops.FP4_FORMATS[fmt], buf.data_ptr() + 2 * off, 0, ldo, M, N, K, None, 0,
+                             torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        got = buf[off: off + M * ldo].view(M, ldo)
+        assert torch.equal(got[:, :N], want)
+        got[:, :N] = 7.0
+        assert bool((buf == 7.0).all())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_product_strided_codes_and_repeatability(cuda_dev, fmt):
+    _, xq = make_rows(150, 1280, fmt, torch.bfloat16, 1, cuda_dev)
+    _, wq = make_rows(200, 1280, fmt, torch.bfloat16, 2, cuda_dev)
+    want = fp4_exec.fp4_gemm(xq, wq, None, torch.float16)
+    wide = torch.full((150, 704), 0xAA, dtype=torch.uint8, device=cuda_dev)
+    for off in (0, 16, 8):                                        # 8: copied first
+        view = wide[:, off: off + 640]
+        view.copy_(xq.codes)
+        got = fp4_exec.fp4_gemm(fp4_exec.Fp4Rows(view, xq.scales, xq.row_scale), wq, None, torch.float16)
+        assert torch.equal(got, want)
+    for _ in range(5):
+        assert torch.equal(fp4_exec.fp4_gemm(xq, wq, None, torch.float16), want)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_refusals(cuda_dev, fmt):
+    x, xq = make_rows(8, 128, fmt, torch.bfloat16, 1, cuda_dev)
+    _, wq = make_rows(16, 128, fmt, torch.bfloat16, 2, cuda_dev)
+    _, other = make_rows(16, 128, "nv" if fmt == "mx" else "mx", torch.bfloat16, 2, cuda_dev)
+    _, longer = make_rows(16, 160, fmt, torch.bfloat16, 2, cuda_dev)
+    R = fp4_exec.Fp4Rows
+    for bad in (lambda: fp4_exec.fp4_gemm(xq, other), lambda: fp4_exec.fp4_gemm(xq, longer),
+                lambda: fp4_exec.fp4_gemm(R(xq.codes, wq.scales[:, :0], xq.row_scale), wq),
+                lambda: fp4_exec.fp4_gemm(R(xq.codes.int(), xq.scales, xq.row_scale), wq),
+                lambda: fp4_exec.fp4_gemm(xq, wq, torch.zeros(15, device=cuda_dev)),
+                lambda: fp4_exec.fp4_gemm(xq, wq, torch.zeros(16, device=cuda_dev, dtype=torch.bfloat16)),
+                lambda: fp4_exec.fp4_gemm(xq, wq, torch.zeros(16)),
+                lambda: fp4_exec.quant_rows_fp4(x[:, :48], fmt)):
+        with pytest.raises(AssertionError):
+            bad()
+    with pytest.raises(TypeError):
+        fp4_exec.quant_rows_fp4(x.float(), fmt)
+    with pytest.raises(TypeError):
+        fp4_exec.fp4_gemm(xq, wq, None, torch.float32)
+    with pytest.raises(ValueError):
+        fp4_exec.quant_rows_fp4(x, "int4")
+
+
+# ------------------------------------------------------------------------------------------------ the Linear
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_runs_its_operators(cuda_dev, fmt, dtype):
+    torch.manual_seed(2)
+    lin = nn.Linear(640, 328).to(dtype)
+    A, B = (torch.randn(640, 32) / 25).to(dtype), (torch.randn(32, 328) / 5).to(dtype)
+    m = fp4_exec.Fp4Linear(lin, device=cuda_dev, fmt=fmt)
+    x = torch.randn(2, 75, 640, device=cuda_dev).to(dtype)
+    y = m(x)
+    xq = fp4_exec.quant_rows_fp4(x.reshape(-1, 640), fmt)
+    assert y.shape == (2, 75, 328) and torch.equal(y.reshape(-1, 328), fp4_exec.fp4_gemm(xq, m.weight_rows, m.bias, dtype))
+    check_product(y.reshape(-1, 328), xq, m.weight_rows, m.bias, fmt)
+    low = fp4_exec.Fp4Linear(lin, device=cuda_dev, fmt=fmt, lowrank=(A, B))
+    yl = low(x)
+    ref = y.double() + ((x.double() @ A.to(cuda_dev).double()).to(dtype).double() @ B.to(cuda_dev).double())
+    # y and the sum are rounded once each, x @ A once (its half step carried through B, 32 terms of |t| |B| <= about 4 * 1)
+    eps = torch.finfo(dtype).eps
+    assert float((yl.double() - ref).abs().max()) <= eps * (float(ref.abs().max()) + float(y.abs().max())) + eps * 32
+    assert m(x[:, :0]).shape == (2, 0, 328)
+    assert torch.equal(m(x[0, 0]), y[0, 0])
+
+
+def test_streams_graphs_and_compile_wrappers(cuda_dev):
+    torch.manual_seed(3)
+    lin = nn.Linear(1280, 640).to(torch.bfloat16)
+    m = fp4_exec.Fp4Linear(lin, device=cuda_dev, fmt="nv")
+    x = torch.randn(300, 1280, device=cuda_dev).to(torch.bfloat16)
+    want = m(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = m(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    with torch.cuda.stream(side):
+        m(x)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    xs = x.clone()
+    with torch.cuda.graph(g1):
+        y1 = m(xs)
+    with torch.cuda.graph(g2):
+        y2 = m(xs * 2)
+    xs.copy_(x)
+    g1.replay(); g2.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y1, want) and torch.equal(y2, m(x * 2))
+    ops_ns = torch.ops.pq_b200
+    c, s, r = ops_ns.quant_rows_fp4(x, "nv")
+    assert torch.equal(ops_ns.fp4_gemm(c, s, r, *m.weight_rows, m.bias, 0), want)
+    assert torch.equal(ops_ns.dequant_rows_fp4(c, s, r, 0), fp4_exec.dequant_rows_fp4(fp4_exec.quant_rows_fp4(x, "nv")))
+    c, s, r = ops_ns.quant_rows_fp4(x, "mx")
+    assert r.numel() == 0
