@@ -110,6 +110,21 @@ int pq_adaln_quant_rows(const void* x, int dtype, int64_t M, int64_t K, int64_t 
                         const void* scale, const void* shift, int64_t ld_mod, int64_t rows_per_sample, float eps,
                         void* x_mod, int64_t ldxm, int8_t* q, float* s, void* stream);
 
+/* Group norm over channels-last rows, with SiLU or without: the norm in front of the SDXL transformer blocks' proj_in and of
+ * its convolutions (no counterpart kernel in the reference, which uses torch's):
+ *   z[b,t,c] = act((x[b,t,c] - mean[b,g]) / sqrt(var[b,g] + eps) * gamma[c] + beta[c]),   g = c / (C / groups),
+ * mean and variance over the T rows and C / groups channels of a group; fp32 throughout, rounded once.
+ *   x [B,T,C] with strides ld_batch, ld_row, 1 (elements); out likewise; gamma, beta [C] in x's type, or fp32 when
+ *   affine_fp32 is set, each NULL for 1 and 0; C % 8 == 0, C <= 8192, C % groups == 0, B <= 65535, strides % 8 == 0,
+ *   16-byte aligned x and out; workspace: pq_group_norm_workspace_bytes (same B, T, C, groups, current device), 8-byte
+ *   aligned.  B == 0 or T == 0 is a no-op. */
+#define PQ_ACT_NONE 0
+#define PQ_ACT_SILU 1
+int64_t pq_group_norm_workspace_bytes(int64_t B, int64_t T, int64_t C, int groups);
+int pq_group_norm(const void* x, int dtype, int64_t B, int64_t T, int64_t C, int64_t ld_row, int64_t ld_batch, int groups,
+                  const void* gamma, const void* beta, int affine_fp32, float eps, int act,
+                  void* out, int64_t ldo_row, int64_t ldo_batch, void* workspace, int64_t ws_bytes, void* stream);
+
 /* Dequantisation of materialised accumulators: out[m,n] = float(acc[m,n]) * (s_row[m] * s_col[n])
  * (+ bias[n]) rounded to out_dtype.  Replaces dequant_epilogue / _dequant_epilogue_kernel
  * (deploy/int8_exec.py:233-243, :104-127); kept for API parity, the fused GEMM never needs it.

@@ -18,6 +18,8 @@ DTYPE_BF16 = 0
 DTYPE_FP16 = 1
 FP4_MX = 0
 FP4_NV = 1
+ACT_NONE = 0
+ACT_SILU = 1
 GEMM_WORKSPACE_BYTES = 256
 
 _lib: Optional[ctypes.CDLL] = None
@@ -38,6 +40,9 @@ SIGNATURES = {
                                       c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "pq_adaln_quant_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64,
                                     ctypes.c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "pq_group_norm_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "pq_group_norm": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int,
+                              ctypes.c_float, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
     "pq_gather_quant_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                      c_void_p, c_void_p]),
     "pq_gather_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,

@@ -169,6 +169,18 @@ class Fp4Linear(nn.Module):
         x2 = x.detach().reshape(-1, shape[-1])                 # no gradient, not even through the low-rank branch alone
         return self._product(quant_rows_fp4(x2, self.fmt), x2).reshape(*shape[:-1], self.out_features)
 
+    def forward_group_norm(self, h: torch.Tensor, groups: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                           eps: float = 1e-6, act: Optional[str] = None) -> torch.Tensor:
+        """``self(act(GroupNorm(h)))`` for channels-last rows h [B, ..., K], the same values as
+        ``norm_exec.group_norm_rows`` followed by the layer."""
+        from . import norm_exec
+        K = h.shape[-1]
+        assert K == self.in_features, (tuple(h.shape), self.in_features)
+        if self.lr_A is not None:                              # the branch reads the 16-bit rows
+            return self.forward(norm_exec.group_norm_rows(h, groups, weight, bias, eps, act))
+        xq = norm_exec.group_norm_quant_fp4(h, groups, weight, bias, eps, act, self.fmt)
+        return fp4_gemm(xq, self.weight_rows, self.bias, h.dtype).reshape(*h.shape[:-1], self.out_features)
+
     def extra_repr(self) -> str:
         return f"in={self.in_features}, out={self.out_features}, 4-bit {self.fmt} W and A, sm_100a tcgen05 kernel"
 

@@ -515,6 +515,28 @@ class Int8Linear(nn.Module):
         out = y2.reshape(*h.shape[:-1], self.out_features)
         return (out, z.reshape(h.shape)) if return_modulated else out
 
+    def forward_group_norm(self, h: torch.Tensor, groups: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                           eps: float = 1e-6, act: Optional[str] = None, return_normed: bool = False):
+        """``self(act(GroupNorm(h)))`` for channels-last rows h [B, ..., K]: the ``norm`` and ``proj_in`` of an SDXL transformer
+        block.  Values are those of ``norm_exec.group_norm_rows`` followed by the layer; the 16-bit normed rows are
+        written out only when the layer has a low-rank branch or the caller wants them (``return_normed``)."""
+        from . import norm_exec
+        lr = self.lr_A is not None
+        K = h.shape[-1]
+        fused = (h.numel() > 0 and h.dtype in ops._DT and K % 16 == 0 and not torch.compiler.is_compiling()
+                 and (not lr or (K % 32 == 0 and self.lr_A.shape[1] == 32 and self.lr_A.dtype == h.dtype
+                                 and self.lr_B.dtype == h.dtype and self.out_features % 8 == 0)))
+        if not fused:
+            z = norm_exec.group_norm_rows(h, groups, weight, bias, eps, act)
+            out = self.forward(z)
+            return (out, z) if return_normed else out
+        xq, sx, z = norm_exec.group_norm_quant_rows(h, groups, weight, bias, eps, act, want_normed=lr or return_normed)
+        t = self._down(z.reshape(-1, K)) if lr else None
+        y2 = ops._gemm_impl(xq, sx, self.weight_int8, self.w_scale, self.bias, t, self.lr_B if lr else None, h.dtype,
+                            lb_t=self._lr_Bt() if lr else None)
+        out = y2.reshape(*h.shape[:-1], self.out_features)
+        return (out, z) if return_normed else out
+
     def _prologue(self, x2: torch.Tensor, x_more: Optional[torch.Tensor] = None):
         """(codes, row scales, t or None) of the layer's input; with ``x_more`` the input is ``[x2 | x_more]`` along the
         features, read from its two sources where the kernels take them and concatenated otherwise."""

@@ -1,0 +1,46 @@
+"""Group norm over channels-last rows, with SiLU or without, and its forms that hand quantised rows to a Linear.
+
+SDXL's transformer blocks put a GroupNorm in front of ``proj_in`` as FLUX's put an adaLN in front of the feed-forward
+(``ops.adaln_quant_rows``); image-token rows [B, T, C] (or [B, H, W, C]) keep a token's channels together, so the norm works
+on them without a transposition:
+
+    z[b,t,c] = act((x[b,t,c] - mean[b,g]) / sqrt(var[b,g] + eps) * weight[c] + bias[c])
+
+Statistics and arithmetic are fp32, the result is rounded once.  CUDA tensors only (AssertionError otherwise); there is no
+gradient: tensors that autograd follows raise RuntimeError.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import ops
+from .fp4_exec import DEFAULT_FORMAT, Fp4Rows, quant_rows_fp4
+from .int8_exec import _eager, quant_rows
+
+
+def group_norm_rows(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                    eps: float = 1e-6, act: Optional[str] = None) -> torch.Tensor:
+    """x [B, ..., C] bf16/fp16, channels last -> normed rows of the same shape and type.  ``act``: None or "silu".
+    weight / bias [C] in x's type or fp32, or None.  C % 8 == 0, C <= 8192, C % groups == 0."""
+    assert x.is_cuda
+    if _eager():
+        return ops._group_norm_impl(x, groups, weight, bias, eps, act)
+    return torch.ops.pq_b200.group_norm_rows(x, groups, weight, bias, eps, act == "silu")
+
+
+def group_norm_quant_rows(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                          eps: float = 1e-6, act: Optional[str] = None,
+                          want_normed: bool = False) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """(q, s, z) with z = group_norm_rows(x, ...) and (q, s) = quant_rows of z's rows; z is None unless ``want_normed``."""
+    z = group_norm_rows(x, groups, weight, bias, eps, act)
+    q, s = quant_rows(z.reshape(-1, z.shape[-1]))
+    return q, s, z if want_normed else None
+
+
+def group_norm_quant_fp4(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                         eps: float = 1e-6, act: Optional[str] = None, fmt: str = DEFAULT_FORMAT) -> Fp4Rows:
+    """quant_rows_fp4 of the rows of group_norm_rows(x, ...); C % 32 == 0."""
+    z = group_norm_rows(x, groups, weight, bias, eps, act)
+    return quant_rows_fp4(z.reshape(-1, z.shape[-1]), fmt)

@@ -217,6 +217,58 @@ def adaln_quant_rows(x2: Tensor, scale: Tensor, shift: Tensor, eps: float = 1e-6
     return q, s, z
 
 
+GROUP_NORM_ACTS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU}
+GROUP_NORM_MAX_C = 8192
+
+
+def group_norm_args(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], act: Optional[str]):
+    """Checks a group norm's operands; returns x as [B, T, C] with rows the kernels take, the affine vectors (both fp32 or both in
+    x's type) and the activation's code."""
+    assert x.is_cuda and x.dim() >= 2, "channels-last rows [B, ..., C] on a GPU"
+    _dt(x.dtype)
+    if act not in GROUP_NORM_ACTS:
+        raise ValueError(f"unknown activation {act!r} (expected one of {tuple(GROUP_NORM_ACTS)})")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        raise RuntimeError("group norm has no gradient here: call it under torch.no_grad() or on detached tensors")
+    C = x.shape[-1]
+    assert groups > 0 and C % groups == 0, f"{C} channels in {groups} groups"
+    assert C % 8 == 0 and 0 < C <= GROUP_NORM_MAX_C, f"{C} channels: a multiple of 8 up to {GROUP_NORM_MAX_C}"
+    for v in (weight, bias):
+        assert v is None or (v.numel() == C and v.device == x.device and v.dtype in (x.dtype, torch.float32)), \
+            "weight and bias: one entry per channel, in the activation type or fp32, on the same device"
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        weight, bias = weight.float(), bias.float()
+    weight = None if weight is None else weight.reshape(-1).contiguous()
+    bias = None if bias is None else bias.reshape(-1).contiguous()
+    T = 1
+    for n in x.shape[1:-1]:
+        T *= n
+    x3 = x.reshape(x.shape[0], T, C)
+    if (x3.stride(2) != 1 or x3.data_ptr() % 16 != 0 or (T > 1 and (x3.stride(1) % 8 != 0 or x3.stride(1) < C))
+            or (x3.shape[0] > 1 and x3.stride(0) % 8 != 0)):
+        x3 = x3.clone(memory_format=torch.contiguous_format)
+    return x3, weight, bias, GROUP_NORM_ACTS[act]
+
+
+def _group_norm_impl(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                     act: Optional[str]) -> Tensor:
+    x3, weight, bias, code = group_norm_args(x, groups, weight, bias, act)
+    B, T, C = x3.shape
+    out = torch.empty((B, T, C), dtype=x.dtype, device=x.device)
+    if out.numel():
+        lib = _LIB()
+        f32 = any(v is not None and v.dtype == torch.float32 for v in (weight, bias))
+        with _on_device(x3):
+            nbytes = lib.pq_group_norm_workspace_bytes(B, T, C, groups)
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
+            rc = lib.pq_group_norm(x3.data_ptr(), _dt(x.dtype), B, T, C, x3.stride(1) if T > 1 else C,
+                                   x3.stride(0) if B > 1 else T * C, groups, _ptr(weight), _ptr(bias), int(f32), float(eps), code,
+                                   out.data_ptr(), C, T * C, ws.data_ptr(), nbytes, _stream(x3))
+        if rc:
+            _lib.check(rc, f"pq_group_norm(B={B}, T={T}, C={C}, groups={groups})")
+    return out.reshape(x.shape)
+
+
 def _gather_quant_rows_impl(canvas: Tensor, row_idx: Tensor) -> Tuple[Tensor, Tensor]:
     canvas = _rows_ok(canvas)
     assert row_idx.is_cuda and row_idx.dtype == torch.int32 and row_idx.dim() == 1 and row_idx.is_contiguous()
@@ -763,6 +815,16 @@ def int8_gemm_g32_op(xq: Tensor, s_a: Tensor, w_int8: Tensor, s_w_gm: Tensor, bi
 @int8_gemm_g32_op.register_fake
 def _(xq, s_a, w_int8, s_w_gm, bias, out_dtype_code):
     return xq.new_empty((xq.shape[0], w_int8.shape[0]), dtype=_CODE2DT[out_dtype_code])
+
+
+@torch.library.custom_op("pq_b200::group_norm_rows", mutates_args=(), device_types="cuda")
+def group_norm_rows_op(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, silu: bool) -> Tensor:
+    return _group_norm_impl(x, groups, weight, bias, eps, "silu" if silu else None)
+
+
+@group_norm_rows_op.register_fake
+def _(x, groups, weight, bias, eps, silu):
+    return x.new_empty(x.shape)
 
 
 # 4-bit rows travel as (codes, scales, row scales); an operator cannot return an optional tensor, so the mx format's absent

@@ -1,0 +1,243 @@
+"""Group norm over channels-last rows against the formula in 64 bits, and its quantising forms against their parts.
+
+Bound.  A thread sums at most L rows of x - pivot one after the other (L <= 64 for the sizes here) and at most 64 merges
+follow: the mean is off by at most (L + 64) 2^-24 mean|x - pivot|, with |x - pivot| taken as at most 8 deviations, plus
+one rounding of its own size, 2^-24 |mean| a few times over; the variance likewise, relative to itself.  So x-hat is off by
+A (1 + |x-hat|) + 4 2^-24 |mean| / std with A = 128 * 8 * 2^-24.  gamma multiplies that, SiLU's slope is at most 1.1 and its own
+evaluation loses (4 + |z|) 2^-23 of its value (exp's argument rounds, exp and the quotient a few units each).  The
+rounding to 16 bits is eps / 2 of the value or half the smallest subnormal.
+"""
+import ctypes
+
+import pytest
+import torch
+import torch.nn as nn
+
+from pyraquant_b200 import _lib, fp4_exec, int8_exec, norm_exec, ops
+
+DTYPES = [torch.bfloat16, torch.float16]
+A = 128 * 8 * 2.0 ** -24
+
+
+def formula(x, groups, w, b, eps, act):
+    """(z, bound before the rounding to 16 bits) in 64 bits; x [B, T, C]."""
+    B, T, C = x.shape
+    v = x.double().reshape(B, T, groups, C // groups)
+    mean = v.mean(dim=(1, 3), keepdim=True)
+    var = ((v - mean) ** 2).mean(dim=(1, 3), keepdim=True)
+    rstd = 1 / torch.sqrt(var + eps)
+    xh = (v - mean) * rstd
+    # with eps > 0 the error of x-hat scales with rstd, not 1 / std
+    err = (A * (torch.sqrt(var) * rstd + xh.abs()) + 4 * 2.0 ** -24 * mean.abs() * rstd).expand_as(v)
+    w = torch.ones(C, dtype=torch.float64) if w is None else w.double()
+    b = torch.zeros(C, dtype=torch.float64) if b is None else b.double()
+    z = xh.reshape(B, T, C) * w + b
+    err = err.reshape(B, T, C) * w.abs() + 2.0 ** -23 * (z.abs() + b.abs())
+    if act == "silu":
+        z, err = z / (1 + torch.exp(-z)), 1.1 * err + (4 + z.abs()) * 2.0 ** -23 * (z / (1 + torch.exp(-z))).abs()
+    return z, err
+
+
+def check(got, x, groups, w, b, eps, act):
+    C = x.shape[-1]
+    z, err = formula(x.cpu().reshape(x.shape[0], -1, C), groups, None if w is None else w.cpu(), None if b is None else b.cpu(), eps, act)
+    fi = torch.finfo(got.dtype)
+    bound = err + (z.abs() + err) * fi.eps / 2 + fi.smallest_normal * fi.eps / 2
+    off = (got.cpu().double().reshape(z.shape) - z).abs()
+    assert bool(torch.isfinite(got).all())
+    worst = float((off / bound).max())
+    assert worst <= 1, f"{worst:.3g} times the bound"
+
+
+def rows(B, T, C, dtype, seed, mean=0.5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, T, C, generator=g) * (0.3 + torch.rand(C, generator=g)) + mean * torch.randn(C, generator=g)
+    return x.to(dtype), (1 + 0.3 * torch.randn(C, generator=g)).to(dtype), (0.3 * torch.randn(C, generator=g)).to(dtype)
+
+
+SHAPES = [(1, 1, 8, 1), (2, 1, 32, 32), (1, 7, 64, 4), (3, 50, 320, 32), (1, 1000, 1280, 32), (2, 333, 640, 32), (1, 4097, 256, 32),
+          (1, 100, 8192, 8), (1, 40, 4104, 3), (300, 3, 32, 4), (149, 2, 64, 8), (4, 2048, 128, 32), (1, 5, 1920, 32), (5, 601, 960, 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,C,groups", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_group_norm(cuda_dev, dtype, B, T, C, groups):
+    x, w, b = (t.to(cuda_dev) for t in rows(B, T, C, dtype, B + T + C))
+    for act in (None, "silu"):
+        check(norm_exec.group_norm_rows(x, groups, w, b, 1e-6, act), x, groups, w, b, 1e-6, act)
+    check(norm_exec.group_norm_rows(x, groups), x, groups, None, None, 1e-6, None)
+    check(norm_exec.group_norm_rows(x, groups, w.float(), b, 1e-5, "silu"), x, groups, w.float(), b, 1e-5, "silu")
+    check(norm_exec.group_norm_rows(x, groups, None, b.float()), x, groups, None, b.float(), 1e-6, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_mean_and_outliers(cuda_dev, dtype):
+    """A mean far above the deviation, rows that begin with an outlier (the pivot of the sums), constant groups."""
+    g = torch.Generator().manual_seed(8)
+    x = (100 + torch.randn(2, 600, 64, generator=g)).to(dtype)
+    x[:, ::97] = 90
+    x[1, :, :16] = 3.0                                            # variance 0
+    check(norm_exec.group_norm_rows(x.to(cuda_dev), 8), x, 8, None, None, 1e-6, None)
+
+
+@pytest.mark.gpu
+def test_layouts(cuda_dev):
+    x, w, b = (t.to(cuda_dev) for t in rows(3, 64, 320, torch.bfloat16, 4))
+    want = norm_exec.group_norm_rows(x, 32, w, b)
+    img = x.reshape(3, 8, 8, 320)
+    assert torch.equal(norm_exec.group_norm_rows(img, 32, w, b), want.reshape(img.shape))
+    nchw = img.permute(0, 3, 1, 2)                                # a channels_last image
+    assert torch.equal(norm_exec.group_norm_rows(nchw.permute(0, 2, 3, 1), 32, w, b), want.reshape(img.shape))
+    wide = torch.randn(3, 70, 400, device=cuda_dev).to(torch.bfloat16)
+    for off in (0, 8, 3):                                         # 3: copied first
+        view = wide[:, 2:66, off: off + 320]
+        view.copy_(x)
+        keep = wide.clone()
+        assert torch.equal(norm_exec.group_norm_rows(view, 32, w, b), want)
+        assert torch.equal(wide, keep)
+    assert torch.equal(norm_exec.group_norm_rows(x[:1].expand(4, 64, 320), 32, w, b), want[:1].expand(4, 64, 320))
+    assert torch.equal(norm_exec.group_norm_rows(x.transpose(1, 2).contiguous().transpose(1, 2), 32, w, b), want)
+    assert norm_exec.group_norm_rows(x[:0], 32, w, b).shape == (0, 64, 320)
+    assert norm_exec.group_norm_rows(x[:, :0], 32, w, b).shape == (3, 0, 320)
+    flat = torch.randn(5, 64, device=cuda_dev).to(torch.float16)   # [B, C]: one row per sample
+    assert torch.equal(norm_exec.group_norm_rows(flat, 4), norm_exec.group_norm_rows(flat[:, None], 4)[:, 0])
+
+
+@pytest.mark.gpu
+def test_nan_stays_in_its_group(cuda_dev):
+    x, w, b = (t.to(cuda_dev) for t in rows(2, 300, 64, torch.float16, 5))
+    want = norm_exec.group_norm_rows(x, 8, w, b)
+    x[1, 17, 20] = float("nan")
+    got = norm_exec.group_norm_rows(x, 8, w, b)
+    assert torch.isnan(got[1, :, 16:24]).all()
+    got[1, :, 16:24] = want[1, :, 16:24]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,C", [(1, 1, 32), (2, 77, 320), (3, 250, 640), (1, 1024, 1280), (2, 40, 2560), (1, 9, 8192), (150, 2, 64)])
+def test_quantising_forms(cuda_dev, dtype, B, T, C):
+    """The forms that quantise in the same call give the codes of the separate steps, bit for bit."""
+    groups = 32 if C >= 320 else 4
+    x, w, b = (t.to(cuda_dev) for t in rows(B, T, C, dtype, 3 * C + T))
+    for act in (None, "silu"):
+        z = norm_exec.group_norm_rows(x, groups, w, b, 1e-6, act)
+        q0, s0 = int8_exec.quant_rows(z.reshape(-1, C))
+        for want_normed in (False, True):
+            q, s, zz = norm_exec.group_norm_quant_rows(x, groups, w, b, 1e-6, act, want_normed=want_normed)
+            assert torch.equal(q, q0) and torch.equal(s, s0)
+            assert zz is None if not want_normed else torch.equal(zz, z)
+        for fmt in ("mx", "nv"):
+            f0, f = fp4_exec.quant_rows_fp4(z.reshape(-1, C), fmt), norm_exec.group_norm_quant_fp4(x, groups, w, b, 1e-6, act, fmt)
+            assert f.fmt == fmt and torch.equal(f.codes, f0.codes)
+            assert torch.equal(fp4_exec.dequant_rows_fp4(f), fp4_exec.dequant_rows_fp4(f0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_in_front_of_a_linear(cuda_dev, dtype):
+    torch.manual_seed(4)
+    lin = nn.Linear(640, 640).to(dtype)
+    low = ((torch.randn(640, 32) / 25).to(dtype), (torch.randn(32, 640) / 6).to(dtype))
+    x, w, b = (t.to(cuda_dev) for t in rows(2, 90, 640, dtype, 6))
+    x = x.reshape(2, 9, 10, 640)
+    z = norm_exec.group_norm_rows(x, 32, w, b)
+    for layer in (int8_exec.Int8Linear(lin, device=cuda_dev), int8_exec.Int8Linear(lin, device=cuda_dev, lowrank=low)):
+        want = layer(z)
+        y, zz = layer.forward_group_norm(x, 32, w, b, return_normed=True)
+        assert y.shape == (2, 9, 10, 640) and torch.equal(zz, z)
+        # the low-rank branch may be summed in another order by the one-launch prologue: a rounding of t, then of y
+        tol = 0 if layer.lr_A is None else 4 * torch.finfo(dtype).eps * float(want.abs().max())
+        assert float((y.float() - want.float()).abs().max()) <= tol
+        assert torch.equal(layer.forward_group_norm(x, 32, w, b), y)
+    for fmt in ("mx", "nv"):
+        for layer in (fp4_exec.Fp4Linear(lin, device=cuda_dev, fmt=fmt), fp4_exec.Fp4Linear(lin, device=cuda_dev, fmt=fmt, lowrank=low)):
+            assert torch.equal(layer.forward_group_norm(x, 32, w, b), layer(z))
+    ops.check_device_status(cuda_dev)
+
+
+@pytest.mark.gpu
+def test_streams_graphs_and_repeats(cuda_dev):
+    x, w, b = (t.to(cuda_dev) for t in rows(2, 5000, 320, torch.bfloat16, 7))
+    want = norm_exec.group_norm_rows(x, 32, w, b, 1e-6, "silu")
+    for _ in range(5):
+        assert torch.equal(norm_exec.group_norm_rows(x, 32, w, b, 1e-6, "silu"), want)
+    assert torch.equal(torch.ops.pq_b200.group_norm_rows(x, 32, w, b, 1e-6, True), want)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append(norm_exec.group_norm_rows(x, 32, w, b, 1e-6, "silu"))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    xs = x.clone()
+    graphs, ys = [], []
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ys.append(norm_exec.group_norm_quant_fp4(xs * (k + 1), 32, w, b, 1e-6, "silu", "nv"))
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for k in range(2):
+        f0 = norm_exec.group_norm_quant_fp4(x * (k + 1), 32, w, b, 1e-6, "silu", "nv")
+        assert torch.equal(ys[k].codes, f0.codes) and torch.equal(ys[k].row_scale, f0.row_scale)
+    with torch.cuda.stream(streams[0]):
+        graphs[0].replay()
+    with torch.cuda.stream(streams[1]):
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(ys[1].codes, f0.codes)
+
+
+@pytest.mark.gpu
+def test_refusals_gpu(cuda_dev):
+    x = torch.randn(2, 5, 64, device=cuda_dev).to(torch.bfloat16)
+    for bad in (lambda: norm_exec.group_norm_rows(x, 7), lambda: norm_exec.group_norm_rows(x[..., :60], 4),
+                lambda: norm_exec.group_norm_rows(x, 8, torch.ones(63, device=cuda_dev)), lambda: norm_exec.group_norm_rows(x, 8, torch.ones(64)),
+                lambda: norm_exec.group_norm_rows(x, 8, torch.ones(64, device=cuda_dev, dtype=torch.float64)),
+                lambda: norm_exec.group_norm_rows(torch.zeros(1, 1, 8200, device=cuda_dev, dtype=torch.float16), 1),
+                lambda: norm_exec.group_norm_rows(x[0, 0], 8), lambda: norm_exec.group_norm_quant_fp4(x[..., :48].contiguous(), 4)):
+        with pytest.raises(AssertionError):
+            bad()
+    with pytest.raises(TypeError):
+        norm_exec.group_norm_rows(x.float(), 8)
+    with pytest.raises(ValueError):
+        norm_exec.group_norm_rows(x, 8, act="gelu")
+    w = nn.Parameter(torch.ones(64, device=cuda_dev, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError):
+        norm_exec.group_norm_rows(x, 8, w)
+    with torch.no_grad():
+        norm_exec.group_norm_rows(x, 8, w)
+    with torch.inference_mode():
+        norm_exec.group_norm_rows(x, 8, w)
+
+
+def test_refusals_on_the_host():
+    with pytest.raises(AssertionError):
+        norm_exec.group_norm_rows(torch.randn(2, 4, 64, dtype=torch.bfloat16), 8)
+
+
+def test_argument_checks():
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 63) & ~63
+    big = 1 << 30
+
+    def gn(x=p, dtype=0, B=1, T=4, C=64, row=64, batch=256, groups=8, w=None, b=None, f32=0, eps=1e-6, act=0, out=p, orow=64,
+           obatch=256, ws=p, wsb=big):
+        return lib.pq_group_norm(x, dtype, B, T, C, row, batch, groups, w, b, f32, eps, act, out, orow, obatch, ws, wsb, None)
+    assert gn(B=0, x=None) == 0 and gn(T=0, x=None) == 0
+    assert gn(x=None) == 1 and gn(out=None) == 1 and gn(ws=None) == 1
+    assert gn(B=-1) == 2 and gn(C=0) == 2 and gn(groups=0) == 2 and gn(groups=7) == 2 and gn(row=56) == 2 and gn(eps=-1.0) == 2
+    assert gn(eps=float("nan")) == 2 and gn(C=8200, row=8200, orow=8200) == 2 and gn(B=65536) == 2
+    assert gn(C=60, groups=4) == 3 and gn(row=68) == 3 and gn(batch=257) == 3 and gn(x=p + 8) == 3 and gn(out=p + 2) == 3 and gn(ws=p + 4) == 3
+    assert gn(w=p + 1) == 3 and gn(b=p + 2, f32=1) == 3
+    assert gn(dtype=2) == 4 and gn(act=2) == 7 and gn(wsb=0) == 8
+    assert lib.pq_group_norm_workspace_bytes(1, 4, 64, 8) >= 64 and lib.pq_group_norm_workspace_bytes(0, 4, 64, 8) == 0
