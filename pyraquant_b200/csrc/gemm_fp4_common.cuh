@@ -30,6 +30,9 @@ struct Fp4GemmParams {
   int vec;                 // rows may be stored 16 bytes at a time
 };
 
+// The CTA-pair kernel (gemm_fp4_pair.cu).  Fills in the tile counts itself.
+int launch_fp4_pair(int fmt, const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, const Fp4GemmParams& p, cudaStream_t st);
+
 namespace {
 
 constexpr int kFp4StageK = 256;                                   // elements per stage = 128 bytes

@@ -1,0 +1,378 @@
+// Block-scaled 4-bit GEMM on CTA pairs (tcgen05 cta_group::2), the kernel of the large products; operands, scales and
+// epilogue arithmetic as in gemm_fp4.cu.
+//
+// A cluster of two CTAs computes a 256 x 256 tile: CTA r owns rows [128 r, +128) of it in its own tensor memory, loads its
+// own 128 activation rows and their scales, HALF of the weight rows, and all 256 rows of weight scales (each SM's tensor
+// core needs them).  Per stage of K = 256 an SM pulls 32 KB of codes and 3 (mx) or 6 (nv) KB of scales from L2 for
+// 512 cycles of MMA; the 128 x 128 tiles of the single-CTA kernel need 34 to 36 KB for 256 cycles.
+//
+// Tensor memory, 512 columns: two accumulators of 256 columns would leave no room for scales, so they overlap:
+//   accumulator 0 [0, 256), accumulator 1 [128, 384), scale sets [384, 512).
+// The epilogue of a tile drains the shared columns [128, 256) first and signals `shared_free`; then the next tile's MMAs
+// may start in the other accumulator while the epilogue goes on with the columns that belong to its own alone.
+// A scale set is written again only once the MMAs that read it have completed: with as many sets as stages (mx) the
+// stage's own hand-over shows that, with two sets (nv) the MMA thread also waits for the stage before last.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-9 epilogue (a 32-row quarter and, step by step, 64 columns each:
+// scale, bias, rounding, swizzled 4 KB staging block, TMA store; plain stores where TMA cannot address the rows).  Tiles go to the pairs in the order of blocks of eight
+// row tiles, columns outside, so that the pairs at work share few activation and weight tiles.  Every wait is bounded; no
+// multicast.
+#include "gemm_fp4_common.cuh"
+
+namespace pq {
+namespace {
+
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = (2 + kPairEpiWarps) * 32;
+constexpr int kPairStages = 5;
+constexpr int kRowBlock = 8;                     // row tiles per block of the tile order
+
+template <int FMT>
+struct Fp4PairSmem {
+  static constexpr int kABytes = BM * BK, kBBytes = 128 * BK;
+  static constexpr int kOperand = kABytes + kBBytes;
+  static constexpr int kSfa = Fp4Fmt<FMT>::kScaleBytes, kSfb = 2 * Fp4Fmt<FMT>::kScaleBytes;
+  static constexpr int kStageBytes = kOperand + kSfa + kSfb;                 // per CTA
+  static constexpr int kOutOff = kPairStages * kOperand;                     // 1024-byte aligned blocks first
+  static constexpr int kOutBlock = 32 * 128;
+  static constexpr int kScaleOff = kOutOff + kPairEpiWarps * kOutBlock;
+  static constexpr int kColOff = kScaleOff + kPairStages * (kSfa + kSfb);    // {scale, bias} of the tile's 256 columns
+  static constexpr int kBarOff = kColOff + 256 * 8;
+  static constexpr int kNumBars = 2 * kPairStages + 2;                       // full, empty, acc_full, shared_free
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kTotal = kMiscOff + 16;
+  static_assert(kTotal <= 232448, "exceeds the 227 KB shared memory of one CTA");
+  static constexpr int kSetCols = 12 * Fp4Fmt<FMT>::kTilesPerStage;          // per tile: 4 columns for A, 8 for B
+  static constexpr int kSets = FMT == PQ_FP4_MX ? kPairStages : 2;
+  static_assert(384 + kSets * kSetCols <= 512, "tensor memory");
+};
+
+// scale tiles: three-dimensional TMA load {word, scale tile, row group}, zero-filled past the ends
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(m), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+template <int FMT>
+__device__ __forceinline__ void tc_mma_fp4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa_tmem,
+                                                uint32_t sfb_tmem, uint32_t acc) {
+  if constexpr (FMT == PQ_FP4_MX)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(acc)
+        : "memory");
+}
+// both CTAs copy the tile at this offset of their own shared memory into their own tensor memory
+__device__ __forceinline__ void tc_cp_scale_tile_pair(uint32_t tmem_addr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem_addr), "l"(desc) : "memory");
+}
+
+struct PairTile { int mt, nt; };
+__device__ __forceinline__ PairTile pair_tile(int t, int mt_total, int nt_total) {
+  const int block = t / (kRowBlock * nt_total);
+  const int rem = t - block * kRowBlock * nt_total;
+  const int left = mt_total - block * kRowBlock;
+  const int hb = left < kRowBlock ? left : kRowBlock;
+  const int col = rem / hb;
+  return PairTile{block * kRowBlock + rem - col * hb, col};
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(kPairThreads, 1)
+pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                        const __grid_constant__ CUtensorMap tmSa, const __grid_constant__ CUtensorMap tmSw,
+                        const __grid_constant__ CUtensorMap tmOut, const Fp4GemmParams p) {
+  using L = Fp4PairSmem<FMT>;
+  using F = Fp4Fmt<FMT>;
+  constexpr int S = kPairStages;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* empty_bar = full_bar + S;
+  uint64_t* acc_full = empty_bar + S;
+  uint64_t* shared_free = acc_full + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_cta_rank();
+  const bool aligned_ok = (smem_u32(smem) & 1023u) == 0;
+  const int pair = static_cast<int>(blockIdx.x) >> 1, pairs = static_cast<int>(gridDim.x) >> 1;
+  const int tiles = p.mt * p.nt;                                   // of 256 x 256
+  const int num_kb = (p.K + kFp4StageK - 1) / kFp4StageK;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmW); tma_prefetch_desc(&tmSa); tma_prefetch_desc(&tmSw);
+    if (p.vec) tma_prefetch_desc(&tmOut);
+    for (int s = 0; s < S; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    mbar_init(acc_full, 1); mbar_init(shared_free, 2 * kPairEpiWarps);
+    *abort_flag = aligned_ok ? 0 : 1;
+    if (!aligned_ok) report_timeout(p.status, 7, 7);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) { tmem_alloc_pair(tmem_holder, 512); tmem_relinquish_pair(); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                 // both CTAs' barriers exist before anyone signals across the pair
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  auto leader_addr = [&](const uint64_t* bar) { return map_to_cta(smem_u32(bar), 0u); };
+  auto peer_addr = [&](const uint64_t* bar) { return map_to_cta(smem_u32(bar), 1u); };
+
+  if (aligned_ok && warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (both CTAs)
+    if (elect_one()) {
+      int stage = 0; uint32_t phase = 0; int issued = 0; bool ok = true;
+#pragma unroll 1
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        const PairTile tile = pair_tile(t, p.mt, p.nt);
+        const int row0 = tile.mt * 256 + static_cast<int>(rank) * BM;
+        const int n0 = tile.nt * 256;
+        const int nhalf0 = n0 + static_cast<int>(rank) * 128;
+#pragma unroll 1
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!wait_or_abort(&empty_bar[stage], phase ^ 1u, abort_flag)) {
+            report_timeout(p.status, 1, 1); *abort_flag = 1; ok = false; break;
+          }
+          uint8_t* a_s = smem + stage * L::kOperand;
+          uint8_t* s_s = smem + L::kScaleOff + stage * (L::kSfa + L::kSfb);
+          const uint32_t fb = leader_addr(&full_bar[stage]);
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kStageBytes);
+          tma_load_2d_pair(a_s, &tmA, fb, kb * BK, row0);
+          tma_load_2d_pair(a_s + L::kABytes, &tmW, fb, kb * BK, nhalf0);
+          tma_load_3d_pair(s_s, &tmSa, fb, 0, kb * F::kTilesPerStage, row0 >> 7);
+          tma_load_3d_pair(s_s + L::kSfa, &tmSw, fb, 0, kb * F::kTilesPerStage, n0 >> 7);
+          if (issued < S) ++issued;
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+      }
+      // copies in flight must land before the CTA may exit: the last stages issued are consumed by MMAs whose
+      // completion is committed to this CTA's empty barriers
+      for (int i = 0; i < issued; ++i) {
+        if (--stage < 0) { stage = S - 1; phase ^= 1u; }
+        if (!wait_or_abort(&empty_bar[stage], phase, abort_flag)) {
+          for (int k = 0; k < 64; ++k) __nanosleep(1000);
+          break;
+        }
+      }
+    }
+  } else if (aligned_ok && warp == 1 && rank == 0) {
+    // ------------------------------------------------------------------ MMA issuer (leader CTA only)
+    if (elect_one()) {
+      int stage = 0; uint32_t phase = 0; uint32_t i = 0; int it = 0; bool ok = true;
+      auto commit_both = [&](uint64_t* bar) { tc_commit_pair(smem_u32(bar)); tc_commit_pair(peer_addr(bar)); };
+#pragma unroll 1
+      for (int t = pair; t < tiles && ok; t += pairs, ++it) {
+        if (it > 0 && !wait_or_abort(shared_free, static_cast<uint32_t>(it - 1) & 1u, abort_flag)) {
+          report_timeout(p.status, 2, 2); *abort_flag = 1; ok = false; break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>((it & 1) * 128);
+#pragma unroll 1
+        for (int kb = 0; kb < num_kb; ++kb, ++i) {
+          bool ready = true;
+          if (L::kSets < S && i >= L::kSets) {             // the scale set's last readers
+            const uint32_t j = i - L::kSets;
+            ready = wait_or_abort(&empty_bar[j % S], (j / S) & 1u, abort_flag);
+          }
+          if (!ready || !wait_or_abort(&full_bar[stage], phase, abort_flag)) {
+            report_timeout(p.status, 2, 1); *abort_flag = 1; ok = false; break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + stage * L::kOperand);
+          const uint32_t s_addr = smem_u32(smem + L::kScaleOff + stage * (L::kSfa + L::kSfb));
+          const uint32_t sfa_t = tmem_base + 384 + (i % L::kSets) * L::kSetCols;
+          const uint32_t sfb_t = sfa_t + 4 * F::kTilesPerStage;
+#pragma unroll
+          for (int j = 0; j < F::kTilesPerStage; ++j) {
+            tc_cp_scale_tile_pair(sfa_t + 4 * j, scale_tile_desc(s_addr + j * 512));
+            tc_cp_scale_tile_pair(sfb_t + 8 * j, scale_tile_desc(s_addr + L::kSfa + j * 512));
+            tc_cp_scale_tile_pair(sfb_t + 8 * j + 4, scale_tile_desc(s_addr + L::kSfa + (F::kTilesPerStage + j) * 512));
+          }
+          const uint64_t a_desc = make_kmajor_sw128_desc(a_addr);
+          const uint64_t b_desc = make_kmajor_sw128_desc(a_addr + L::kABytes);
+          const int left = p.K - kb * kFp4StageK;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j * 64 < left) {
+              const int s = j * 64 / F::kTileK;
+              const uint32_t idesc = make_idesc_fp4(2 * BM, 256, FMT == PQ_FP4_MX, FMT == PQ_FP4_MX ? 2 * (j & 1) : 0);
+              tc_mma_fp4_pair<FMT>(d_tmem, a_desc + static_cast<uint64_t>(2 * j), b_desc + static_cast<uint64_t>(2 * j), idesc,
+                                   sfa_t + 4 * s, sfb_t + 8 * s, (kb > 0 || j > 0) ? 1u : 0u);
+            }
+          }
+          commit_both(&empty_bar[stage]);
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        commit_both(acc_full);
+      }
+    }
+  } else if (aligned_ok && warp >= 2) {
+    // ------------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, h = (warp - 2) >> 2, et = static_cast<int>(threadIdx.x) - 64;
+    float2* cols = reinterpret_cast<float2*>(smem + L::kColOff);
+    uint8_t* block = smem + L::kOutOff + (warp - 2) * L::kOutBlock;
+    const uint32_t block_row = smem_u32(block) + lane * 128;
+    int it = 0, cur_col = -1;
+    bool ok = true;                     // after a wait that gave up a warp only keeps the column barriers' company
+#pragma unroll 1
+    for (int t = pair; t < tiles; t += pairs, ++it) {
+      const PairTile tile = pair_tile(t, p.mt, p.nt);
+      const int row0 = tile.mt * 256 + static_cast<int>(rank) * BM + quarter * 32;
+      const int n0 = tile.nt * 256;
+      if (tile.nt != cur_col) {
+        cur_col = tile.nt;
+        asm volatile("bar.sync 1, %0;" ::"n"(kPairEpiWarps * 32) : "memory");         // the last tile's are used up
+        const int n = n0 + et;
+        cols[et] = make_float2((p.s_col != nullptr && n < p.N) ? p.s_col[n] : 1.0f, (p.bias != nullptr && n < p.N) ? p.bias[n] : 0.0f);
+        asm volatile("bar.sync 1, %0;" ::"n"(kPairEpiWarps * 32) : "memory");
+      }
+      if (!ok) continue;
+      const int row = row0 + lane;
+      const float s_row = (p.s_row != nullptr && row < p.M) ? p.s_row[row] : 1.0f;
+      const bool landed = wait_or_abort(acc_full, static_cast<uint32_t>(it) & 1u, abort_flag);
+      if (!__all_sync(0xffffffffu, landed)) { report_timeout(p.status, 3, 2); *abort_flag = 1; ok = false; continue; }
+      tc_fence_after();
+      const int buf = it & 1;
+#pragma unroll 1
+      for (int step = 0; step < 2; ++step) {
+        // columns shared with the other accumulator first: the upper half of accumulator 0, the lower of accumulator 1
+        const int c0 = ((buf ^ step) == 0 ? 128 : 0) + h * 64;
+        uint32_t v[64];
+        const uint32_t src = tmem_base + static_cast<uint32_t>(buf * 128 + c0) + (static_cast<uint32_t>(quarter * 32) << 16);
+        tmem_ld_32x32b_x32(src, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        tmem_ld_32x32b_x32(src + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        tc_wait_ld();
+        if (step == 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(leader_addr(shared_free));
+        }
+        if (lane == 0) bulk_wait_group_read0();               // the staging block's last store has been read
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float4 sb = *reinterpret_cast<const float4*>(&cols[c0 + 8 * j + 2 * k]);     // {scale, bias} twice
+            w[k] = pack2_any(fmaf(__uint_as_float(v[8 * j + 2 * k]), s_row * sb.x, sb.y),
+                             fmaf(__uint_as_float(v[8 * j + 2 * k + 1]), s_row * sb.z, sb.w), p.bf16);
+          }
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(block_row + ((j ^ (lane & 7)) << 4)), "r"(w[0]), "r"(w[1]),
+                       "r"(w[2]), "r"(w[3])
+                       : "memory");
+        }
+        if (p.vec) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && n0 + c0 < p.N && row0 < p.M) tma_store_2d(&tmOut, block, n0 + c0, row0);
+          if (lane == 0) bulk_commit_group();
+        } else {
+          // rows that TMA cannot address (it stores 16 bytes at a time): the block's rows, 32 elements per instruction
+          __syncwarp();
+#pragma unroll 1
+          for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
+            unsigned short* o = static_cast<unsigned short*>(p.out) + static_cast<int64_t>(row0 + r) * p.ldo + n0 + c0;
+#pragma unroll
+            for (int c = lane; c < 64; c += 32)
+              if (n0 + c0 + c < p.N) o[c] = *reinterpret_cast<const unsigned short*>(block + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_group0();
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync_all();                 // neither CTA leaves while its peer may still signal it or read its shared memory
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
+// scale tiles as words: [row groups][tiles][128], box {128, tiles of a stage, groups}
+int make_scale_map(CUtensorMap* map, const void* base, int64_t rows, int tiles, int box_tiles, int box_groups) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return PQ_ERR_CUDA;
+  cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(tiles), static_cast<cuuint64_t>((rows + 127) / 128)};
+  cuuint64_t strides[2] = {512, static_cast<cuuint64_t>(tiles) * 512};
+  cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_tiles), static_cast<cuuint32_t>(box_groups)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { g_last_cuda_error = static_cast<int>(r); return PQ_ERR_CUDA; }
+  return PQ_OK;
+}
+// output rows, box 64 columns x 32 rows, 128-byte swizzle; what lies past M or N is not written
+int make_out_map(CUtensorMap* map, const void* base, int64_t M, int64_t N, int64_t ldo) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return PQ_ERR_CUDA;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(M)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldo) * 2};
+  cuuint32_t box[2] = {64, 32};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { g_last_cuda_error = static_cast<int>(r); return PQ_ERR_CUDA; }
+  return PQ_OK;
+}
+
+template <int FMT>
+int launch_pair(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, Fp4GemmParams p, cudaStream_t st) {
+  using L = Fp4PairSmem<FMT>;
+  using F = Fp4Fmt<FMT>;
+  p.mt = (p.M + 255) / 256;
+  p.nt = (p.N + 255) / 256;
+  const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt;
+  if (tiles > 0x3fffffff) return PQ_ERR_SHAPE;
+  p.vec = p.vec && p.N % 8 == 0;
+  CUtensorMap tmA, tmW, tmSa, tmSw, tmOut = {};
+  int rc;
+  if ((rc = make_tile_map(&tmA, xq, p.M, p.K / 2, ldx, BM)) != PQ_OK || (rc = make_tile_map(&tmW, w, p.N, p.K / 2, ldw, 128)) != PQ_OK ||
+      (rc = make_scale_map(&tmSa, p.sfa, p.M, p.tiles_k, F::kTilesPerStage, 1)) != PQ_OK ||
+      (rc = make_scale_map(&tmSw, p.sfb, p.N, p.tiles_k, F::kTilesPerStage, 2)) != PQ_OK ||
+      (p.vec && (rc = make_out_map(&tmOut, p.out, p.M, p.N, p.ldo)) != PQ_OK))
+    return rc;
+  auto kern = pq_fp4_gemm_pair_kernel<FMT>;
+  static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes
+  int dev = 0;
+  PQ_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const int pairs = sm_count() / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2u * static_cast<unsigned>(tiles < pairs ? tiles : pairs));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = L::kTotal;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmW, tmSa, tmSw, tmOut, p));
+  return PQ_OK;
+}
+
+}  // namespace
+
+int launch_fp4_pair(int fmt, const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, const Fp4GemmParams& p, cudaStream_t st) {
+  return fmt == PQ_FP4_MX ? launch_pair<PQ_FP4_MX>(xq, ldx, w, ldw, p, st) : launch_pair<PQ_FP4_NV>(xq, ldx, w, ldw, p, st);
+}
+
+}  // namespace pq

@@ -24,6 +24,7 @@ DTYPES = [torch.bfloat16, torch.float16]
 @pytest.fixture(autouse=True)
 def _status_clean(cuda_dev):
     yield
+    _lib.set_option("fp4_pair", 1)
     ops.check_device_status(cuda_dev)
 
 
@@ -168,9 +169,31 @@ def test_product_many_tiles(cuda_dev, fmt, M, N, K):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-def test_product_leaves_its_neighbourhood_alone(cuda_dev, fmt):
+@pytest.mark.parametrize("M,N,K,bias", [(256, 256, 64, False), (1, 8, 32, True), (300, 520, 288, True), (129, 640, 2592, False),
+                                        (520, 264, 1280, True), (2300, 2312, 96, True), (3000, 2560, 1600, False), (4173, 640, 2560, True), (700, 333, 160, True), (257, 257, 64, False)])
+def test_product_on_cta_pairs(cuda_dev, fmt, M, N, K, bias):
+    """The CTA-pair kernel at sizes below and above one tile per pair, ragged in every direction."""
+    g = torch.Generator().manual_seed(M + N)
+    x = torch.randn(M, K, generator=g).to(torch.float16).to(cuda_dev)
+    w = torch.randn(N, K, generator=g).to(torch.bfloat16).to(cuda_dev)
+    xq, wq = fp4_exec.quant_rows_fp4(x, fmt), fp4_exec.quant_rows_fp4(w, fmt)
+    b = torch.randn(N, generator=g).to(cuda_dev) if bias else None
+    _lib.set_option("fp4_pair", 2)
+    try:
+        y = fp4_exec.fp4_gemm(xq, wq, b, torch.float16)
+        again = fp4_exec.fp4_gemm(xq, wq, b, torch.float16)
+    finally:
+        _lib.set_option("fp4_pair", 1)
+    check_product(y, xq, wq, b, fmt)
+    assert torch.equal(y, again)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("pair", [1, 2])
+def test_product_leaves_its_neighbourhood_alone(cuda_dev, fmt, pair):
     """Rows behind the last one, columns behind the last one and the bytes around the output stay as they were."""
     M, N, K = 70, 90, 128
+    _lib.set_option("fp4_pair", pair)
     _, xq = make_rows(M, K, fmt, torch.bfloat16, 1, cuda_dev)
     _, wq = make_rows(N, K, fmt, torch.bfloat16, 2, cuda_dev)
     want = fp4_exec.fp4_gemm(xq, wq, None, torch.bfloat16)
@@ -186,6 +209,7 @@ def test_product_leaves_its_neighbourhood_alone(cuda_dev, fmt):
         assert torch.equal(got[:, :N], want)
         got[:, :N] = 7.0
         assert bool((buf == 7.0).all())
+    _lib.set_option("fp4_pair", 1)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
