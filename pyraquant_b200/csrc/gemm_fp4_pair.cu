@@ -11,7 +11,8 @@
 // The epilogue of a tile drains the shared columns [128, 256) first and signals `shared_free`; then the next tile's MMAs
 // may start in the other accumulator while the epilogue goes on with the columns that belong to its own alone.
 // A scale set is written again only once the MMAs that read it have completed: with as many sets as stages (mx) the
-// stage's own hand-over shows that, with two sets (nv) the MMA thread also waits for the stage before last.
+// stage's own hand-over shows that; nv needs twice the columns, so its sets are those of half a stage, five of them, and
+// each has a barrier that the MMAs commit to.
 //
 // Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-9 epilogue (a 32-row quarter and, step by step, 64 columns each:
 // scale, bias, rounding, swizzled 4 KB staging block, TMA store; plain stores where TMA cannot address the rows).  Tiles go to the pairs in the order of blocks of eight
@@ -36,14 +37,17 @@ struct Fp4PairSmem {
   static constexpr int kOutOff = kPairStages * kOperand;                     // 1024-byte aligned blocks first
   static constexpr int kOutBlock = 32 * 128;
   static constexpr int kScaleOff = kOutOff + kPairEpiWarps * kOutBlock;
-  static constexpr int kColOff = kScaleOff + kPairStages * (kSfa + kSfb);    // {scale, bias} of the tile's 256 columns
-  static constexpr int kBarOff = kColOff + 256 * 8;
-  static constexpr int kNumBars = 2 * kPairStages + 2;                       // full, empty, acc_full, shared_free
+  static constexpr int kColOff = kScaleOff + kPairStages * (kSfa + kSfb);    // {scale, bias} of 256 columns, two tiles
+  static constexpr int kBarOff = kColOff + 2 * 256 * 8;
+  static constexpr int kNumBars = 2 * kPairStages + 2 + 5;                   // full, empty, acc_full, shared_free, scale sets
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kTotal = kMiscOff + 16;
   static_assert(kTotal <= 232448, "exceeds the 227 KB shared memory of one CTA");
-  static constexpr int kSetCols = 12 * Fp4Fmt<FMT>::kTilesPerStage;          // per tile: 4 columns for A, 8 for B
-  static constexpr int kSets = FMT == PQ_FP4_MX ? kPairStages : 2;
+  // scale columns are handed over in units of a stage (mx) or half a stage (nv): per scale tile 4 columns for A, 8 for B
+  static constexpr int kUnits = FMT == PQ_FP4_MX ? 1 : 2;
+  static constexpr int kTilesPerUnit = Fp4Fmt<FMT>::kTilesPerStage / kUnits;
+  static constexpr int kSetCols = 12 * kTilesPerUnit;
+  static constexpr int kSets = 5;
   static_assert(384 + kSets * kSetCols <= 512, "tensor memory");
 };
 
@@ -75,17 +79,38 @@ __device__ __forceinline__ void tc_cp_scale_tile_pair(uint32_t tmem_addr, uint64
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem_addr), "l"(desc) : "memory");
 }
 
-struct PairTile { int mt, nt; };
-__device__ __forceinline__ PairTile pair_tile(int t, int mt_total, int nt_total) {
-  const int block = t / (kRowBlock * nt_total);
-  const int rem = t - block * kRowBlock * nt_total;
-  const int left = mt_total - block * kRowBlock;
-  const int hb = left < kRowBlock ? left : kRowBlock;
-  const int col = rem / hb;
-  return PairTile{block * kRowBlock + rem - col * hb, col};
+// a load that stays where it is written (the compiler would move an ordinary one down to its use)
+__device__ __forceinline__ float ld_now(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
 }
 
-template <int FMT>
+// Tile order: blocks of kRowBlock row tiles, inside a block column after column, rows innermost.  A pair visits every
+// `stride`-th tile; the step needs no division (two of them took a third of the epilogue's time per tile) except in a last
+// block of fewer rows.
+struct Fp4PairWalker {
+  int t, stride, tiles, nt_total, mt_total;
+  int block_t0, block_row0;             // first tile and first row tile of the current block
+  int mt, nt;                           // row tile, column tile
+  __device__ __forceinline__ void init(int pair, int pairs, int mt_total_, int nt_total_) {
+    t = pair; stride = pairs; mt_total = mt_total_; nt_total = nt_total_; tiles = mt_total * nt_total;
+    block_t0 = block_row0 = 0;
+    place();
+  }
+  __device__ __forceinline__ bool valid() const { return t < tiles; }
+  __device__ __forceinline__ void place() {
+    if (t >= tiles) return;
+    const int full = kRowBlock * nt_total;
+    while (t - block_t0 >= full) { block_t0 += full; block_row0 += kRowBlock; }
+    const int rem = t - block_t0, left = mt_total - block_row0;
+    nt = left >= kRowBlock ? rem / kRowBlock : rem / left;
+    mt = block_row0 + rem - nt * (left >= kRowBlock ? kRowBlock : left);
+  }
+  __device__ __forceinline__ void advance() { t += stride; place(); }
+};
+
+template <int FMT, bool SCALED, typename OutT>
 __global__ void __launch_bounds__(kPairThreads, 1)
 pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                         const __grid_constant__ CUtensorMap tmSa, const __grid_constant__ CUtensorMap tmSw,
@@ -98,6 +123,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   uint64_t* empty_bar = full_bar + S;
   uint64_t* acc_full = empty_bar + S;
   uint64_t* shared_free = acc_full + 1;
+  uint64_t* set_bar = shared_free + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
 
@@ -113,6 +139,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     if (p.vec) tma_prefetch_desc(&tmOut);
     for (int s = 0; s < S; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
     mbar_init(acc_full, 1); mbar_init(shared_free, 2 * kPairEpiWarps);
+    for (int s = 0; s < L::kSets; ++s) mbar_init(&set_bar[s], 1);
     *abort_flag = aligned_ok ? 0 : 1;
     if (!aligned_ok) report_timeout(p.status, 7, 7);
     fence_mbar_init();
@@ -131,11 +158,11 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (elect_one()) {
       int stage = 0; uint32_t phase = 0; int issued = 0; bool ok = true;
+      Fp4PairWalker w; w.init(pair, pairs, p.mt, p.nt);
 #pragma unroll 1
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        const PairTile tile = pair_tile(t, p.mt, p.nt);
-        const int row0 = tile.mt * 256 + static_cast<int>(rank) * BM;
-        const int n0 = tile.nt * 256;
+      for (; w.valid() && ok; w.advance()) {
+        const int row0 = w.mt * 256 + static_cast<int>(rank) * BM;
+        const int n0 = w.nt * 256;
         const int nhalf0 = n0 + static_cast<int>(rank) * 128;
 #pragma unroll 1
         for (int kb = 0; kb < num_kb; ++kb) {
@@ -167,50 +194,68 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   } else if (aligned_ok && warp == 1 && rank == 0) {
     // ------------------------------------------------------------------ MMA issuer (leader CTA only)
     if (elect_one()) {
-      int stage = 0; uint32_t phase = 0; uint32_t i = 0; int it = 0; bool ok = true;
+      int stage = 0; uint32_t phase = 0; int it = 0; bool ok = true;
+      uint32_t set = 0, set_use = 0;                       // scale set and how often the ring of sets has come round
       auto commit_both = [&](uint64_t* bar) { tc_commit_pair(smem_u32(bar)); tc_commit_pair(peer_addr(bar)); };
+      // Barriers are probed one step ahead of their use: a probe takes a few hundred cycles while the tensor cores and TMA
+      // saturate shared memory, as long as a stage's MMAs.
+      bool full_ready = false;
 #pragma unroll 1
       for (int t = pair; t < tiles && ok; t += pairs, ++it) {
-        if (it > 0 && !wait_or_abort(shared_free, static_cast<uint32_t>(it - 1) & 1u, abort_flag)) {
-          report_timeout(p.status, 2, 2); *abort_flag = 1; ok = false; break;
-        }
-        tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>((it & 1) * 128);
 #pragma unroll 1
-        for (int kb = 0; kb < num_kb; ++kb, ++i) {
-          bool ready = true;
-          if (L::kSets < S && i >= L::kSets) {             // the scale set's last readers
-            const uint32_t j = i - L::kSets;
-            ready = wait_or_abort(&empty_bar[j % S], (j / S) & 1u, abort_flag);
-          }
-          if (!ready || !wait_or_abort(&full_bar[stage], phase, abort_flag)) {
+        for (int kb = 0; kb < num_kb && ok; ++kb) {
+          if (!full_ready && !wait_or_abort(&full_bar[stage], phase, abort_flag)) {
             report_timeout(p.status, 2, 1); *abort_flag = 1; ok = false; break;
           }
           tc_fence_after();
+          const int next = stage + 1 == S ? 0 : stage + 1;
+          full_ready = mbar_test_wait(&full_bar[next], next == 0 ? phase ^ 1u : phase);
           const uint32_t a_addr = smem_u32(smem + stage * L::kOperand);
           const uint32_t s_addr = smem_u32(smem + L::kScaleOff + stage * (L::kSfa + L::kSfb));
-          const uint32_t sfa_t = tmem_base + 384 + (i % L::kSets) * L::kSetCols;
-          const uint32_t sfb_t = sfa_t + 4 * F::kTilesPerStage;
-#pragma unroll
-          for (int j = 0; j < F::kTilesPerStage; ++j) {
-            tc_cp_scale_tile_pair(sfa_t + 4 * j, scale_tile_desc(s_addr + j * 512));
-            tc_cp_scale_tile_pair(sfb_t + 8 * j, scale_tile_desc(s_addr + L::kSfa + j * 512));
-            tc_cp_scale_tile_pair(sfb_t + 8 * j + 4, scale_tile_desc(s_addr + L::kSfa + (F::kTilesPerStage + j) * 512));
-          }
           const uint64_t a_desc = make_kmajor_sw128_desc(a_addr);
           const uint64_t b_desc = make_kmajor_sw128_desc(a_addr + L::kABytes);
           const int left = p.K - kb * kFp4StageK;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (j * 64 < left) {
-              const int s = j * 64 / F::kTileK;
-              const uint32_t idesc = make_idesc_fp4(2 * BM, 256, FMT == PQ_FP4_MX, FMT == PQ_FP4_MX ? 2 * (j & 1) : 0);
-              tc_mma_fp4_pair<FMT>(d_tmem, a_desc + static_cast<uint64_t>(2 * j), b_desc + static_cast<uint64_t>(2 * j), idesc,
-                                   sfa_t + 4 * s, sfb_t + 8 * s, (kb > 0 || j > 0) ? 1u : 0u);
+          for (int u = 0; u < L::kUnits; ++u) {
+            // the last readers of the unit's scale columns
+            if (L::kSets < S * L::kUnits && set_use > 0 &&
+                !wait_or_abort(&set_bar[set], (set_use - 1) & 1u, abort_flag)) {
+              report_timeout(p.status, 2, 3); *abort_flag = 1; ok = false; break;
             }
+            const uint32_t sfa_t = tmem_base + 384 + set * L::kSetCols;
+            const uint32_t sfb_t = sfa_t + 4 * L::kTilesPerUnit;
+#pragma unroll
+            for (int j = 0; j < L::kTilesPerUnit; ++j) {
+              const int tile = u * L::kTilesPerUnit + j;
+              tc_cp_scale_tile_pair(sfa_t + 4 * j, scale_tile_desc(s_addr + tile * 512));
+              tc_cp_scale_tile_pair(sfb_t + 8 * j, scale_tile_desc(s_addr + L::kSfa + tile * 512));
+              tc_cp_scale_tile_pair(sfb_t + 8 * j + 4, scale_tile_desc(s_addr + L::kSfa + (F::kTilesPerStage + tile) * 512));
+            }
+            // the scales of a tile's first stage are under way before the accumulator is free
+            if (u == 0 && kb == 0 && it > 0) {
+              if (!wait_or_abort(shared_free, static_cast<uint32_t>(it - 1) & 1u, abort_flag)) {
+                report_timeout(p.status, 2, 2); *abort_flag = 1; ok = false; break;
+              }
+              tc_fence_after();
+            }
+#pragma unroll
+            for (int m = 0; m < 4 / L::kUnits; ++m) {
+              const int j = u * (4 / L::kUnits) + m;
+              if (j * 64 < left) {
+                const int s = m * 64 / F::kTileK;
+                const uint32_t idesc = make_idesc_fp4(2 * BM, 256, FMT == PQ_FP4_MX, FMT == PQ_FP4_MX ? 2 * (j & 1) : 0);
+                tc_mma_fp4_pair<FMT>(d_tmem, a_desc + static_cast<uint64_t>(2 * j), b_desc + static_cast<uint64_t>(2 * j), idesc,
+                                     sfa_t + 4 * s, sfb_t + 8 * s, (kb > 0 || j > 0) ? 1u : 0u);
+              }
+            }
+            if (L::kSets < S * L::kUnits) tc_commit_pair(smem_u32(&set_bar[set]));
+            if (++set == L::kSets) { set = 0; ++set_use; }
           }
+          if (!ok) break;
           commit_both(&empty_bar[stage]);
-          if (++stage == S) { stage = 0; phase ^= 1u; }
+          if (next == 0) phase ^= 1u;
+          stage = next;
         }
         if (!ok) break;
         commit_both(acc_full);
@@ -219,38 +264,58 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   } else if (aligned_ok && warp >= 2) {
     // ------------------------------------------------------------------ epilogue
     const int quarter = warp & 3, h = (warp - 2) >> 2, et = static_cast<int>(threadIdx.x) - 64;
-    float2* cols = reinterpret_cast<float2*>(smem + L::kColOff);
     uint8_t* block = smem + L::kOutOff + (warp - 2) * L::kOutBlock;
-    const uint32_t block_row = smem_u32(block) + lane * 128;
-    int it = 0, cur_col = -1;
+    const int g = lane >> 2, q = lane & 3;       // accumulator fragments: rows g, g + 8 (+ 16), column pairs 8 j + 2 q
+    const uint32_t block_addr = smem_u32(block) + g * 128 + q * 4;
+    // A tile's column scales, bias and row scales are requested one tile ahead: in front of the accumulator's barrier their
+    // latency would be paid on every tile.
+    float2 next_col = make_float2(1.0f, 0.0f);
+    float next_row[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    Fp4PairWalker w; w.init(pair, pairs, p.mt, p.nt);
+    auto request = [&]() {
+      if (!w.valid()) return;
+      const int n = w.nt * 256 + et, row = w.mt * 256 + static_cast<int>(rank) * BM + quarter * 32 + g;
+      if (SCALED && p.s_col != nullptr) next_col.x = n < p.N ? ld_now(p.s_col + n) : 1.0f;
+      if (p.bias != nullptr) next_col.y = n < p.N ? ld_now(p.bias + n) : 0.0f;
+      if (SCALED && p.s_row != nullptr) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) next_row[r] = row + 8 * r < p.M ? ld_now(p.s_row + row + 8 * r) : 1.0f;
+      }
+    };
+    request();
+    int it = 0;
     bool ok = true;                     // after a wait that gave up a warp only keeps the column barriers' company
 #pragma unroll 1
-    for (int t = pair; t < tiles; t += pairs, ++it) {
-      const PairTile tile = pair_tile(t, p.mt, p.nt);
-      const int row0 = tile.mt * 256 + static_cast<int>(rank) * BM + quarter * 32;
-      const int n0 = tile.nt * 256;
-      if (tile.nt != cur_col) {
-        cur_col = tile.nt;
-        asm volatile("bar.sync 1, %0;" ::"n"(kPairEpiWarps * 32) : "memory");         // the last tile's are used up
-        const int n = n0 + et;
-        cols[et] = make_float2((p.s_col != nullptr && n < p.N) ? p.s_col[n] : 1.0f, (p.bias != nullptr && n < p.N) ? p.bias[n] : 0.0f);
-        asm volatile("bar.sync 1, %0;" ::"n"(kPairEpiWarps * 32) : "memory");
-      }
+    for (; w.valid(); ++it) {
+      const int row0 = w.mt * 256 + static_cast<int>(rank) * BM + quarter * 32;
+      const int n0 = w.nt * 256;
+      // two buffers: the one written here was last read two tiles ago, before the barrier of the last tile
+      float2* cols = reinterpret_cast<float2*>(smem + L::kColOff) + (it & 1) * 256;
+      cols[et] = next_col;
+      float s_row[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s_row[r] = next_row[r];
+      asm volatile("bar.sync 1, %0;" ::"n"(kPairEpiWarps * 32) : "memory");
+      w.advance();
+      request();
       if (!ok) continue;
-      const int row = row0 + lane;
-      const float s_row = (p.s_row != nullptr && row < p.M) ? p.s_row[row] : 1.0f;
-      const bool landed = wait_or_abort(acc_full, static_cast<uint32_t>(it) & 1u, abort_flag);
-      if (!__all_sync(0xffffffffu, landed)) { report_timeout(p.status, 3, 2); *abort_flag = 1; ok = false; continue; }
-      tc_fence_after();
       const int buf = it & 1;
 #pragma unroll 1
       for (int step = 0; step < 2; ++step) {
         // columns shared with the other accumulator first: the upper half of accumulator 0, the lower of accumulator 1
         const int c0 = ((buf ^ step) == 0 ? 128 : 0) + h * 64;
-        uint32_t v[64];
+        float4 sb[8];                                           // {scale, bias} of two columns
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sb[j] = *reinterpret_cast<const float4*>(&cols[c0 + 8 * j + 2 * q]);
+        if (step == 0) {
+          const bool landed = wait_or_abort(acc_full, static_cast<uint32_t>(it) & 1u, abort_flag);
+          if (!__all_sync(0xffffffffu, landed)) { report_timeout(p.status, 3, 2); *abort_flag = 1; ok = false; break; }
+          tc_fence_after();
+        }
+        uint32_t v[2][32];
         const uint32_t src = tmem_base + static_cast<uint32_t>(buf * 128 + c0) + (static_cast<uint32_t>(quarter * 32) << 16);
-        tmem_ld_32x32b_x32(src, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld_32x32b_x32(src + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        tmem_ld_16x256b_x8(src, v[0]);
+        tmem_ld_16x256b_x8(src + (16u << 16), v[1]);
         tc_wait_ld();
         if (step == 0) {
           tc_fence_before();
@@ -260,18 +325,24 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         if (lane == 0) bulk_wait_group_read0();               // the staging block's last store has been read
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t w[4];
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float4 sb = *reinterpret_cast<const float4*>(&cols[c0 + 8 * j + 2 * k]);     // {scale, bias} twice
-            w[k] = pack2_any(fmaf(__uint_as_float(v[8 * j + 2 * k]), s_row * sb.x, sb.y),
-                             fmaf(__uint_as_float(v[8 * j + 2 * k + 1]), s_row * sb.z, sb.w), p.bf16);
-          }
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(block_row + ((j ^ (lane & 7)) << 4)), "r"(w[0]), "r"(w[1]),
-                       "r"(w[2]), "r"(w[3])
-                       : "memory");
-        }
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float2 y = make_float2(__uint_as_float(v[half][4 * j + 2 * r]), __uint_as_float(v[half][4 * j + 2 * r + 1]));
+              const float2 b = make_float2(sb[j].y, sb[j].w);
+              if constexpr (SCALED) {
+                const float sr = s_row[2 * half + r];
+                y = __ffma2_rn(y, __fmul2_rn(make_float2(sb[j].x, sb[j].z), make_float2(sr, sr)), b);
+              } else {
+                y = __fadd2_rn(y, b);
+              }
+              // row 16 half + 8 r + g of the block, 16-byte chunk j at its swizzled place: a warp's words fall into 32 banks
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(block_addr + (16 * half + 8 * r) * 128 + ((j ^ g) << 4)),
+                           "r"(pack2(y.x, y.y, OutT{}))
+                           : "memory");
+            }
         if (p.vec) {
           fence_proxy_async_smem();
           __syncwarp();
@@ -329,7 +400,7 @@ int make_out_map(CUtensorMap* map, const void* base, int64_t M, int64_t N, int64
   return PQ_OK;
 }
 
-template <int FMT>
+template <int FMT, bool SCALED, typename OutT>
 int launch_pair(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, Fp4GemmParams p, cudaStream_t st) {
   using L = Fp4PairSmem<FMT>;
   using F = Fp4Fmt<FMT>;
@@ -345,7 +416,7 @@ int launch_pair(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, F
       (rc = make_scale_map(&tmSw, p.sfb, p.N, p.tiles_k, F::kTilesPerStage, 2)) != PQ_OK ||
       (p.vec && (rc = make_out_map(&tmOut, p.out, p.M, p.N, p.ldo)) != PQ_OK))
     return rc;
-  auto kern = pq_fp4_gemm_pair_kernel<FMT>;
+  auto kern = pq_fp4_gemm_pair_kernel<FMT, SCALED, OutT>;
   static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes
   int dev = 0;
   PQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -369,10 +440,17 @@ int launch_pair(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, F
   return PQ_OK;
 }
 
+template <typename OutT>
+int launch_pair_as(int fmt, const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, const Fp4GemmParams& p, cudaStream_t st) {
+  if (fmt == PQ_FP4_NV) return launch_pair<PQ_FP4_NV, true, OutT>(xq, ldx, w, ldw, p, st);
+  if (p.s_row != nullptr || p.s_col != nullptr) return launch_pair<PQ_FP4_MX, true, OutT>(xq, ldx, w, ldw, p, st);
+  return launch_pair<PQ_FP4_MX, false, OutT>(xq, ldx, w, ldw, p, st);
+}
+
 }  // namespace
 
 int launch_fp4_pair(int fmt, const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, const Fp4GemmParams& p, cudaStream_t st) {
-  return fmt == PQ_FP4_MX ? launch_pair<PQ_FP4_MX>(xq, ldx, w, ldw, p, st) : launch_pair<PQ_FP4_NV>(xq, ldx, w, ldw, p, st);
+  return p.bf16 ? launch_pair_as<__nv_bfloat16>(fmt, xq, ldx, w, ldw, p, st) : launch_pair_as<__half>(fmt, xq, ldx, w, ldw, p, st);
 }
 
 }  // namespace pq
