@@ -261,7 +261,7 @@ int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, 
   const int sms = sm_count();
   const int num_kb = (p.K + kFp4StageK - 1) / kFp4StageK;
   const int64_t pair_tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (options().fp4_pair == 2 || (options().fp4_pair == 1 && 2 * pair_tiles >= sms))
+  if ((p.s_row != nullptr) == (p.s_col != nullptr) && (options().fp4_pair == 2 || (options().fp4_pair == 1 && 2 * pair_tiles >= sms)))
     return launch_fp4_pair(FMT, xq, ldx, w, ldw, p, st);
   const bool wide = static_cast<int64_t>(p.mt) * ((p.N + 127) / 128) >= sms;
   const int bn = wide ? 128 : 64;

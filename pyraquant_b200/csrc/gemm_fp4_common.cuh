@@ -30,7 +30,7 @@ struct Fp4GemmParams {
   int vec;                 // rows may be stored 16 bytes at a time
 };
 
-// The CTA-pair kernel (gemm_fp4_pair.cu).  Fills in the tile counts itself.
+// The CTA-pair kernel (gemm_fp4_pair.cu): both row scales or neither.  Fills in the tile counts itself.
 int launch_fp4_pair(int fmt, const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, const Fp4GemmParams& p, cudaStream_t st);
 
 namespace {

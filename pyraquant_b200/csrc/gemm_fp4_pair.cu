@@ -12,7 +12,8 @@
 // may start in the other accumulator while the epilogue goes on with the columns that belong to its own alone.
 // A scale set is written again only once the MMAs that read it have completed: with as many sets as stages (mx) the
 // stage's own hand-over shows that; nv needs twice the columns, so its sets are those of half a stage, five of them, and
-// each has a barrier that the MMAs commit to.
+// before a stage the MMA thread waits for the first half of the stage before last, whose completion covers the last
+// readers of both sets it is about to write.
 //
 // Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-9 epilogue (a 32-row quarter and, step by step, 64 columns each:
 // scale, bias, rounding, swizzled 4 KB staging block, TMA store; plain stores where TMA cannot address the rows).  Tiles go to the pairs in the order of blocks of eight
@@ -39,7 +40,7 @@ struct Fp4PairSmem {
   static constexpr int kScaleOff = kOutOff + kPairEpiWarps * kOutBlock;
   static constexpr int kColOff = kScaleOff + kPairStages * (kSfa + kSfb);    // {scale, bias} of 256 columns, two tiles
   static constexpr int kBarOff = kColOff + 2 * 256 * 8;
-  static constexpr int kNumBars = 2 * kPairStages + 2 + 5;                   // full, empty, acc_full, shared_free, scale sets
+  static constexpr int kNumBars = 3 * kPairStages + 2;                       // full, empty, acc_full, shared_free, half
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kTotal = kMiscOff + 16;
   static_assert(kTotal <= 232448, "exceeds the 227 KB shared memory of one CTA");
@@ -123,7 +124,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   uint64_t* empty_bar = full_bar + S;
   uint64_t* acc_full = empty_bar + S;
   uint64_t* shared_free = acc_full + 1;
-  uint64_t* set_bar = shared_free + 1;
+  uint64_t* half_bar = shared_free + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
 
@@ -139,7 +140,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     if (p.vec) tma_prefetch_desc(&tmOut);
     for (int s = 0; s < S; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
     mbar_init(acc_full, 1); mbar_init(shared_free, 2 * kPairEpiWarps);
-    for (int s = 0; s < L::kSets; ++s) mbar_init(&set_bar[s], 1);
+    for (int s = 0; s < S; ++s) mbar_init(&half_bar[s], 1);
     *abort_flag = aligned_ok ? 0 : 1;
     if (!aligned_ok) report_timeout(p.status, 7, 7);
     fence_mbar_init();
@@ -195,7 +196,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     // ------------------------------------------------------------------ MMA issuer (leader CTA only)
     if (elect_one()) {
       int stage = 0; uint32_t phase = 0; int it = 0; bool ok = true;
-      uint32_t set = 0, set_use = 0;                       // scale set and how often the ring of sets has come round
+      uint32_t set = 0; int issued = 0;                    // next scale set; stages issued (up to 2)
       auto commit_both = [&](uint64_t* bar) { tc_commit_pair(smem_u32(bar)); tc_commit_pair(peer_addr(bar)); };
       // Barriers are probed one step ahead of their use: a probe takes a few hundred cycles while the tensor cores and TMA
       // saturate shared memory, as long as a stage's MMAs.
@@ -205,6 +206,14 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>((it & 1) * 128);
 #pragma unroll 1
         for (int kb = 0; kb < num_kb && ok; ++kb) {
+          // nv: the scale columns of this stage were last read by MMAs up to the first half of the stage before last
+          if (L::kUnits > 1 && issued >= 2) {
+            const int back = stage >= 2 ? stage - 2 : stage - 2 + S;
+            if (!wait_or_abort(&half_bar[back], stage >= 2 ? phase : phase ^ 1u, abort_flag)) {
+              report_timeout(p.status, 2, 3); *abort_flag = 1; ok = false; break;
+            }
+          }
+          if (issued < 2) ++issued;
           if (!full_ready && !wait_or_abort(&full_bar[stage], phase, abort_flag)) {
             report_timeout(p.status, 2, 1); *abort_flag = 1; ok = false; break;
           }
@@ -218,11 +227,6 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           const int left = p.K - kb * kFp4StageK;
 #pragma unroll
           for (int u = 0; u < L::kUnits; ++u) {
-            // the last readers of the unit's scale columns
-            if (L::kSets < S * L::kUnits && set_use > 0 &&
-                !wait_or_abort(&set_bar[set], (set_use - 1) & 1u, abort_flag)) {
-              report_timeout(p.status, 2, 3); *abort_flag = 1; ok = false; break;
-            }
             const uint32_t sfa_t = tmem_base + 384 + set * L::kSetCols;
             const uint32_t sfb_t = sfa_t + 4 * L::kTilesPerUnit;
 #pragma unroll
@@ -249,8 +253,8 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                                      sfa_t + 4 * s, sfb_t + 8 * s, (kb > 0 || j > 0) ? 1u : 0u);
               }
             }
-            if (L::kSets < S * L::kUnits) tc_commit_pair(smem_u32(&set_bar[set]));
-            if (++set == L::kSets) { set = 0; ++set_use; }
+            if (L::kUnits > 1 && u == 0) tc_commit_pair(smem_u32(&half_bar[stage]));
+            if (++set == L::kSets) set = 0;
           }
           if (!ok) break;
           commit_both(&empty_bar[stage]);
@@ -269,17 +273,18 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     const uint32_t block_addr = smem_u32(block) + g * 128 + q * 4;
     // A tile's column scales, bias and row scales are requested one tile ahead: in front of the accumulator's barrier their
     // latency would be paid on every tile.
-    float2 next_col = make_float2(1.0f, 0.0f);
+    float next_scale = 1.0f, next_bias = 0.0f;
     float next_row[4] = {1.0f, 1.0f, 1.0f, 1.0f};
     Fp4PairWalker w; w.init(pair, pairs, p.mt, p.nt);
     auto request = [&]() {
       if (!w.valid()) return;
-      const int n = w.nt * 256 + et, row = w.mt * 256 + static_cast<int>(rank) * BM + quarter * 32 + g;
-      if (SCALED && p.s_col != nullptr) next_col.x = n < p.N ? ld_now(p.s_col + n) : 1.0f;
-      if (p.bias != nullptr) next_col.y = n < p.N ? ld_now(p.bias + n) : 0.0f;
-      if (SCALED && p.s_row != nullptr) {
+      // indices are clamped, not tested: branches one after the other cost as much as the tile's conversion
+      const int n = min(w.nt * 256 + et, p.N - 1), row = w.mt * 256 + static_cast<int>(rank) * BM + quarter * 32 + g;
+      if (p.bias != nullptr) next_bias = ld_now(p.bias + n);
+      if constexpr (SCALED) {
+        next_scale = ld_now(p.s_col + n);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) next_row[r] = row + 8 * r < p.M ? ld_now(p.s_row + row + 8 * r) : 1.0f;
+        for (int r = 0; r < 4; ++r) next_row[r] = ld_now(p.s_row + min(row + 8 * r, p.M - 1));
       }
     };
     request();
@@ -289,9 +294,11 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     for (; w.valid(); ++it) {
       const int row0 = w.mt * 256 + static_cast<int>(rank) * BM + quarter * 32;
       const int n0 = w.nt * 256;
-      // two buffers: the one written here was last read two tiles ago, before the barrier of the last tile
-      float2* cols = reinterpret_cast<float2*>(smem + L::kColOff) + (it & 1) * 256;
-      cols[et] = next_col;
+      // {scale, scale, bias, bias} of column pairs, two buffers: the one written here was last read two tiles ago, before the
+      // barrier of the last tile
+      float* cols = reinterpret_cast<float*>(smem + L::kColOff) + (it & 1) * 512;
+      cols[(et >> 1) * 4 + (et & 1)] = next_scale;
+      cols[(et >> 1) * 4 + 2 + (et & 1)] = next_bias;
       float s_row[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) s_row[r] = next_row[r];
@@ -304,9 +311,9 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
       for (int step = 0; step < 2; ++step) {
         // columns shared with the other accumulator first: the upper half of accumulator 0, the lower of accumulator 1
         const int c0 = ((buf ^ step) == 0 ? 128 : 0) + h * 64;
-        float4 sb[8];                                           // {scale, bias} of two columns
+        float4 sb[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sb[j] = *reinterpret_cast<const float4*>(&cols[c0 + 8 * j + 2 * q]);
+        for (int j = 0; j < 8; ++j) sb[j] = *reinterpret_cast<const float4*>(&cols[(c0 + 8 * j + 2 * q) * 2]);
         if (step == 0) {
           const bool landed = wait_or_abort(acc_full, static_cast<uint32_t>(it) & 1u, abort_flag);
           if (!__all_sync(0xffffffffu, landed)) { report_timeout(p.status, 3, 2); *abort_flag = 1; ok = false; break; }
@@ -331,10 +338,10 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               float2 y = make_float2(__uint_as_float(v[half][4 * j + 2 * r]), __uint_as_float(v[half][4 * j + 2 * r + 1]));
-              const float2 b = make_float2(sb[j].y, sb[j].w);
+              const float2 b = make_float2(sb[j].z, sb[j].w);
               if constexpr (SCALED) {
                 const float sr = s_row[2 * half + r];
-                y = __ffma2_rn(y, __fmul2_rn(make_float2(sb[j].x, sb[j].z), make_float2(sr, sr)), b);
+                y = __ffma2_rn(y, __fmul2_rn(make_float2(sb[j].x, sb[j].y), make_float2(sr, sr)), b);
               } else {
                 y = __fadd2_rn(y, b);
               }
@@ -443,7 +450,7 @@ int launch_pair(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, F
 template <typename OutT>
 int launch_pair_as(int fmt, const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, const Fp4GemmParams& p, cudaStream_t st) {
   if (fmt == PQ_FP4_NV) return launch_pair<PQ_FP4_NV, true, OutT>(xq, ldx, w, ldw, p, st);
-  if (p.s_row != nullptr || p.s_col != nullptr) return launch_pair<PQ_FP4_MX, true, OutT>(xq, ldx, w, ldw, p, st);
+  if (p.s_row != nullptr) return launch_pair<PQ_FP4_MX, true, OutT>(xq, ldx, w, ldw, p, st);
   return launch_pair<PQ_FP4_MX, false, OutT>(xq, ldx, w, ldw, p, st);
 }
 
