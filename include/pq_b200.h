@@ -119,13 +119,27 @@ int pq_adaln_quant_rows(const void* x, int dtype, int64_t M, int64_t K, int64_t 
  *   x [B,T,C] with strides ld_batch, ld_row, 1 (elements); out likewise; gamma, beta [C] in x's type, or fp32 when
  *   affine_fp32 is set, each NULL for 1 and 0; C % 8 == 0, C <= 8192, C % groups == 0, B <= 65535, strides % 8 == 0,
  *   16-byte aligned x and out; workspace: pq_group_norm_workspace_bytes (same B, T, C, groups, current device), 8-byte
- *   aligned.  B == 0 or T == 0 is a no-op. */
+ *   aligned; status: NULL or a status word as in the GEMMs' workspace.  B == 0 or T == 0 is a no-op.
+ * One launch, cooperative when a sample is shared by several CTAs. */
 #define PQ_ACT_NONE 0
 #define PQ_ACT_SILU 1
 int64_t pq_group_norm_workspace_bytes(int64_t B, int64_t T, int64_t C, int groups);
 int pq_group_norm(const void* x, int dtype, int64_t B, int64_t T, int64_t C, int64_t ld_row, int64_t ld_batch, int groups,
                   const void* gamma, const void* beta, int affine_fp32, float eps, int act,
-                  void* out, int64_t ldo_row, int64_t ldo_batch, void* workspace, int64_t ws_bytes, void* stream);
+                  void* out, int64_t ldo_row, int64_t ldo_batch, void* workspace, int64_t ws_bytes, void* status, void* stream);
+
+/* pq_group_norm whose rows leave quantised, in the same launch: (q, s) = pq_quant_rows(z) with q [B T, C] and s [B T], or
+ * (codes, scales, row_scale) = pq_quant_rows_fp4(z), bit for bit.  x_norm: NULL, or [B,T,C] that receives z (strides ldn_batch,
+ * ldn_row).  C % 16 == 0 (INT8), C % 32 == 0 (4-bit); 16-byte aligned q, codes and scales.  PQ_ERR_UNSUPPORTED, with nothing
+ * launched, when the rows do not fit into the GPU's shared memory (about 29 MB): normalise and quantise in two calls then. */
+int pq_group_norm_quant_rows(const void* x, int dtype, int64_t B, int64_t T, int64_t C, int64_t ld_row, int64_t ld_batch,
+                             int groups, const void* gamma, const void* beta, int affine_fp32, float eps, int act,
+                             void* x_norm, int64_t ldn_row, int64_t ldn_batch, int8_t* q, float* s,
+                             void* workspace, int64_t ws_bytes, void* status, void* stream);
+int pq_group_norm_quant_fp4(const void* x, int dtype, int64_t B, int64_t T, int64_t C, int64_t ld_row, int64_t ld_batch,
+                            int groups, const void* gamma, const void* beta, int affine_fp32, float eps, int act, int fmt,
+                            uint8_t* codes, uint8_t* scales, float* row_scale,
+                            void* workspace, int64_t ws_bytes, void* status, void* stream);
 
 /* Dequantisation of materialised accumulators: out[m,n] = float(acc[m,n]) * (s_row[m] * s_col[n])
  * (+ bias[n]) rounded to out_dtype.  Replaces dequant_epilogue / _dequant_epilogue_kernel

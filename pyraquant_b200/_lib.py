@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libpq_b200.so"
 
 PQ_OK = 0
 PQ_ERR_TIMEOUT = 6
+PQ_ERR_UNSUPPORTED = 7
 DTYPE_BF16 = 0
 DTYPE_FP16 = 1
 FP4_MX = 0
@@ -42,7 +43,13 @@ SIGNATURES = {
                                     ctypes.c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
     "pq_group_norm_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
     "pq_group_norm": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int,
-                              ctypes.c_float, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+                              ctypes.c_float, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "pq_group_norm_quant_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                                         c_int, ctypes.c_float, c_int, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                         c_int64, c_void_p, c_void_p]),
+    "pq_group_norm_quant_fp4": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                                        c_int, ctypes.c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                        c_void_p, c_void_p]),
     "pq_gather_quant_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                      c_void_p, c_void_p]),
     "pq_gather_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,

@@ -1,57 +1,51 @@
 // Group norm over channels-last rows: z[b,t,c] = act((x[b,t,c] - mean[b,g]) * rstd[b,g] * gamma[c] + beta[c]), statistics over
-// the T rows and C / groups channels of a group, act nothing or SiLU (z * sigmoid(z)), one rounding to the 16-bit type.
+// the T rows and C / groups channels of a group, act nothing or SiLU (z * sigmoid(z)), one rounding to the 16-bit type;
+// with or without the per-row quantisation of z (INT8, mx, nv) in the same launch.
 //
-// Two launches.  Both cut the T rows of every sample into P consecutive chunks, one per CTA, and give a thread a fixed
-// column of eight channels (one 16-byte load) and every R-th row.
-//   1. statistics: a thread sums x - pivot and its square per channel, the pivot being its first value (so that the sum of
-//      squares does not cancel when the mean is large against the deviation); means and centred sums of squares of
-//      channels, threads and chunks are merged pairwise in a fixed order:
-//        n = nA + nB, mean = mA + (mB - mA) nB / n, M2 = M2A + M2B + (mB - mA)^2 nA nB / n.
-//   2. the merged statistics of the sample's P chunks, then the normalisation.
+// HBM-bound: 2 bytes read and 2 (z), 1 (INT8) or 0.53 to 0.56 (4-bit) written per element, provided x is read once although the
+// statistics are needed before the first output.  So one cooperative launch of one CTA per SM: the T rows of a sample are
+// cut into P consecutive chunks, one per CTA, which a CTA keeps in shared memory (200 KB, 30 MB over the GPU) across a
+// grid barrier.  Rows beyond that are read from memory twice, the second time in reverse order (the last ones read are
+// the likeliest to be in L2 still).
+//   1. The rows come by bulk copies in eight segments.  A thread has a fixed column of eight channels and every R-th row
+//      and sums x - pivot and its square per channel, the pivot being its first value (the sum of squares must not cancel
+//      when the mean is large against the deviation).  The CTA's mean of a group is the sum of the threads' sums, its
+//      centred sum of squares that of M2_thread + n (mean_thread - mean)^2: no cancellation, fixed order.
+//   2. After the barrier every CTA does the same with the P chunks of its sample, and normalises its rows.
+// The quantising forms put z back into shared memory, take every row's largest magnitude on the way (an atomic maximum of
+// bit patterns, independent of order) and write codes in a second sweep; they need all rows of a chunk in shared memory.
 // All statistics and arithmetic are fp32.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+#include "fp4_common.cuh"
 #include "quant_common.cuh"
 
 namespace pq {
 namespace {
 
 constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxC = 8192;
+constexpr int kSegments = 8;
 constexpr int kUnroll = 4;
+constexpr int kSmemMax = 232448;
+
+enum Mode { kOut16 = 0, kInt8 = 1, kMx = 2, kNv = 3 };
 
 struct NormArgs {
   const void* x; int64_t ld_row, ld_batch;         // elements
   const void* gamma; const void* beta; int affine_f32;
-  void* out; int64_t out_row, out_batch;
-  float2* part;                                     // [B][P][groups] mean, M2
+  void* out; int64_t out_row, out_batch;            // z (NULL: not wanted)
+  uint8_t* codes;                                   // INT8 [B T, C] or packed E2M1 [B T, C / 2]
+  uint8_t* scales;                                  // 4-bit: scale tiles
+  float* row_scale;                                 // INT8, nv
+  float2* part;                                     // [B][groups][P] mean, M2
+  int32_t* status;
   int B, T, C, groups, P, silu;
+  int cap;                                          // rows a CTA keeps in shared memory
   float eps;
 };
-
-struct Stat { float n, mean, m2; };
-__device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
-  Stat r;
-  r.n = a.n + b.n;
-  const float d = b.mean - a.mean;
-  const float w = r.n > 0.0f ? b.n / r.n : 0.0f;
-  r.mean = fmaf(d, w, a.mean);
-  r.m2 = a.m2 + b.m2 + d * d * a.n * w;
-  // an empty side must not bring in what its fields hold
-  if (b.n == 0.0f) r = a;
-  if (a.n == 0.0f) r = b;
-  return r;
-}
-__device__ __forceinline__ Stat merge_warp(Stat s) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    Stat t;
-    t.n = __shfl_down_sync(0xffffffffu, s.n, o);
-    t.mean = __shfl_down_sync(0xffffffffu, s.mean, o);
-    t.m2 = __shfl_down_sync(0xffffffffu, s.m2, o);
-    s = merge(s, t);                                // lane 0 merges lanes 0..31 in order
-  }
-  return s;
-}
 
 // threads over the columns of eight channels: `cols` a pass, R rows side by side
 struct Lanes { int ncol, cols, R; };
@@ -64,90 +58,18 @@ __host__ __device__ __forceinline__ Lanes lanes_of(int C) {
 }
 __host__ __device__ __forceinline__ int chunk_begin(int T, int P, int p) { return static_cast<int>(static_cast<int64_t>(T) * p / P); }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-pq_group_norm_stats_kernel(const NormArgs a) {
-  extern __shared__ float sm[];                     // [R][C] means, [R][C] M2
-  T tag{};
-  const Lanes l = lanes_of(a.C);
-  const int p = blockIdx.x, b = blockIdx.y;
-  const int r0 = chunk_begin(a.T, a.P, p), r1 = chunk_begin(a.T, a.P, p + 1);
-  const int rl = static_cast<int>(threadIdx.x) / l.cols;
-  const T* xb = static_cast<const T*>(a.x) + static_cast<int64_t>(b) * a.ld_batch;
-  float* s_mean = sm;
-  float* s_m2 = sm + l.R * a.C;
-  if (rl < l.R) {
-    for (int col = static_cast<int>(threadIdx.x) % l.cols; col < l.ncol; col += l.cols) {
-      float piv[8] = {}, s1[8] = {}, s2[8] = {};
-      const T* xc = xb + col * 8;
-      int n = 0;
-      auto unpack = [&](const uint4& v, float (&f)[8]) {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { f[2 * i] = lo_f32(w[i], tag); f[2 * i + 1] = hi_f32(w[i], tag); }
-      };
-      if (r0 + rl < r1) {
-        float f[8];
-        unpack(ld_v4(xc + static_cast<int64_t>(r0 + rl) * a.ld_row), f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) piv[i] = f[i];
-      }
-      for (int r = r0 + rl; r < r1; r += l.R * kUnroll) {
-        uint4 v[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (r + u * l.R < r1) v[u] = ld_v4(xc + static_cast<int64_t>(r + u * l.R) * a.ld_row);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (r + u * l.R < r1) {
-            float f[8];
-            unpack(v[u], f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { const float d = f[i] - piv[i]; s1[i] += d; s2[i] = fmaf(d, d, s2[i]); }
-            ++n;
-          }
-      }
-      const float inv = n > 0 ? 1.0f / static_cast<float>(n) : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s_mean[rl * a.C + col * 8 + i] = fmaf(s1[i], inv, piv[i]);
-        s_m2[rl * a.C + col * 8 + i] = fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f);
-      }
-    }
-  }
-  __syncthreads();
-  const int cpg = a.C / a.groups;
-  const int rows = r1 - r0;
-  for (int g = static_cast<int>(threadIdx.x) >> 5; g < a.groups; g += kThreads / 32) {
-    Stat s{0.0f, 0.0f, 0.0f};
-    for (int i = static_cast<int>(threadIdx.x) & 31; i < l.R * cpg; i += 32) {
-      const int lane_row = i / cpg, c = g * cpg + i % cpg;
-      const int n = rows > lane_row ? (rows - lane_row + l.R - 1) / l.R : 0;
-      s = merge(s, Stat{static_cast<float>(n), s_mean[lane_row * a.C + c], s_m2[lane_row * a.C + c]});
-    }
-    s = merge_warp(s);
-    if ((threadIdx.x & 31) == 0) a.part[(static_cast<int64_t>(b) * a.P + p) * a.groups + g] = make_float2(s.mean, s.m2);
-  }
-}
-
-__device__ __forceinline__ float silu(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
-
-// statistics of the sample's groups from its chunks: s_stat[g] = mean, s_stat[groups + g] = 1 / sqrt(var + eps)
-__device__ __forceinline__ void merge_chunks(const NormArgs& a, int b, float* s_stat) {
-  const int cpg = a.C / a.groups;
-  for (int g = static_cast<int>(threadIdx.x) >> 5; g < a.groups; g += kThreads / 32) {
-    Stat s{0.0f, 0.0f, 0.0f};
-    for (int p = static_cast<int>(threadIdx.x) & 31; p < a.P; p += 32) {
-      const float2 v = a.part[(static_cast<int64_t>(b) * a.P + p) * a.groups + g];
-      const float n = static_cast<float>(chunk_begin(a.T, a.P, p + 1) - chunk_begin(a.T, a.P, p)) * static_cast<float>(cpg);
-      s = merge(s, Stat{n, v.x, v.y});
-    }
-    s = merge_warp(s);
-    if ((threadIdx.x & 31) == 0) {
-      s_stat[g] = s.mean;
-      s_stat[a.groups + g] = 1.0f / sqrtf(s.m2 / s.n + a.eps);
-    }
-  }
+// shared memory: rows, then per-thread sums [R][C], group statistics [2][groups], row maxima, barriers
+struct NormSmem {
+  int red, stat, amax, bars, total;
+};
+__host__ __device__ __forceinline__ NormSmem smem_of(int C, int groups, int cap) {
+  NormSmem s;
+  s.red = (cap * C * 2 + 127) & ~127;
+  s.stat = s.red + lanes_of(C).R * C * 4;
+  s.amax = s.stat + 2 * groups * 4;
+  s.bars = (s.amax + cap * 4 + 7) & ~7;
+  s.total = s.bars + kSegments * 8;
+  return s;
 }
 
 template <typename T>
@@ -156,75 +78,419 @@ __device__ __forceinline__ float affine_at(const void* v, int c, int f32, float 
   if (f32) return static_cast<const float*>(v)[c];
   return lo_f32(static_cast<const unsigned short*>(v)[c], T{});
 }
+__device__ __forceinline__ float silu(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-pq_group_norm_apply_kernel(const NormArgs a) {
-  extern __shared__ float sm[];                     // [2][groups]
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
   T tag{};
-  const Lanes l = lanes_of(a.C);
-  const int p = blockIdx.x, b = blockIdx.y;
-  const int r0 = chunk_begin(a.T, a.P, p), r1 = chunk_begin(a.T, a.P, p + 1);
-  merge_chunks(a, b, sm);
-  __syncthreads();
-  const int rl = static_cast<int>(threadIdx.x) / l.cols;
-  if (rl >= l.R) return;
-  const int cpg = a.C / a.groups;
-  for (int col = static_cast<int>(threadIdx.x) % l.cols; col < l.ncol; col += l.cols) {
-    float mean[8], mul[8], add[8];
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = lo_f32(w[i], tag); f[2 * i + 1] = hi_f32(w[i], tag); }
+}
+// contiguous copy global -> shared, completion bytes on a barrier of this CTA; 16-byte aligned, size % 16 == 0
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t a, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// running sums of one column of eight channels; after finish(): means in piv, centred sums of squares in s2
+struct ColumnSums {
+  float piv[8], s1[8], s2[8], count;
+  int n;
+  __device__ __forceinline__ float mean(int i) const { return piv[i]; }
+  __device__ __forceinline__ float m2(int i) const { return s2[i]; }
+  __device__ __forceinline__ void finish() {
+    count = static_cast<float>(n);
+    const float inv = n > 0 ? 1.0f / count : 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = col * 8 + i, g = c / cpg;
-      mean[i] = sm[g];
-      mul[i] = sm[a.groups + g] * affine_at<T>(a.gamma, c, a.affine_f32, 1.0f);
+      s2[i] = fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f);
+      piv[i] = fmaf(s1[i], inv, piv[i]);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) piv[i] = s1[i] = s2[i] = 0.0f;
+  }
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4& v) {
+    float f[8];
+    unpack8<T>(v, f);
+    if (n == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) piv[i] = f[i];
+    }
+    ++n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { const float d = f[i] - piv[i]; s1[i] += d; s2[i] = fmaf(d, d, s2[i]); }
+  }
+};
+
+template <typename F>
+__device__ __forceinline__ void put8(float* dst, F&& f) {
+  *reinterpret_cast<float4*>(dst) = make_float4(f(0), f(1), f(2), f(3));
+  *reinterpret_cast<float4*>(dst + 4) = make_float4(f(4), f(5), f(6), f(7));
+}
+
+// the normalisation of eight channels
+template <typename T>
+struct Affine8 {
+  float mean[8], mul[8], add[8];
+  __device__ __forceinline__ Affine8(const NormArgs& a, const float* stat, int c0, int cpg) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = c0 + i, g = c / cpg;
+      mean[i] = stat[g];
+      mul[i] = stat[a.groups + g] * affine_at<T>(a.gamma, c, a.affine_f32, 1.0f);
       add[i] = affine_at<T>(a.beta, c, a.affine_f32, 0.0f);
     }
-    const T* xc = static_cast<const T*>(a.x) + static_cast<int64_t>(b) * a.ld_batch + col * 8;
-    T* oc = static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.out_batch + col * 8;
-    for (int r = r0 + rl; r < r1; r += l.R * kUnroll) {
-      uint4 v[kUnroll];
+  }
+  __device__ __forceinline__ uint4 operator()(const uint4& v, int with_silu) const {
+    float f[8];
+    unpack8<T>(v, f);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (r + u * l.R < r1) v[u] = ld_v4(xc + static_cast<int64_t>(r + u * l.R) * a.ld_row);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (r + u * l.R < r1) {
-          const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-          uint32_t o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float z0 = fmaf(lo_f32(w[i], tag) - mean[2 * i], mul[2 * i], add[2 * i]);
-            float z1 = fmaf(hi_f32(w[i], tag) - mean[2 * i + 1], mul[2 * i + 1], add[2 * i + 1]);
-            if (a.silu) { z0 = silu(z0); z1 = silu(z1); }
-            o[i] = pack2(z0, z1, tag);
-          }
-          st_v4(oc + static_cast<int64_t>(r + u * l.R) * a.out_row, make_uint4(o[0], o[1], o[2], o[3]));
-        }
+    for (int i = 0; i < 8; ++i) {
+      f[i] = fmaf(f[i] - mean[i], mul[i], add[i]);
+      if (with_silu) f[i] = silu(f[i]);
     }
+    T tag{};
+    return make_uint4(pack2(f[0], f[1], tag), pack2(f[2], f[3], tag), pack2(f[4], f[5], tag), pack2(f[6], f[7], tag));
+  }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// sums over the R x cpg entries of every group of `red`, one warp per group, in a fixed order
+template <typename F>
+__device__ __forceinline__ void sum_groups(const float* red, int R, int C, int groups, int cpg, F&& put) {
+  const int lane = threadIdx.x & 31;
+  for (int g = static_cast<int>(threadIdx.x) >> 5; g < groups; g += kWarps) {
+    float s = 0.0f;
+    if (cpg >= 32) {
+      for (int r = 0; r < R; ++r)
+        for (int c = lane; c < cpg; c += 32) s += red[r * C + g * cpg + c];
+    } else {
+      // lanes in rows of cpg: floor(32 / cpg) rows at a time
+      const int per = 32 / cpg, r0 = lane / cpg, c = lane - r0 * cpg;
+      if (r0 < per)
+        for (int r = r0; r < R; r += per) s += red[r * C + g * cpg + c];
+    }
+    s = warp_sum(s);
+    if (lane == 0) put(g, s);
   }
 }
 
-// chunks per sample: all SMs busy, at least one unrolled step of rows per CTA
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+pq_group_norm_kernel(const NormArgs a) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  T tag{};
+  const Lanes l = lanes_of(a.C);
+  const NormSmem lay = smem_of(a.C, a.groups, a.cap);
+  float* red = reinterpret_cast<float*>(smem + lay.red);
+  float* stat = reinterpret_cast<float*>(smem + lay.stat);              // mean, then 1 / sqrt(var + eps)
+  uint32_t* amax = reinterpret_cast<uint32_t*>(smem + lay.amax);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lay.bars);
+  const uint32_t rows_s = smem_u32(smem);
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  const int p = static_cast<int>(blockIdx.x) % a.P;
+  const int r0 = chunk_begin(a.T, a.P, p), rows = chunk_begin(a.T, a.P, p + 1) - r0;
+  const int resident = rows < a.cap ? rows : a.cap;
+  const int seg_rows = (resident + kSegments - 1) / kSegments > 0 ? (resident + kSegments - 1) / kSegments : 1;
+  const int cpg = a.C / a.groups;
+  const int rl = tid / l.cols, col0 = tid - rl * l.cols;
+  const int row_bytes = a.C * 2;
+
+  if (tid == 0) {
+    for (int s = 0; s < kSegments; ++s) mbar_init(&bars[s], 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+
+  uint32_t phase = 0;
+#pragma unroll 1
+  for (int b = static_cast<int>(blockIdx.x) / a.P; b < a.B; b += static_cast<int>(gridDim.x) / a.P, phase ^= 1u) {
+    const T* xb = static_cast<const T*>(a.x) + static_cast<int64_t>(b) * a.ld_batch + static_cast<int64_t>(r0) * a.ld_row;
+    // ---------------------------------------------------------------- rows into shared memory
+    if (warp == 0) {
+      for (int s = 0; s < kSegments; ++s) {
+        const int from = s * seg_rows < resident ? s * seg_rows : resident;
+        const int to = from + seg_rows < resident ? from + seg_rows : resident;
+        if (lane == 0) mbar_arrive_expect_tx(&bars[s], static_cast<uint32_t>((to - from) * row_bytes));
+        __syncwarp();
+        if (a.ld_row == a.C) {                                          // one piece
+          if (lane == 0 && to > from)
+            bulk_copy(rows_s + from * row_bytes, xb + static_cast<int64_t>(from) * a.C, static_cast<uint32_t>((to - from) * row_bytes), &bars[s]);
+        } else {
+          for (int r = from + lane; r < to; r += 32)
+            bulk_copy(rows_s + r * row_bytes, xb + static_cast<int64_t>(r) * a.ld_row, static_cast<uint32_t>(row_bytes), &bars[s]);
+        }
+      }
+    }
+    if (MODE != kOut16)
+      for (int r = tid; r < resident; r += kThreads) amax[r] = 0u;
+
+    // ---------------------------------------------------------------- statistics of the chunk
+    ColumnSums cs[2];                                                    // two columns a thread only for C > 4096
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      cs[k].clear();
+      const int col = col0 + k * l.cols;
+      if (rl < l.R && col < l.ncol) {
+        const T* xc = xb + col * 8;
+        int r = resident + rl;
+        for (; r < rows; r += l.R * kUnroll) {                           // rows that stay in memory
+          uint4 v[kUnroll];
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u)
+            if (r + u * l.R < rows) v[u] = ld_v4(xc + static_cast<int64_t>(r + u * l.R) * a.ld_row);
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u)
+            if (r + u * l.R < rows) cs[k].template add<T>(v[u]);
+        }
+        int seg_end = 0, seg = -1;
+        for (r = rl; r < resident; r += l.R) {
+          while (r >= seg_end) {
+            ++seg; seg_end += seg_rows;
+            if (!mbar_wait_bounded(&bars[seg], phase)) report_timeout(a.status, 8, 1);
+          }
+          cs[k].template add<T>(ld_shared_v4(rows_s + r * row_bytes + col * 16));
+        }
+        cs[k].finish();
+        put8(red + rl * a.C + col * 8, [&](int i) { return cs[k].mean(i) * cs[k].count; });
+      }
+    }
+    __syncthreads();
+    const float count = static_cast<float>(rows) * static_cast<float>(cpg);
+    sum_groups(red, l.R, a.C, a.groups, cpg, [&](int g, float s) { stat[g] = s / count; });
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int col = col0 + k * l.cols;
+      if (rl < l.R && col < l.ncol)
+        put8(red + rl * a.C + col * 8, [&](int i) {
+          const float d = cs[k].mean(i) - stat[(col * 8 + i) / cpg];
+          return fmaf(d * d, cs[k].count, cs[k].m2(i));
+        });
+    }
+    __syncthreads();
+    sum_groups(red, l.R, a.C, a.groups, cpg, [&](int g, float s) { stat[a.groups + g] = s; });
+    __syncthreads();
+
+    // ---------------------------------------------------------------- statistics of the sample
+    if (a.P > 1) {
+      for (int g = tid; g < a.groups; g += kThreads)
+        a.part[(static_cast<int64_t>(b) * a.groups + g) * a.P + p] = make_float2(stat[g], stat[a.groups + g]);
+      cooperative_groups::this_grid().sync();
+      const float total = static_cast<float>(a.T) * static_cast<float>(cpg);
+      for (int g = warp; g < a.groups; g += kWarps) {
+        const float2* part = a.part + (static_cast<int64_t>(b) * a.groups + g) * a.P;
+        float s = 0.0f;
+        for (int i = lane; i < a.P; i += 32)
+          s += __ldcg(part + i).x * (static_cast<float>(chunk_begin(a.T, a.P, i + 1) - chunk_begin(a.T, a.P, i)) * static_cast<float>(cpg));
+        const float mean = warp_sum(s) / total;
+        float m2 = 0.0f;
+        for (int i = lane; i < a.P; i += 32) {
+          const float2 v = __ldcg(part + i);
+          const float d = v.x - mean, n = static_cast<float>(chunk_begin(a.T, a.P, i + 1) - chunk_begin(a.T, a.P, i)) * static_cast<float>(cpg);
+          m2 += fmaf(d * d, n, v.y);
+        }
+        m2 = warp_sum(m2);
+        if (lane == 0) { stat[g] = mean; stat[a.groups + g] = 1.0f / sqrtf(m2 / total + a.eps); }
+      }
+    } else {
+      for (int g = tid; g < a.groups; g += kThreads) stat[a.groups + g] = 1.0f / sqrtf(stat[a.groups + g] / count + a.eps);
+    }
+    __syncthreads();
+
+    // ---------------------------------------------------------------- normalisation
+    const int64_t out0 = static_cast<int64_t>(b) * a.out_batch + static_cast<int64_t>(r0) * a.out_row;
+    if constexpr (MODE == kOut16) {
+#pragma unroll 1
+      for (int col = col0; rl < l.R && col < l.ncol; col += l.cols) {
+        const Affine8<T> f(a, stat, col * 8, cpg);
+        const T* xc = xb + col * 8;
+        T* oc = static_cast<T*>(a.out) + out0 + col * 8;
+        const int far = rows - resident;                                  // rows to read again, the last ones first
+        for (int r = rl; r < far; r += l.R * kUnroll) {
+          uint4 v[kUnroll];
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u)
+            if (r + u * l.R < far) v[u] = ld_stream_v4(xc + static_cast<int64_t>(rows - 1 - r - u * l.R) * a.ld_row);
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u)
+            if (r + u * l.R < far) st_v4_cs(oc + static_cast<int64_t>(rows - 1 - r - u * l.R) * a.out_row, f(v[u], a.silu));
+        }
+        for (int r = rl; r < resident; r += l.R)
+          st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, f(ld_shared_v4(rows_s + r * row_bytes + col * 16), a.silu));
+      }
+    } else {
+      // a thread has a fixed column of 16 channels and every R2-th row
+      const int nch = a.C >> 4, R2 = kThreads / nch;
+      const int r2 = tid / nch, ci = tid - r2 * nch;
+      const bool active = r2 < R2;
+      {
+        const Affine8<T> f0(a, stat, active ? ci * 16 : 0, cpg), f1(a, stat, active ? ci * 16 + 8 : 0, cpg);
+#pragma unroll 1
+        for (int rb = 0; rb < rows; rb += R2) {
+          const int r = rb + r2;
+          const bool ok = active && r < rows;
+          uint32_t m = 0u;
+          if (ok) {
+            const uint32_t at = rows_s + r * row_bytes + ci * 32;
+            const uint4 z0 = f0(ld_shared_v4(at), a.silu), z1 = f1(ld_shared_v4(at + 16), a.silu);
+            st_shared_v4(at, z0); st_shared_v4(at + 16, z1);
+            if (a.out != nullptr) {
+              T* o = static_cast<T*>(a.out) + out0 + static_cast<int64_t>(r) * a.out_row + ci * 16;
+              st_v4(o, z0); st_v4(o + 8, z1);
+            }
+            m = max_pattern(absmax_chunk<T>(absmax_chunk<T>(0u, z0), z1));
+          }
+          if constexpr (MODE != kMx) {
+            // lanes of one row first, as far as rows divide into equal shares of lanes
+            int share = 1;
+            if ((nch & 1) == 0) { m = max(m, __shfl_xor_sync(0xffffffffu, m, 1)); share = 2; }
+            if ((nch & 3) == 0) { m = max(m, __shfl_xor_sync(0xffffffffu, m, 2)); share = 4; }
+            if (ok && (tid & (share - 1)) == 0) atomicMax(&amax[r], m);
+          }
+        }
+      }
+      __syncthreads();
+      const int64_t tiles = MODE == kInt8 ? 0 : fp4_scale_tiles(a.C, MODE == kMx ? PQ_FP4_MX : PQ_FP4_NV);
+#pragma unroll 1
+      for (int rb = 0; rb < rows; rb += R2) {
+        const int r = rb + r2;
+        const bool ok = active && r < rows;
+        const int64_t row = static_cast<int64_t>(b) * a.T + r0 + r;
+        uint4 z0 = make_uint4(0u, 0u, 0u, 0u), z1 = z0;
+        if (ok) {
+          const uint32_t at = rows_s + r * row_bytes + ci * 32;
+          z0 = ld_shared_v4(at); z1 = ld_shared_v4(at + 16);
+        }
+        if constexpr (MODE == kInt8) {
+          if (!ok) continue;
+          const QuantScale qs = make_quant_scale(lo_f32(amax[r], tag));
+          if (ci == 0) a.row_scale[row] = qs.scale;
+          uint4 q;
+          quant_chunk<T>(z0, qs, q.x, q.y);
+          quant_chunk<T>(z1, qs, q.z, q.w);
+          st_v4(a.codes + row * a.C + ci * 16, q);
+        } else {
+          const Chunk16 c{{z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w}};
+          uint32_t m = max_pattern(absmax_chunk16(c));
+          BlockScale s;
+          if constexpr (MODE == kMx) {
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));               // C % 32 == 0: a block is two neighbours
+            s = mx_block_scale(lo_f32(m, tag));
+          } else {
+            const float top = ok ? lo_f32(amax[r], tag) : 0.0f;
+            const bool bad = (__float_as_int(top) >> 23) == 255;
+            const float s_row = bad ? 1.0f : nv_row_scale(top);
+            s = nv_block_scale(lo_f32(m, tag), s_row, bad);
+            if (ok && ci == 0) a.row_scale[row] = bad ? __int_as_float(0x7FC00000) : s_row;
+          }
+          if (!ok) continue;
+          const uint2 q = quant_chunk16<T, MODE == kMx ? PQ_FP4_MX : PQ_FP4_NV>(c, s);
+          st_v2(a.codes + row * (a.C >> 1) + ci * 8, q.x, q.y);
+          const int blk = MODE == kMx ? ci >> 1 : ci, blocks = MODE == kMx ? nch >> 1 : nch;
+          if (MODE == kNv || (ci & 1) == 0) {
+            uint8_t* sp = a.scales + fp4_scale_off(row, blk >> 2, tiles) + (blk & 3);
+            *sp = static_cast<uint8_t>(s.byte);
+            if (blk == blocks - 1)
+              for (int k = (blk & 3) + 1; k < 4; ++k) *++sp = 0;           // the row's last scale word
+          }
+        }
+      }
+    }
+    fence_proxy_async_smem();                                             // before the next sample's copies overwrite the rows
+    __syncthreads();
+  }
+}
+
+// chunks per sample: all SMs busy, at least one step of rows per CTA
 int chunks_of(int B, int T, int C) {
   const Lanes l = lanes_of(C);
-  int P = 2 * sm_count() / B;
-  const int most = (T + l.R * kUnroll - 1) / (l.R * kUnroll);
+  int P = sm_count() / B;
+  const int most = (T + l.R - 1) / l.R;
   if (P > most) P = most;
   return P < 1 ? 1 : P;
 }
 
-template <typename T>
-int launch_norm(const NormArgs& a, cudaStream_t st) {
-  const Lanes l = lanes_of(a.C);
-  const dim3 grid(static_cast<unsigned>(a.P), static_cast<unsigned>(a.B));
-  const int smem = 2 * l.R * a.C * static_cast<int>(sizeof(float));
-  if (smem > 48 * 1024)
-    PQ_CUDA_TRY(cudaFuncSetAttribute(pq_group_norm_stats_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  pq_group_norm_stats_kernel<T><<<grid, kThreads, smem, st>>>(a);
-  PQ_CUDA_TRY(cudaGetLastError());
-  pq_group_norm_apply_kernel<T><<<grid, kThreads, 2 * a.groups * static_cast<int>(sizeof(float)), st>>>(a);
-  PQ_CUDA_TRY(cudaGetLastError());
+template <typename T, int MODE>
+int launch_norm(NormArgs a, cudaStream_t st) {
+  const int longest = (a.T + a.P - 1) / a.P;
+  const int fixed = smem_of(a.C, a.groups, 0).total + 256;
+  int cap = (kSmemMax - fixed) / (a.C * 2 + 4);
+  if (cap > longest) cap = longest;
+  if (cap < 0) return PQ_ERR_UNSUPPORTED;
+  if (MODE != kOut16 && cap < longest) return PQ_ERR_UNSUPPORTED;          // the rows do not fit on the chip
+  a.cap = cap;
+  const NormSmem lay = smem_of(a.C, a.groups, cap);
+  if (lay.total > kSmemMax) return PQ_ERR_UNSUPPORTED;
+  auto kern = pq_group_norm_kernel<T, MODE>;
+  static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes
+  int dev = 0;
+  PQ_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    PQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const int sms = sm_count();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.P * (a.B < sms ? a.B : sms)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(lay.total);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = a.P > 1 ? 1 : 0;                                         // nobody waits for another CTA otherwise
+  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a));
   return PQ_OK;
+}
+
+template <int MODE>
+int group_norm_any(const void* x, int dtype, int64_t B, int64_t T, int64_t C, int64_t ld_row, int64_t ld_batch, int groups,
+                   const void* gamma, const void* beta, int affine_fp32, float eps, int act, void* out, int64_t ldo_row,
+                   int64_t ldo_batch, uint8_t* codes, uint8_t* scales, float* row_scale, void* workspace, int64_t ws_bytes,
+                   void* status, void* stream) {
+  if (B < 0 || T < 0 || C <= 0 || groups <= 0 || B > 65535 || T > 0x7fffffffLL || C > kMaxC || C % groups != 0) return PQ_ERR_SHAPE;
+  if (!(eps >= 0.0f) || ld_row < C || ld_batch < 0 || (out != nullptr && (ldo_row < C || ldo_batch < 0))) return PQ_ERR_SHAPE;
+  if (dtype != PQ_DTYPE_BF16 && dtype != PQ_DTYPE_FP16) return PQ_ERR_DTYPE;
+  if (act != PQ_ACT_NONE && act != PQ_ACT_SILU) return PQ_ERR_UNSUPPORTED;
+  if (B == 0 || T == 0) return PQ_OK;
+  if (x == nullptr || workspace == nullptr || (MODE == kOut16 && out == nullptr)) return PQ_ERR_NULL;
+  if (MODE != kOut16 && (codes == nullptr || (MODE != kMx && row_scale == nullptr) || (MODE >= kMx && scales == nullptr))) return PQ_ERR_NULL;
+  if (C % (MODE == kOut16 ? 8 : (MODE == kInt8 ? 16 : 32)) != 0 || ld_row % 8 != 0 || ld_batch % 8 != 0) return PQ_ERR_ALIGN;
+  if (out != nullptr && (ldo_row % 8 != 0 || ldo_batch % 8 != 0 || !aligned_to(out, 16))) return PQ_ERR_ALIGN;
+  if (!aligned_to(x, 16) || !aligned_to(workspace, 8) || !aligned_to(gamma, affine_fp32 ? 4 : 2) ||
+      !aligned_to(beta, affine_fp32 ? 4 : 2) || !aligned_to(codes, 16) || !aligned_to(scales, 16) || !aligned_to(row_scale, 4))
+    return PQ_ERR_ALIGN;
+  if (ws_bytes < pq_group_norm_workspace_bytes(B, T, C, groups)) return PQ_ERR_WORKSPACE;
+  NormArgs a{};
+  a.x = x; a.ld_row = ld_row; a.ld_batch = ld_batch; a.gamma = gamma; a.beta = beta; a.affine_f32 = affine_fp32 != 0;
+  a.out = out; a.out_row = ldo_row; a.out_batch = ldo_batch; a.codes = codes; a.scales = scales; a.row_scale = row_scale;
+  a.part = static_cast<float2*>(workspace); a.status = static_cast<int32_t*>(status);
+  a.B = static_cast<int>(B); a.T = static_cast<int>(T); a.C = static_cast<int>(C); a.groups = groups;
+  a.P = chunks_of(a.B, a.T, a.C); a.silu = act == PQ_ACT_SILU; a.eps = eps;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == PQ_DTYPE_BF16 ? launch_norm<__nv_bfloat16, MODE>(a, st) : launch_norm<__half, MODE>(a, st);
 }
 
 }  // namespace
@@ -239,23 +505,29 @@ extern "C" int64_t pq_group_norm_workspace_bytes(int64_t B, int64_t T, int64_t C
 
 extern "C" int pq_group_norm(const void* x, int dtype, int64_t B, int64_t T, int64_t C, int64_t ld_row, int64_t ld_batch,
                              int groups, const void* gamma, const void* beta, int affine_fp32, float eps, int act,
-                             void* out, int64_t ldo_row, int64_t ldo_batch, void* workspace, int64_t ws_bytes, void* stream) {
-  if (B < 0 || T < 0 || C <= 0 || groups <= 0 || B > 65535 || T > 0x7fffffffLL || C > kMaxC || C % groups != 0) return PQ_ERR_SHAPE;
-  if (!(eps >= 0.0f) || ld_row < C || ldo_row < C || ld_batch < 0 || ldo_batch < 0) return PQ_ERR_SHAPE;
-  if (dtype != PQ_DTYPE_BF16 && dtype != PQ_DTYPE_FP16) return PQ_ERR_DTYPE;
-  if (act != PQ_ACT_NONE && act != PQ_ACT_SILU) return PQ_ERR_UNSUPPORTED;
-  if (B == 0 || T == 0) return PQ_OK;
-  if (x == nullptr || out == nullptr || workspace == nullptr) return PQ_ERR_NULL;
-  if (C % 8 != 0 || ld_row % 8 != 0 || ld_batch % 8 != 0 || ldo_row % 8 != 0 || ldo_batch % 8 != 0) return PQ_ERR_ALIGN;
-  if (!aligned_to(x, 16) || !aligned_to(out, 16) || !aligned_to(workspace, 8) || !aligned_to(gamma, affine_fp32 ? 4 : 2) ||
-      !aligned_to(beta, affine_fp32 ? 4 : 2))
-    return PQ_ERR_ALIGN;
-  if (ws_bytes < pq_group_norm_workspace_bytes(B, T, C, groups)) return PQ_ERR_WORKSPACE;
-  NormArgs a{};
-  a.x = x; a.ld_row = ld_row; a.ld_batch = ld_batch; a.gamma = gamma; a.beta = beta; a.affine_f32 = affine_fp32 != 0;
-  a.out = out; a.out_row = ldo_row; a.out_batch = ldo_batch; a.part = static_cast<float2*>(workspace);
-  a.B = static_cast<int>(B); a.T = static_cast<int>(T); a.C = static_cast<int>(C); a.groups = groups;
-  a.P = chunks_of(a.B, a.T, a.C); a.silu = act == PQ_ACT_SILU; a.eps = eps;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == PQ_DTYPE_BF16 ? launch_norm<__nv_bfloat16>(a, st) : launch_norm<__half>(a, st);
+                             void* out, int64_t ldo_row, int64_t ldo_batch, void* workspace, int64_t ws_bytes, void* status,
+                             void* stream) {
+  return group_norm_any<kOut16>(x, dtype, B, T, C, ld_row, ld_batch, groups, gamma, beta, affine_fp32, eps, act, out, ldo_row,
+                                ldo_batch, nullptr, nullptr, nullptr, workspace, ws_bytes, status, stream);
+}
+
+extern "C" int pq_group_norm_quant_rows(const void* x, int dtype, int64_t B, int64_t T, int64_t C, int64_t ld_row,
+                                        int64_t ld_batch, int groups, const void* gamma, const void* beta, int affine_fp32,
+                                        float eps, int act, void* x_norm, int64_t ldn_row, int64_t ldn_batch, int8_t* q, float* s,
+                                        void* workspace, int64_t ws_bytes, void* status, void* stream) {
+  return group_norm_any<kInt8>(x, dtype, B, T, C, ld_row, ld_batch, groups, gamma, beta, affine_fp32, eps, act, x_norm, ldn_row,
+                               ldn_batch, reinterpret_cast<uint8_t*>(q), nullptr, s, workspace, ws_bytes, status, stream);
+}
+
+extern "C" int pq_group_norm_quant_fp4(const void* x, int dtype, int64_t B, int64_t T, int64_t C, int64_t ld_row,
+                                       int64_t ld_batch, int groups, const void* gamma, const void* beta, int affine_fp32,
+                                       float eps, int act, int fmt, uint8_t* codes, uint8_t* scales, float* row_scale,
+                                       void* workspace, int64_t ws_bytes, void* status, void* stream) {
+  if (fmt == PQ_FP4_MX)
+    return group_norm_any<kMx>(x, dtype, B, T, C, ld_row, ld_batch, groups, gamma, beta, affine_fp32, eps, act, nullptr, 0, 0, codes,
+                               scales, row_scale, workspace, ws_bytes, status, stream);
+  if (fmt == PQ_FP4_NV)
+    return group_norm_any<kNv>(x, dtype, B, T, C, ld_row, ld_batch, groups, gamma, beta, affine_fp32, eps, act, nullptr, 0, 0, codes,
+                               scales, row_scale, workspace, ws_bytes, status, stream);
+  return PQ_ERR_UNSUPPORTED;
 }

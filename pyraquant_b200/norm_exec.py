@@ -33,7 +33,13 @@ def group_norm_rows(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor]
 def group_norm_quant_rows(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                           eps: float = 1e-6, act: Optional[str] = None,
                           want_normed: bool = False) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
-    """(q, s, z) with z = group_norm_rows(x, ...) and (q, s) = quant_rows of z's rows; z is None unless ``want_normed``."""
+    """(q, s, z) with z = group_norm_rows(x, ...) and (q, s) = quant_rows of z's rows; z is None unless ``want_normed``.  One
+    launch where the rows fit into the GPU's shared memory (about 29 MB) and C % 16 == 0, two otherwise; the same codes."""
+    assert x.is_cuda
+    if _eager():
+        r = ops.group_norm_quant_rows_fused(x, groups, weight, bias, eps, act, want_normed)
+        if r is not None:
+            return r
     z = group_norm_rows(x, groups, weight, bias, eps, act)
     q, s = quant_rows(z.reshape(-1, z.shape[-1]))
     return q, s, z if want_normed else None
@@ -41,6 +47,11 @@ def group_norm_quant_rows(x: torch.Tensor, groups: int, weight: Optional[torch.T
 
 def group_norm_quant_fp4(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                          eps: float = 1e-6, act: Optional[str] = None, fmt: str = DEFAULT_FORMAT) -> Fp4Rows:
-    """quant_rows_fp4 of the rows of group_norm_rows(x, ...); C % 32 == 0."""
+    """quant_rows_fp4 of the rows of group_norm_rows(x, ...), C % 32 == 0; launches as group_norm_quant_rows."""
+    assert x.is_cuda
+    if _eager():
+        r = ops.group_norm_quant_fp4_fused(x, groups, weight, bias, eps, act, fmt)
+        if r is not None:
+            return Fp4Rows(*r)
     z = group_norm_rows(x, groups, weight, bias, eps, act)
     return quant_rows_fp4(z.reshape(-1, z.shape[-1]), fmt)

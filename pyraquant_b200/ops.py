@@ -250,23 +250,70 @@ def group_norm_args(x: Tensor, groups: int, weight: Optional[Tensor], bias: Opti
     return x3, weight, bias, GROUP_NORM_ACTS[act]
 
 
-def _group_norm_impl(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
-                     act: Optional[str]) -> Tensor:
+def _group_norm_call(name: str, x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                     act: Optional[str], outputs):
+    """Runs one of the pq_group_norm entry points on x; `outputs(x3)` allocates and returns (result, the entry point's output
+    arguments).  None when the entry point does not take the size (its rows do not fit on the chip)."""
     x3, weight, bias, code = group_norm_args(x, groups, weight, bias, act)
     B, T, C = x3.shape
-    out = torch.empty((B, T, C), dtype=x.dtype, device=x.device)
-    if out.numel():
-        lib = _LIB()
-        f32 = any(v is not None and v.dtype == torch.float32 for v in (weight, bias))
-        with _on_device(x3):
-            nbytes = lib.pq_group_norm_workspace_bytes(B, T, C, groups)
-            ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
-            rc = lib.pq_group_norm(x3.data_ptr(), _dt(x.dtype), B, T, C, x3.stride(1) if T > 1 else C,
-                                   x3.stride(0) if B > 1 else T * C, groups, _ptr(weight), _ptr(bias), int(f32), float(eps), code,
-                                   out.data_ptr(), C, T * C, ws.data_ptr(), nbytes, _stream(x3))
-        if rc:
-            _lib.check(rc, f"pq_group_norm(B={B}, T={T}, C={C}, groups={groups})")
-    return out.reshape(x.shape)
+    result, args = outputs(x3)
+    if x3.numel() == 0:
+        return result
+    lib = _LIB()
+    f32 = (weight is not None and weight.dtype == torch.float32) or (bias is not None and bias.dtype == torch.float32)
+    with _on_device(x3):
+        nbytes = lib.pq_group_norm_workspace_bytes(B, T, C, groups)
+        ws = x3.new_empty((nbytes,), dtype=torch.uint8)
+        rc = getattr(lib, name)(x3.data_ptr(), _DT[x.dtype], B, T, C, x3.stride(1) if T > 1 else C, x3.stride(0) if B > 1 else T * C,
+                                groups, _ptr(weight), _ptr(bias), int(f32), float(eps), code, *args, ws.data_ptr(), nbytes,
+                                status_word(x3.device).data_ptr(), _stream(x3))
+    if rc == _lib.PQ_ERR_UNSUPPORTED:
+        return None
+    if rc:
+        _lib.check(rc, f"{name}(B={B}, T={T}, C={C}, groups={groups})")
+    return result
+
+
+def _group_norm_impl(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                     act: Optional[str]) -> Tensor:
+    def outputs(x3):
+        B, T, C = x3.shape
+        out = x3.new_empty((B, T, C))
+        return out, (out.data_ptr(), C, T * C)
+    out = _group_norm_call("pq_group_norm", x, groups, weight, bias, eps, act, outputs)
+    assert out is not None
+    return out if out.shape == x.shape else out.reshape(x.shape)
+
+
+def group_norm_quant_rows_fused(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                                act: Optional[str], want_normed: bool):
+    """(q, s, z or None) in one launch (pq_group_norm_quant_rows), or None when the size does not fit."""
+    C = x.shape[-1]
+    if C % 16:
+        return None
+
+    def outputs(x3):
+        B, T, C = x3.shape
+        z = x3.new_empty((B, T, C)) if want_normed else None
+        q, s = x3.new_empty((B * T, C), dtype=torch.int8), x3.new_empty((B * T,), dtype=torch.float32)
+        return (q, s, z if z is None else z.reshape(x.shape)), (_ptr(z), C, T * C, q.data_ptr(), s.data_ptr())
+    return _group_norm_call("pq_group_norm_quant_rows", x, groups, weight, bias, eps, act, outputs)
+
+
+def group_norm_quant_fp4_fused(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                               act: Optional[str], fmt: str):
+    """(codes, scales, row scales or None) in one launch (pq_group_norm_quant_fp4), or None when the size does not fit."""
+    code = _fp4_code(fmt)
+    C = x.shape[-1]
+    assert C % 32 == 0, f"K={C} must be a multiple of 32"
+
+    def outputs(x3):
+        M = x3.shape[0] * x3.shape[1]
+        codes = x3.new_empty((M, C // 2), dtype=torch.uint8)
+        scales = x3.new_empty(fp4_scale_shape(M, C, fmt), dtype=torch.uint8)
+        row = x3.new_empty((M,), dtype=torch.float32) if fmt == "nv" else None
+        return (codes, scales, row), (code, codes.data_ptr(), scales.data_ptr(), _ptr(row))
+    return _group_norm_call("pq_group_norm_quant_fp4", x, groups, weight, bias, eps, act, outputs)
 
 
 def _gather_quant_rows_impl(canvas: Tensor, row_idx: Tensor) -> Tuple[Tensor, Tensor]:

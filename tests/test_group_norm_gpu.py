@@ -106,6 +106,23 @@ def test_layouts(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,C,groups", [(1, 30000, 640, 32), (3, 4000, 1536, 32), (2, 1500, 8192, 16)])
+def test_more_rows_than_the_chip_holds(cuda_dev, dtype, B, T, C, groups):
+    """Rows beyond shared memory are read twice; the quantising forms fall back to two launches."""
+    x, w, b = (t.to(cuda_dev) for t in rows(B, T, C, dtype, 11))
+    z = norm_exec.group_norm_rows(x, groups, w, b, 1e-6, "silu")
+    check(z, x, groups, w, b, 1e-6, "silu")
+    assert torch.equal(norm_exec.group_norm_rows(x, groups, w, b, 1e-6, "silu"), z)
+    q, s, zz = norm_exec.group_norm_quant_rows(x, groups, w, b, 1e-6, "silu", want_normed=True)
+    q0, s0 = int8_exec.quant_rows(z.reshape(-1, C))
+    assert torch.equal(zz, z) and torch.equal(q, q0) and torch.equal(s, s0)
+    wide = torch.zeros(B, T, C + 64, device=cuda_dev, dtype=dtype)
+    wide[..., 32: 32 + C] = x
+    assert torch.equal(norm_exec.group_norm_rows(wide[..., 32: 32 + C], groups, w, b, 1e-6, "silu"), z)
+
+
+@pytest.mark.gpu
 def test_nan_stays_in_its_group(cuda_dev):
     x, w, b = (t.to(cuda_dev) for t in rows(2, 300, 64, torch.float16, 5))
     want = norm_exec.group_norm_rows(x, 8, w, b)
@@ -118,10 +135,12 @@ def test_nan_stays_in_its_group(cuda_dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("B,T,C", [(1, 1, 32), (2, 77, 320), (3, 250, 640), (1, 1024, 1280), (2, 40, 2560), (1, 9, 8192), (150, 2, 64)])
+@pytest.mark.parametrize("B,T,C", [(1, 1, 32), (2, 77, 320), (3, 250, 640), (1, 1024, 1280), (2, 40, 2560), (1, 9, 8192), (150, 2, 64), (400, 3, 96),
+                                   (2, 3000, 224)])
 def test_quantising_forms(cuda_dev, dtype, B, T, C):
     """The forms that quantise in the same call give the codes of the separate steps, bit for bit."""
     groups = 32 if C >= 320 else 4
+    assert ops.group_norm_quant_rows_fused(torch.zeros(B, T, C, device=cuda_dev, dtype=dtype), groups, None, None, 1e-6, None, False) is not None
     x, w, b = (t.to(cuda_dev) for t in rows(B, T, C, dtype, 3 * C + T))
     for act in (None, "silu"):
         z = norm_exec.group_norm_rows(x, groups, w, b, 1e-6, act)
@@ -194,6 +213,7 @@ def test_streams_graphs_and_repeats(cuda_dev):
         graphs[1].replay()
     torch.cuda.synchronize()
     assert torch.equal(ys[1].codes, f0.codes)
+    ops.check_device_status(cuda_dev)
 
 
 @pytest.mark.gpu
@@ -232,7 +252,7 @@ def test_argument_checks():
 
     def gn(x=p, dtype=0, B=1, T=4, C=64, row=64, batch=256, groups=8, w=None, b=None, f32=0, eps=1e-6, act=0, out=p, orow=64,
            obatch=256, ws=p, wsb=big):
-        return lib.pq_group_norm(x, dtype, B, T, C, row, batch, groups, w, b, f32, eps, act, out, orow, obatch, ws, wsb, None)
+        return lib.pq_group_norm(x, dtype, B, T, C, row, batch, groups, w, b, f32, eps, act, out, orow, obatch, ws, wsb, None, None)
     assert gn(B=0, x=None) == 0 and gn(T=0, x=None) == 0
     assert gn(x=None) == 1 and gn(out=None) == 1 and gn(ws=None) == 1
     assert gn(B=-1) == 2 and gn(C=0) == 2 and gn(groups=0) == 2 and gn(groups=7) == 2 and gn(row=56) == 2 and gn(eps=-1.0) == 2
@@ -240,4 +260,12 @@ def test_argument_checks():
     assert gn(C=60, groups=4) == 3 and gn(row=68) == 3 and gn(batch=257) == 3 and gn(x=p + 8) == 3 and gn(out=p + 2) == 3 and gn(ws=p + 4) == 3
     assert gn(w=p + 1) == 3 and gn(b=p + 2, f32=1) == 3
     assert gn(dtype=2) == 4 and gn(act=2) == 7 and gn(wsb=0) == 8
+
+    def q8(C=64, z=None, q=p, s=p, x=p):
+        return lib.pq_group_norm_quant_rows(x, 0, 1, 4, C, C, 4 * C, 8, None, None, 0, 1e-6, 0, z, C, 4 * C, q, s, p, big, None, None)
+    assert q8(q=None) == 1 and q8(s=None) == 1 and q8(C=72) == 3 and q8(q=p + 8) == 3 and q8(z=p + 8) == 3 and q8(x=None) == 1
+
+    def q4(C=64, fmt=1, codes=p, scales=p, row=p):
+        return lib.pq_group_norm_quant_fp4(p, 0, 1, 4, C, C, 4 * C, 8, None, None, 0, 1e-6, 0, fmt, codes, scales, row, p, big, None, None)
+    assert q4(fmt=2) == 7 and q4(codes=None) == 1 and q4(scales=None) == 1 and q4(row=None) == 1 and q4(C=80) == 3 and q4(scales=p + 4) == 3
     assert lib.pq_group_norm_workspace_bytes(1, 4, 64, 8) >= 64 and lib.pq_group_norm_workspace_bytes(0, 4, 64, 8) == 0
