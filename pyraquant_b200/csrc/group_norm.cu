@@ -28,8 +28,9 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxC = 8192;
 constexpr int kSegments = 8;
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 8;
 constexpr int kSmemMax = 232448;
+constexpr int kPartsPerLane = 8;                  // chunks of a sample: at most 256
 
 enum Mode { kOut16 = 0, kInt8 = 1, kMx = 2, kNv = 3 };
 
@@ -44,6 +45,7 @@ struct NormArgs {
   int32_t* status;
   int B, T, C, groups, P, silu;
   int cap;                                          // rows a CTA keeps in shared memory
+  int chunk, longer;                                // rows per chunk; the first `longer` chunks have one more
   float eps;
 };
 
@@ -56,7 +58,6 @@ __host__ __device__ __forceinline__ Lanes lanes_of(int C) {
   l.R = kThreads / l.cols;
   return l;
 }
-__host__ __device__ __forceinline__ int chunk_begin(int T, int P, int p) { return static_cast<int>(static_cast<int64_t>(T) * p / P); }
 
 // shared memory: rows, then per-thread sums [R][C], group statistics [2][groups], row maxima, barriers
 struct NormSmem {
@@ -78,7 +79,29 @@ __device__ __forceinline__ float affine_at(const void* v, int c, int f32, float 
   if (f32) return static_cast<const float*>(v)[c];
   return lo_f32(static_cast<const unsigned short*>(v)[c], T{});
 }
-__device__ __forceinline__ float silu(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
+// c / cpg for 0 <= c < 8192: (c + 1/2) / cpg is at least 1 / (2 cpg) away from an integer and its rounding error below
+// c / cpg * 2^-22, which is less as long as C < 2^21
+__device__ __forceinline__ int group_of(int c, float inv_cpg) { return static_cast<int>((static_cast<float>(c) + 0.5f) * inv_cpg); }
+
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// z * sigmoid(z) for four values with one reciprocal: with E = exp(-|z|) in [0, 1] the sigmoid is 1 / (1 + E) or E / (1 + E), and the
+// product of two or four denominators stays within [1, 16].  (Two special-function operations per value, an exponential and a
+// reciprocal, bound the normalisation of bf16 rows otherwise.)
+__device__ __forceinline__ void silu4(float (&z)[8], int i) {
+  float e[4], d[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) { e[k] = __expf(-fabsf(z[i + k])); d[k] = 1.0f + e[k]; }
+  const float p01 = d[0] * d[1], p23 = d[2] * d[3];
+  const float r = rcp_approx(p01 * p23);
+  const float r01 = r * p23, r23 = r * p01;
+  const float inv[4] = {r01 * d[1], r01 * d[0], r23 * d[3], r23 * d[2]};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) z[i + k] *= (z[i + k] < 0.0f ? e[k] : 1.0f) * inv[k];
+}
 
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
@@ -142,27 +165,31 @@ __device__ __forceinline__ void put8(float* dst, F&& f) {
   *reinterpret_cast<float4*>(dst + 4) = make_float4(f(4), f(5), f(6), f(7));
 }
 
-// the normalisation of eight channels
+// The normalisation of eight channels: gamma and beta are requested before the grid barrier, the statistics come after it.
 template <typename T>
 struct Affine8 {
   float mean[8], mul[8], add[8];
-  __device__ __forceinline__ Affine8(const NormArgs& a, const float* stat, int c0, int cpg) {
+  __device__ __forceinline__ void request(const NormArgs& a, int c0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = c0 + i, g = c / cpg;
+      mul[i] = affine_at<T>(a.gamma, c0 + i, a.affine_f32, 1.0f);
+      add[i] = affine_at<T>(a.beta, c0 + i, a.affine_f32, 0.0f);
+    }
+  }
+  __device__ __forceinline__ void complete(const float* stat, int groups, int c0, float inv_cpg) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int g = group_of(c0 + i, inv_cpg);
       mean[i] = stat[g];
-      mul[i] = stat[a.groups + g] * affine_at<T>(a.gamma, c, a.affine_f32, 1.0f);
-      add[i] = affine_at<T>(a.beta, c, a.affine_f32, 0.0f);
+      mul[i] *= stat[groups + g];
     }
   }
   __device__ __forceinline__ uint4 operator()(const uint4& v, int with_silu) const {
     float f[8];
     unpack8<T>(v, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = fmaf(f[i] - mean[i], mul[i], add[i]);
-      if (with_silu) f[i] = silu(f[i]);
-    }
+    for (int i = 0; i < 8; ++i) f[i] = fmaf(f[i] - mean[i], mul[i], add[i]);
+    if (with_silu) { silu4(f, 0); silu4(f, 4); }
     T tag{};
     return make_uint4(pack2(f[0], f[1], tag), pack2(f[2], f[3], tag), pack2(f[4], f[5], tag), pack2(f[6], f[7], tag));
   }
@@ -174,27 +201,51 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// sums over the R x cpg entries of every group of `red`, one warp per group, in a fixed order
+// Sums over the R x cpg entries of every group of `red`, a warp for two groups at a time, in a fixed order.
 template <typename F>
-__device__ __forceinline__ void sum_groups(const float* red, int R, int C, int groups, int cpg, F&& put) {
-  const int lane = threadIdx.x & 31;
-  for (int g = static_cast<int>(threadIdx.x) >> 5; g < groups; g += kWarps) {
-    float s = 0.0f;
-    if (cpg >= 32) {
-      for (int r = 0; r < R; ++r)
-        for (int c = lane; c < cpg; c += 32) s += red[r * C + g * cpg + c];
-    } else {
-      // lanes in rows of cpg: floor(32 / cpg) rows at a time
-      const int per = 32 / cpg, r0 = lane / cpg, c = lane - r0 * cpg;
-      if (r0 < per)
-        for (int r = r0; r < R; r += per) s += red[r * C + g * cpg + c];
+__device__ __forceinline__ void sum_groups(const float* red, int R, int C, int groups, int cpg, float inv_cpg, F&& put) {
+  const int lane = threadIdx.x & 31, items = R * cpg;
+  if (items <= 128) {                                // any C whose columns nearly fill the threads, with 32 groups
+    int off[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = lane + 32 * k, r = group_of(i, inv_cpg);
+      off[k] = i < items ? r * C + i - r * cpg : -1;
     }
-    s = warp_sum(s);
-    if (lane == 0) put(g, s);
+    for (int g = static_cast<int>(threadIdx.x) >> 5; g < groups; g += 2 * kWarps) {
+      const int h = g + kWarps;
+      const float* rg = red + g * cpg;
+      const float* rh = red + h * cpg;
+      float s = 0.0f, t = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (off[k] >= 0) s += rg[off[k]];
+        if (off[k] >= 0 && h < groups) t += rh[off[k]];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); t += __shfl_xor_sync(0xffffffffu, t, o); }
+      if (lane == 0) put(g, s);
+      if (lane == 1 && h < groups) put(h, t);
+    }
+  } else {
+    for (int g = static_cast<int>(threadIdx.x) >> 5; g < groups; g += kWarps) {
+      float s = 0.0f;
+      if (cpg >= 32) {
+        for (int r = 0; r < R; ++r)
+          for (int c = lane; c < cpg; c += 32) s += red[r * C + g * cpg + c];
+      } else {
+        const int per = 32 / cpg, r0 = lane / cpg, c = lane - r0 * cpg;      // floor(32 / cpg) rows at a time
+        if (r0 < per)
+          for (int r = r0; r < R; r += per) s += red[r * C + g * cpg + c];
+      }
+      s = warp_sum(s);
+      if (lane == 0) put(g, s);
+    }
   }
 }
 
-template <typename T, int MODE>
+// COLS: columns of eight channels per thread, two only for C > 4096
+template <typename T, int MODE, int COLS>
 __global__ void __launch_bounds__(kThreads, 1)
 pq_group_norm_kernel(const NormArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -208,19 +259,20 @@ pq_group_norm_kernel(const NormArgs a) {
   const uint32_t rows_s = smem_u32(smem);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int p = static_cast<int>(blockIdx.x) % a.P;
-  const int r0 = chunk_begin(a.T, a.P, p), rows = chunk_begin(a.T, a.P, p + 1) - r0;
+  const int r0 = p * a.chunk + (p < a.longer ? p : a.longer), rows = a.chunk + (p < a.longer ? 1 : 0);
   const int resident = rows < a.cap ? rows : a.cap;
   const int seg_rows = (resident + kSegments - 1) / kSegments > 0 ? (resident + kSegments - 1) / kSegments : 1;
   const int cpg = a.C / a.groups;
+  const float inv_cpg = 1.0f / static_cast<float>(cpg);
   const int rl = tid / l.cols, col0 = tid - rl * l.cols;
   const int row_bytes = a.C * 2;
 
-  if (tid == 0) {
-    for (int s = 0; s < kSegments; ++s) mbar_init(&bars[s], 1);
+  if (tid < kSegments) {
+    mbar_init(&bars[tid], 1);
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  __syncthreads();
+  __syncwarp();
 
   uint32_t phase = 0;
 #pragma unroll 1
@@ -228,27 +280,25 @@ pq_group_norm_kernel(const NormArgs a) {
     const T* xb = static_cast<const T*>(a.x) + static_cast<int64_t>(b) * a.ld_batch + static_cast<int64_t>(r0) * a.ld_row;
     // ---------------------------------------------------------------- rows into shared memory
     if (warp == 0) {
-      for (int s = 0; s < kSegments; ++s) {
-        const int from = s * seg_rows < resident ? s * seg_rows : resident;
-        const int to = from + seg_rows < resident ? from + seg_rows : resident;
-        if (lane == 0) mbar_arrive_expect_tx(&bars[s], static_cast<uint32_t>((to - from) * row_bytes));
-        __syncwarp();
-        if (a.ld_row == a.C) {                                          // one piece
-          if (lane == 0 && to > from)
-            bulk_copy(rows_s + from * row_bytes, xb + static_cast<int64_t>(from) * a.C, static_cast<uint32_t>((to - from) * row_bytes), &bars[s]);
-        } else {
-          for (int r = from + lane; r < to; r += 32)
-            bulk_copy(rows_s + r * row_bytes, xb + static_cast<int64_t>(r) * a.ld_row, static_cast<uint32_t>(row_bytes), &bars[s]);
-        }
+      if (lane < kSegments) {
+        const int from = min(lane * seg_rows, resident), to = min(from + seg_rows, resident);
+        mbar_arrive_expect_tx(&bars[lane], static_cast<uint32_t>((to - from) * row_bytes));
+        if (a.ld_row == a.C && to > from)                               // contiguous: one piece a segment
+          bulk_copy(rows_s + from * row_bytes, xb + static_cast<int64_t>(from) * a.C, static_cast<uint32_t>((to - from) * row_bytes), &bars[lane]);
       }
+      __syncwarp();
+      if (a.ld_row != a.C)
+        for (int r = lane; r < resident; r += 32)
+          bulk_copy(rows_s + r * row_bytes, xb + static_cast<int64_t>(r) * a.ld_row, static_cast<uint32_t>(row_bytes), &bars[r / seg_rows]);
     }
     if (MODE != kOut16)
       for (int r = tid; r < resident; r += kThreads) amax[r] = 0u;
+    __syncthreads();                                                     // barriers and row maxima are there
 
     // ---------------------------------------------------------------- statistics of the chunk
-    ColumnSums cs[2];                                                    // two columns a thread only for C > 4096
+    ColumnSums cs[COLS];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < COLS; ++k) {
       cs[k].clear();
       const int col = col0 + k * l.cols;
       if (rl < l.R && col < l.ncol) {
@@ -277,20 +327,23 @@ pq_group_norm_kernel(const NormArgs a) {
     }
     __syncthreads();
     const float count = static_cast<float>(rows) * static_cast<float>(cpg);
-    sum_groups(red, l.R, a.C, a.groups, cpg, [&](int g, float s) { stat[g] = s / count; });
+    sum_groups(red, l.R, a.C, a.groups, cpg, inv_cpg, [&](int g, float s) { stat[g] = s / count; });
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < COLS; ++k) {
       const int col = col0 + k * l.cols;
       if (rl < l.R && col < l.ncol)
         put8(red + rl * a.C + col * 8, [&](int i) {
-          const float d = cs[k].mean(i) - stat[(col * 8 + i) / cpg];
+          const float d = cs[k].mean(i) - stat[group_of(col * 8 + i, inv_cpg)];
           return fmaf(d * d, cs[k].count, cs[k].m2(i));
         });
     }
     __syncthreads();
-    sum_groups(red, l.R, a.C, a.groups, cpg, [&](int g, float s) { stat[a.groups + g] = s; });
+    sum_groups(red, l.R, a.C, a.groups, cpg, inv_cpg, [&](int g, float s) { stat[a.groups + g] = s; });
     __syncthreads();
+
+    Affine8<T> f;
+    if (rl < l.R) f.request(a, col0 * 8);
 
     // ---------------------------------------------------------------- statistics of the sample
     if (a.P > 1) {
@@ -298,17 +351,21 @@ pq_group_norm_kernel(const NormArgs a) {
         a.part[(static_cast<int64_t>(b) * a.groups + g) * a.P + p] = make_float2(stat[g], stat[a.groups + g]);
       cooperative_groups::this_grid().sync();
       const float total = static_cast<float>(a.T) * static_cast<float>(cpg);
+      const float n_long = static_cast<float>((a.chunk + 1) * cpg), n_short = static_cast<float>(a.chunk * cpg);
       for (int g = warp; g < a.groups; g += kWarps) {
         const float2* part = a.part + (static_cast<int64_t>(b) * a.groups + g) * a.P;
+        float2 v[kPartsPerLane];
+#pragma unroll
+        for (int k = 0; k < kPartsPerLane; ++k) v[k] = lane + 32 * k < a.P ? __ldcg(part + lane + 32 * k) : make_float2(0.0f, 0.0f);
         float s = 0.0f;
-        for (int i = lane; i < a.P; i += 32)
-          s += __ldcg(part + i).x * (static_cast<float>(chunk_begin(a.T, a.P, i + 1) - chunk_begin(a.T, a.P, i)) * static_cast<float>(cpg));
+#pragma unroll
+        for (int k = 0; k < kPartsPerLane; ++k) s = fmaf(v[k].x, lane + 32 * k < a.longer ? n_long : n_short, s);
         const float mean = warp_sum(s) / total;
         float m2 = 0.0f;
-        for (int i = lane; i < a.P; i += 32) {
-          const float2 v = __ldcg(part + i);
-          const float d = v.x - mean, n = static_cast<float>(chunk_begin(a.T, a.P, i + 1) - chunk_begin(a.T, a.P, i)) * static_cast<float>(cpg);
-          m2 += fmaf(d * d, n, v.y);
+#pragma unroll
+        for (int k = 0; k < kPartsPerLane; ++k) {
+          const float d = v[k].x - mean;
+          if (lane + 32 * k < a.P) m2 += fmaf(d * d, lane + 32 * k < a.longer ? n_long : n_short, v[k].y);
         }
         m2 = warp_sum(m2);
         if (lane == 0) { stat[g] = mean; stat[a.groups + g] = 1.0f / sqrtf(m2 / total + a.eps); }
@@ -320,10 +377,13 @@ pq_group_norm_kernel(const NormArgs a) {
 
     // ---------------------------------------------------------------- normalisation
     const int64_t out0 = static_cast<int64_t>(b) * a.out_batch + static_cast<int64_t>(r0) * a.out_row;
-    if constexpr (MODE == kOut16) {
 #pragma unroll 1
-      for (int col = col0; rl < l.R && col < l.ncol; col += l.cols) {
-        const Affine8<T> f(a, stat, col * 8, cpg);
+    for (int k = 0; k < COLS; ++k) {
+      const int col = col0 + k * l.cols;
+      if (rl >= l.R || col >= l.ncol) break;
+      if (k > 0) f.request(a, col * 8);
+      f.complete(stat, a.groups, col * 8, inv_cpg);
+      if constexpr (MODE == kOut16) {
         const T* xc = xb + col * 8;
         T* oc = static_cast<T*>(a.out) + out0 + col * 8;
         const int far = rows - resident;                                  // rows to read again, the last ones first
@@ -336,16 +396,26 @@ pq_group_norm_kernel(const NormArgs a) {
           for (int u = 0; u < kUnroll; ++u)
             if (r + u * l.R < far) st_v4_cs(oc + static_cast<int64_t>(rows - 1 - r - u * l.R) * a.out_row, f(v[u], a.silu));
         }
+#pragma unroll 2
         for (int r = rl; r < resident; r += l.R)
           st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, f(ld_shared_v4(rows_s + r * row_bytes + col * 16), a.silu));
+      } else {
+#pragma unroll 2
+        for (int r = rl; r < rows; r += l.R) {
+          const uint32_t at = rows_s + r * row_bytes + col * 16;
+          const uint4 z = f(ld_shared_v4(at), a.silu);
+          st_shared_v4(at, z);
+          if (a.out != nullptr) st_v4(static_cast<T*>(a.out) + out0 + static_cast<int64_t>(r) * a.out_row + col * 8, z);
+        }
       }
-    } else {
+    }
+    if constexpr (MODE != kOut16) {
+      __syncthreads();
       // a thread has a fixed column of 16 channels and every R2-th row
       const int nch = a.C >> 4, R2 = kThreads / nch;
       const int r2 = tid / nch, ci = tid - r2 * nch;
       const bool active = r2 < R2;
-      {
-        const Affine8<T> f0(a, stat, active ? ci * 16 : 0, cpg), f1(a, stat, active ? ci * 16 + 8 : 0, cpg);
+      if constexpr (MODE != kMx) {
 #pragma unroll 1
         for (int rb = 0; rb < rows; rb += R2) {
           const int r = rb + r2;
@@ -353,24 +423,16 @@ pq_group_norm_kernel(const NormArgs a) {
           uint32_t m = 0u;
           if (ok) {
             const uint32_t at = rows_s + r * row_bytes + ci * 32;
-            const uint4 z0 = f0(ld_shared_v4(at), a.silu), z1 = f1(ld_shared_v4(at + 16), a.silu);
-            st_shared_v4(at, z0); st_shared_v4(at + 16, z1);
-            if (a.out != nullptr) {
-              T* o = static_cast<T*>(a.out) + out0 + static_cast<int64_t>(r) * a.out_row + ci * 16;
-              st_v4(o, z0); st_v4(o + 8, z1);
-            }
-            m = max_pattern(absmax_chunk<T>(absmax_chunk<T>(0u, z0), z1));
+            m = max_pattern(absmax_chunk<T>(absmax_chunk<T>(0u, ld_shared_v4(at)), ld_shared_v4(at + 16)));
           }
-          if constexpr (MODE != kMx) {
-            // lanes of one row first, as far as rows divide into equal shares of lanes
-            int share = 1;
-            if ((nch & 1) == 0) { m = max(m, __shfl_xor_sync(0xffffffffu, m, 1)); share = 2; }
-            if ((nch & 3) == 0) { m = max(m, __shfl_xor_sync(0xffffffffu, m, 2)); share = 4; }
-            if (ok && (tid & (share - 1)) == 0) atomicMax(&amax[r], m);
-          }
+          // lanes of one row first, as far as rows divide into equal shares of lanes
+          int share = 1;
+          if ((nch & 1) == 0) { m = max(m, __shfl_xor_sync(0xffffffffu, m, 1)); share = 2; }
+          if ((nch & 3) == 0) { m = max(m, __shfl_xor_sync(0xffffffffu, m, 2)); share = 4; }
+          if (ok && (tid & (share - 1)) == 0) atomicMax(&amax[r], m);
         }
+        __syncthreads();
       }
-      __syncthreads();
       const int64_t tiles = MODE == kInt8 ? 0 : fp4_scale_tiles(a.C, MODE == kMx ? PQ_FP4_MX : PQ_FP4_NV);
 #pragma unroll 1
       for (int rb = 0; rb < rows; rb += R2) {
@@ -428,10 +490,11 @@ int chunks_of(int B, int T, int C) {
   int P = sm_count() / B;
   const int most = (T + l.R - 1) / l.R;
   if (P > most) P = most;
+  if (P > 32 * kPartsPerLane) P = 32 * kPartsPerLane;
   return P < 1 ? 1 : P;
 }
 
-template <typename T, int MODE>
+template <typename T, int MODE, int COLS>
 int launch_norm(NormArgs a, cudaStream_t st) {
   const int longest = (a.T + a.P - 1) / a.P;
   const int fixed = smem_of(a.C, a.groups, 0).total + 256;
@@ -440,9 +503,10 @@ int launch_norm(NormArgs a, cudaStream_t st) {
   if (cap < 0) return PQ_ERR_UNSUPPORTED;
   if (MODE != kOut16 && cap < longest) return PQ_ERR_UNSUPPORTED;          // the rows do not fit on the chip
   a.cap = cap;
+  a.chunk = a.T / a.P; a.longer = a.T % a.P;
   const NormSmem lay = smem_of(a.C, a.groups, cap);
   if (lay.total > kSmemMax) return PQ_ERR_UNSUPPORTED;
-  auto kern = pq_group_norm_kernel<T, MODE>;
+  auto kern = pq_group_norm_kernel<T, MODE, COLS>;
   static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes
   int dev = 0;
   PQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -490,7 +554,9 @@ int group_norm_any(const void* x, int dtype, int64_t B, int64_t T, int64_t C, in
   a.B = static_cast<int>(B); a.T = static_cast<int>(T); a.C = static_cast<int>(C); a.groups = groups;
   a.P = chunks_of(a.B, a.T, a.C); a.silu = act == PQ_ACT_SILU; a.eps = eps;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == PQ_DTYPE_BF16 ? launch_norm<__nv_bfloat16, MODE>(a, st) : launch_norm<__half, MODE>(a, st);
+  if (lanes_of(a.C).ncol > kThreads)
+    return dtype == PQ_DTYPE_BF16 ? launch_norm<__nv_bfloat16, MODE, 2>(a, st) : launch_norm<__half, MODE, 2>(a, st);
+  return dtype == PQ_DTYPE_BF16 ? launch_norm<__nv_bfloat16, MODE, 1>(a, st) : launch_norm<__half, MODE, 1>(a, st);
 }
 
 }  // namespace
