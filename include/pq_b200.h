@@ -118,7 +118,7 @@ int pq_adaln_quant_rows(const void* x, int dtype, int64_t M, int64_t K, int64_t 
  * mean and variance over the T rows and C / groups channels of a group; fp32 throughout, rounded once.
  *   x [B,T,C] with strides ld_batch, ld_row, 1 (elements); out likewise; gamma, beta [C] in x's type, or fp32 when
  *   affine_fp32 is set, each NULL for 1 and 0; C % 8 == 0, C <= 8192, C % groups == 0, B <= 65535, strides % 8 == 0,
- *   16-byte aligned x and out; workspace: pq_group_norm_workspace_bytes (same B, T, C, groups, current device), 8-byte
+ *   16-byte aligned x, out, gamma and beta; workspace: pq_group_norm_workspace_bytes (same B, T, C, groups, current device), 8-byte
  *   aligned; status: NULL or a status word as in the GEMMs' workspace.  B == 0 or T == 0 is a no-op.
  * One launch, cooperative when a sample is shared by several CTAs. */
 #define PQ_ACT_NONE 0

@@ -34,21 +34,6 @@ constexpr int kPartsPerLane = 8;                  // chunks of a sample: at most
 
 enum Mode { kOut16 = 0, kInt8 = 1, kMx = 2, kNv = 3 };
 
-struct NormArgs {
-  const void* x; int64_t ld_row, ld_batch;         // elements
-  const void* gamma; const void* beta; int affine_f32;
-  void* out; int64_t out_row, out_batch;            // z (NULL: not wanted)
-  uint8_t* codes;                                   // INT8 [B T, C] or packed E2M1 [B T, C / 2]
-  uint8_t* scales;                                  // 4-bit: scale tiles
-  float* row_scale;                                 // INT8, nv
-  float2* part;                                     // [B][groups][P] mean, M2
-  int32_t* status;
-  int B, T, C, groups, P, silu;
-  int cap;                                          // rows a CTA keeps in shared memory
-  int chunk, longer;                                // rows per chunk; the first `longer` chunks have one more
-  float eps;
-};
-
 // threads over the columns of eight channels: `cols` a pass, R rows side by side
 struct Lanes { int ncol, cols, R; };
 __host__ __device__ __forceinline__ Lanes lanes_of(int C) {
@@ -73,12 +58,26 @@ __host__ __device__ __forceinline__ NormSmem smem_of(int C, int groups, int cap)
   return s;
 }
 
-template <typename T>
-__device__ __forceinline__ float affine_at(const void* v, int c, int f32, float none) {
-  if (v == nullptr) return none;
-  if (f32) return static_cast<const float*>(v)[c];
-  return lo_f32(static_cast<const unsigned short*>(v)[c], T{});
-}
+struct NormArgs {
+  const void* x; int64_t ld_row, ld_batch;         // elements
+  const void* gamma; const void* beta; int affine_f32;
+  void* out; int64_t out_row, out_batch;            // z (NULL: not wanted)
+  uint8_t* codes;                                   // INT8 [B T, C] or packed E2M1 [B T, C / 2]
+  uint8_t* scales;                                  // 4-bit: scale tiles
+  float* row_scale;                                 // INT8, nv
+  float2* part;                                     // [B][groups][P] mean, M2
+  int32_t* status;
+  int B, T, C, groups, P, silu;
+  int cap;                                          // rows a CTA keeps in shared memory
+  int chunk, longer;                                // rows per chunk; the first `longer` chunks have one more
+  // what follows from the sizes, worked out on the host: a division on the way to the first copy costs a tenth of a
+  // microsecond, and there would be eight of them
+  Lanes l; NormSmem lay;
+  int cpg, nch, R2;                                 // channels per group; units of 16 channels, rows of them side by side
+  float inv_cpg, inv_cols, inv_nch;
+  float eps;
+};
+
 // c / cpg for 0 <= c < 8192: (c + 1/2) / cpg is at least 1 / (2 cpg) away from an integer and its rounding error below
 // c / cpg * 2^-22, which is less as long as C < 2^21
 __device__ __forceinline__ int group_of(int c, float inv_cpg) { return static_cast<int>((static_cast<float>(c) + 0.5f) * inv_cpg); }
@@ -88,27 +87,32 @@ __device__ __forceinline__ float rcp_approx(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// z * sigmoid(z) for four values with one reciprocal: with E = exp(-|z|) in [0, 1] the sigmoid is 1 / (1 + E) or E / (1 + E), and the
-// product of two or four denominators stays within [1, 16].  (Two special-function operations per value, an exponential and a
-// reciprocal, bound the normalisation of bf16 rows otherwise.)
-__device__ __forceinline__ void silu4(float (&z)[8], int i) {
-  float e[4], d[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) { e[k] = __expf(-fabsf(z[i + k])); d[k] = 1.0f + e[k]; }
-  const float p01 = d[0] * d[1], p23 = d[2] * d[3];
-  const float r = rcp_approx(p01 * p23);
-  const float r01 = r * p23, r23 = r * p01;
-  const float inv[4] = {r01 * d[1], r01 * d[0], r23 * d[3], r23 * d[2]};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) z[i + k] *= (z[i + k] < 0.0f ? e[k] : 1.0f) * inv[k];
+__device__ __forceinline__ float ex2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// z * sigmoid(z) for four values with one reciprocal: with E = exp(-|z|) in [0, 1] and h = E / (1 + E), it is z - z h for z >= 0
+// and z h below, max(z, 0) - |z| h in both cases; the product of four denominators stays within [1, 16].  (Two special-function
+// operations per value, an exponential and a reciprocal, bound the normalisation of bf16 rows otherwise.)
+__device__ __forceinline__ void silu4(float2 (&z)[4], int i) {
+  const float2 a0 = make_float2(fabsf(z[i].x), fabsf(z[i].y)), a1 = make_float2(fabsf(z[i + 1].x), fabsf(z[i + 1].y));
+  const float2 neg_log2e = make_float2(-1.4426950408889634f, -1.4426950408889634f), one = make_float2(1.0f, 1.0f);
+  const float2 t0 = __fmul2_rn(a0, neg_log2e), t1 = __fmul2_rn(a1, neg_log2e);
+  const float2 e0 = make_float2(ex2_approx(t0.x), ex2_approx(t0.y)), e1 = make_float2(ex2_approx(t1.x), ex2_approx(t1.y));
+  const float2 d0 = __fadd2_rn(e0, one), d1 = __fadd2_rn(e1, one);
+  const float p0 = d0.x * d0.y, p1 = d1.x * d1.y;
+  const float r = rcp_approx(p0 * p1);
+  const float r0 = r * p1, r1 = r * p0;
+  const float2 h0 = __fmul2_rn(e0, __fmul2_rn(make_float2(d0.y, d0.x), make_float2(r0, r0)));
+  const float2 h1 = __fmul2_rn(e1, __fmul2_rn(make_float2(d1.y, d1.x), make_float2(r1, r1)));
+  z[i] = __ffma2_rn(make_float2(-a0.x, -a0.y), h0, make_float2(fmaxf(z[i].x, 0.0f), fmaxf(z[i].y, 0.0f)));
+  z[i + 1] = __ffma2_rn(make_float2(-a1.x, -a1.y), h1, make_float2(fmaxf(z[i + 1].x, 0.0f), fmaxf(z[i + 1].y, 0.0f)));
 }
 
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
-  T tag{};
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { f[2 * i] = lo_f32(w[i], tag); f[2 * i + 1] = hi_f32(w[i], tag); }
+__device__ __forceinline__ void unpack8(const uint4& v, float2 (&f)[4]) {
+  f[0] = unpack2<T>(v.x); f[1] = unpack2<T>(v.y); f[2] = unpack2<T>(v.z); f[3] = unpack2<T>(v.w);
 }
 // contiguous copy global -> shared, completion bytes on a barrier of this CTA; 16-byte aligned, size % 16 == 0
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -125,37 +129,42 @@ __device__ __forceinline__ void st_shared_v4(uint32_t a, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// running sums of one column of eight channels; after finish(): means in piv, centred sums of squares in s2
+// running sums of one column of eight channels; after finish(): means in neg (negated), centred sums of squares in s2
 struct ColumnSums {
-  float piv[8], s1[8], s2[8], count;
+  float2 neg[4], s1[4], s2[4];          // -pivot, sum of x - pivot, of its square
+  float count;
   int n;
-  __device__ __forceinline__ float mean(int i) const { return piv[i]; }
-  __device__ __forceinline__ float m2(int i) const { return s2[i]; }
+  __device__ __forceinline__ float mean(int i) const { return -(i & 1 ? neg[i >> 1].y : neg[i >> 1].x); }
+  __device__ __forceinline__ float m2(int i) const { return i & 1 ? s2[i >> 1].y : s2[i >> 1].x; }
+  __device__ __forceinline__ void clear() {
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) neg[i] = s1[i] = s2[i] = make_float2(0.0f, 0.0f);
+  }
+  template <typename T>
+  __device__ __forceinline__ void add(const uint4& v) {
+    float2 f[4];
+    unpack8<T>(v, f);
+    if (n == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) neg[i] = make_float2(-f[i].x, -f[i].y);
+    }
+    ++n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 d = __fadd2_rn(f[i], neg[i]);
+      s1[i] = __fadd2_rn(s1[i], d);
+      s2[i] = __ffma2_rn(d, d, s2[i]);
+    }
+  }
   __device__ __forceinline__ void finish() {
     count = static_cast<float>(n);
     const float inv = n > 0 ? 1.0f / count : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s2[i] = fmaxf(s2[i] - s1[i] * s1[i] * inv, 0.0f);
-      piv[i] = fmaf(s1[i], inv, piv[i]);
+    for (int i = 0; i < 4; ++i) {
+      s2[i] = make_float2(fmaxf(s2[i].x - s1[i].x * s1[i].x * inv, 0.0f), fmaxf(s2[i].y - s1[i].y * s1[i].y * inv, 0.0f));
+      neg[i] = make_float2(fmaf(-s1[i].x, inv, neg[i].x), fmaf(-s1[i].y, inv, neg[i].y));
     }
-  }
-  __device__ __forceinline__ void clear() {
-    n = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) piv[i] = s1[i] = s2[i] = 0.0f;
-  }
-  template <typename T>
-  __device__ __forceinline__ void add(const uint4& v) {
-    float f[8];
-    unpack8<T>(v, f);
-    if (n == 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) piv[i] = f[i];
-    }
-    ++n;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { const float d = f[i] - piv[i]; s1[i] += d; s2[i] = fmaf(d, d, s2[i]); }
   }
 };
 
@@ -165,33 +174,55 @@ __device__ __forceinline__ void put8(float* dst, F&& f) {
   *reinterpret_cast<float4*>(dst + 4) = make_float4(f(4), f(5), f(6), f(7));
 }
 
-// The normalisation of eight channels: gamma and beta are requested before the grid barrier, the statistics come after it.
+// The normalisation of eight channels: gamma and beta are requested before the grid barrier (and left as they were loaded:
+// converting them would wait for them), the statistics come after it.
 template <typename T>
 struct Affine8 {
-  float mean[8], mul[8], add[8];
+  uint4 raw[2][2];                        // gamma, beta: eight 16-bit values in [0], or eight fp32 ones
+  float2 neg_mean[4], mul[4], add[4];
   __device__ __forceinline__ void request(const NormArgs& a, int c0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      mul[i] = affine_at<T>(a.gamma, c0 + i, a.affine_f32, 1.0f);
-      add[i] = affine_at<T>(a.beta, c0 + i, a.affine_f32, 0.0f);
+    for (int k = 0; k < 2; ++k) {
+      const void* v = k == 0 ? a.gamma : a.beta;
+      if (v == nullptr) continue;
+      if (a.affine_f32) {
+        raw[k][0] = ld_v4(static_cast<const float*>(v) + c0);
+        raw[k][1] = ld_v4(static_cast<const float*>(v) + c0 + 4);
+      } else {
+        raw[k][0] = ld_v4(static_cast<const T*>(v) + c0);
+      }
     }
   }
-  __device__ __forceinline__ void complete(const float* stat, int groups, int c0, float inv_cpg) {
+  __device__ __forceinline__ void values(const NormArgs& a, int k, float none, float2 (&o)[4]) const {
+    if ((k == 0 ? a.gamma : a.beta) == nullptr) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int g = group_of(c0 + i, inv_cpg);
-      mean[i] = stat[g];
-      mul[i] *= stat[groups + g];
+      for (int i = 0; i < 4; ++i) o[i] = make_float2(none, none);
+    } else if (a.affine_f32) {
+      const uint4 u = raw[k][0], w = raw[k][1];
+      o[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y)); o[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+      o[2] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y)); o[3] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+    } else {
+      unpack8<T>(raw[k][0], o);
+    }
+  }
+  __device__ __forceinline__ void complete(const NormArgs& a, const float* stat, int c0) {
+    values(a, 0, 1.0f, mul);
+    values(a, 1, 0.0f, add);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int g0 = group_of(c0 + 2 * i, a.inv_cpg), g1 = group_of(c0 + 2 * i + 1, a.inv_cpg);
+      neg_mean[i] = make_float2(-stat[g0], -stat[g1]);
+      mul[i] = __fmul2_rn(mul[i], make_float2(stat[a.groups + g0], stat[a.groups + g1]));
     }
   }
   __device__ __forceinline__ uint4 operator()(const uint4& v, int with_silu) const {
-    float f[8];
+    float2 f[4];
     unpack8<T>(v, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = fmaf(f[i] - mean[i], mul[i], add[i]);
-    if (with_silu) { silu4(f, 0); silu4(f, 4); }
+    for (int i = 0; i < 4; ++i) f[i] = __ffma2_rn(__fadd2_rn(f[i], neg_mean[i]), mul[i], add[i]);
+    if (with_silu) { silu4(f, 0); silu4(f, 2); }
     T tag{};
-    return make_uint4(pack2(f[0], f[1], tag), pack2(f[2], f[3], tag), pack2(f[4], f[5], tag), pack2(f[6], f[7], tag));
+    return make_uint4(pack2(f[0].x, f[0].y, tag), pack2(f[1].x, f[1].y, tag), pack2(f[2].x, f[2].y, tag), pack2(f[3].x, f[3].y, tag));
   }
 };
 
@@ -250,21 +281,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 pq_group_norm_kernel(const NormArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   T tag{};
-  const Lanes l = lanes_of(a.C);
-  const NormSmem lay = smem_of(a.C, a.groups, a.cap);
+  const Lanes l = a.l;
+  const NormSmem lay = a.lay;
   float* red = reinterpret_cast<float*>(smem + lay.red);
   float* stat = reinterpret_cast<float*>(smem + lay.stat);              // mean, then 1 / sqrt(var + eps)
   uint32_t* amax = reinterpret_cast<uint32_t*>(smem + lay.amax);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lay.bars);
   const uint32_t rows_s = smem_u32(smem);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
-  const int p = static_cast<int>(blockIdx.x) % a.P;
+  const int p = static_cast<int>(blockIdx.x);
   const int r0 = p * a.chunk + (p < a.longer ? p : a.longer), rows = a.chunk + (p < a.longer ? 1 : 0);
   const int resident = rows < a.cap ? rows : a.cap;
-  const int seg_rows = (resident + kSegments - 1) / kSegments > 0 ? (resident + kSegments - 1) / kSegments : 1;
-  const int cpg = a.C / a.groups;
-  const float inv_cpg = 1.0f / static_cast<float>(cpg);
-  const int rl = tid / l.cols, col0 = tid - rl * l.cols;
+  const int seg_rows = max((resident + kSegments - 1) / kSegments, 1);
+  const int cpg = a.cpg;
+  const float inv_cpg = a.inv_cpg;
+  const int rl = group_of(tid, a.inv_cols), col0 = tid - rl * l.cols;
   const int row_bytes = a.C * 2;
 
   if (tid < kSegments) {
@@ -276,7 +307,7 @@ pq_group_norm_kernel(const NormArgs a) {
 
   uint32_t phase = 0;
 #pragma unroll 1
-  for (int b = static_cast<int>(blockIdx.x) / a.P; b < a.B; b += static_cast<int>(gridDim.x) / a.P, phase ^= 1u) {
+  for (int b = static_cast<int>(blockIdx.y); b < a.B; b += static_cast<int>(gridDim.y), phase ^= 1u) {
     const T* xb = static_cast<const T*>(a.x) + static_cast<int64_t>(b) * a.ld_batch + static_cast<int64_t>(r0) * a.ld_row;
     // ---------------------------------------------------------------- rows into shared memory
     if (warp == 0) {
@@ -382,7 +413,7 @@ pq_group_norm_kernel(const NormArgs a) {
       const int col = col0 + k * l.cols;
       if (rl >= l.R || col >= l.ncol) break;
       if (k > 0) f.request(a, col * 8);
-      f.complete(stat, a.groups, col * 8, inv_cpg);
+      f.complete(a, stat, col * 8);
       if constexpr (MODE == kOut16) {
         const T* xc = xb + col * 8;
         T* oc = static_cast<T*>(a.out) + out0 + col * 8;
@@ -412,8 +443,8 @@ pq_group_norm_kernel(const NormArgs a) {
     if constexpr (MODE != kOut16) {
       __syncthreads();
       // a thread has a fixed column of 16 channels and every R2-th row
-      const int nch = a.C >> 4, R2 = kThreads / nch;
-      const int r2 = tid / nch, ci = tid - r2 * nch;
+      const int nch = a.nch, R2 = a.R2;
+      const int r2 = group_of(tid, a.inv_nch), ci = tid - r2 * nch;
       const bool active = r2 < R2;
       if constexpr (MODE != kMx) {
 #pragma unroll 1
@@ -504,8 +535,12 @@ int launch_norm(NormArgs a, cudaStream_t st) {
   if (MODE != kOut16 && cap < longest) return PQ_ERR_UNSUPPORTED;          // the rows do not fit on the chip
   a.cap = cap;
   a.chunk = a.T / a.P; a.longer = a.T % a.P;
-  const NormSmem lay = smem_of(a.C, a.groups, cap);
-  if (lay.total > kSmemMax) return PQ_ERR_UNSUPPORTED;
+  a.l = lanes_of(a.C);
+  a.lay = smem_of(a.C, a.groups, cap);
+  if (a.lay.total > kSmemMax) return PQ_ERR_UNSUPPORTED;
+  a.cpg = a.C / a.groups; a.inv_cpg = 1.0f / static_cast<float>(a.cpg);
+  a.inv_cols = 1.0f / static_cast<float>(a.l.cols);
+  a.nch = a.C >> 4; a.R2 = a.nch > 0 ? kThreads / a.nch : 0; a.inv_nch = a.nch > 0 ? 1.0f / static_cast<float>(a.nch) : 0.0f;
   auto kern = pq_group_norm_kernel<T, MODE, COLS>;
   static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes
   int dev = 0;
@@ -516,9 +551,9 @@ int launch_norm(NormArgs a, cudaStream_t st) {
   }
   const int sms = sm_count();
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.P * (a.B < sms ? a.B : sms)));
+  cfg.gridDim = dim3(static_cast<unsigned>(a.P), static_cast<unsigned>(a.B < sms ? a.B : sms));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(lay.total);
+  cfg.dynamicSmemBytes = static_cast<size_t>(a.lay.total);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeCooperative;
@@ -543,8 +578,7 @@ int group_norm_any(const void* x, int dtype, int64_t B, int64_t T, int64_t C, in
   if (MODE != kOut16 && (codes == nullptr || (MODE != kMx && row_scale == nullptr) || (MODE >= kMx && scales == nullptr))) return PQ_ERR_NULL;
   if (C % (MODE == kOut16 ? 8 : (MODE == kInt8 ? 16 : 32)) != 0 || ld_row % 8 != 0 || ld_batch % 8 != 0) return PQ_ERR_ALIGN;
   if (out != nullptr && (ldo_row % 8 != 0 || ldo_batch % 8 != 0 || !aligned_to(out, 16))) return PQ_ERR_ALIGN;
-  if (!aligned_to(x, 16) || !aligned_to(workspace, 8) || !aligned_to(gamma, affine_fp32 ? 4 : 2) ||
-      !aligned_to(beta, affine_fp32 ? 4 : 2) || !aligned_to(codes, 16) || !aligned_to(scales, 16) || !aligned_to(row_scale, 4))
+  if (!aligned_to(x, 16) || !aligned_to(workspace, 8) || !aligned_to(gamma, 16) || !aligned_to(beta, 16) || !aligned_to(codes, 16) || !aligned_to(scales, 16) || !aligned_to(row_scale, 4))
     return PQ_ERR_ALIGN;
   if (ws_bytes < pq_group_norm_workspace_bytes(B, T, C, groups)) return PQ_ERR_WORKSPACE;
   NormArgs a{};

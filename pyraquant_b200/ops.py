@@ -221,6 +221,13 @@ GROUP_NORM_ACTS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU}
 GROUP_NORM_MAX_C = 8192
 
 
+def _affine_vector(v: Optional[Tensor]) -> Optional[Tensor]:
+    """A contiguous vector that starts on a 16-byte border."""
+    if v is None or (v.dim() == 1 and v.is_contiguous() and v.data_ptr() % 16 == 0):
+        return v
+    return v.reshape(-1).clone(memory_format=torch.contiguous_format)
+
+
 def group_norm_args(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], act: Optional[str]):
     """Checks a group norm's operands; returns x as [B, T, C] with rows the kernels take, the affine vectors (both fp32 or both in
     x's type) and the activation's code."""
@@ -238,8 +245,7 @@ def group_norm_args(x: Tensor, groups: int, weight: Optional[Tensor], bias: Opti
             "weight and bias: one entry per channel, in the activation type or fp32, on the same device"
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         weight, bias = weight.float(), bias.float()
-    weight = None if weight is None else weight.reshape(-1).contiguous()
-    bias = None if bias is None else bias.reshape(-1).contiguous()
+    weight, bias = _affine_vector(weight), _affine_vector(bias)
     T = 1
     for n in x.shape[1:-1]:
         T *= n

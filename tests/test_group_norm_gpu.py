@@ -4,7 +4,9 @@ Bound.  A thread sums at most L rows of x - pivot one after the other (L <= 64 f
 follow: the mean is off by at most (L + 64) 2^-24 mean|x - pivot|, with |x - pivot| taken as at most 8 deviations, plus
 one rounding of its own size, 2^-24 |mean| a few times over; the variance likewise, relative to itself.  So x-hat is off by
 A (1 + |x-hat|) + 4 2^-24 |mean| / std with A = 128 * 8 * 2^-24.  gamma multiplies that, SiLU's slope is at most 1.1 and its own
-evaluation loses (4 + |z|) 2^-23 of its value (exp's argument rounds, exp and the quotient a few units each).  The
+evaluation, max(z, 0) - |z| h with h = E / (1 + E), E = exp(-|z|) and one reciprocal for four denominators, loses (in units of
+2^-24): |z| (E's argument rounds) + 4 (exponential) in E, 1 in each denominator that does not cancel, 2 in the reciprocal, 6 in
+the products around it, 1 in the sum: (14 + |z|) 2^-24 of |z| h, which is the value below 0 and at most the value above.  The
 rounding to 16 bits is eps / 2 of the value or half the smallest subnormal.
 """
 import ctypes
@@ -34,7 +36,7 @@ def formula(x, groups, w, b, eps, act):
     z = xh.reshape(B, T, C) * w + b
     err = err.reshape(B, T, C) * w.abs() + 2.0 ** -23 * (z.abs() + b.abs())
     if act == "silu":
-        z, err = z / (1 + torch.exp(-z)), 1.1 * err + (4 + z.abs()) * 2.0 ** -23 * (z / (1 + torch.exp(-z))).abs()
+        z, err = z / (1 + torch.exp(-z)), 1.1 * err + (14 + z.abs()) * 2.0 ** -24 * (z / (1 + torch.exp(-z))).abs()
     return z, err
 
 
@@ -101,6 +103,10 @@ def test_layouts(cuda_dev):
     assert torch.equal(norm_exec.group_norm_rows(x.transpose(1, 2).contiguous().transpose(1, 2), 32, w, b), want)
     assert norm_exec.group_norm_rows(x[:0], 32, w, b).shape == (0, 64, 320)
     assert norm_exec.group_norm_rows(x[:, :0], 32, w, b).shape == (3, 0, 320)
+    odd = torch.randn(700, device=cuda_dev).to(torch.bfloat16)
+    odd[3:323], odd[323:643] = w, b                                # affine vectors off 16-byte borders, and strided ones
+    assert torch.equal(norm_exec.group_norm_rows(x, 32, odd[3:323], odd[323:643]), want)
+    assert torch.equal(norm_exec.group_norm_rows(x, 32, torch.stack([w, b], 1)[:, 0], torch.stack([w, b], 1)[:, 1]), want)
     flat = torch.randn(5, 64, device=cuda_dev).to(torch.float16)   # [B, C]: one row per sample
     assert torch.equal(norm_exec.group_norm_rows(flat, 4), norm_exec.group_norm_rows(flat[:, None], 4)[:, 0])
 
@@ -258,7 +264,7 @@ def test_argument_checks():
     assert gn(B=-1) == 2 and gn(C=0) == 2 and gn(groups=0) == 2 and gn(groups=7) == 2 and gn(row=56) == 2 and gn(eps=-1.0) == 2
     assert gn(eps=float("nan")) == 2 and gn(C=8200, row=8200, orow=8200) == 2 and gn(B=65536) == 2
     assert gn(C=60, groups=4) == 3 and gn(row=68) == 3 and gn(batch=257) == 3 and gn(x=p + 8) == 3 and gn(out=p + 2) == 3 and gn(ws=p + 4) == 3
-    assert gn(w=p + 1) == 3 and gn(b=p + 2, f32=1) == 3
+    assert gn(w=p + 2) == 3 and gn(b=p + 8, f32=1) == 3
     assert gn(dtype=2) == 4 and gn(act=2) == 7 and gn(wsb=0) == 8
 
     def q8(C=64, z=None, q=p, s=p, x=p):
