@@ -101,8 +101,15 @@ __device__ __forceinline__ float nv_row_scale(float amax) {
   return __int_as_float(bits == 0 ? 0x3F800000 : e << 23);
 }
 
-// Multiplier and divisor of one block.  code = e2m1(x / div): the quotient is estimated with the rounded reciprocal and
-// corrected once, which gives exact quotients exactly (ties must stay ties).  div == 0 marks a block of zero codes.
+// Multiplier and divisor of one block.  code = e2m1(x / div): the quotient is estimated with the approximate reciprocal and
+// corrected once.  With inv = (1 + e') / div and q0 = (1 + e) x / div, the corrected value is (1 - e e') x / div, e and e' below
+// 2^-21, before its rounding: quotients that fp32 holds, the ties among them, come out exactly.  div == 0 marks a block of
+// zero codes.
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 struct BlockScale { uint32_t byte; float inv, div; };
 __device__ __forceinline__ BlockScale mx_block_scale(float amax) {
   BlockScale b;
@@ -121,16 +128,17 @@ __device__ __forceinline__ BlockScale nv_block_scale(float amax, float s_row, bo
   const float v = __fmaf_rn(__fmaf_rn(-q0, 6.0f, t), r6, q0);
   b.byte = bad_row ? 0u : e4m3_of(v);
   b.div = e4m3_value(b.byte) * s_row;
-  b.inv = __frcp_rn(b.div);
+  b.inv = rcp_approx(b.div);
   if (bad_row) b.div = 0.0f;
   return b;
 }
 
 template <int FMT>
-__device__ __forceinline__ float e2m1_quotient(float x, const BlockScale& b) {
-  const float q0 = __fmul_rn(x, b.inv);
+__device__ __forceinline__ float2 e2m1_quotient(float2 x, const BlockScale& b) {
+  const float2 inv = make_float2(b.inv, b.inv);
+  const float2 q0 = __fmul2_rn(x, inv);
   if constexpr (FMT == PQ_FP4_MX) return q0;
-  return __fmaf_rn(__fmaf_rn(-q0, b.div, x), b.inv, q0);
+  return __ffma2_rn(__ffma2_rn(q0, make_float2(-b.div, -b.div), x), inv, q0);
 }
 
 // 16 packed elements of one block (or half of an mx block) -> 8 bytes of codes
@@ -143,9 +151,9 @@ __device__ __forceinline__ uint2 quant_chunk16(const Chunk16& c, const BlockScal
     float v[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack2<T>(c.w[4 * h + i]);
-      v[2 * i] = e2m1_quotient<FMT>(f.x, b);
-      v[2 * i + 1] = e2m1_quotient<FMT>(f.y, b);
+      const float2 f = e2m1_quotient<FMT>(unpack2<T>(c.w[4 * h + i]), b);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
     }
     (h == 0 ? r.x : r.y) = pack_e2m1x8(v);
   }

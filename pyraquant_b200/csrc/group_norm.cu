@@ -82,11 +82,6 @@ struct NormArgs {
 // c / cpg * 2^-22, which is less as long as C < 2^21
 __device__ __forceinline__ int group_of(int c, float inv_cpg) { return static_cast<int>((static_cast<float>(c) + 0.5f) * inv_cpg); }
 
-__device__ __forceinline__ float rcp_approx(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float ex2_approx(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));

@@ -133,6 +133,7 @@ pq_quant_rows_fp4_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restri
 __device__ __forceinline__ float finite16(float v, __half) { return v > 65504.0f ? 65504.0f : (v < -65504.0f ? -65504.0f : v); }
 __device__ __forceinline__ float finite16(float v, __nv_bfloat16) { return v; }
 
+// A thread turns units of 16 codes (8 bytes and a scale byte) into one 32-byte store each, five units at a time.
 template <typename T, int FMT, int TPR>
 __global__ void __launch_bounds__(kThreads)
 pq_dequant_rows_fp4_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
@@ -143,29 +144,44 @@ pq_dequant_rows_fp4_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
   if (row >= M) return;
   const int nchunk = K >> 4;
-  const int64_t tiles = fp4_scale_tiles(K, FMT);
-  const float s_row = FMT == PQ_FP4_NV ? row_scale[row] : 1.0f;
+  const uint8_t* srow = scales + fp4_scale_off(row, 0, fp4_scale_tiles(K, FMT));
+  const float s_row = FMT == PQ_FP4_NV ? __ldg(row_scale + row) : 1.0f;
   const uint8_t* crow = codes + row * ldc;
   T* orow = out + row * ldo;
-  for (int c = lane; c < nchunk; c += TPR) {
-    const int blk = FMT == PQ_FP4_MX ? c >> 1 : c;
-    const uint32_t byte = scales[fp4_scale_off(row, blk >> 2, tiles) + (blk & 3)];
-    const uint2 w = *reinterpret_cast<const uint2*>(crow + static_cast<int64_t>(c) * 8);
-    float s;
-    if constexpr (FMT == PQ_FP4_MX)                        // 2^(byte - 127); 2^-127 is subnormal, 255 is NaN
-      s = __int_as_float(byte == 255u ? 0x7FC00000 : (byte == 0u ? 0x00400000 : static_cast<int>(byte) << 23));
-    else
-      s = e4m3_value(byte) * s_row;
-    Chunk16 o;
+  for (int c0 = lane; c0 < nchunk; c0 += kUnits * TPR) {
+    uint2 w[kUnits];
+    uint32_t byte[kUnits];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t v[4];
-      unpack_e2m1x8(h == 0 ? w.x : w.y, v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o.w[4 * h + i] = pack2(finite16(lo_f32(v[i], __half{}) * s, tag), finite16(hi_f32(v[i], __half{}) * s, tag), tag);
+    for (int j = 0; j < kUnits; ++j) {
+      const int c = c0 + j * TPR;
+      if (c < nchunk) {
+        const int blk = FMT == PQ_FP4_MX ? c >> 1 : c;
+        w[j] = __ldg(reinterpret_cast<const uint2*>(crow + static_cast<int64_t>(c) * 8));
+        byte[j] = __ldg(srow + (blk >> 2) * 512 + (blk & 3));
+      }
     }
-    st_chunk16(orow + static_cast<int64_t>(c) * 16, o);
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j) {
+      const int c = c0 + j * TPR;
+      if (c >= nchunk) break;
+      float s;
+      if constexpr (FMT == PQ_FP4_MX)                      // 2^(byte - 127); 2^-127 is subnormal, 255 is NaN
+        s = __int_as_float(byte[j] == 255u ? 0x7FC00000 : (byte[j] == 0u ? 0x00400000 : static_cast<int>(byte[j]) << 23));
+      else
+        s = e4m3_value(byte[j]) * s_row;
+      Chunk16 o;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[4];
+        unpack_e2m1x8(h == 0 ? w[j].x : w[j].y, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __fmul2_rn(unpack2<__half>(v[i]), make_float2(s, s));
+          o.w[4 * h + i] = pack2(finite16(f.x, tag), finite16(f.y, tag), tag);
+        }
+      }
+      st_chunk16(orow + static_cast<int64_t>(c) * 16, o);
+    }
   }
 }
 
@@ -212,9 +228,10 @@ template <typename T, int FMT>
 int dispatch_dequant(const void* codes, int64_t ldc, const void* scales, const float* row_scale, void* out, int64_t ldo,
                      int64_t M, int K, cudaStream_t st) {
   const int n = K >> 4;
-  if (n <= 16) return launch_dequant<T, FMT, 8>(codes, ldc, scales, row_scale, out, ldo, M, K, st);
-  if (n <= 128) return launch_dequant<T, FMT, 32>(codes, ldc, scales, row_scale, out, ldo, M, K, st);
-  return launch_dequant<T, FMT, 128>(codes, ldc, scales, row_scale, out, ldo, M, K, st);
+  if (n <= 8 * kUnits) return launch_dequant<T, FMT, 8>(codes, ldc, scales, row_scale, out, ldo, M, K, st);
+  if (n <= 16 * kUnits) return launch_dequant<T, FMT, 16>(codes, ldc, scales, row_scale, out, ldo, M, K, st);
+  if (n <= 32 * kUnits) return launch_dequant<T, FMT, 32>(codes, ldc, scales, row_scale, out, ldo, M, K, st);
+  return launch_dequant<T, FMT, 64>(codes, ldc, scales, row_scale, out, ldo, M, K, st);
 }
 
 }  // namespace
