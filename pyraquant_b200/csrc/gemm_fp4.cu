@@ -3,8 +3,8 @@
 //
 // One 128 x BN tile per CTA, 192 threads: warp 0 fills a ring of {activations, weights, scales of both} stages by TMA,
 // warp 1 copies a stage's scales to tensor memory (tcgen05.cp) and issues its four MMAs, warps 2-5 scale, add the bias
-// and store.  Two sets of scale columns alternate; a set is written again only after the MMAs that read it have
-// completed (the commit of the stage before last).
+// and store.  Every stage has scale columns of its own, so a full stage also says that the MMAs that read them last have
+// completed (its operands could not have been overwritten otherwise).
 //   BN = 128, three stages: two CTAs share an SM, so one's epilogue overlaps the other's main loop.
 //   BN = 64, seven stages, for launches of few tiles, where the weights have to be streamed by as many SMs as possible:
 //   a cluster of up to eight CTAs splits K, each leaves its fp32 partial tile in shared memory, and every CTA adds up
@@ -32,10 +32,11 @@ struct Fp4Smem {
   static constexpr int kRedStride = BN + 4;                          // fp32 partial tile of a split launch
   static_assert(BM * kRedStride * 4 <= kScaleOff, "partial tile lies over the operand stages");
   static_assert(kTotal <= 232448, "exceeds the 227 KB shared memory of one CTA");
-  // accumulator, then two sets of scale columns
+  // accumulator, then a set of scale columns per stage
   static constexpr int kSetCols = 2 * 4 * Fp4Fmt<FMT>::kTilesPerStage;
-  static constexpr int kTmemCols = BN + 2 * kSetCols <= 128 ? 128 : 256;
-  static_assert(BN + 2 * kSetCols <= kTmemCols, "tensor memory");
+  static constexpr int kCols = BN + STAGES * kSetCols;
+  static constexpr int kTmemCols = kCols <= 128 ? 128 : (kCols <= 256 ? 256 : 512);
+  static_assert(kCols <= (STAGES == 3 ? 256 : 512), "tensor memory: two CTAs an SM with three stages");
 };
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
@@ -45,7 +46,7 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 }
 
 template <int FMT, int BN, int STAGES, bool SPLIT>
-__global__ void __launch_bounds__(kFp4Threads, BN == 128 ? 2 : 1)
+__global__ void __launch_bounds__(kFp4Threads, STAGES == 3 ? 2 : 1)
 pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const Fp4GemmParams p,
                    int split) {
   using L = Fp4Smem<FMT, BN, STAGES>;
@@ -100,7 +101,7 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         uint8_t* s_s = smem + L::kScaleOff + stage * 2 * L::kScale;
         const int t0 = kb * F::kTilesPerStage;
         const uint32_t sbytes = static_cast<uint32_t>(p.tiles_k - t0 < F::kTilesPerStage ? p.tiles_k - t0 : F::kTilesPerStage) * 512u;
-        mbar_arrive_expect_tx(&full_bar[stage], L::kOperand + 2 * sbytes);
+        mbar_arrive_expect_tx(&full_bar[stage], static_cast<uint32_t>(p.a_rows * BK + L::kBBytes) + 2 * sbytes);
         tma_load_2d(a_s, &tmA, &full_bar[stage], kb * BK, row0);
         tma_load_2d(a_s + L::kABytes, &tmW, &full_bar[stage], kb * BK, n0);
         bulk_load(s_s, sfa + static_cast<int64_t>(t0) * 512, sbytes, &full_bar[stage]);
@@ -118,16 +119,14 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll 1
       for (int kb = kb0; kb < kb1; ++kb) {
         const int i = kb - kb0, stage = i % STAGES;
-        // the scale set's last readers: the MMAs of two stages ago
-        if ((i >= 2 && !wait_or_abort(&empty_bar[(i - 2) % STAGES], ((i - 2) / STAGES) & 1, abort_flag)) ||
-            !wait_or_abort(&full_bar[stage], (i / STAGES) & 1, abort_flag)) {
+        if (!wait_or_abort(&full_bar[stage], (i / STAGES) & 1, abort_flag)) {
           report_timeout(p.status, 2, 1); *abort_flag = 1; ok = false;
           break;
         }
         tc_fence_after();
         const uint32_t a_addr = smem_u32(smem + stage * L::kOperand);
         const uint32_t s_addr = smem_u32(smem + L::kScaleOff + stage * 2 * L::kScale);
-        const uint32_t sfa_t = tmem_base + BN + (i & 1) * L::kSetCols;
+        const uint32_t sfa_t = tmem_base + BN + stage * L::kSetCols;
         const uint32_t sfb_t = sfa_t + 4 * F::kTilesPerStage;
         const int left = p.K - kb * kFp4StageK;                      // elements of this stage and beyond
 #pragma unroll
@@ -263,20 +262,30 @@ int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, 
   const int64_t pair_tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
   if ((p.s_row != nullptr) == (p.s_col != nullptr) && (options().fp4_pair == 2 || (options().fp4_pair == 1 && 2 * pair_tiles >= sms)))
     return launch_fp4_pair(FMT, xq, ldx, w, ldw, p, st);
-  const bool wide = static_cast<int64_t>(p.mt) * ((p.N + 127) / 128) >= sms;
+  bool wide = static_cast<int64_t>(p.mt) * ((p.N + 127) / 128) >= sms;
+  if (options().fp4_block_n != 0) wide = options().fp4_block_n == 128;
   const int bn = wide ? 128 : 64;
   p.nt = (p.N + bn - 1) / bn;
   if (static_cast<int64_t>(p.mt) * p.nt > 0x0fffffff) return PQ_ERR_SHAPE;
   CUtensorMap tmA, tmW;
-  int rc = make_tile_map(&tmA, xq, p.M, p.K / 2, ldx, BM);
+  // a single tile of few rows loads only those: what the others hold ends up in rows that nobody stores
+  p.a_rows = p.M < BM ? (p.M + 7) / 8 * 8 : BM;
+  int rc = make_tile_map(&tmA, xq, p.M, p.K / 2, ldx, p.a_rows);
   if (rc != PQ_OK) return rc;
   rc = make_tile_map(&tmW, w, p.N, p.K / 2, ldw, bn);
   if (rc != PQ_OK) return rc;
   if (wide) return launch_fp4<FMT, 128, 3, false>(tmA, tmW, p, 1, st);
   int split = 1;
   while (split < 8 && p.mt * p.nt * split * 2 <= sms && split * 2 <= num_kb) split *= 2;
-  if (split == 1) return launch_fp4<FMT, 64, 7, false>(tmA, tmW, p, 1, st);
-  return launch_fp4<FMT, 64, 7, true>(tmA, tmW, p, split, st);
+  const int want = options().fp4_split;
+  if (want == 1 || want == 2 || want == 4 || want == 8) {
+    split = want;
+    while (split > num_kb) split /= 2;
+  }
+  if (split > 1) return launch_fp4<FMT, 64, 7, true>(tmA, tmW, p, split, st);
+  // more tiles than SMs: two CTAs an SM instead of a second round (1 x 1280 -> 10240, 160 tiles: 9.6 us in two rounds)
+  if (p.mt * p.nt > sms) return launch_fp4<FMT, 64, 3, false>(tmA, tmW, p, 1, st);
+  return launch_fp4<FMT, 64, 7, false>(tmA, tmW, p, 1, st);
 }
 
 }  // namespace

@@ -26,6 +26,7 @@ struct Fp4GemmParams {
   int M, N, K;
   int tiles_k;             // scale tiles per row group
   int mt, nt;              // row and column tiles
+  int a_rows;              // rows of an activation tile that are loaded (single-CTA kernel)
   int bf16;                // output type
   int vec;                 // rows may be stored 16 bytes at a time
 };
