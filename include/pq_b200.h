@@ -68,7 +68,6 @@ int pq_last_cuda_error(void);
  *   "fp4_pair"          4-bit GEMM: 0 = never use the CTA-pair kernel, 1 = where its tiles fill the SM pairs (default), 2 =
  *                       always;
  *   "fp4_split"         4-bit GEMM outside the CTA-pair kernel: CTAs that share a tile's K (1, 2, 4 or 8);
- *   "fp4_block_n"       and its column tile (64 or 128);
  *   "g32_variant"       group-32 GEMM: 0 = tile width by the size of the launch, 1 = 128 columns, 2 = 64 columns.
  * Unknown keys return PQ_ERR_UNSUPPORTED.  Not part of the reference API. */
 int pq_set_option(const char* key, int value);

@@ -54,7 +54,6 @@ int* option_slot(const char* key) {
   if (key == nullptr) return nullptr;
   if (std::strcmp(key, "fp4_pair") == 0) return &o.fp4_pair;
   if (std::strcmp(key, "fp4_split") == 0) return &o.fp4_split;
-  if (std::strcmp(key, "fp4_block_n") == 0) return &o.fp4_block_n;
   if (std::strcmp(key, "quant_tpr") == 0) return &o.quant_tpr;
   if (std::strcmp(key, "gemm_stages") == 0) return &o.gemm_stages;
   if (std::strcmp(key, "gemm_block_n") == 0) return &o.gemm_block_n;

@@ -50,7 +50,6 @@ struct Options {
   int gemm_l2_hints = 0;   // CTA-pair kernel: bit 0 weights evict-last, bit 1 activations evict-first, bit 2 activations evict-last, bit 3 streaming output stores
   int fp4_pair = 1;        // 4-bit GEMM: CTA-pair kernel 0 never, 1 for launches that fill the SM pairs, 2 whenever it applies
   int fp4_split = 0;       // 4-bit GEMM, single-CTA tiles: CTAs that share a tile's K (0 automatic; 1, 2, 4, 8)
-  int fp4_block_n = 0;     // 4-bit GEMM, single-CTA tiles: columns (0 automatic; 64, 128)
   int g32_variant = 0;     // group-32 GEMM tiles: 0 by the size of the launch, 1 128 columns, 2 64 columns
 };
 Options& options();

@@ -1,24 +1,27 @@
 // Block-scaled 4-bit GEMM: out = (sum_k a s_a * w s_w) * (s_row x s_col) (+ bias), E2M1 codes with E8M0 (mx) or E4M3 (nv)
 // block scales applied by the tensor cores, fp32 accumulation in tensor memory (formats: fp4_common.cuh).
 //
-// One 128 x BN tile per CTA, 192 threads: warp 0 fills a ring of {activations, weights, scales of both} stages by TMA,
-// warp 1 copies a stage's scales to tensor memory (tcgen05.cp) and issues its four MMAs, warps 2-5 scale, add the bias
-// and store.  Every stage has scale columns of its own, so a full stage also says that the MMAs that read them last have
-// completed (its operands could not have been overwritten otherwise).
-//   BN = 128, three stages: two CTAs share an SM, so one's epilogue overlaps the other's main loop.
-//   BN = 64, seven stages, for launches of few tiles, where the weights have to be streamed by as many SMs as possible:
-//   a cluster of up to eight CTAs splits K, each leaves its fp32 partial tile in shared memory, and every CTA adds up
-//   and stores a share of the outputs (in rank order, so results do not depend on timing).
-// Every wait is bounded; no multicast.
+// The kernel of small and narrow products (the others run on CTA pairs, gemm_fp4_pair.cu).  One 128 x 64 tile per CTA, 192
+// threads: warp 0 fills a ring of {activations, weights, scales of both} stages by TMA, warp 1 copies a stage's scales to
+// tensor memory (tcgen05.cp) and issues its four MMAs, warps 2-5 scale, add the bias and store.  Every stage has scale
+// columns of its own, so a full stage also says that the MMAs that read them last have completed (its operands could not
+// have been overwritten otherwise).
+// What bounds it is latency: 3.6 us for a launch of one stage, 0.31 us for every further one (nv; mx 0.25), whatever the
+// tile's width.  With few tiles and a long K a cluster of up to eight CTAs splits K: each leaves its fp32 partial tile in
+// shared memory, and every CTA adds up and stores a share of the outputs (in rank order, so results do not depend on
+// timing).  1 x 5120 -> 1280: 9.9 us by 20 CTAs, 6.2 by 80; 1 x 10240 -> 640: 15.7 by 10, 6.5 by 80.
+// Seven stages and one CTA per SM; three stages and two CTAs per SM when there are more tiles than SMs (1 x 1280 -> 10240,
+// 160 tiles: 5.5 instead of 9.6 us).  Every wait is bounded; no multicast.
 #include "gemm_fp4_common.cuh"
 
 namespace pq {
 namespace {
 
+constexpr int BN = 64;                           // tile columns
 constexpr int kFp4Threads = 192;
 constexpr int kEpiThreads = 128;
 
-template <int FMT, int BN, int STAGES>
+template <int FMT, int STAGES>
 struct Fp4Smem {
   static constexpr int kABytes = BM * BK;
   static constexpr int kBBytes = BN * BK;
@@ -45,11 +48,11 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
-template <int FMT, int BN, int STAGES, bool SPLIT>
+template <int FMT, int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(kFp4Threads, STAGES == 3 ? 2 : 1)
 pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const Fp4GemmParams p,
                    int split) {
-  using L = Fp4Smem<FMT, BN, STAGES>;
+  using L = Fp4Smem<FMT, STAGES>;
   using F = Fp4Fmt<FMT>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
@@ -114,7 +117,7 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     // ------------------------------------------------------------------ MMA issuer
     if (elect_one()) {
       // columns [64, 128) of a weight row group start two scale words further on
-      const uint32_t sfb_shift = BN == 64 ? static_cast<uint32_t>((n0 & 64) >> 5) : 0u;
+      const uint32_t sfb_shift = static_cast<uint32_t>((n0 & 64) >> 5);
       bool ok = true;
 #pragma unroll 1
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -229,10 +232,10 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   if (warp == 1) tmem_dealloc(tmem_base, L::kTmemCols);
 }
 
-template <int FMT, int BN, int STAGES, bool SPLIT>
+template <int FMT, int STAGES, bool SPLIT>
 int launch_fp4(const CUtensorMap& tmA, const CUtensorMap& tmW, const Fp4GemmParams& p, int split, cudaStream_t st) {
-  using L = Fp4Smem<FMT, BN, STAGES>;
-  auto kern = pq_fp4_gemm_kernel<FMT, BN, STAGES, SPLIT>;
+  using L = Fp4Smem<FMT, STAGES>;
+  auto kern = pq_fp4_gemm_kernel<FMT, STAGES, SPLIT>;
   static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes
   int dev = 0;
   PQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -259,33 +262,36 @@ template <int FMT>
 int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, Fp4GemmParams& p, cudaStream_t st) {
   const int sms = sm_count();
   const int num_kb = (p.K + kFp4StageK - 1) / kFp4StageK;
+  // 256 x 256 tiles on CTA pairs from a quarter of the SMs on, measured in us, pair / single: 4096 x 640 -> 640 (48 tiles) 6.9 / 8.2,
+  // 2048 x 1280 -> 1280 (40) 7.5 / 8.9, 1024 x 1280 -> 1280 (20) 7.2 / 6.5.  Narrow outputs leave half a tile or more unused:
+  // 16384 x 640 -> 128 (64) 7.2 / 5.8, 65536 x 1280 -> 128 (256) 18.7 / 25.4, 65536 x 640 -> 64 13.7 / 10.0.
   const int64_t pair_tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if ((p.s_row != nullptr) == (p.s_col != nullptr) && (options().fp4_pair == 2 || (options().fp4_pair == 1 && 2 * pair_tiles >= sms)))
+  const bool pair = p.N > 128 ? 4 * pair_tiles >= sms : (p.N > 64 && pair_tiles >= sms);
+  if ((p.s_row != nullptr) == (p.s_col != nullptr) && (options().fp4_pair == 2 || (options().fp4_pair == 1 && pair)))
     return launch_fp4_pair(FMT, xq, ldx, w, ldw, p, st);
-  bool wide = static_cast<int64_t>(p.mt) * ((p.N + 127) / 128) >= sms;
-  if (options().fp4_block_n != 0) wide = options().fp4_block_n == 128;
-  const int bn = wide ? 128 : 64;
-  p.nt = (p.N + bn - 1) / bn;
-  if (static_cast<int64_t>(p.mt) * p.nt > 0x0fffffff) return PQ_ERR_SHAPE;
+  p.nt = (p.N + BN - 1) / BN;
+  const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt;
+  if (tiles > 0x0fffffff) return PQ_ERR_SHAPE;
   CUtensorMap tmA, tmW;
   // a single tile of few rows loads only those: what the others hold ends up in rows that nobody stores
   p.a_rows = p.M < BM ? (p.M + 7) / 8 * 8 : BM;
   int rc = make_tile_map(&tmA, xq, p.M, p.K / 2, ldx, p.a_rows);
   if (rc != PQ_OK) return rc;
-  rc = make_tile_map(&tmW, w, p.N, p.K / 2, ldw, bn);
+  rc = make_tile_map(&tmW, w, p.N, p.K / 2, ldw, BN);
   if (rc != PQ_OK) return rc;
-  if (wide) return launch_fp4<FMT, 128, 3, false>(tmA, tmW, p, 1, st);
+  // Clusters cost 1.5 us more than they save below ten stages (77 x 2048 -> 1280: 6.2 us unsplit, 6.5 split in four), and run in
+  // rounds when they do not all find room at once (2560 -> 2560, 40 tiles: 6.2 us split in two, 9.9 in four).
   int split = 1;
-  while (split < 8 && p.mt * p.nt * split * 2 <= sms && split * 2 <= num_kb) split *= 2;
+  if (num_kb >= 10)
+    while (split < 8 && tiles * split * 2 <= sms * 3 / 4 && split * 4 <= num_kb) split *= 2;
   const int want = options().fp4_split;
   if (want == 1 || want == 2 || want == 4 || want == 8) {
     split = want;
     while (split > num_kb) split /= 2;
   }
-  if (split > 1) return launch_fp4<FMT, 64, 7, true>(tmA, tmW, p, split, st);
-  // more tiles than SMs: two CTAs an SM instead of a second round (1 x 1280 -> 10240, 160 tiles: 9.6 us in two rounds)
-  if (p.mt * p.nt > sms) return launch_fp4<FMT, 64, 3, false>(tmA, tmW, p, 1, st);
-  return launch_fp4<FMT, 64, 7, false>(tmA, tmW, p, 1, st);
+  if (split > 1) return launch_fp4<FMT, 7, true>(tmA, tmW, p, split, st);
+  if (tiles > sms) return launch_fp4<FMT, 3, false>(tmA, tmW, p, 1, st);
+  return launch_fp4<FMT, 7, false>(tmA, tmW, p, 1, st);
 }
 
 }  // namespace

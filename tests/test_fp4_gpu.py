@@ -25,6 +25,7 @@ DTYPES = [torch.bfloat16, torch.float16]
 def _status_clean(cuda_dev):
     yield
     _lib.set_option("fp4_pair", 1)
+    _lib.set_option("fp4_split", 0)
     ops.check_device_status(cuda_dev)
 
 
@@ -53,7 +54,12 @@ def check_product(y, xq, wq, bias, fmt):
         bound = bound + 2.0 ** -24 * (S + bias.cpu().double().abs())
     fi = torch.finfo(y.dtype)
     bound = bound + (ref.abs() + bound) * fi.eps / 2 + fi.smallest_normal * fi.eps / 2
-    err = (y.cpu().double() - ref).abs()
+    got = y.cpu().double()
+    # 16-bit rounding: from half a step above the largest finite value on, an infinity of the sum's sign
+    border = fi.max * (2 - fi.eps / 2) / (2 - fi.eps)
+    beyond, inside = ref.abs() - bound >= border, ref.abs() + bound < border
+    assert torch.equal(got[beyond], torch.sign(ref[beyond]) * float("inf")) and bool(torch.isfinite(got[inside]).all())
+    err = torch.where(inside, (got - ref).abs(), torch.zeros_like(ref))
     worst = float((err / bound).max())
     assert worst <= 1, f"error {worst:.3g} times the bound at {divmod(int((err / bound).argmax()), y.shape[1])}"
 
@@ -166,6 +172,31 @@ def test_product_many_tiles(cuda_dev, fmt, M, N, K):
     xq, wq = fp4_exec.quant_rows_fp4(x, fmt), fp4_exec.quant_rows_fp4(w, fmt)
     bias = torch.randn(N, generator=g).to(cuda_dev)
     check_product(fp4_exec.fp4_gemm(xq, wq, bias, torch.bfloat16), xq, wq, bias, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("split", [1, 2, 4, 8])
+@pytest.mark.parametrize("M,N,K", [(1, 640, 2560), (77, 200, 2080), (130, 70, 5120), (300, 64, 288)])
+def test_product_with_k_split(cuda_dev, fmt, split, M, N, K):
+    """Single-CTA tiles with K shared by a cluster, stages divided evenly or not."""
+    _, xq = make_rows(M, K, fmt, torch.bfloat16, 3, cuda_dev)
+    _, wq = make_rows(N, K, fmt, torch.bfloat16, 4, cuda_dev)
+    bias = torch.randn(N, device=cuda_dev)
+    _lib.set_option("fp4_pair", 0)
+    _lib.set_option("fp4_split", split)
+    y = fp4_exec.fp4_gemm(xq, wq, bias, torch.float16)
+    check_product(y, xq, wq, bias, fmt)
+    assert torch.equal(fp4_exec.fp4_gemm(xq, wq, bias, torch.float16), y)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", [(2048, 640, 640), (5000, 100, 160), (20000, 60, 96)])
+def test_product_more_single_tiles_than_sms(cuda_dev, fmt, M, N, K):
+    g = torch.Generator().manual_seed(8)
+    xq = fp4_exec.quant_rows_fp4(torch.randn(M, K, generator=g).to(torch.bfloat16).to(cuda_dev), fmt)
+    wq = fp4_exec.quant_rows_fp4(torch.randn(N, K, generator=g).to(torch.bfloat16).to(cuda_dev), fmt)
+    _lib.set_option("fp4_pair", 0)
+    check_product(fp4_exec.fp4_gemm(xq, wq, None, torch.bfloat16), xq, wq, None, fmt)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
