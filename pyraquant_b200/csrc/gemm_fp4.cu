@@ -263,10 +263,11 @@ int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, 
   const int sms = sm_count();
   const int num_kb = (p.K + kFp4StageK - 1) / kFp4StageK;
   // 256 x 256 tiles on CTA pairs from a quarter of the SMs on, measured in us, pair / single: 4096 x 640 -> 640 (48 tiles) 6.9 / 8.2,
-  // 2048 x 1280 -> 1280 (40) 7.5 / 8.9, 1024 x 1280 -> 1280 (20) 7.2 / 6.5.  Narrow outputs leave half a tile or more unused:
-  // 16384 x 640 -> 128 (64) 7.2 / 5.8, 65536 x 1280 -> 128 (256) 18.7 / 25.4, 65536 x 640 -> 64 13.7 / 10.0.
+  // 256 x 1280 -> 10240 (40) 7.6 / 10.3, 1024 x 1280 -> 1280 (20) 7.2 / 6.5.  Up to 128 rows or columns half a tile or more is
+  // unused: 128 x 1280 -> 10240 (40) 7.9 / 6.9, 128 x 4096 -> 32768 (128) 22.0 / 25.0; 16384 x 640 -> 128 (64) 7.2 / 5.8,
+  // 65536 x 1280 -> 128 (256) 18.7 / 25.4, 65536 x 640 -> 64 13.7 / 10.0.
   const int64_t pair_tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
-  const bool pair = p.N > 128 ? 4 * pair_tiles >= sms : (p.N > 64 && pair_tiles >= sms);
+  const bool pair = p.N > 128 ? (p.M > 128 ? 4 : 2) * pair_tiles >= sms : (p.N > 64 && pair_tiles >= sms);
   if ((p.s_row != nullptr) == (p.s_col != nullptr) && (options().fp4_pair == 2 || (options().fp4_pair == 1 && pair)))
     return launch_fp4_pair(FMT, xq, ldx, w, ldw, p, st);
   p.nt = (p.N + BN - 1) / BN;
