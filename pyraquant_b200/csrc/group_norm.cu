@@ -4,16 +4,16 @@
 //
 // HBM-bound: 2 bytes read and 2 (z), 1 (INT8) or 0.53 to 0.56 (4-bit) written per element, provided x is read once although the
 // statistics are needed before the first output.  So one cooperative launch of one CTA per SM: the T rows of a sample are
-// cut into P consecutive chunks, one per CTA, which a CTA keeps in shared memory (200 KB, 30 MB over the GPU) across a
-// grid barrier.  Rows beyond that are read from memory twice, the second time in reverse order (the last ones read are
-// the likeliest to be in L2 still).
-//   1. The rows come by bulk copies in eight segments.  A thread has a fixed column of eight channels and every R-th row
-//      and sums x - pivot and its square per channel, the pivot being its first value (the sum of squares must not cancel
-//      when the mean is large against the deviation).  The CTA's mean of a group is the sum of the threads' sums, its
-//      centred sum of squares that of M2_thread + n (mean_thread - mean)^2: no cancellation, fixed order.
-//   2. After the barrier every CTA does the same with the P chunks of its sample, and normalises its rows.
-// The quantising forms put z back into shared memory, take every row's largest magnitude on the way (an atomic maximum of
-// bit patterns, independent of order) and write codes in a second sweep; they need all rows of a chunk in shared memory.
+// cut into P consecutive chunks, one per CTA, which pass through a ring of eight segments in shared memory (200 KB, 30 MB
+// over the GPU) by bulk copies, and what the ring holds at the end of the first pass is not read again for the second.
+//   1. First to last segment: a thread has a fixed column of eight channels and every R-th row and sums x - pivot and its
+//      square per channel, the pivot being its first value (the sum of squares must not cancel when the mean is large
+//      against the deviation).  The CTA's mean of a group is the sum of the threads' sums, its centred sum of squares that
+//      of M2_thread + n (mean_thread - mean)^2: no cancellation, fixed order.
+//   2. After a grid barrier every CTA does the same with the P chunks of its sample, and normalises its rows, last to
+//      first segment: the last eight are there, of the others the ones read last are the likeliest to be in L2 still.
+// The quantising forms put z back into shared memory, take every row's largest magnitude (an atomic maximum of bit patterns,
+// independent of order) and write codes in a third sweep; they need all rows of a chunk in the ring.
 // All statistics and arithmetic are fp32.
 #include <cooperative_groups.h>
 
@@ -27,9 +27,9 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxC = 8192;
-constexpr int kSegments = 8;
-constexpr int kUnroll = 8;
+constexpr int kSlots = 8;                         // segments in shared memory
 constexpr int kSmemMax = 232448;
+constexpr int kApplyUnroll = 2;
 constexpr int kPartsPerLane = 8;                  // chunks of a sample: at most 256
 
 enum Mode { kOut16 = 0, kInt8 = 1, kMx = 2, kNv = 3 };
@@ -44,17 +44,18 @@ __host__ __device__ __forceinline__ Lanes lanes_of(int C) {
   return l;
 }
 
-// shared memory: rows, then per-thread sums [R][C], group statistics [2][groups], row maxima, barriers
+// shared memory: ring of rows, then per-thread sums [R][C], group statistics [2][groups], row maxima (quantising forms, whose rows
+// all fit), barriers full[kSlots], empty[kSlots]
 struct NormSmem {
   int red, stat, amax, bars, total;
 };
-__host__ __device__ __forceinline__ NormSmem smem_of(int C, int groups, int cap) {
+__host__ __device__ __forceinline__ NormSmem smem_of(int C, int groups, int ring_rows) {
   NormSmem s;
-  s.red = (cap * C * 2 + 127) & ~127;
+  s.red = (ring_rows * C * 2 + 127) & ~127;
   s.stat = s.red + lanes_of(C).R * C * 4;
   s.amax = s.stat + 2 * groups * 4;
-  s.bars = (s.amax + cap * 4 + 7) & ~7;
-  s.total = s.bars + kSegments * 8;
+  s.bars = (s.amax + ring_rows * 4 + 7) & ~7;
+  s.total = s.bars + 2 * kSlots * 8;
   return s;
 }
 
@@ -68,7 +69,7 @@ struct NormArgs {
   float2* part;                                     // [B][groups][P] mean, M2
   int32_t* status;
   int B, T, C, groups, P, silu;
-  int cap;                                          // rows a CTA keeps in shared memory
+  int seg_rows;                                     // rows of a segment
   int chunk, longer;                                // rows per chunk; the first `longer` chunks have one more
   // what follows from the sizes, worked out on the host: a division on the way to the first copy costs a tenth of a
   // microsecond, and there would be eight of them
@@ -227,48 +228,57 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sums over the R x cpg entries of every group of `red`, a warp for two groups at a time, in a fixed order.
-template <typename F>
-__device__ __forceinline__ void sum_groups(const float* red, int R, int C, int groups, int cpg, float inv_cpg, F&& put) {
-  const int lane = threadIdx.x & 31, items = R * cpg;
-  if (items <= 128) {                                // any C whose columns nearly fill the threads, with 32 groups
-    int off[4];
+// Sums over the R x cpg entries of every group of `red`, in a fixed order; a warp for two groups at a time in the usual case of at
+// most 128 entries (32 groups whose columns nearly fill the threads), whose places are worked out once.
+struct GroupSums {
+  int off[4], R, C, groups, cpg;
+  __device__ __forceinline__ void init(const NormArgs& a) {
+    R = a.l.R; C = a.C; groups = a.groups; cpg = a.cpg;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int i = lane + 32 * k, r = group_of(i, inv_cpg);
-      off[k] = i < items ? r * C + i - r * cpg : -1;
-    }
-    for (int g = static_cast<int>(threadIdx.x) >> 5; g < groups; g += 2 * kWarps) {
-      const int h = g + kWarps;
-      const float* rg = red + g * cpg;
-      const float* rh = red + h * cpg;
-      float s = 0.0f, t = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (off[k] >= 0) s += rg[off[k]];
-        if (off[k] >= 0 && h < groups) t += rh[off[k]];
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); t += __shfl_xor_sync(0xffffffffu, t, o); }
-      if (lane == 0) put(g, s);
-      if (lane == 1 && h < groups) put(h, t);
-    }
-  } else {
-    for (int g = static_cast<int>(threadIdx.x) >> 5; g < groups; g += kWarps) {
-      float s = 0.0f;
-      if (cpg >= 32) {
-        for (int r = 0; r < R; ++r)
-          for (int c = lane; c < cpg; c += 32) s += red[r * C + g * cpg + c];
-      } else {
-        const int per = 32 / cpg, r0 = lane / cpg, c = lane - r0 * cpg;      // floor(32 / cpg) rows at a time
-        if (r0 < per)
-          for (int r = r0; r < R; r += per) s += red[r * C + g * cpg + c];
-      }
-      s = warp_sum(s);
-      if (lane == 0) put(g, s);
+      const int i = lane + 32 * k, r = group_of(i, a.inv_cpg);
+      off[k] = i < R * cpg ? r * C + i - r * cpg : -1;
     }
   }
-}
+  template <typename F>
+  __device__ __forceinline__ void operator()(const float* red, F&& put) const {
+    const int lane = threadIdx.x & 31;
+    if (R * cpg <= 128) {
+      for (int g = static_cast<int>(threadIdx.x) >> 5; g < groups; g += 2 * kWarps) {
+        const int h = g + kWarps;
+        const float* rg = red + g * cpg;
+        const float* rh = red + h * cpg;
+        float s = 0.0f, t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (off[k] >= 0) s += rg[off[k]];
+          if (off[k] >= 0 && h < groups) t += rh[off[k]];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); t += __shfl_xor_sync(0xffffffffu, t, o); }
+        if (lane == 0) put(g, s);
+        if (lane == 1 && h < groups) put(h, t);
+      }
+    } else {
+#pragma unroll 1
+      for (int g = static_cast<int>(threadIdx.x) >> 5; g < groups; g += kWarps) {
+        float s = 0.0f;
+        if (cpg >= 32) {
+#pragma unroll 1
+          for (int r = 0; r < R; ++r)
+            for (int c = lane; c < cpg; c += 32) s += red[r * C + g * cpg + c];
+        } else {
+          const int per = 32 / cpg, r0 = lane / cpg, c = lane - r0 * cpg;      // floor(32 / cpg) rows at a time
+          if (r0 < per)
+            for (int r = r0; r < R; r += per) s += red[r * C + g * cpg + c];
+        }
+        s = warp_sum(s);
+        if (lane == 0) put(g, s);
+      }
+    }
+  }
+};
 
 // COLS: columns of eight channels per thread, two only for C > 4096
 template <typename T, int MODE, int COLS>
@@ -286,74 +296,97 @@ pq_group_norm_kernel(const NormArgs a) {
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int p = static_cast<int>(blockIdx.x);
   const int r0 = p * a.chunk + (p < a.longer ? p : a.longer), rows = a.chunk + (p < a.longer ? 1 : 0);
-  const int resident = rows < a.cap ? rows : a.cap;
-  const int seg_rows = max((resident + kSegments - 1) / kSegments, 1);
+  const int segs = (rows + a.seg_rows - 1) / a.seg_rows;
   const int cpg = a.cpg;
   const float inv_cpg = a.inv_cpg;
   const int rl = group_of(tid, a.inv_cols), col0 = tid - rl * l.cols;
-  const int row_bytes = a.C * 2;
+  const int row_bytes = a.C * 2, slot_bytes = a.seg_rows * row_bytes;
+  uint64_t* empty = bars + kSlots;
 
-  if (tid < kSegments) {
-    mbar_init(&bars[tid], 1);
-    fence_mbar_init();
-    fence_proxy_async_smem();
-  }
-  __syncwarp();
-
-  uint32_t phase = 0;
 #pragma unroll 1
-  for (int b = static_cast<int>(blockIdx.y); b < a.B; b += static_cast<int>(gridDim.y), phase ^= 1u) {
+  for (int b = static_cast<int>(blockIdx.y); b < a.B; b += static_cast<int>(gridDim.y)) {
     const T* xb = static_cast<const T*>(a.x) + static_cast<int64_t>(b) * a.ld_batch + static_cast<int64_t>(r0) * a.ld_row;
-    // ---------------------------------------------------------------- rows into shared memory
+    // segment s into its slot; one lane for contiguous rows, the lanes of a warp side by side for others
+    auto load = [&](int s) {
+      const int from = s * a.seg_rows, n = min(a.seg_rows, rows - from);
+      const uint32_t dst = rows_s + (s % kSlots) * slot_bytes;
+      uint64_t* bar = &bars[s % kSlots];
+      if (a.ld_row == a.C) {
+        mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n * row_bytes));
+        bulk_copy(dst, xb + static_cast<int64_t>(from) * a.C, static_cast<uint32_t>(n * row_bytes), bar);
+      } else {
+        if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n * row_bytes));
+        __syncwarp();
+        for (int r = lane; r < n; r += 32)
+          bulk_copy(dst + r * row_bytes, xb + static_cast<int64_t>(from + r) * a.ld_row, static_cast<uint32_t>(row_bytes), bar);
+      }
+    };
+    // In both passes the segment's wait has the parity of s / kSlots: the first pass fills a slot L + 1 times, with its segments
+    // 0 .. L, the second refills it with L - 1 .. 0, fill number 2 L - q for segment q.  The slot is given back once per
+    // segment and pass, 2 L + 1 - q times before by segment q of the second pass.
+    auto wait_full = [&](int s) {
+      if (!mbar_wait_bounded(&bars[s % kSlots], (s / kSlots) & 1)) report_timeout(a.status, 8, 1);
+    };
+    auto refill = [&](int used, int s, uint32_t parity) {             // warp 0: segment s once everybody is done with `used`
+      if (a.ld_row != a.C || lane == 0) {
+        if (!mbar_wait_bounded(&empty[used % kSlots], parity)) report_timeout(a.status, 8, 2);
+        load(s);
+      }
+      __syncwarp();
+    };
+    // ---------------------------------------------------------------- the first segments on their way
     if (warp == 0) {
-      if (lane < kSegments) {
-        const int from = min(lane * seg_rows, resident), to = min(from + seg_rows, resident);
-        mbar_arrive_expect_tx(&bars[lane], static_cast<uint32_t>((to - from) * row_bytes));
-        if (a.ld_row == a.C && to > from)                               // contiguous: one piece a segment
-          bulk_copy(rows_s + from * row_bytes, xb + static_cast<int64_t>(from) * a.C, static_cast<uint32_t>((to - from) * row_bytes), &bars[lane]);
+      if (lane < kSlots) {
+        if (b != static_cast<int>(blockIdx.y)) {                      // another sample: barriers from the start
+          asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars[lane])) : "memory");
+          asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(&empty[lane])) : "memory");
+        }
+        mbar_init(&bars[lane], 1);
+        mbar_init(&empty[lane], kWarps);
+        fence_mbar_init();
+        fence_proxy_async_smem();
+        if (a.ld_row == a.C && lane < segs) load(lane);
       }
       __syncwarp();
       if (a.ld_row != a.C)
-        for (int r = lane; r < resident; r += 32)
-          bulk_copy(rows_s + r * row_bytes, xb + static_cast<int64_t>(r) * a.ld_row, static_cast<uint32_t>(row_bytes), &bars[r / seg_rows]);
+        for (int s = 0; s < min(segs, kSlots); ++s) load(s);
     }
     if (MODE != kOut16)
-      for (int r = tid; r < resident; r += kThreads) amax[r] = 0u;
+      for (int r = tid; r < rows; r += kThreads) amax[r] = 0u;
+    GroupSums group_sums;
+    group_sums.init(a);
+    const float inv_count = 1.0f / (static_cast<float>(rows) * static_cast<float>(cpg));
     __syncthreads();                                                     // barriers and row maxima are there
 
     // ---------------------------------------------------------------- statistics of the chunk
     ColumnSums cs[COLS];
 #pragma unroll
-    for (int k = 0; k < COLS; ++k) {
-      cs[k].clear();
-      const int col = col0 + k * l.cols;
-      if (rl < l.R && col < l.ncol) {
-        const T* xc = xb + col * 8;
-        int r = resident + rl;
-        for (; r < rows; r += l.R * kUnroll) {                           // rows that stay in memory
-          uint4 v[kUnroll];
+    for (int k = 0; k < COLS; ++k) cs[k].clear();
+#pragma unroll 1
+    for (int s = 0; s < segs; ++s) {
+      wait_full(s);
+      const int n = min(a.seg_rows, rows - s * a.seg_rows);
+      const uint32_t at = rows_s + (s % kSlots) * slot_bytes + col0 * 16;
 #pragma unroll
-          for (int u = 0; u < kUnroll; ++u)
-            if (r + u * l.R < rows) v[u] = ld_v4(xc + static_cast<int64_t>(r + u * l.R) * a.ld_row);
-#pragma unroll
-          for (int u = 0; u < kUnroll; ++u)
-            if (r + u * l.R < rows) cs[k].template add<T>(v[u]);
+      for (int k = 0; k < COLS; ++k)
+        if (rl < l.R && col0 + k * l.cols < l.ncol) {
+#pragma unroll 2
+          for (int r = rl; r < n; r += l.R) cs[k].template add<T>(ld_shared_v4(at + r * row_bytes + k * l.cols * 16));
         }
-        int seg_end = 0, seg = -1;
-        for (r = rl; r < resident; r += l.R) {
-          while (r >= seg_end) {
-            ++seg; seg_end += seg_rows;
-            if (!mbar_wait_bounded(&bars[seg], phase)) report_timeout(a.status, 8, 1);
-          }
-          cs[k].template add<T>(ld_shared_v4(rows_s + r * row_bytes + col * 16));
-        }
-        cs[k].finish();
-        put8(red + rl * a.C + col * 8, [&](int i) { return cs[k].mean(i) * cs[k].count; });
+      if (segs > kSlots) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s % kSlots]);
+        if (warp == 0 && s >= 1 && s - 1 + kSlots < segs) refill(s - 1, s - 1 + kSlots, ((s - 1) / kSlots) & 1);
       }
     }
+#pragma unroll
+    for (int k = 0; k < COLS; ++k) {
+      cs[k].finish();
+      const int col = col0 + k * l.cols;
+      if (rl < l.R && col < l.ncol) put8(red + rl * a.C + col * 8, [&](int i) { return cs[k].mean(i) * cs[k].count; });
+    }
     __syncthreads();
-    const float count = static_cast<float>(rows) * static_cast<float>(cpg);
-    sum_groups(red, l.R, a.C, a.groups, cpg, inv_cpg, [&](int g, float s) { stat[g] = s / count; });
+    group_sums(red, [&](int g, float s) { stat[g] = s * inv_count; });
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < COLS; ++k) {
@@ -365,7 +398,7 @@ pq_group_norm_kernel(const NormArgs a) {
         });
     }
     __syncthreads();
-    sum_groups(red, l.R, a.C, a.groups, cpg, inv_cpg, [&](int g, float s) { stat[a.groups + g] = s; });
+    group_sums(red, [&](int g, float s) { stat[a.groups + g] = s; });
     __syncthreads();
 
     Affine8<T> f;
@@ -397,42 +430,36 @@ pq_group_norm_kernel(const NormArgs a) {
         if (lane == 0) { stat[g] = mean; stat[a.groups + g] = 1.0f / sqrtf(m2 / total + a.eps); }
       }
     } else {
-      for (int g = tid; g < a.groups; g += kThreads) stat[a.groups + g] = 1.0f / sqrtf(stat[a.groups + g] / count + a.eps);
+      for (int g = tid; g < a.groups; g += kThreads) stat[a.groups + g] = 1.0f / sqrtf(stat[a.groups + g] * inv_count + a.eps);
     }
     __syncthreads();
 
     // ---------------------------------------------------------------- normalisation
     const int64_t out0 = static_cast<int64_t>(b) * a.out_batch + static_cast<int64_t>(r0) * a.out_row;
 #pragma unroll 1
-    for (int k = 0; k < COLS; ++k) {
-      const int col = col0 + k * l.cols;
-      if (rl >= l.R || col >= l.ncol) break;
-      if (k > 0) f.request(a, col * 8);
-      f.complete(a, stat, col * 8);
-      if constexpr (MODE == kOut16) {
-        const T* xc = xb + col * 8;
-        T* oc = static_cast<T*>(a.out) + out0 + col * 8;
-        const int far = rows - resident;                                  // rows to read again, the last ones first
-        for (int r = rl; r < far; r += l.R * kUnroll) {
-          uint4 v[kUnroll];
-#pragma unroll
-          for (int u = 0; u < kUnroll; ++u)
-            if (r + u * l.R < far) v[u] = ld_stream_v4(xc + static_cast<int64_t>(rows - 1 - r - u * l.R) * a.ld_row);
-#pragma unroll
-          for (int u = 0; u < kUnroll; ++u)
-            if (r + u * l.R < far) st_v4_cs(oc + static_cast<int64_t>(rows - 1 - r - u * l.R) * a.out_row, f(v[u], a.silu));
+    for (int s = segs - 1; s >= 0; --s) {
+      if (s < segs - kSlots) wait_full(s);
+      const int n = min(a.seg_rows, rows - s * a.seg_rows);
+      const uint32_t at = rows_s + (s % kSlots) * slot_bytes;
+#pragma unroll 1
+      for (int k = 0; k < COLS; ++k) {
+        const int col = col0 + k * l.cols;
+        if (rl >= l.R || col >= l.ncol) break;
+        if (COLS > 1) f.request(a, col * 8);
+        if (COLS > 1 || s == segs - 1) f.complete(a, stat, col * 8);
+        T* oc = static_cast<T*>(a.out) + out0 + static_cast<int64_t>(s * a.seg_rows) * a.out_row + col * 8;
+#pragma unroll kApplyUnroll
+        for (int r = rl; r < n; r += l.R) {
+          const uint4 z = f(ld_shared_v4(at + r * row_bytes + col * 16), a.silu);
+          if constexpr (MODE != kOut16) st_shared_v4(at + r * row_bytes + col * 16, z);
+          if (MODE == kOut16 || a.out != nullptr) st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, z);
         }
-#pragma unroll 2
-        for (int r = rl; r < resident; r += l.R)
-          st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, f(ld_shared_v4(rows_s + r * row_bytes + col * 16), a.silu));
-      } else {
-#pragma unroll 2
-        for (int r = rl; r < rows; r += l.R) {
-          const uint32_t at = rows_s + r * row_bytes + col * 16;
-          const uint4 z = f(ld_shared_v4(at), a.silu);
-          st_shared_v4(at, z);
-          if (a.out != nullptr) st_v4(static_cast<T*>(a.out) + out0 + static_cast<int64_t>(r) * a.out_row + col * 8, z);
-        }
+      }
+      if (segs > kSlots) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s % kSlots]);
+        // the segment done before this one makes room; its slot's next one, going down, is kSlots before it
+        if (warp == 0 && s + 1 < segs && s + 1 - kSlots >= 0) refill(s + 1, s + 1 - kSlots, (((s + 1) / kSlots) & 1) ^ 1u);
       }
     }
     if constexpr (MODE != kOut16) {
@@ -524,14 +551,20 @@ template <typename T, int MODE, int COLS>
 int launch_norm(NormArgs a, cudaStream_t st) {
   const int longest = (a.T + a.P - 1) / a.P;
   const int fixed = smem_of(a.C, a.groups, 0).total + 256;
-  int cap = (kSmemMax - fixed) / (a.C * 2 + 4);
-  if (cap > longest) cap = longest;
-  if (cap < 0) return PQ_ERR_UNSUPPORTED;
-  if (MODE != kOut16 && cap < longest) return PQ_ERR_UNSUPPORTED;          // the rows do not fit on the chip
-  a.cap = cap;
-  a.chunk = a.T / a.P; a.longer = a.T % a.P;
+  const int most = fixed < kSmemMax ? (kSmemMax - fixed) / (a.C * 2 + 4) : 0;     // rows of the ring
   a.l = lanes_of(a.C);
-  a.lay = smem_of(a.C, a.groups, cap);
+  // segments of whole steps of R rows where that leaves all rows in the ring, then of an eighth of the rows, then of an eighth
+  // of the ring
+  const int R = a.l.R, eighth = (longest + kSlots - 1) / kSlots, steps = (eighth + R - 1) / R * R;
+  auto ring = [&](int rows) { return (longest + rows - 1) / rows * rows; };
+  int seg = ring(steps) <= most ? steps : (ring(eighth) <= most ? eighth : most / kSlots);
+  if (ring(seg) > most && seg > R) seg = seg / R * R;
+  if (seg < 1) return PQ_ERR_UNSUPPORTED;                                  // thousands of groups of thousands of channels
+  if (MODE != kOut16 && static_cast<int64_t>(seg) * kSlots < longest) return PQ_ERR_UNSUPPORTED;      // rows beyond the chip's shared memory
+  a.seg_rows = seg;
+  const int slots = (longest + seg - 1) / seg < kSlots ? (longest + seg - 1) / seg : kSlots;
+  a.chunk = a.T / a.P; a.longer = a.T % a.P;
+  a.lay = smem_of(a.C, a.groups, slots * seg);
   if (a.lay.total > kSmemMax) return PQ_ERR_UNSUPPORTED;
   a.cpg = a.C / a.groups; a.inv_cpg = 1.0f / static_cast<float>(a.cpg);
   a.inv_cols = 1.0f / static_cast<float>(a.l.cols);
