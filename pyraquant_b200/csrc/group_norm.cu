@@ -30,7 +30,7 @@ constexpr int kMaxC = 8192;
 constexpr int kSlots = 8;                         // segments in shared memory
 constexpr int kSmemMax = 232448;
 constexpr int kApplyUnroll = 2;
-constexpr int kPartsPerLane = 8;                  // chunks of a sample: at most 256
+constexpr int kPartsPerLane = 5;                  // chunks of a sample: at most 160
 
 enum Mode { kOut16 = 0, kInt8 = 1, kMx = 2, kNv = 3 };
 
@@ -90,20 +90,20 @@ __device__ __forceinline__ float ex2_approx(float v) {
 }
 // z * sigmoid(z) for four values with one reciprocal: with E = exp(-|z|) in [0, 1] and h = E / (1 + E), it is z - z h for z >= 0
 // and z h below, max(z, 0) - |z| h in both cases; the product of four denominators stays within [1, 16].  (Two special-function
-// operations per value, an exponential and a reciprocal, bound the normalisation of bf16 rows otherwise.)
-__device__ __forceinline__ void silu4(float2 (&z)[4], int i) {
-  const float2 a0 = make_float2(fabsf(z[i].x), fabsf(z[i].y)), a1 = make_float2(fabsf(z[i + 1].x), fabsf(z[i + 1].y));
-  const float2 neg_log2e = make_float2(-1.4426950408889634f, -1.4426950408889634f), one = make_float2(1.0f, 1.0f);
-  const float2 t0 = __fmul2_rn(a0, neg_log2e), t1 = __fmul2_rn(a1, neg_log2e);
+// operations per value, an exponential and a reciprocal, bound the normalisation of bf16 rows otherwise.)  With
+// t = -|z| log2(e), the argument of the exponential to the base 2, -|z| h = t (ln(2) h).
+__device__ __forceinline__ void silu4(float2& u, float2& v) {
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  const float2 t0 = make_float2(fabsf(u.x) * -kLog2e, fabsf(u.y) * -kLog2e), t1 = make_float2(fabsf(v.x) * -kLog2e, fabsf(v.y) * -kLog2e);
   const float2 e0 = make_float2(ex2_approx(t0.x), ex2_approx(t0.y)), e1 = make_float2(ex2_approx(t1.x), ex2_approx(t1.y));
+  const float2 one = make_float2(1.0f, 1.0f);
   const float2 d0 = __fadd2_rn(e0, one), d1 = __fadd2_rn(e1, one);
   const float p0 = d0.x * d0.y, p1 = d1.x * d1.y;
-  const float r = rcp_approx(p0 * p1);
+  const float r = rcp_approx(p0 * p1) * kLn2;
   const float r0 = r * p1, r1 = r * p0;
-  const float2 h0 = __fmul2_rn(e0, __fmul2_rn(make_float2(d0.y, d0.x), make_float2(r0, r0)));
-  const float2 h1 = __fmul2_rn(e1, __fmul2_rn(make_float2(d1.y, d1.x), make_float2(r1, r1)));
-  z[i] = __ffma2_rn(make_float2(-a0.x, -a0.y), h0, make_float2(fmaxf(z[i].x, 0.0f), fmaxf(z[i].y, 0.0f)));
-  z[i + 1] = __ffma2_rn(make_float2(-a1.x, -a1.y), h1, make_float2(fmaxf(z[i + 1].x, 0.0f), fmaxf(z[i + 1].y, 0.0f)));
+  const float2 h0 = __fmul2_rn(e0, make_float2(r0 * d0.y, r0 * d0.x)), h1 = __fmul2_rn(e1, make_float2(r1 * d1.y, r1 * d1.x));
+  u = __ffma2_rn(t0, h0, make_float2(fmaxf(u.x, 0.0f), fmaxf(u.y, 0.0f)));
+  v = __ffma2_rn(t1, h1, make_float2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f)));
 }
 
 template <typename T>
@@ -216,7 +216,7 @@ struct Affine8 {
     unpack8<T>(v, f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = __ffma2_rn(__fadd2_rn(f[i], neg_mean[i]), mul[i], add[i]);
-    if (with_silu) { silu4(f, 0); silu4(f, 2); }
+    if (with_silu) { silu4(f[0], f[1]); silu4(f[2], f[3]); }
     T tag{};
     return make_uint4(pack2(f[0].x, f[0].y, tag), pack2(f[1].x, f[1].y, tag), pack2(f[2].x, f[2].y, tag), pack2(f[3].x, f[3].y, tag));
   }
@@ -409,25 +409,41 @@ pq_group_norm_kernel(const NormArgs a) {
       for (int g = tid; g < a.groups; g += kThreads)
         a.part[(static_cast<int64_t>(b) * a.groups + g) * a.P + p] = make_float2(stat[g], stat[a.groups + g]);
       cooperative_groups::this_grid().sync();
-      const float total = static_cast<float>(a.T) * static_cast<float>(cpg);
+      const float inv_total = 1.0f / (static_cast<float>(a.T) * static_cast<float>(cpg));
       const float n_long = static_cast<float>((a.chunk + 1) * cpg), n_short = static_cast<float>(a.chunk * cpg);
-      for (int g = warp; g < a.groups; g += kWarps) {
-        const float2* part = a.part + (static_cast<int64_t>(b) * a.groups + g) * a.P;
-        float2 v[kPartsPerLane];
-#pragma unroll
-        for (int k = 0; k < kPartsPerLane; ++k) v[k] = lane + 32 * k < a.P ? __ldcg(part + lane + 32 * k) : make_float2(0.0f, 0.0f);
-        float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kPartsPerLane; ++k) s = fmaf(v[k].x, lane + 32 * k < a.longer ? n_long : n_short, s);
-        const float mean = warp_sum(s) / total;
-        float m2 = 0.0f;
+      // a warp for two groups at a time: their loads are in flight together
+#pragma unroll 1
+      for (int g = warp; g < a.groups; g += 2 * kWarps) {
+        const int h = g + kWarps < a.groups ? g + kWarps : g;
+        const float2* part_g = a.part + (static_cast<int64_t>(b) * a.groups + g) * a.P;
+        const float2* part_h = a.part + (static_cast<int64_t>(b) * a.groups + h) * a.P;
+        float2 u[kPartsPerLane], v[kPartsPerLane];
 #pragma unroll
         for (int k = 0; k < kPartsPerLane; ++k) {
-          const float d = v[k].x - mean;
-          if (lane + 32 * k < a.P) m2 += fmaf(d * d, lane + 32 * k < a.longer ? n_long : n_short, v[k].y);
+          const int i = lane + 32 * k;
+          u[k] = i < a.P ? __ldcg(part_g + i) : make_float2(0.0f, 0.0f);
+          v[k] = i < a.P ? __ldcg(part_h + i) : make_float2(0.0f, 0.0f);
         }
-        m2 = warp_sum(m2);
-        if (lane == 0) { stat[g] = mean; stat[a.groups + g] = 1.0f / sqrtf(m2 / total + a.eps); }
+        float n[kPartsPerLane], su = 0.0f, sv = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPartsPerLane; ++k) {
+          const int i = lane + 32 * k;
+          n[k] = i < a.longer ? n_long : (i < a.P ? n_short : 0.0f);
+          su = fmaf(u[k].x, n[k], su); sv = fmaf(v[k].x, n[k], sv);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { su += __shfl_xor_sync(0xffffffffu, su, o); sv += __shfl_xor_sync(0xffffffffu, sv, o); }
+        const float mean_u = su * inv_total, mean_v = sv * inv_total;
+        su = sv = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPartsPerLane; ++k) {
+          const float du = u[k].x - mean_u, dv = v[k].x - mean_v;
+          su += fmaf(du * du, n[k], u[k].y); sv += fmaf(dv * dv, n[k], v[k].y);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { su += __shfl_xor_sync(0xffffffffu, su, o); sv += __shfl_xor_sync(0xffffffffu, sv, o); }
+        if (lane == 0) { stat[g] = mean_u; stat[a.groups + g] = 1.0f / sqrtf(su * inv_total + a.eps); }
+        if (lane == 1) { stat[h] = mean_v; stat[a.groups + h] = 1.0f / sqrtf(sv * inv_total + a.eps); }
       }
     } else {
       for (int g = tid; g < a.groups; g += kThreads) stat[a.groups + g] = 1.0f / sqrtf(stat[a.groups + g] * inv_count + a.eps);
@@ -436,30 +452,61 @@ pq_group_norm_kernel(const NormArgs a) {
 
     // ---------------------------------------------------------------- normalisation
     const int64_t out0 = static_cast<int64_t>(b) * a.out_batch + static_cast<int64_t>(r0) * a.out_row;
+    if constexpr (MODE == kOut16) {
+      const bool ring = segs > kSlots;                                    // else one sweep over rows that are all there
 #pragma unroll 1
-    for (int s = segs - 1; s >= 0; --s) {
-      if (s < segs - kSlots) wait_full(s);
-      const int n = min(a.seg_rows, rows - s * a.seg_rows);
-      const uint32_t at = rows_s + (s % kSlots) * slot_bytes;
+      for (int s = ring ? segs - 1 : 0; s >= 0; --s) {
+        if (s < segs - kSlots) wait_full(s);
+        const int n = ring ? min(a.seg_rows, rows - s * a.seg_rows) : rows;
+        const uint32_t at = rows_s + (s % kSlots) * slot_bytes;
+#pragma unroll 1
+        for (int k = 0; k < COLS; ++k) {
+          const int col = col0 + k * l.cols;
+          if (rl >= l.R || col >= l.ncol) break;
+          if (COLS > 1) f.request(a, col * 8);
+          if (COLS > 1 || !ring || s == segs - 1) f.complete(a, stat, col * 8);
+          T* oc = static_cast<T*>(a.out) + out0 + static_cast<int64_t>(s * a.seg_rows) * a.out_row + col * 8;
+#pragma unroll kApplyUnroll
+          for (int r = rl; r < n; r += l.R)
+            st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, f(ld_shared_v4(at + r * row_bytes + col * 16), a.silu));
+        }
+        if (ring) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[s % kSlots]);
+          // the segment done before this one makes room; its slot's next one, going down, is kSlots before it
+          if (warp == 0 && s + 1 < segs && s + 1 - kSlots >= 0) refill(s + 1, s + 1 - kSlots, (((s + 1) / kSlots) & 1) ^ 1u);
+        }
+      }
+    } else {
+      // lanes of one row that share an atomic maximum: eight, four, two or one neighbours, as the columns divide
+      const int share = (l.ncol & 7) == 0 ? 8 : ((l.ncol & 3) == 0 ? 4 : ((l.ncol & 1) == 0 ? 2 : 1));
 #pragma unroll 1
       for (int k = 0; k < COLS; ++k) {
         const int col = col0 + k * l.cols;
-        if (rl >= l.R || col >= l.ncol) break;
-        if (COLS > 1) f.request(a, col * 8);
-        if (COLS > 1 || s == segs - 1) f.complete(a, stat, col * 8);
-        T* oc = static_cast<T*>(a.out) + out0 + static_cast<int64_t>(s * a.seg_rows) * a.out_row + col * 8;
-#pragma unroll kApplyUnroll
-        for (int r = rl; r < n; r += l.R) {
-          const uint4 z = f(ld_shared_v4(at + r * row_bytes + col * 16), a.silu);
-          if constexpr (MODE != kOut16) st_shared_v4(at + r * row_bytes + col * 16, z);
-          if (MODE == kOut16 || a.out != nullptr) st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, z);
+        const bool mine = rl < l.R && col < l.ncol;
+        if (mine) {
+          if (COLS > 1) f.request(a, col * 8);
+          f.complete(a, stat, col * 8);
         }
-      }
-      if (segs > kSlots) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s % kSlots]);
-        // the segment done before this one makes room; its slot's next one, going down, is kSlots before it
-        if (warp == 0 && s + 1 < segs && s + 1 - kSlots >= 0) refill(s + 1, s + 1 - kSlots, (((s + 1) / kSlots) & 1) ^ 1u);
+#pragma unroll 2
+        for (int rb = 0; rb < rows; rb += l.R) {
+          const int r = rb + rl;
+          const bool ok = mine && r < rows;
+          uint32_t m = 0u;
+          if (ok) {
+            const uint32_t at = rows_s + r * row_bytes + col * 16;
+            const uint4 z = f(ld_shared_v4(at), a.silu);
+            st_shared_v4(at, z);
+            if (a.out != nullptr) st_v4_cs(static_cast<T*>(a.out) + out0 + static_cast<int64_t>(r) * a.out_row + col * 8, z);
+            if constexpr (MODE != kMx) m = max_pattern(absmax_chunk<T>(0u, z));
+          }
+          if constexpr (MODE != kMx) {
+            if (share >= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            if (share >= 4) m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            if (share >= 8) m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            if (ok && (tid & (share - 1)) == 0) atomicMax(&amax[r], m);
+          }
+        }
       }
     }
     if constexpr (MODE != kOut16) {
@@ -468,24 +515,6 @@ pq_group_norm_kernel(const NormArgs a) {
       const int nch = a.nch, R2 = a.R2;
       const int r2 = group_of(tid, a.inv_nch), ci = tid - r2 * nch;
       const bool active = r2 < R2;
-      if constexpr (MODE != kMx) {
-#pragma unroll 1
-        for (int rb = 0; rb < rows; rb += R2) {
-          const int r = rb + r2;
-          const bool ok = active && r < rows;
-          uint32_t m = 0u;
-          if (ok) {
-            const uint32_t at = rows_s + r * row_bytes + ci * 32;
-            m = max_pattern(absmax_chunk<T>(absmax_chunk<T>(0u, ld_shared_v4(at)), ld_shared_v4(at + 16)));
-          }
-          // lanes of one row first, as far as rows divide into equal shares of lanes
-          int share = 1;
-          if ((nch & 1) == 0) { m = max(m, __shfl_xor_sync(0xffffffffu, m, 1)); share = 2; }
-          if ((nch & 3) == 0) { m = max(m, __shfl_xor_sync(0xffffffffu, m, 2)); share = 4; }
-          if (ok && (tid & (share - 1)) == 0) atomicMax(&amax[r], m);
-        }
-        __syncthreads();
-      }
       const int64_t tiles = MODE == kInt8 ? 0 : fp4_scale_tiles(a.C, MODE == kMx ? PQ_FP4_MX : PQ_FP4_NV);
 #pragma unroll 1
       for (int rb = 0; rb < rows; rb += R2) {
