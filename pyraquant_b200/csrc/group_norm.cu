@@ -75,7 +75,7 @@ struct NormArgs {
   // microsecond, and there would be eight of them
   Lanes l; NormSmem lay;
   int cpg, nch, R2;                                 // channels per group; units of 16 channels, rows of them side by side
-  float inv_cpg, inv_cols, inv_nch;
+  float inv_cpg, inv_cols, inv_nch, inv_R;
   float eps;
 };
 
@@ -88,22 +88,16 @@ __device__ __forceinline__ float ex2_approx(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// z * sigmoid(z) for four values with one reciprocal: with E = exp(-|z|) in [0, 1] and h = E / (1 + E), it is z - z h for z >= 0
-// and z h below, max(z, 0) - |z| h in both cases; the product of four denominators stays within [1, 16].  (Two special-function
-// operations per value, an exponential and a reciprocal, bound the normalisation of bf16 rows otherwise.)  With
-// t = -|z| log2(e), the argument of the exponential to the base 2, -|z| h = t (ln(2) h).
-__device__ __forceinline__ void silu4(float2& u, float2& v) {
-  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  const float2 t0 = make_float2(fabsf(u.x) * -kLog2e, fabsf(u.y) * -kLog2e), t1 = make_float2(fabsf(v.x) * -kLog2e, fabsf(v.y) * -kLog2e);
-  const float2 e0 = make_float2(ex2_approx(t0.x), ex2_approx(t0.y)), e1 = make_float2(ex2_approx(t1.x), ex2_approx(t1.y));
-  const float2 one = make_float2(1.0f, 1.0f);
-  const float2 d0 = __fadd2_rn(e0, one), d1 = __fadd2_rn(e1, one);
-  const float p0 = d0.x * d0.y, p1 = d1.x * d1.y;
-  const float r = rcp_approx(p0 * p1) * kLn2;
-  const float r0 = r * p1, r1 = r * p0;
-  const float2 h0 = __fmul2_rn(e0, make_float2(r0 * d0.y, r0 * d0.x)), h1 = __fmul2_rn(e1, make_float2(r1 * d1.y, r1 * d1.x));
-  u = __ffma2_rn(t0, h0, make_float2(fmaxf(u.x, 0.0f), fmaxf(u.y, 0.0f)));
-  v = __ffma2_rn(t1, h1, make_float2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f)));
+// z * sigmoid(z) = z / (1 + 2^t), t = -z log2(e), for two values with one reciprocal: 1 / d0 = d1 / (d0 d1).  An exponential and a
+// reciprocal per value would keep the special-function pipe busy for 16 cycles a warp; this takes 12, next to about nine
+// instructions a value in all.  t is held at 60 so that the product stays finite: below z = -41.6, where the result is under
+// 4e-17 in size, it comes out as z 2^-60.
+__device__ __forceinline__ float2 silu2(float2 z) {
+  const float2 t = __fmul2_rn(z, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  const float2 e = make_float2(ex2_approx(fminf(t.x, 60.0f)), ex2_approx(fminf(t.y, 60.0f)));
+  const float2 d = __fadd2_rn(e, make_float2(1.0f, 1.0f));
+  const float r = rcp_approx(d.x * d.y);
+  return __fmul2_rn(z, make_float2(r * d.y, r * d.x));
 }
 
 template <typename T>
@@ -129,23 +123,23 @@ __device__ __forceinline__ void st_shared_v4(uint32_t a, const uint4& v) {
 struct ColumnSums {
   float2 neg[4], s1[4], s2[4];          // -pivot, sum of x - pivot, of its square
   float count;
-  int n;
   __device__ __forceinline__ float mean(int i) const { return -(i & 1 ? neg[i >> 1].y : neg[i >> 1].x); }
   __device__ __forceinline__ float m2(int i) const { return i & 1 ? s2[i >> 1].y : s2[i >> 1].x; }
   __device__ __forceinline__ void clear() {
-    n = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) neg[i] = s1[i] = s2[i] = make_float2(0.0f, 0.0f);
+  }
+  template <typename T>
+  __device__ __forceinline__ void pivot(const uint4& v) {
+    float2 f[4];
+    unpack8<T>(v, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) neg[i] = make_float2(-f[i].x, -f[i].y);
   }
   template <typename T>
   __device__ __forceinline__ void add(const uint4& v) {
     float2 f[4];
     unpack8<T>(v, f);
-    if (n == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) neg[i] = make_float2(-f[i].x, -f[i].y);
-    }
-    ++n;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 d = __fadd2_rn(f[i], neg[i]);
@@ -153,7 +147,7 @@ struct ColumnSums {
       s2[i] = __ffma2_rn(d, d, s2[i]);
     }
   }
-  __device__ __forceinline__ void finish() {
+  __device__ __forceinline__ void finish(int n) {
     count = static_cast<float>(n);
     const float inv = n > 0 ? 1.0f / count : 0.0f;
 #pragma unroll
@@ -216,7 +210,10 @@ struct Affine8 {
     unpack8<T>(v, f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = __ffma2_rn(__fadd2_rn(f[i], neg_mean[i]), mul[i], add[i]);
-    if (with_silu) { silu4(f[0], f[1]); silu4(f[2], f[3]); }
+    if (with_silu) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = silu2(f[i]);
+    }
     T tag{};
     return make_uint4(pack2(f[0].x, f[0].y, tag), pack2(f[1].x, f[1].y, tag), pack2(f[2].x, f[2].y, tag), pack2(f[3].x, f[3].y, tag));
   }
@@ -362,6 +359,7 @@ pq_group_norm_kernel(const NormArgs a) {
     ColumnSums cs[COLS];
 #pragma unroll
     for (int k = 0; k < COLS; ++k) cs[k].clear();
+    int taken = 0;
 #pragma unroll 1
     for (int s = 0; s < segs; ++s) {
       wait_full(s);
@@ -370,9 +368,11 @@ pq_group_norm_kernel(const NormArgs a) {
 #pragma unroll
       for (int k = 0; k < COLS; ++k)
         if (rl < l.R && col0 + k * l.cols < l.ncol) {
+          if (taken == 0 && rl < n) cs[k].template pivot<T>(ld_shared_v4(at + rl * row_bytes + k * l.cols * 16));
 #pragma unroll 2
           for (int r = rl; r < n; r += l.R) cs[k].template add<T>(ld_shared_v4(at + r * row_bytes + k * l.cols * 16));
         }
+      if (rl < n) taken += group_of(n - rl + l.R - 1, a.inv_R);           // rows this thread has taken
       if (segs > kSlots) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s % kSlots]);
@@ -381,7 +381,7 @@ pq_group_norm_kernel(const NormArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < COLS; ++k) {
-      cs[k].finish();
+      cs[k].finish(taken);
       const int col = col0 + k * l.cols;
       if (rl < l.R && col < l.ncol) put8(red + rl * a.C + col * 8, [&](int i) { return cs[k].mean(i) * cs[k].count; });
     }
@@ -596,7 +596,7 @@ int launch_norm(NormArgs a, cudaStream_t st) {
   a.lay = smem_of(a.C, a.groups, slots * seg);
   if (a.lay.total > kSmemMax) return PQ_ERR_UNSUPPORTED;
   a.cpg = a.C / a.groups; a.inv_cpg = 1.0f / static_cast<float>(a.cpg);
-  a.inv_cols = 1.0f / static_cast<float>(a.l.cols);
+  a.inv_cols = 1.0f / static_cast<float>(a.l.cols); a.inv_R = 1.0f / static_cast<float>(a.l.R);
   a.nch = a.C >> 4; a.R2 = a.nch > 0 ? kThreads / a.nch : 0; a.inv_nch = a.nch > 0 ? 1.0f / static_cast<float>(a.nch) : 0.0f;
   auto kern = pq_group_norm_kernel<T, MODE, COLS>;
   static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes

@@ -4,10 +4,9 @@ Bound.  A thread sums at most L rows of x - pivot one after the other (L <= 64 f
 follow: the mean is off by at most (L + 64) 2^-24 mean|x - pivot|, with |x - pivot| taken as at most 8 deviations, plus
 one rounding of its own size, 2^-24 |mean| a few times over; the variance likewise, relative to itself.  So x-hat is off by
 A (1 + |x-hat|) + 4 2^-24 |mean| / std with A = 128 * 8 * 2^-24.  gamma multiplies that, SiLU's slope is at most 1.1 and its own
-evaluation, max(z, 0) + t (ln(2) h) with t = -|z| log2(e), h = E / (1 + E), E = 2^t and one reciprocal for four denominators,
-loses (in units of 2^-24): |z| (t rounds) + 4 (exponential) in E, 2 in the products of denominators and 1 in theirs, 2 in the
-reciprocal, 2 with ln(2), 3 in the products around it, 1 in t itself, 1 in the sum: (16 + |z|) 2^-24 of |z| h, which is the value
-below 0 and at most the value above.  The
+evaluation, z / (1 + 2^t) with t = -z log2(e) and one reciprocal for two denominators, loses (in units of 2^-24): 1 + |z| (t rounds)
+and 4 (exponential) in 2^t, 1 in the denominator that does not cancel, 1 in the product of the two, 2 in the reciprocal, 1 + 1 in
+the products with it: (11 + |z|) 2^-24 of the value.  The
 rounding to 16 bits is eps / 2 of the value or half the smallest subnormal.
 """
 import ctypes
@@ -37,7 +36,7 @@ def formula(x, groups, w, b, eps, act):
     z = xh.reshape(B, T, C) * w + b
     err = err.reshape(B, T, C) * w.abs() + 2.0 ** -23 * (z.abs() + b.abs())
     if act == "silu":
-        z, err = z / (1 + torch.exp(-z)), 1.1 * err + (16 + z.abs()) * 2.0 ** -24 * (z / (1 + torch.exp(-z))).abs()
+        z, err = z / (1 + torch.exp(-z)), 1.1 * err + (11 + z.abs()) * 2.0 ** -24 * (z / (1 + torch.exp(-z))).abs()
     return z, err
 
 
