@@ -29,7 +29,6 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxC = 8192;
 constexpr int kSlots = 8;                         // segments in shared memory
 constexpr int kSmemMax = 232448;
-constexpr int kApplyUnroll = 2;
 constexpr int kPartsPerLane = 5;                  // chunks of a sample: at most 160
 
 enum Mode { kOut16 = 0, kInt8 = 1, kMx = 2, kNv = 3 };
@@ -204,6 +203,23 @@ struct Affine8 {
       neg_mean[i] = make_float2(-stat[g0], -stat[g1]);
       mul[i] = __fmul2_rn(mul[i], make_float2(stat[a.groups + g0], stat[a.groups + g1]));
     }
+  }
+  __device__ __forceinline__ void both(const uint4& v, const uint4& w, int with_silu, uint4& zv, uint4& zw) const {
+    float2 f[4], g[4];
+    unpack8<T>(v, f);
+    unpack8<T>(w, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i] = __ffma2_rn(__fadd2_rn(f[i], neg_mean[i]), mul[i], add[i]);
+      g[i] = __ffma2_rn(__fadd2_rn(g[i], neg_mean[i]), mul[i], add[i]);
+    }
+    if (with_silu) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { f[i] = silu2(f[i]); g[i] = silu2(g[i]); }
+    }
+    T tag{};
+    zv = make_uint4(pack2(f[0].x, f[0].y, tag), pack2(f[1].x, f[1].y, tag), pack2(f[2].x, f[2].y, tag), pack2(f[3].x, f[3].y, tag));
+    zw = make_uint4(pack2(g[0].x, g[0].y, tag), pack2(g[1].x, g[1].y, tag), pack2(g[2].x, g[2].y, tag), pack2(g[3].x, g[3].y, tag));
   }
   __device__ __forceinline__ uint4 operator()(const uint4& v, int with_silu) const {
     float2 f[4];
@@ -466,9 +482,17 @@ pq_group_norm_kernel(const NormArgs a) {
           if (COLS > 1) f.request(a, col * 8);
           if (COLS > 1 || !ring || s == segs - 1) f.complete(a, stat, col * 8);
           T* oc = static_cast<T*>(a.out) + out0 + static_cast<int64_t>(s * a.seg_rows) * a.out_row + col * 8;
-#pragma unroll kApplyUnroll
-          for (int r = rl; r < n; r += l.R)
-            st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, f(ld_shared_v4(at + r * row_bytes + col * 16), a.silu));
+          // two rows at a time: their chains of dependent operations interleave
+          int r = rl;
+#pragma unroll 1
+          for (; r + l.R < n; r += 2 * l.R) {
+            const uint4 v0 = ld_shared_v4(at + r * row_bytes + col * 16), v1 = ld_shared_v4(at + (r + l.R) * row_bytes + col * 16);
+            uint4 z0, z1;
+            f.both(v0, v1, a.silu, z0, z1);
+            st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, z0);
+            st_v4_cs(oc + static_cast<int64_t>(r + l.R) * a.out_row, z1);
+          }
+          if (r < n) st_v4_cs(oc + static_cast<int64_t>(r) * a.out_row, f(ld_shared_v4(at + r * row_bytes + col * 16), a.silu));
         }
         if (ring) {
           __syncwarp();
