@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from .int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR, _eager, is_bf16_whitelisted
+from .int8_exec import LOWRANK_A_ATTR, LOWRANK_B_ATTR, LowRankFactors, _eager, is_bf16_whitelisted
 
 FORMATS = tuple(ops.FP4_FORMATS)
 DEFAULT_FORMAT = "nv"
@@ -108,7 +108,7 @@ def quantize_weight_fp4(w: torch.Tensor, fmt: str = DEFAULT_FORMAT) -> Fp4Rows:
 
 
 # --------------------------------------------------------------------------- module
-class Fp4Linear(nn.Module):
+class Fp4Linear(LowRankFactors, nn.Module):
     """4-bit stand-in for ``nn.Linear``: packed weights held as buffers, activations quantised per call in the same
     format.  A low-rank branch (``lowrank=(A, B)`` or the ``_lowrank_A`` / ``_lowrank_B`` attributes that
     ``Int8Linear`` reads too) is added in the activation type after the product, ``y += (x @ A) @ B``.
@@ -160,7 +160,7 @@ class Fp4Linear(nn.Module):
     def _product(self, xq: Fp4Rows, x2: torch.Tensor) -> torch.Tensor:
         y = fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype)
         if self.lr_A is not None:
-            y.addmm_((x2.to(self.lr_A.dtype) @ self.lr_A).to(y.dtype), self.lr_B.to(y.dtype))
+            y.addmm_(self._down(x2).to(y.dtype), self.lr_B.to(y.dtype))
         return y
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

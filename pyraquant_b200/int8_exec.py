@@ -266,7 +266,37 @@ FLUX_SHARED_INPUT_GROUPS = (
 )
 
 
-class Int8Linear(nn.Module):
+class LowRankFactors:
+    """What the Linears with a low-rank branch share: K-major copies of the factors, made once, and the down-projection."""
+
+    def _lr_Bt(self) -> torch.Tensor:
+        """K-major copy of lr_B for the tensor-core low-rank path, made once per device/dtype (not part of the state)."""
+        return self._transposed("lr_B")
+
+    def _lr_At(self) -> torch.Tensor:
+        """K-major copy of lr_A ([32, K]) for the native down-projection kernel, made once (not part of the state)."""
+        return self._transposed("lr_A")
+
+    def _transposed(self, name: str) -> torch.Tensor:
+        """Contiguous transpose of a low-rank factor, remade whenever the buffer is replaced, converted (.to / .half),
+        moved or written in place."""
+        src = getattr(self, name)
+        key = (src.data_ptr(), src.dtype, src.device, tuple(src.shape), ops.tensor_version(src))
+        c = self.__dict__.get("_t_cache_" + name)
+        if c is None or c[0] != key:
+            c = (key, src.t().contiguous())
+            self.__dict__["_t_cache_" + name] = c
+        return c[1]
+
+    def _down(self, x2: torch.Tensor) -> torch.Tensor:
+        """t = x2 @ lr_A rounded to the activation dtype (reference :390): the native streaming kernel for rank 32
+        on inputs it takes as they are (any row count), torch's matmul otherwise (other ranks, dtypes, unaligned rows)."""
+        if self.lr_A.shape[1] == 32 and self.lr_A.dtype == x2.dtype and ops.lowrank_down_ok(x2):
+            return ops.lowrank_down(x2, self._lr_At())
+        return x2.to(self.lr_A.dtype) @ self.lr_A
+
+
+class Int8Linear(LowRankFactors, nn.Module):
     """INT8 stand-in for ``nn.Linear``: per-channel INT8 weights held as buffers, per-token dynamic INT8
     activations, optional rank-r low-rank branch executed for real (down-projection as a small GEMM,
     up-projection inside the INT8 GEMM epilogue)."""
@@ -305,32 +335,6 @@ class Int8Linear(nn.Module):
     def __getstate__(self):
         """Copies and pickles leave the address caches behind (they are remade on the first forward)."""
         return {k: v for k, v in self.__dict__.items() if k != "_lean_cache"}
-
-    def _lr_Bt(self) -> torch.Tensor:
-        """K-major copy of lr_B for the tensor-core low-rank path, made once per device/dtype (not part of the state)."""
-        return self._transposed("lr_B")
-
-    def _lr_At(self) -> torch.Tensor:
-        """K-major copy of lr_A ([32, K]) for the native down-projection kernel, made once (not part of the state)."""
-        return self._transposed("lr_A")
-
-    def _transposed(self, name: str) -> torch.Tensor:
-        """Contiguous transpose of a low-rank factor, remade whenever the buffer is replaced, converted (.to / .half),
-        moved or written in place."""
-        src = getattr(self, name)
-        key = (src.data_ptr(), src.dtype, src.device, tuple(src.shape), ops.tensor_version(src))
-        c = self.__dict__.get("_t_cache_" + name)
-        if c is None or c[0] != key:
-            c = (key, src.t().contiguous())
-            self.__dict__["_t_cache_" + name] = c
-        return c[1]
-
-    def _down(self, x2: torch.Tensor) -> torch.Tensor:
-        """t = x2 @ lr_A rounded to the activation dtype (reference :390): the native streaming kernel for rank 32
-        on inputs it takes as they are (any row count), torch's matmul otherwise (other ranks, dtypes, unaligned rows)."""
-        if self.lr_A.shape[1] == 32 and self.lr_A.dtype == x2.dtype and ops.lowrank_down_ok(x2):
-            return ops.lowrank_down(x2, self._lr_At())
-        return x2.to(self.lr_A.dtype) @ self.lr_A
 
     def _one_launch_prologue(self, x2: torch.Tensor) -> bool:
         return (self.lr_A.shape[1] == 32 and self.lr_A.dtype == x2.dtype and ops.quant_lowrank_ok(x2)

@@ -42,13 +42,17 @@ def _stream(t: Tensor) -> int:
         return torch.cuda.current_stream(t.device).cuda_stream
 
 
+# torch.cuda.current_device() without its check that CUDA is initialised (a tensor of the device exists already)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 class _on_device:
     """`with torch.cuda.device(...)` only when the tensor lives on another device than the current one: the
     context manager costs several microseconds, which matters for the small 1K-stage layers."""
     __slots__ = ("ctx",)
 
     def __init__(self, t: Tensor):
-        self.ctx = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+        self.ctx = None if t.get_device() == _current_device() else torch.cuda.device(t.device)
 
     def __enter__(self):
         if self.ctx is not None:
