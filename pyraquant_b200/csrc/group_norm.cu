@@ -4,14 +4,14 @@
 //
 // HBM-bound: 2 bytes read and 2 (z), 1 (INT8) or 0.53 to 0.56 (4-bit) written per element, provided x is read once although the
 // statistics are needed before the first output.  So one cooperative launch of one CTA per SM: the T rows of a sample are
-// cut into P consecutive chunks, one per CTA, which pass through a ring of eight segments in shared memory (200 KB, 30 MB
+// cut into P consecutive chunks, one per CTA, which pass through a ring of four segments in shared memory (200 KB, 30 MB
 // over the GPU) by bulk copies, and what the ring holds at the end of the first pass is not read again for the second.
 //   1. First to last segment: a thread has a fixed column of eight channels and every R-th row and sums x - pivot and its
 //      square per channel, the pivot being its first value (the sum of squares must not cancel when the mean is large
 //      against the deviation).  The CTA's mean of a group is the sum of the threads' sums, its centred sum of squares that
 //      of M2_thread + n (mean_thread - mean)^2: no cancellation, fixed order.
 //   2. After a grid barrier every CTA does the same with the P chunks of its sample, and normalises its rows, last to
-//      first segment: the last eight are there, of the others the ones read last are the likeliest to be in L2 still.
+//      first segment: the last four are there, of the others the ones read last are the likeliest to be in L2 still.
 // The quantising forms put z back into shared memory, take every row's largest magnitude (an atomic maximum of bit patterns,
 // independent of order) and write codes in a third sweep; they need all rows of a chunk in the ring.
 // All statistics and arithmetic are fp32.
@@ -27,7 +27,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxC = 8192;
-constexpr int kSlots = 8;                         // segments in shared memory
+constexpr int kSlots = 4;                         // segments in shared memory (1 x 262144 x 256: eight 75.5 us, four 73.6)
 constexpr int kSmemMax = 232448;
 constexpr int kPartsPerLane = 5;                  // chunks of a sample: at most 160
 
@@ -168,7 +168,7 @@ __device__ __forceinline__ void put8(float* dst, F&& f) {
 template <typename T>
 struct Affine8 {
   uint4 raw[2][2];                        // gamma, beta: eight 16-bit values in [0], or eight fp32 ones
-  float2 neg_mean[4], mul[4], add[4];
+  float2 mul[4], add[4];                  // z = x mul + add; add holds -mean mul too, which costs half a unit of 2^-24 |mean| / std
   __device__ __forceinline__ void request(const NormArgs& a, int c0) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -200,8 +200,8 @@ struct Affine8 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int g0 = group_of(c0 + 2 * i, a.inv_cpg), g1 = group_of(c0 + 2 * i + 1, a.inv_cpg);
-      neg_mean[i] = make_float2(-stat[g0], -stat[g1]);
       mul[i] = __fmul2_rn(mul[i], make_float2(stat[a.groups + g0], stat[a.groups + g1]));
+      add[i] = __ffma2_rn(make_float2(-stat[g0], -stat[g1]), mul[i], add[i]);
     }
   }
   __device__ __forceinline__ void both(const uint4& v, const uint4& w, int with_silu, uint4& zv, uint4& zw) const {
@@ -210,8 +210,8 @@ struct Affine8 {
     unpack8<T>(w, g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f[i] = __ffma2_rn(__fadd2_rn(f[i], neg_mean[i]), mul[i], add[i]);
-      g[i] = __ffma2_rn(__fadd2_rn(g[i], neg_mean[i]), mul[i], add[i]);
+      f[i] = __ffma2_rn(f[i], mul[i], add[i]);
+      g[i] = __ffma2_rn(g[i], mul[i], add[i]);
     }
     if (with_silu) {
 #pragma unroll
@@ -225,7 +225,7 @@ struct Affine8 {
     float2 f[4];
     unpack8<T>(v, f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = __ffma2_rn(__fadd2_rn(f[i], neg_mean[i]), mul[i], add[i]);
+    for (int i = 0; i < 4; ++i) f[i] = __ffma2_rn(f[i], mul[i], add[i]);
     if (with_silu) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = silu2(f[i]);
@@ -606,11 +606,11 @@ int launch_norm(NormArgs a, cudaStream_t st) {
   const int fixed = smem_of(a.C, a.groups, 0).total + 256;
   const int most = fixed < kSmemMax ? (kSmemMax - fixed) / (a.C * 2 + 4) : 0;     // rows of the ring
   a.l = lanes_of(a.C);
-  // segments of whole steps of R rows where that leaves all rows in the ring, then of an eighth of the rows, then of an eighth
+  // segments of whole steps of R rows where that leaves all rows in the ring, then of a quarter of the rows, then of a quarter
   // of the ring
-  const int R = a.l.R, eighth = (longest + kSlots - 1) / kSlots, steps = (eighth + R - 1) / R * R;
+  const int R = a.l.R, quarter = (longest + kSlots - 1) / kSlots, steps = (quarter + R - 1) / R * R;
   auto ring = [&](int rows) { return (longest + rows - 1) / rows * rows; };
-  int seg = ring(steps) <= most ? steps : (ring(eighth) <= most ? eighth : most / kSlots);
+  int seg = ring(steps) <= most ? steps : (ring(quarter) <= most ? quarter : most / kSlots);
   if (ring(seg) > most && seg > R) seg = seg / R * R;
   if (seg < 1) return PQ_ERR_UNSUPPORTED;                                  // thousands of groups of thousands of channels
   if (MODE != kOut16 && static_cast<int64_t>(seg) * kSlots < longest) return PQ_ERR_UNSUPPORTED;      // rows beyond the chip's shared memory

@@ -3,7 +3,8 @@
 Bound.  A thread sums at most L rows of x - pivot one after the other (L <= 64 for the sizes here) and at most 64 merges
 follow: the mean is off by at most (L + 64) 2^-24 mean|x - pivot|, with |x - pivot| taken as at most 8 deviations, plus
 one rounding of its own size, 2^-24 |mean| a few times over; the variance likewise, relative to itself.  So x-hat is off by
-A (1 + |x-hat|) + 4 2^-24 |mean| / std with A = 128 * 8 * 2^-24.  gamma multiplies that, SiLU's slope is at most 1.1 and its own
+A (1 + |x-hat|) + 4 2^-24 |mean| / std with A = 128 * 8 * 2^-24 (a unit of the last term goes to the product of mean and
+slope, which is rounded into the added constant).  gamma multiplies that, SiLU's slope is at most 1.1 and its own
 evaluation, z / (1 + 2^t) with t = -z log2(e) and one reciprocal for two denominators, loses (in units of 2^-24): 1 + |z| (t rounds)
 and 4 (exponential) in 2^t, 1 in the denominator that does not cancel, 1 in the product of the two, 2 in the reciprocal, 1 + 1 in
 the products with it: (11 + |z|) 2^-24 of the value.  The
