@@ -24,6 +24,7 @@ ACT_SILU = 1
 GEMM_WORKSPACE_BYTES = 256
 
 _lib: Optional[ctypes.CDLL] = None
+_binding = None
 
 # name -> (restype, argtypes); mirrors include/pq_b200.h
 SIGNATURES = {
@@ -129,6 +130,19 @@ def load() -> ctypes.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def binding():
+    """The CPython module over the library (csrc/bind.cpp), loaded once; like the library it has no substitute."""
+    global _binding
+    if _binding is None:
+        load()
+        try:
+            from . import _bind
+        except ImportError as e:
+            raise RuntimeError(f"pyraquant_b200/_bind.so does not load ({e}): run `python -m pyraquant_b200.build`") from e
+        _binding = _bind
+    return _binding
 
 
 def status_str(rc: int) -> str:

@@ -1,0 +1,215 @@
+// The eager call of the 4-bit and group-norm operators as CPython functions over the C ABI.
+//
+// A call through ctypes costs 13 to 19 us on the host (operand checks, one to three allocations, twenty argument
+// conversions), a multiple of what these kernels take for few rows.  The functions here do the same for the usual case --
+// CUDA tensors of a supported type whose rows the kernels take as they are -- and return None for every other: the
+// Python layer then does it step by step, with its copies, its other cases and its errors.  No kernel and no arithmetic
+// here.
+#include <Python.h>
+
+#include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include "../../include/pq_b200.h"
+
+namespace {
+
+using at::Tensor;
+
+// the tensor behind a Python object, or nullptr for anything else
+const Tensor* tensor_of(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+
+bool aligned(const Tensor& t, uintptr_t a) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % a == 0; }
+int dtype_code(at::ScalarType t) { return t == at::kBFloat16 ? PQ_DTYPE_BF16 : (t == at::kHalf ? PQ_DTYPE_FP16 : -1); }
+bool plain(const Tensor& t, at::ScalarType type, c10::Device device) {
+  return t.scalar_type() == type && t.device() == device && t.layout() == at::kStrided && t.is_contiguous();
+}
+Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::empty(sizes, like.options().dtype(type)); }
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+PyObject* none() { Py_RETURN_NONE; }
+PyObject* fail(const char* what, int rc) {
+  if (rc == PQ_ERR_CUDA) PyErr_Format(PyExc_RuntimeError, "%s: %s (cudaError %d)", what, pq_status_str(rc), pq_last_cuda_error());
+  else PyErr_Format(PyExc_RuntimeError, "%s: %s", what, pq_status_str(rc));
+  return nullptr;
+}
+// a tuple of new references; an undefined tensor becomes None
+PyObject* tuple3(const Tensor& a, const Tensor& b, const Tensor& c) {
+  PyObject* t = PyTuple_New(3);
+  if (t == nullptr) return nullptr;
+  const Tensor* v[3] = {&a, &b, &c};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* o = v[i]->defined() ? THPVariable_Wrap(*v[i]) : Py_NewRef(Py_None);
+    if (o == nullptr) { Py_DECREF(t); return nullptr; }
+    PyTuple_SET_ITEM(t, i, o);
+  }
+  return t;
+}
+
+// C++ exceptions (allocation failures, a bad device) become Python's
+template <typename F>
+PyObject* guarded(F&& f) {
+  try {
+    return f();
+  } catch (const c10::OutOfMemoryError& e) {
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type = torch != nullptr ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    PyErr_SetString(type != nullptr ? type : PyExc_RuntimeError, e.what_without_backtrace());
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
+  } catch (const c10::Error& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
+Tensor scale_tensor(int64_t M, int64_t K, int fmt, const Tensor& like) {
+  const int64_t per = fmt == PQ_FP4_MX ? 128 : 64;
+  return make({(M + 127) / 128, (K + per - 1) / per, 512}, at::kByte, like);
+}
+// packed rows as the quantising operators return them; `row` nullptr: mx
+bool plain_rows(const Tensor* codes, const Tensor* scales, const Tensor* row) {
+  if (codes == nullptr || scales == nullptr || !codes->is_cuda() || codes->dim() != 2) return false;
+  const int64_t M = codes->size(0), K2 = codes->size(1), per = row == nullptr ? 64 : 32;
+  return plain(*codes, at::kByte, codes->device()) && aligned(*codes, 16) && K2 > 0 && K2 % 16 == 0 && plain(*scales, at::kByte, codes->device()) &&
+         scales->dim() == 3 && scales->size(0) == (M + 127) / 128 && scales->size(1) == (K2 + per - 1) / per && scales->size(2) == 512 &&
+         (row == nullptr || (plain(*row, at::kFloat, codes->device()) && row->dim() == 1 && row->size(0) == M));
+}
+// an argument that is a tensor or None; false for anything else
+bool optional_tensor(PyObject* o, const Tensor** t) {
+  *t = o == Py_None ? nullptr : tensor_of(o);
+  return o == Py_None || *t != nullptr;
+}
+
+// quant_rows_fp4(x [M,K], fmt) -> (codes, scales, row scales or None), or None
+PyObject* quant_rows_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const Tensor* xp = n == 2 ? tensor_of(a[0]) : nullptr;
+    if (xp == nullptr || !xp->is_cuda() || xp->dim() != 2 || xp->layout() != at::kStrided) return none();
+    const Tensor& x = *xp;
+    const int code = dtype_code(x.scalar_type()), fmt = static_cast<int>(PyLong_AsLong(a[1]));
+    const int64_t M = x.size(0), K = x.size(1);
+    if (code < 0 || K <= 0 || K % 32 != 0 || x.stride(1) != 1 || (M > 1 && (x.stride(0) % 16 != 0 || x.stride(0) < K)) || !aligned(x, 32)) return none();
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor codes = make({M, K / 2}, at::kByte, x), scales = scale_tensor(M, K, fmt, x), row;
+    if (fmt == PQ_FP4_NV) row = make({M}, at::kFloat, x);
+    const int rc = pq_quant_rows_fp4(x.data_ptr(), code, M, K, M > 1 ? x.stride(0) : K, fmt, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
+                                     row.defined() ? row.data_ptr<float>() : nullptr, stream_of(x));
+    return rc == PQ_OK ? tuple3(codes, scales, row) : fail("pq_quant_rows_fp4", rc);
+  });
+}
+
+// dequant_rows_fp4(codes, scales, row scales or None, bf16?) -> [M,K], or None
+PyObject* dequant_rows_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const Tensor* row;
+    if (n != 4 || !optional_tensor(a[2], &row)) return none();
+    const Tensor *codes = tensor_of(a[0]), *scales = tensor_of(a[1]);
+    if (!plain_rows(codes, scales, row)) return none();
+    const bool bf16 = a[3] == Py_True;
+    c10::cuda::CUDAGuard guard(codes->device());
+    const int64_t M = codes->size(0), K = codes->size(1) * 2;
+    Tensor out = make({M, K}, bf16 ? at::kBFloat16 : at::kHalf, *codes);
+    const int rc = pq_dequant_rows_fp4(codes->data_ptr<uint8_t>(), K / 2, scales->data_ptr<uint8_t>(), row != nullptr ? row->data_ptr<float>() : nullptr,
+                                       row != nullptr ? PQ_FP4_NV : PQ_FP4_MX, out.data_ptr(), bf16 ? PQ_DTYPE_BF16 : PQ_DTYPE_FP16, K, M, K,
+                                       stream_of(*codes));
+    return rc == PQ_OK ? THPVariable_Wrap(out) : fail("pq_dequant_rows_fp4", rc);
+  });
+}
+
+// fp4_gemm(codes, scales, rows or None of x, the same of w, bias or None, bf16?, workspace, its bytes) -> [M,N], or None
+PyObject* fp4_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const Tensor *x_row, *w_row, *bias;
+    if (n != 10 || !optional_tensor(a[2], &x_row) || !optional_tensor(a[5], &w_row) || !optional_tensor(a[6], &bias)) return none();
+    const Tensor *xq = tensor_of(a[0]), *xs = tensor_of(a[1]), *wq = tensor_of(a[3]), *ws = tensor_of(a[4]);
+    if (!plain_rows(xq, xs, x_row) || !plain_rows(wq, ws, w_row) || (x_row == nullptr) != (w_row == nullptr) ||
+        wq->device() != xq->device() || wq->size(1) != xq->size(1) || wq->size(0) == 0)
+      return none();
+    const int64_t M = xq->size(0), N = wq->size(0), K = xq->size(1) * 2;
+    if (bias != nullptr && (!plain(*bias, at::kFloat, xq->device()) || bias->numel() != N)) return none();
+    const bool bf16 = a[7] == Py_True;
+    c10::cuda::CUDAGuard guard(xq->device());
+    Tensor out = make({M, N}, bf16 ? at::kBFloat16 : at::kHalf, *xq);
+    const int rc = pq_fp4_gemm(xq->data_ptr<uint8_t>(), K / 2, xs->data_ptr<uint8_t>(), x_row != nullptr ? x_row->data_ptr<float>() : nullptr,
+                               wq->data_ptr<uint8_t>(), K / 2, ws->data_ptr<uint8_t>(), w_row != nullptr ? w_row->data_ptr<float>() : nullptr,
+                               bias != nullptr ? bias->data_ptr<float>() : nullptr, x_row != nullptr ? PQ_FP4_NV : PQ_FP4_MX, out.data_ptr(),
+                               bf16 ? PQ_DTYPE_BF16 : PQ_DTYPE_FP16, N, M, N, K, PyLong_AsVoidPtr(a[8]), static_cast<size_t>(PyLong_AsSize_t(a[9])),
+                               stream_of(*xq));
+    return rc == PQ_OK ? THPVariable_Wrap(out) : fail("pq_fp4_gemm", rc);
+  });
+}
+
+// group_norm(x [B,T,C], groups, weight or None, bias or None, eps, act, mode, z wanted?, status word) with mode 0: z, 1: INT8, 2: mx, 3: nv
+// -> z, (q, s, z or None), (codes, scales, row scales or None); None where the Python layer has to look; False for a size
+// that the quantising forms do not take
+PyObject* group_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const Tensor *w, *b;
+    const Tensor* xp = n == 9 ? tensor_of(a[0]) : nullptr;
+    if (xp == nullptr || !optional_tensor(a[2], &w) || !optional_tensor(a[3], &b)) return none();
+    const Tensor& x = *xp;
+    if (!x.is_cuda() || x.dim() != 3 || !PyLong_Check(a[1])) return none();
+    const int code = dtype_code(x.scalar_type());
+    const int64_t B = x.size(0), T = x.size(1), C = x.size(2);
+    const long groups = PyLong_AsLong(a[1]);
+    const double eps = PyFloat_AsDouble(a[4]);
+    const int act = static_cast<int>(PyLong_AsLong(a[5])), mode = static_cast<int>(PyLong_AsLong(a[6]));
+    if (PyErr_Occurred() != nullptr) { PyErr_Clear(); return none(); }
+    if (code < 0 || !plain(x, x.scalar_type(), x.device()) || !aligned(x, 16) || B * T == 0 || B > 65535 || groups <= 0 || groups > C || C % groups != 0 ||
+        C % 8 != 0 || C > 8192 || (mode == 1 && C % 16 != 0) || (mode >= 2 && C % 32 != 0))
+      return none();
+    const bool grad = c10::GradMode::is_enabled();
+    if (grad && x.requires_grad()) return none();
+    for (const Tensor* v : {w, b})
+      if (v != nullptr && (!plain(*v, x.scalar_type(), x.device()) || v->dim() != 1 || v->size(0) != C || !aligned(*v, 16) || (grad && v->requires_grad())))
+        return none();
+    c10::cuda::CUDAGuard guard(x.device());
+    const void* wp = w != nullptr ? w->data_ptr() : nullptr;
+    const void* bp = b != nullptr ? b->data_ptr() : nullptr;
+    const int64_t bytes = pq_group_norm_workspace_bytes(B, T, C, static_cast<int>(groups));
+    Tensor ws = make({bytes}, at::kByte, x);
+    void* status = PyLong_AsVoidPtr(a[8]);
+    void* st = stream_of(x);
+    const float e = static_cast<float>(eps);
+    const int g = static_cast<int>(groups);
+    if (mode == 0) {
+      Tensor z = make({B, T, C}, x.scalar_type(), x);
+      const int rc = pq_group_norm(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, z.data_ptr(), C, T * C, ws.data_ptr(), bytes, status, st);
+      if (rc == PQ_ERR_UNSUPPORTED) return none();
+      return rc == PQ_OK ? THPVariable_Wrap(z) : fail("pq_group_norm", rc);
+    }
+    int rc;
+    PyObject* result = nullptr;
+    if (mode == 1) {
+      Tensor z, q = make({B * T, C}, at::kChar, x), s = make({B * T}, at::kFloat, x);
+      if (a[7] == Py_True) z = make({B, T, C}, x.scalar_type(), x);
+      rc = pq_group_norm_quant_rows(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, z.defined() ? z.data_ptr() : nullptr, C, T * C,
+                                    q.data_ptr<int8_t>(), s.data_ptr<float>(), ws.data_ptr(), bytes, status, st);
+      if (rc == PQ_OK) result = tuple3(q, s, z);
+    } else {
+      const int fmt = mode == 2 ? PQ_FP4_MX : PQ_FP4_NV;
+      Tensor codes = make({B * T, C / 2}, at::kByte, x), scales = scale_tensor(B * T, C, fmt, x), row;
+      if (fmt == PQ_FP4_NV) row = make({B * T}, at::kFloat, x);
+      rc = pq_group_norm_quant_fp4(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, fmt, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
+                                   row.defined() ? row.data_ptr<float>() : nullptr, ws.data_ptr(), bytes, status, st);
+      if (rc == PQ_OK) result = tuple3(codes, scales, row);
+    }
+    if (rc == PQ_ERR_UNSUPPORTED) Py_RETURN_FALSE;
+    return rc == PQ_OK ? result : fail("pq_group_norm_quant", rc);
+  });
+}
+
+#define PQ_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+PyMethodDef kMethods[] = {PQ_FAST(quant_rows_fp4), PQ_FAST(dequant_rows_fp4), PQ_FAST(fp4_gemm), PQ_FAST(group_norm), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bind", "eager calls of the 4-bit and group-norm operators", -1, kMethods,
+                       nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__bind() { return PyModule_Create(&kModule); }

@@ -89,6 +89,17 @@ def _LIB():
     return _lib_handle
 
 
+_bind_handle = None
+
+
+def _BIND():
+    """The one-step calls of csrc/bind.cpp; each returns None for operands that need the steps written out here."""
+    global _bind_handle
+    if _bind_handle is None:
+        _bind_handle = _lib.binding()
+    return _bind_handle
+
+
 def status_word(device: torch.device) -> Tensor:
     """Per-device workspace whose word 0 the GEMM kernels set when a bounded wait gives up."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -260,86 +271,67 @@ def group_norm_args(x: Tensor, groups: int, weight: Optional[Tensor], bias: Opti
     return x3, weight, bias, GROUP_NORM_ACTS[act]
 
 
-_sm_counts: Dict[int, int] = {}
-_norm_workspaces: Dict[Tuple[int, int], Tensor] = {}
-_NORM_WORKSPACE_BYTES = 1 << 20
-
-
-def _norm_workspace(x: Tensor, index: int, stream: int, nbytes: int) -> Tensor:
-    """The chunk statistics' buffer: one per (device, stream), whose launches follow one another, for the eager calls; a fresh one
-    while the stream is captured (graphs may be replayed side by side) and for the rare larger sizes."""
-    if nbytes > _NORM_WORKSPACE_BYTES or torch.cuda.is_current_stream_capturing():
-        return x.new_empty((nbytes,), dtype=torch.uint8)
-    ws = _norm_workspaces.get((index, stream))
-    if ws is None:
-        with torch.inference_mode(False):
-            ws = torch.empty((_NORM_WORKSPACE_BYTES,), dtype=torch.uint8, device=x.device)
-        _norm_workspaces[(index, stream)] = ws
-    return ws
-
-
 def _group_norm_call(name: str, x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
                      act: Optional[str], outputs):
-    """Runs one of the pq_group_norm entry points on x; `outputs(x, B, T, C)` allocates and returns (result, the entry point's
-    output arguments).  None when the entry point does not take the size (its rows do not fit on the chip)."""
-    shape = x.shape
-    dtype = x.dtype
-    C = shape[-1]
-    index = x.get_device()
-    # contiguous rows and plain vectors of their type, the usual case, are recognised without the general checks
-    if (index >= 0 and len(shape) == 3 and dtype in _DT and x.is_contiguous() and x.data_ptr() % 16 == 0 and groups > 0
-            and C % 8 == 0 and 0 < C <= GROUP_NORM_MAX_C and C % groups == 0 and act in GROUP_NORM_ACTS
-            and not (x.requires_grad and torch.is_grad_enabled())
-            and (weight is None or _plain_affine(weight, dtype, C, index))
-            and (bias is None or _plain_affine(bias, dtype, C, index))):
-        x3, code, f32 = x, GROUP_NORM_ACTS[act], 0
-        B, T, _ = shape
-        ld, ld_batch = C, T * C
-    else:
-        x3, weight, bias, code = group_norm_args(x, groups, weight, bias, act)
-        B, T, C = x3.shape
-        ld, ld_batch = x3.stride(1) if T > 1 else C, x3.stride(0) if B > 1 else T * C
-        f32 = int((weight is not None and weight.dtype == torch.float32) or (bias is not None and bias.dtype == torch.float32))
+    """Runs one of the pq_group_norm entry points on x, step by step, for what the one-step call (csrc/bind.cpp) leaves to it.
+    `outputs(x3, B, T, C)` allocates and returns (result, the entry point's output arguments).  None when the entry point does
+    not take the size (its rows do not fit on the chip)."""
+    x3, weight, bias, code = group_norm_args(x, groups, weight, bias, act)
+    B, T, C = x3.shape
     result, args = outputs(x3, B, T, C)
     if B * T == 0:
         return result
-    sms = _sm_counts.get(index)
-    if sms is None:
-        sms = _sm_counts[index] = torch.cuda.get_device_properties(index).multi_processor_count
-    nbytes = (sms if sms > B else B) * groups * 8               # B times the chunks of a sample, or more
+    lib = _LIB()
+    f32 = (weight is not None and weight.dtype == torch.float32) or (bias is not None and bias.dtype == torch.float32)
     with _on_device(x3):
-        stream = _stream(x3)
-        rc = getattr(_LIB(), name)(x3.data_ptr(), _DT[dtype], B, T, C, ld, ld_batch, groups, _ptr(weight), _ptr(bias), f32, eps, code,
-                                   *args, _norm_workspace(x3, index, stream, nbytes).data_ptr(), nbytes,
-                                   status_word(x3.device).data_ptr(), stream)
+        nbytes = lib.pq_group_norm_workspace_bytes(B, T, C, groups)
+        ws = x3.new_empty((nbytes,), dtype=torch.uint8)
+        rc = getattr(lib, name)(x3.data_ptr(), _DT[x.dtype], B, T, C, x3.stride(1) if T > 1 else C, x3.stride(0) if B > 1 else T * C,
+                                groups, _ptr(weight), _ptr(bias), int(f32), float(eps), code, *args, ws.data_ptr(), nbytes,
+                                status_word(x3.device).data_ptr(), _stream(x3))
+    if rc == _lib.PQ_ERR_UNSUPPORTED:
+        return None
     if rc:
-        if rc == _lib.PQ_ERR_UNSUPPORTED:
-            return None
         _lib.check(rc, f"{name}(B={B}, T={T}, C={C}, groups={groups})")
     return result
 
 
-def _plain_affine(v: Tensor, dtype: torch.dtype, C: int, index: int) -> bool:
-    return (v.dtype is dtype and v.dim() == 1 and v.numel() == C and v.is_contiguous() and v.get_device() == index
-            and v.data_ptr() % 16 == 0 and not (v.requires_grad and torch.is_grad_enabled()))
+# what csrc/bind.cpp calls the forms of the norm
+_NORM_Z, _NORM_INT8, _NORM_FP4 = 0, 1, {"mx": 2, "nv": 3}
+
+
+def _group_norm_bound(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, act: Optional[str],
+                      mode: int, want_z: bool):
+    """The one-step call: its result, None for operands that need the general one, False for rows that do not fit."""
+    code = GROUP_NORM_ACTS.get(act, -1)
+    if code < 0 or x.dim() != 3 or not x.is_cuda:
+        return None
+    return _BIND().group_norm(x, groups, weight, bias, eps, code, mode, want_z, status_word(x.device).data_ptr())
 
 
 def _group_norm_impl(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
                      act: Optional[str]) -> Tensor:
+    out = _group_norm_bound(x, groups, weight, bias, eps, act, _NORM_Z, True)
+    if out is not None:
+        return out
+
     def outputs(x3, B, T, C):
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        return out, (out.data_ptr(), C, T * C)
+        z = torch.empty_like(x, memory_format=torch.contiguous_format)
+        return z, (z.data_ptr(), C, T * C)
     out = _group_norm_call("pq_group_norm", x, groups, weight, bias, eps, act, outputs)
-    assert out is not None
+    if out is None:
+        raise RuntimeError(f"pq_group_norm: {groups} groups of {x.shape[-1]} channels leave no room for a row on the chip")
     return out
 
 
 def group_norm_quant_rows_fused(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
                                 act: Optional[str], want_normed: bool):
     """(q, s, z or None) in one launch (pq_group_norm_quant_rows), or None when the size does not fit."""
-    C = x.shape[-1]
-    if C % 16:
+    if x.shape[-1] % 16:
         return None
+    r = _group_norm_bound(x, groups, weight, bias, eps, act, _NORM_INT8, want_normed)
+    if r is not None:
+        return r or None
 
     def outputs(x3, B, T, C):
         z = torch.empty_like(x, memory_format=torch.contiguous_format) if want_normed else None
@@ -352,8 +344,10 @@ def group_norm_quant_fp4_fused(x: Tensor, groups: int, weight: Optional[Tensor],
                                act: Optional[str], fmt: str):
     """(codes, scales, row scales or None) in one launch (pq_group_norm_quant_fp4), or None when the size does not fit."""
     code = _fp4_code(fmt)
-    C = x.shape[-1]
-    assert C % 32 == 0, f"K={C} must be a multiple of 32"
+    assert x.shape[-1] % 32 == 0, f"K={x.shape[-1]} must be a multiple of 32"
+    r = _group_norm_bound(x, groups, weight, bias, eps, act, _NORM_FP4[fmt], False)
+    if r is not None:
+        return r or None
 
     def outputs(x3, B, T, C):
         M = B * T
@@ -544,25 +538,20 @@ def fp4_rows_aligned(x2: Tensor) -> Tensor:
 
 
 def _quant_rows_fp4_impl(x2: Tensor, fmt: str) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
-    code = FP4_FORMATS.get(fmt)
-    if code is None:
-        code = _fp4_code(fmt)
-    dt = _DT.get(x2.dtype)
-    if dt is None:
-        dt = _dt(x2.dtype)
+    code = _fp4_code(fmt)
+    r = _BIND().quant_rows_fp4(x2, code)
+    if r is not None:
+        return r
+    dt = _dt(x2.dtype)
+    x2 = fp4_rows_aligned(x2)
     M, K = x2.shape
     assert K > 0 and K % 32 == 0, f"K={K} must be a multiple of 32"
-    ld, ptr = x2.stride(0), x2.data_ptr()
-    if x2.stride(1) != 1 or ptr % 32 or (M > 1 and ld % 16):
-        x2 = fp4_rows_aligned(x2)
-        ld, ptr = x2.stride(0), x2.data_ptr()
     codes = x2.new_empty((M, K // 2), dtype=torch.uint8)
-    block = FP4_BLOCK[fmt]
-    scales = x2.new_empty(((M + 127) // 128, (K + 4 * block - 1) // (4 * block), 512), dtype=torch.uint8)
-    row_scale = x2.new_empty((M,), dtype=torch.float32) if code == _lib.FP4_NV else None
+    scales = x2.new_empty(fp4_scale_shape(M, K, fmt), dtype=torch.uint8)
+    row_scale = x2.new_empty((M,), dtype=torch.float32) if fmt == "nv" else None
     with _on_device(x2):
-        rc = _LIB().pq_quant_rows_fp4(ptr, dt, M, K, ld if M > 1 else K, code, codes.data_ptr(), scales.data_ptr(),
-                                      None if row_scale is None else row_scale.data_ptr(), _stream(x2))
+        rc = _LIB().pq_quant_rows_fp4(x2.data_ptr(), dt, M, K, x2.stride(0) if M > 1 else K, code, codes.data_ptr(),
+                                      scales.data_ptr(), _ptr(row_scale), _stream(x2))
     if rc:
         _lib.check(rc, f"pq_quant_rows_fp4(M={M}, K={K}, {fmt})")
     return codes, scales, row_scale
@@ -588,56 +577,45 @@ def _codes_aligned(codes: Tensor) -> Tensor:
     return codes
 
 
-def _plain_fp4_rows(codes: Tensor, scales: Tensor, row_scale: Optional[Tensor], index: int) -> bool:
-    """Packed rows as the quantising operators return them: what check_fp4_rows and _codes_aligned accept without a copy."""
-    M, K2 = codes.shape
-    per = 64 if row_scale is None else 32                        # bytes of codes per scale tile
-    return (codes.dtype is torch.uint8 and codes.is_contiguous() and codes.get_device() == index and codes.data_ptr() % 16 == 0
-            and K2 % 16 == 0 and K2 > 0 and scales.dtype is torch.uint8 and scales.is_contiguous() and scales.get_device() == index
-            and scales.shape == ((M + 127) // 128, (K2 + per - 1) // per, 512)
-            and (row_scale is None or (row_scale.dtype is torch.float32 and row_scale.is_contiguous()
-                                       and row_scale.get_device() == index and row_scale.shape == (M,))))
-
-
 def _dequant_rows_fp4_impl(codes: Tensor, scales: Tensor, row_scale: Optional[Tensor], dtype: torch.dtype) -> Tensor:
-    index = codes.get_device()
-    if not (index >= 0 and codes.dim() == 2 and _plain_fp4_rows(codes, scales, row_scale, index)):
-        check_fp4_rows(codes, scales, row_scale, "dequant_rows_fp4")
-        codes = _codes_aligned(codes)
-    M, K = codes.shape[0], codes.shape[1] * 2
+    dt = _dt(dtype)
+    out = _BIND().dequant_rows_fp4(codes, scales, row_scale, dtype is torch.bfloat16)
+    if out is not None:
+        return out
+    fmt, M, K = check_fp4_rows(codes, scales, row_scale, "dequant_rows_fp4")
+    codes = _codes_aligned(codes)
     out = codes.new_empty((M, K), dtype=dtype)
     with _on_device(codes):
         rc = _LIB().pq_dequant_rows_fp4(codes.data_ptr(), codes.stride(0) if M > 1 else K // 2, scales.data_ptr(),
-                                        _ptr(row_scale), _lib.FP4_MX if row_scale is None else _lib.FP4_NV, out.data_ptr(),
-                                        _dt(dtype), K, M, K, _stream(codes))
+                                        _ptr(row_scale), FP4_FORMATS[fmt], out.data_ptr(), dt, K, M, K, _stream(codes))
     if rc:
-        _lib.check(rc, f"pq_dequant_rows_fp4(M={M}, K={K})")
+        _lib.check(rc, f"pq_dequant_rows_fp4(M={M}, K={K}, {fmt})")
     return out
 
 
 def _fp4_gemm_impl(xq: Tensor, xs: Tensor, x_row: Optional[Tensor], wq: Tensor, ws: Tensor, w_row: Optional[Tensor],
                    bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
-    index = xq.get_device()
-    if not (index >= 0 and xq.dim() == 2 and wq.dim() == 2 and xq.shape[1] == wq.shape[1] and (x_row is None) == (w_row is None)
-            and wq.shape[0] > 0 and _plain_fp4_rows(xq, xs, x_row, index) and _plain_fp4_rows(wq, ws, w_row, index)):
-        fmt, _, K = check_fp4_rows(xq, xs, x_row, "fp4_gemm, activations")
-        fmt_w, N, K_w = check_fp4_rows(wq, ws, w_row, "fp4_gemm, weights")
-        assert fmt_w == fmt and K_w == K, f"{fmt} activations with K={K}, {fmt_w} weights with K={K_w}"
-        assert N > 0 and wq.device == xq.device
-        xq = _codes_aligned(xq); wq = _codes_aligned(wq)
-    M, K2 = xq.shape
-    N = wq.shape[0]
-    assert bias is None or (bias.dtype is torch.float32 and bias.numel() == N and bias.is_contiguous()
-                            and bias.get_device() == index), "bias is an fp32 vector with one entry per output channel"
+    dt = _dt(out_dtype)
+    if xq.is_cuda:
+        out = _BIND().fp4_gemm(xq, xs, x_row, wq, ws, w_row, bias, out_dtype is torch.bfloat16, status_word(xq.device).data_ptr(),
+                               _lib.GEMM_WORKSPACE_BYTES)
+        if out is not None:
+            return out
+    fmt, M, K = check_fp4_rows(xq, xs, x_row, "fp4_gemm, activations")
+    fmt_w, N, K_w = check_fp4_rows(wq, ws, w_row, "fp4_gemm, weights")
+    assert fmt_w == fmt and K_w == K, f"{fmt} activations with K={K}, {fmt_w} weights with K={K_w}"
+    assert N > 0 and wq.device == xq.device
+    assert bias is None or (bias.dtype == torch.float32 and bias.numel() == N and bias.is_contiguous()
+                            and bias.device == xq.device), "bias is an fp32 vector with one entry per output channel"
+    xq = _codes_aligned(xq); wq = _codes_aligned(wq)
     out = xq.new_empty((M, N), dtype=out_dtype)
     st = status_word(xq.device)
     with _on_device(xq):
-        rc = _LIB().pq_fp4_gemm(xq.data_ptr(), xq.stride(0) if M > 1 else K2, xs.data_ptr(), _ptr(x_row), wq.data_ptr(),
-                                wq.stride(0) if N > 1 else K2, ws.data_ptr(), _ptr(w_row), _ptr(bias),
-                                _lib.FP4_MX if x_row is None else _lib.FP4_NV, out.data_ptr(), _dt(out_dtype), N, M, N, 2 * K2,
-                                st.data_ptr(), _lib.GEMM_WORKSPACE_BYTES, _stream(xq))
+        rc = _LIB().pq_fp4_gemm(xq.data_ptr(), xq.stride(0) if M > 1 else K // 2, xs.data_ptr(), _ptr(x_row), wq.data_ptr(),
+                                wq.stride(0) if N > 1 else K // 2, ws.data_ptr(), _ptr(w_row), _ptr(bias), FP4_FORMATS[fmt],
+                                out.data_ptr(), dt, N, M, N, K, st.data_ptr(), st.numel() * 4, _stream(xq))
     if rc:
-        _lib.check(rc, f"pq_fp4_gemm(M={M}, N={N}, K={2 * K2})")
+        _lib.check(rc, f"pq_fp4_gemm(M={M}, N={N}, K={K}, {fmt})")
     return out
 
 

@@ -259,6 +259,28 @@ def test_product_strided_codes_and_repeatability(cuda_dev, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+def test_general_path_agrees_with_the_one_step_calls(cuda_dev, fmt, monkeypatch):
+    """Operands that the one-step calls refuse take the step-by-step path; both give the same bytes."""
+    x, xq = make_rows(150, 640, fmt, torch.bfloat16, 1, cuda_dev)
+    _, wq = make_rows(200, 640, fmt, torch.bfloat16, 2, cuda_dev)
+    bias = torch.randn(200, device=cuda_dev)
+    bind = ops._BIND()
+    code = ops.FP4_FORMATS[fmt]
+    assert bind.quant_rows_fp4(x, code) is not None
+    for odd in (x.float(), x[:, ::2], x[:, 8:], x[:, :48], x[0], x.t()):
+        assert bind.quant_rows_fp4(odd, code) is None
+    assert bind.fp4_gemm(*xq, *wq, bias.double(), True, 0, 0) is None and bind.fp4_gemm(*xq, *wq, bias[1:], True, 0, 0) is None
+    assert bind.fp4_gemm(xq.codes[:, ::2], *xq[1:], *wq, None, True, 0, 0) is None
+    one = (fp4_exec.quant_rows_fp4(x, fmt), fp4_exec.dequant_rows_fp4(xq), fp4_exec.fp4_gemm(xq, wq, bias, torch.float16))
+    class Refuses:
+        def __getattr__(self, name):
+            return lambda *a: None
+    monkeypatch.setattr(ops, "_bind_handle", Refuses())
+    step = (fp4_exec.quant_rows_fp4(x, fmt), fp4_exec.dequant_rows_fp4(xq), fp4_exec.fp4_gemm(xq, wq, bias, torch.float16))
+    assert torch.equal(one[0].codes, step[0].codes) and torch.equal(one[1], step[1]) and torch.equal(one[2], step[2])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 def test_refusals(cuda_dev, fmt):
     x, xq = make_rows(8, 128, fmt, torch.bfloat16, 1, cuda_dev)
     _, wq = make_rows(16, 128, fmt, torch.bfloat16, 2, cuda_dev)

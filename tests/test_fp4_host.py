@@ -93,6 +93,18 @@ def test_refusals():
             call()                                               # CPU tensors
 
 
+def test_one_step_calls_leave_other_operands_to_the_general_path():
+    """The one-step calls answer None, without touching anything, for what they do not take as it is."""
+    bind = _lib.binding()
+    x = torch.randn(4, 64, dtype=torch.bfloat16)
+    q = fp4_exec.quantize_weight_fp4(x)
+    assert bind.quant_rows_fp4(x, 1) is None and bind.quant_rows_fp4(None, 1) is None and bind.quant_rows_fp4(3, 1) is None
+    assert bind.dequant_rows_fp4(*q, True) is None and bind.dequant_rows_fp4(q.codes, 5, None, True) is None
+    assert bind.fp4_gemm(*q, *q, None, True, 0, 0) is None and bind.fp4_gemm(*q, *q, "bias", True, 0, 0) is None
+    assert bind.group_norm(x[None], 4, None, None, 1e-6, 0, 0, True, 0) is None
+    assert bind.group_norm(x[None], 4.0, "w", None, 1e-6, 0, 0, True, 0) is None
+
+
 def test_argument_checks():
     lib = _lib.load()
     buf = ctypes.create_string_buffer(8192)

@@ -186,6 +186,34 @@ def test_in_front_of_a_linear(cuda_dev, dtype):
 
 
 @pytest.mark.gpu
+def test_general_path_agrees_with_the_one_step_calls(cuda_dev, monkeypatch):
+    x, w, b = (t.to(cuda_dev) for t in rows(2, 300, 320, torch.float16, 9))
+    calls = (lambda: norm_exec.group_norm_rows(x, 32, w, b, 1e-6, "silu"),
+             lambda: norm_exec.group_norm_quant_rows(x, 32, w, b, want_normed=True),
+             lambda: norm_exec.group_norm_quant_fp4(x, 32, w, b, fmt="nv"), lambda: norm_exec.group_norm_quant_fp4(x, 32, None, b, fmt="mx"))
+    one = [c() for c in calls]
+
+    class Refuses:
+        def __getattr__(self, name):
+            return lambda *a: None
+    monkeypatch.setattr(ops, "_bind_handle", Refuses())
+    for a, c in zip(one, calls):
+        s = c()
+        if isinstance(a, torch.Tensor):
+            assert torch.equal(a, s)
+        elif isinstance(a, fp4_exec.Fp4Rows):
+            assert torch.equal(fp4_exec.dequant_rows_fp4(fp4_exec.Fp4Rows(*(t if t is None else t.clone() for t in a))).float(), _values(s))
+        else:
+            assert all(torch.equal(p, q) for p, q in zip(a, s))
+
+
+def _values(q):
+    from oracle import fp4 as ofp4
+    v = ofp4.packed_values(q.codes.cpu(), q.scales.cpu(), None if q.row_scale is None else q.row_scale.cpu(), q.fmt)
+    return v.to(torch.bfloat16).float().to(q.codes.device)
+
+
+@pytest.mark.gpu
 def test_streams_graphs_and_repeats(cuda_dev):
     x, w, b = (t.to(cuda_dev) for t in rows(2, 5000, 320, torch.bfloat16, 7))
     want = norm_exec.group_norm_rows(x, 32, w, b, 1e-6, "silu")
