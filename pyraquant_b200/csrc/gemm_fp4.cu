@@ -32,8 +32,13 @@ struct Fp4Smem {
   static constexpr int kBarOff = kColOff + 2 * BN * 4;
   static constexpr int kMiscOff = kBarOff + (2 * STAGES + 1) * 8;
   static constexpr int kTotal = kMiscOff + 16;
-  static constexpr int kRedStride = BN + 4;                          // fp32 partial tile of a split launch
-  static_assert(BM * kRedStride * 4 <= kScaleOff, "partial tile lies over the operand stages");
+  // What lies over the operand stages once they are used up: the fp32 partial tile of a split launch, or the rounded rows of the
+  // output, at a stride of 144 bytes so that eight lanes' 16-byte stores meet different banks.  From there whole rows go out; a lane
+  // that stores its own row's pieces took (us, it / this) 560 x 1440 -> 1068 13.5 / 8.5, 1375 x 64 -> 358 12.1 / 7.0, 1024 x 1280 ->
+  // 1280 5.9 / 5.7.
+  static constexpr int kRedStride = BN + 4;
+  static constexpr int kRowStride = 2 * BN + 16;
+  static_assert(BM * kRedStride * 4 <= kScaleOff && BM * kRowStride <= kScaleOff, "tiles over the operand stages");
   static_assert(kTotal <= 232448, "exceeds the 227 KB shared memory of one CTA");
   // accumulator, then a set of scale columns per stage
   static constexpr int kSetCols = 2 * 4 * Fp4Fmt<FMT>::kTilesPerStage;
@@ -46,6 +51,32 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
+}
+
+// eight consecutive outputs of one row, columns [col, col + 8)
+__device__ __forceinline__ void store8(const Fp4GemmParams& p, int row, int col, const float (&y)[8]) {
+  unsigned short* o = static_cast<unsigned short*>(p.out) + static_cast<int64_t>(row) * p.ldo + col;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack2_any(y[2 * i], y[2 * i + 1], p.bf16);
+  if (p.vec && col + 8 <= p.N) {
+    st_v4(o, make_uint4(w[0], w[1], w[2], w[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < p.N) o[i] = static_cast<unsigned short>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu);
+  }
+}
+// Up to 64 columns of one output row by a warp, rows that start on any 2-byte border: one 4-byte store per lane from the first
+// 4-byte border on, single elements at the ends; n may be zero or less, then nothing is stored.  `read(c)` gives element c.
+template <typename Read>
+__device__ __forceinline__ void store_row64(unsigned short* o, int n, int lane, Read&& read) {
+  const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(o) >> 1) & 1;
+  if (n > 64) n = 64;
+  const int c = 2 * lane + odd;
+  if (odd && lane == 0 && n > 0) o[0] = static_cast<unsigned short>(read(0));
+  if (c + 1 < n) *reinterpret_cast<uint32_t*>(o + c) = read(c) | (read(c + 1) << 16);
+  else if (c < n) o[c] = static_cast<unsigned short>(read(c));
 }
 
 template <int FMT, int STAGES, bool SPLIT>
@@ -184,15 +215,38 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             for (int j = 0; j < 8; ++j)
               *reinterpret_cast<uint4*>(red + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
-        } else if (row < p.M) {
+        } else {
+          uint8_t* line = smem + r * L::kRowStride + 2 * c;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float y[8];
+            uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              y[k] = fmaf(__uint_as_float(v[8 * j + k]), s_row * col_scale[c + 8 * j + k], col_bias[c + 8 * j + k]);
-            if (n0 + c + 8 * j < p.N) store8(p, row, n0 + c + 8 * j, y);
+            for (int k = 0; k < 4; ++k) {
+              const int i = 8 * j + 2 * k;
+              w[k] = pack2_any(fmaf(__uint_as_float(v[i]), s_row * col_scale[c + i], col_bias[c + i]),
+                               fmaf(__uint_as_float(v[i + 1]), s_row * col_scale[c + i + 1], col_bias[c + i + 1]), p.bf16);
+            }
+            *reinterpret_cast<uint4*>(line + 16 * j) = make_uint4(w[0], w[1], w[2], w[3]);
           }
+        }
+      }
+    }
+    if constexpr (!SPLIT) {
+      // every warp stores a quarter of the rows that there are, whole rows at a time; all reach this barrier, landed or not
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+      if (__all_sync(0xffffffffu, landed)) {
+        unsigned short* const out = static_cast<unsigned short*>(p.out) + static_cast<int64_t>(row0) * p.ldo + n0;
+        const int rows = p.M - row0 < BM ? p.M - row0 : BM;
+        if (p.vec && n0 + BN <= p.N) {                     // four rows of eight 16-byte pieces
+#pragma unroll 2
+          for (int q = 4 * quarter + (lane >> 3); q < rows; q += 16)
+            st_v4(out + q * p.ldo + (lane & 7) * 8, *reinterpret_cast<const uint4*>(smem + q * L::kRowStride + (lane & 7) * 16));
+        } else {
+#pragma unroll 2
+          for (int q = quarter; q < rows; q += 4)
+            store_row64(out + q * p.ldo, p.N - n0, lane, [&](int c) {
+              return static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(smem + q * L::kRowStride + 2 * c));
+            });
         }
       }
     }
@@ -201,7 +255,8 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 
   __syncthreads();
   if constexpr (SPLIT) {
-    // Partial tiles stand in the CTAs' shared memory; this CTA adds up its share of the 8-column pieces.
+    // Partial tiles stand in the CTAs' shared memory; this CTA adds up its share of the 8-column pieces.  (Two columns a lane, so
+    // that a warp stores whole rows, is slower for its four times as many reads: 64 x 10240 -> 2560 11.6 us instead of 10.7.)
     const bool ok = *abort_flag == 0;
     cluster_sync_all();
     if (ok) {
@@ -262,10 +317,10 @@ template <int FMT>
 int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, Fp4GemmParams& p, cudaStream_t st) {
   const int sms = sm_count();
   const int num_kb = (p.K + kFp4StageK - 1) / kFp4StageK;
-  // 256 x 256 tiles on CTA pairs from a quarter of the SMs on, measured in us, pair / single: 4096 x 640 -> 640 (48 tiles) 6.9 / 8.2,
-  // 256 x 1280 -> 10240 (40) 7.6 / 10.3, 1024 x 1280 -> 1280 (20) 7.2 / 6.5.  Up to 128 rows or columns half a tile or more is
-  // unused: 128 x 1280 -> 10240 (40) 7.9 / 6.9, 128 x 4096 -> 32768 (128) 22.0 / 25.0; 16384 x 640 -> 128 (64) 7.2 / 5.8,
-  // 65536 x 1280 -> 128 (256) 18.7 / 25.4, 65536 x 640 -> 64 13.7 / 10.0.
+  // 256 x 256 tiles on CTA pairs from a quarter of the SMs on, measured in us (mx, nv within 0.7), pair / single: 4096 x 640 -> 640
+  // (48 tiles) 6.2 / 7.6, 1024 x 1280 -> 2560 (40) 7.2 / 9.3, -> 1920 (32) 7.2 / 6.2, -> 1280 (20) 7.2 / 5.9.  Up to 128 rows or
+  // columns half a tile or more is unused: 128 x 1280 -> 10240 (40) 7.4 / 5.9, 128 x 4096 -> 32768 (128) 21.4 / 23.4;
+  // 16384 x 640 -> 128 (64) 7.2 / 5.5, 65536 x 1280 -> 128 (256) 16.8 / 23.7, 65536 x 640 -> 64 12.7 / 8.9.
   const int64_t pair_tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
   const bool pair = p.N > 128 ? (p.M > 128 ? 4 : 2) * pair_tiles >= sms : (p.N > 64 && pair_tiles >= sms);
   if ((p.s_row != nullptr) == (p.s_col != nullptr) && (options().fp4_pair == 2 || (options().fp4_pair == 1 && pair)))
@@ -280,10 +335,14 @@ int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, 
   if (rc != PQ_OK) return rc;
   rc = make_tile_map(&tmW, w, p.N, p.K / 2, ldw, BN);
   if (rc != PQ_OK) return rc;
-  // Clusters cost 1.5 us more than they save below ten stages (77 x 2048 -> 1280: 6.2 us unsplit, 6.5 split in four), and run in
-  // rounds when they do not all find room at once (2560 -> 2560, 40 tiles: 6.2 us split in two, 9.9 in four).
+  // Along K a stage takes 0.26 us; a cluster costs 1 to 2 us, the more the more rows the joined tiles have, and runs in rounds when
+  // the clusters do not all find room at once (2560 -> 2560, 40 tiles: 6.0 us split in two, 10.2 in four).  Measured in us,
+  // unsplit / in two / in four, by stages: 77 rows -> 640 (10 tiles) 8 stages 5.5 / 6.6 / 6.5 (-> 1280), 10: 6.2 / 6.9 / 6.5,
+  // 13: 6.9 / 7.2 / 6.5, 40: 13.7 / 10.6 / 8.6.  Where only two find room, 40 tiles of 16 rows 13: 6.9 / 6.9, 16: 7.6 / 6.9,
+  // 50 tiles of 128 rows 16: 7.9 / 8.6, 20: 8.9 / 8.9, 40: 13.8 / 11.6.
   int split = 1;
-  if (num_kb >= 10)
+  const bool only_two = tiles * 4 > sms * 3 / 4;
+  if (num_kb >= (!only_two ? 10 : p.M <= 64 ? 14 : 20))
     while (split < 8 && tiles * split * 2 <= sms * 3 / 4 && split * 4 <= num_kb) split *= 2;
   const int want = options().fp4_split;
   if (want == 1 || want == 2 || want == 4 || want == 8) {

@@ -96,20 +96,6 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
 __device__ __forceinline__ uint32_t pack2_any(float a, float b, int bf16) {
   return bf16 ? pack2(a, b, __nv_bfloat16{}) : pack2(a, b, __half{});
 }
-// eight consecutive outputs of one row, columns [col, col + 8)
-__device__ __forceinline__ void store8(const Fp4GemmParams& p, int row, int col, const float (&y)[8]) {
-  unsigned short* o = static_cast<unsigned short*>(p.out) + static_cast<int64_t>(row) * p.ldo + col;
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack2_any(y[2 * i], y[2 * i + 1], p.bf16);
-  if (p.vec && col + 8 <= p.N) {
-    st_v4(o, make_uint4(w[0], w[1], w[2], w[3]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < p.N) o[i] = static_cast<unsigned short>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu);
-  }
-}
 
 }  // namespace
 }  // namespace pq

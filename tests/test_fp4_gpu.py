@@ -243,6 +243,36 @@ def test_product_leaves_its_neighbourhood_alone(cuda_dev, fmt, pair):
     _lib.set_option("fp4_pair", 1)
 
 
+@pytest.mark.parametrize("M,N,K,options", [(130, 1, 96, {"fp4_pair": 0}), (70, 131, 96, {"fp4_pair": 0}), (2500, 587, 64, {"fp4_pair": 0}),
+                                           (33, 67, 1280, {"fp4_pair": 0, "fp4_split": 4}), (1, 63, 1280, {"fp4_pair": 0, "fp4_split": 2}),
+                                           (290, 577, 96, {"fp4_pair": 2}), (290, 263, 96, {"fp4_pair": 2})])
+def test_product_rows_at_every_border(cuda_dev, M, N, K, options):
+    """Rows of odd length, odd stride and odd start in every variant: exactly the outputs are written."""
+    _, xq = make_rows(M, K, "mx", torch.bfloat16, 1, cuda_dev)
+    _, wq = make_rows(N, K, "mx", torch.bfloat16, 2, cuda_dev)
+    lib = _lib.load()
+    for k, v in options.items():
+        _lib.set_option(k, v)
+    try:
+        want = None
+        for ldo, off in ((-(-N // 8) * 8, 8), (N, 0), (N + 1, 1), (N + 2, 2), (N + 3, 5)):
+            buf = torch.full((M * ldo + 16,), 7.0, dtype=torch.float16, device=cuda_dev)
+            rc = lib.pq_fp4_gemm(xq.codes.data_ptr(), K // 2, xq.scales.data_ptr(), None, wq.codes.data_ptr(), K // 2, wq.scales.data_ptr(),
+                                 None, None, ops.FP4_FORMATS["mx"], buf.data_ptr() + 2 * off, 1, ldo, M, N, K, None, 0,
+                                 torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            got = buf[off: off + M * ldo].view(M, ldo)
+            if want is None:
+                want = got[:, :N].clone()
+                check_product(want, xq, wq, None, "mx")
+            assert torch.equal(got[:, :N], want)
+            got[:, :N] = 7.0
+            assert bool((buf == 7.0).all())
+    finally:
+        _lib.set_option("fp4_pair", 1)
+        _lib.set_option("fp4_split", 0)
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_product_strided_codes_and_repeatability(cuda_dev, fmt):
     _, xq = make_rows(150, 1280, fmt, torch.bfloat16, 1, cuda_dev)
