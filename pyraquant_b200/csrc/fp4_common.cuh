@@ -21,6 +21,23 @@
 namespace pq {
 namespace {
 
+// Chained launches.  The kernels that take or make 4-bit rows follow one another on a stream, a few microseconds each, so they are
+// launched with programmatic serialisation: a kernel's blocks may become resident, set up barriers and tensor memory and fetch
+// descriptors while the kernel before it is still at work.  Every thread then waits for the end of that kernel, memory included,
+// before its first access to global memory, so that nothing is read or overwritten early; a chain of such kernels waits link by
+// link, as no block ends before its own wait.  Their loads are no read-only ones, which might be asked for ahead of the wait.
+// Quantisation and product, us, plain launches / chained: 1 x 1280 -> 1280 6.6 / 5.7, 77 x 1280 -> 640 7.9 / 6.5, 4096 x 640 -> 640
+// 10.1 / 9.1, 16384 x 1280 -> 1280 31.0 / 29.0.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// once all blocks have said so (or ended) the next kernel's may take what room is left
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+inline cudaLaunchAttribute chained_launch() {
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  return at;
+}
+
 // scale tiles per row group of 128 rows
 __host__ __device__ __forceinline__ int64_t fp4_scale_tiles(int64_t K, int fmt) {
   const int64_t per = fmt == PQ_FP4_MX ? 128 : 64;                 // elements per four scales
@@ -35,9 +52,9 @@ __device__ __forceinline__ int64_t fp4_scale_off(int64_t m, int64_t kt, int64_t 
 struct Chunk16 { uint32_t w[8]; };
 __device__ __forceinline__ Chunk16 ld_stream_chunk16(const void* p) {
   Chunk16 c;
-  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(c.w[0]), "=r"(c.w[1]), "=r"(c.w[2]), "=r"(c.w[3]), "=r"(c.w[4]), "=r"(c.w[5]), "=r"(c.w[6]), "=r"(c.w[7])
-               : "l"(p));
+               : "l"(p) : "memory");
   return c;
 }
 __device__ __forceinline__ void st_chunk16(void* p, const Chunk16& c) {

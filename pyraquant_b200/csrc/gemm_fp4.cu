@@ -117,6 +117,8 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  wait_for_previous_kernel();
+  allow_next_kernel();
 
   if (aligned_ok && warp == 0) {
     // ------------------------------------------------------------------ TMA producer
@@ -303,12 +305,12 @@ int launch_fp4(const CUtensorMap& tmA, const CUtensorMap& tmW, const Fp4GemmPara
   cfg.blockDim = dim3(kFp4Threads);
   cfg.dynamicSmemBytes = L::kTotal;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = static_cast<unsigned>(SPLIT ? split : 1);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2] = {chained_launch()};
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = static_cast<unsigned>(SPLIT ? split : 1);
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = SPLIT ? 1 : 0;
+  cfg.numAttrs = SPLIT ? 2 : 1;
   PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmW, p, split));
   return PQ_OK;
 }

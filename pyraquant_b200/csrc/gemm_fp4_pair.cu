@@ -83,7 +83,7 @@ __device__ __forceinline__ void tc_cp_scale_tile_pair(uint32_t tmem_addr, uint64
 // a load that stays where it is written (the compiler would move an ordinary one down to its use)
 __device__ __forceinline__ float ld_now(const float* p) {
   float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
   return v;
 }
 
@@ -152,6 +152,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   cluster_sync_all();                 // both CTAs' barriers exist before anyone signals across the pair
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  wait_for_previous_kernel();         // (the next kernel is not let in early: 16384 x 1280 -> 1280 and its quantisation 29.0 us, 32.1 if so)
   auto leader_addr = [&](const uint64_t* bar) { return map_to_cta(smem_u32(bar), 0u); };
   auto peer_addr = [&](const uint64_t* bar) { return map_to_cta(smem_u32(bar), 1u); };
 
@@ -437,12 +438,12 @@ int launch_pair(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, F
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = L::kTotal;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2] = {chained_launch()};
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmW, tmSa, tmSw, tmOut, p));
   return PQ_OK;
 }

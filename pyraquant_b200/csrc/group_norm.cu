@@ -298,6 +298,7 @@ template <typename T, int MODE, int COLS>
 __global__ void __launch_bounds__(kThreads, 1)
 pq_group_norm_kernel(const NormArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
+  if constexpr (MODE != kOut16) allow_next_kernel();                     // the product that takes these rows
   T tag{};
   const Lanes l = a.l;
   const NormSmem lay = a.lay;

@@ -76,10 +76,11 @@ __device__ __forceinline__ float team_amax(uint32_t acc, float* part, int tid) {
 
 template <typename T, int FMT, int TPR, bool LONG>
 __global__ void __launch_bounds__(kThreads, LONG ? 2 : 3)
-pq_quant_rows_fp4_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                         float* __restrict__ row_scale, int64_t M, int K) {
+pq_quant_rows_fp4_kernel(const T* x, int64_t ldx, uint8_t* codes, uint8_t* scales, float* row_scale, int64_t M, int K) {
   constexpr int RPB = kThreads / TPR;
   __shared__ float part[kThreads / 32];
+  wait_for_previous_kernel();
+  allow_next_kernel();
   const int tid = threadIdx.x;
   const int lane = tid % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + tid / TPR;
@@ -136,16 +137,18 @@ __device__ __forceinline__ float finite16(float v, __nv_bfloat16) { return v; }
 // A thread turns units of 16 codes (8 bytes and a scale byte) into one 32-byte store each, five units at a time.
 template <typename T, int FMT, int TPR>
 __global__ void __launch_bounds__(kThreads)
-pq_dequant_rows_fp4_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
-                           const float* __restrict__ row_scale, T* __restrict__ out, int64_t ldo, int64_t M, int K) {
+pq_dequant_rows_fp4_kernel(const uint8_t* codes, int64_t ldc, const uint8_t* scales, const float* row_scale, T* out, int64_t ldo,
+                           int64_t M, int K) {
   constexpr int RPB = kThreads / TPR;
   T tag{};
+  wait_for_previous_kernel();
+  allow_next_kernel();
   const int lane = threadIdx.x % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
   if (row >= M) return;
   const int nchunk = K >> 4;
   const uint8_t* srow = scales + fp4_scale_off(row, 0, fp4_scale_tiles(K, FMT));
-  const float s_row = FMT == PQ_FP4_NV ? __ldg(row_scale + row) : 1.0f;
+  const float s_row = FMT == PQ_FP4_NV ? row_scale[row] : 1.0f;
   const uint8_t* crow = codes + row * ldc;
   T* orow = out + row * ldo;
   for (int c0 = lane; c0 < nchunk; c0 += kUnits * TPR) {
@@ -156,8 +159,8 @@ pq_dequant_rows_fp4_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const
       const int c = c0 + j * TPR;
       if (c < nchunk) {
         const int blk = FMT == PQ_FP4_MX ? c >> 1 : c;
-        w[j] = __ldg(reinterpret_cast<const uint2*>(crow + static_cast<int64_t>(c) * 8));
-        byte[j] = __ldg(srow + (blk >> 2) * 512 + (blk & 3));
+        w[j] = *reinterpret_cast<const uint2*>(crow + static_cast<int64_t>(c) * 8);
+        byte[j] = srow[(blk >> 2) * 512 + (blk & 3)];
       }
     }
 #pragma unroll
@@ -189,15 +192,26 @@ struct Args {
   const void* x; int64_t ldx; uint8_t* codes; uint8_t* scales; float* row_scale; int64_t M; int K;
 };
 
+template <typename... P, typename... A>
+int launch_chained(void (*kern)(P...), int64_t blocks, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at = chained_launch();
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
+  return PQ_OK;
+}
+
 template <typename T, int FMT, int TPR, bool LONG>
 int launch_quant(const Args& a, cudaStream_t st) {
   constexpr int RPB = kThreads / TPR;
   const int64_t blocks = (a.M + RPB - 1) / RPB;
   if (blocks > 0x7fffffffLL) return PQ_ERR_SHAPE;
-  pq_quant_rows_fp4_kernel<T, FMT, TPR, LONG><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(
-      static_cast<const T*>(a.x), a.ldx, a.codes, a.scales, a.row_scale, a.M, a.K);
-  PQ_CUDA_TRY(cudaGetLastError());
-  return PQ_OK;
+  return launch_chained(pq_quant_rows_fp4_kernel<T, FMT, TPR, LONG>, blocks, st, static_cast<const T*>(a.x), a.ldx, a.codes, a.scales,
+                        a.row_scale, a.M, a.K);
 }
 
 // the smallest team that keeps the row in registers
@@ -219,10 +233,8 @@ int launch_dequant(const void* codes, int64_t ldc, const void* scales, const flo
   constexpr int RPB = kThreads / TPR;
   const int64_t blocks = (M + RPB - 1) / RPB;
   if (blocks > 0x7fffffffLL) return PQ_ERR_SHAPE;
-  pq_dequant_rows_fp4_kernel<T, FMT, TPR><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(
-      static_cast<const uint8_t*>(codes), ldc, static_cast<const uint8_t*>(scales), row_scale, static_cast<T*>(out), ldo, M, K);
-  PQ_CUDA_TRY(cudaGetLastError());
-  return PQ_OK;
+  return launch_chained(pq_dequant_rows_fp4_kernel<T, FMT, TPR>, blocks, st, static_cast<const uint8_t*>(codes), ldc,
+                        static_cast<const uint8_t*>(scales), row_scale, static_cast<T*>(out), ldo, M, K);
 }
 template <typename T, int FMT>
 int dispatch_dequant(const void* codes, int64_t ldc, const void* scales, const float* row_scale, void* out, int64_t ldo,

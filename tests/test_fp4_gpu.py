@@ -388,3 +388,42 @@ def test_streams_graphs_and_compile_wrappers(cuda_dev):
     assert torch.equal(ops_ns.dequant_rows_fp4(c, s, r, 0), fp4_exec.dequant_rows_fp4(fp4_exec.quant_rows_fp4(x, "nv")))
     c, s, r = ops_ns.quant_rows_fp4(x, "mx")
     assert r.numel() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", [(1, 640, 640), (77, 1280, 640), (1000, 640, 2560), (4096, 1280, 640)])
+def test_kernels_in_a_row_wait_for_one_another(cuda_dev, fmt, M, N, K):
+    """Quantisation, product, read-back, group norm and product again, eager and replayed, on memory that every call takes over from
+    the one before: the results of calls that are synchronised one by one."""
+    from pyraquant_b200 import norm_exec
+    g = torch.Generator().manual_seed(M + N)
+    xs = [torch.randn(M, K, generator=g).to(torch.bfloat16).to(cuda_dev) for _ in range(3)]
+    wq = fp4_exec.quant_rows_fp4(torch.randn(N, K, generator=g).to(torch.bfloat16).to(cuda_dev), fmt)
+    b = torch.randn(N, generator=g).to(cuda_dev)
+    gamma, beta = torch.randn(K, generator=g).to(cuda_dev).bfloat16(), torch.randn(K, generator=g).to(cuda_dev).bfloat16()
+
+    def run(x, between):
+        q = fp4_exec.quant_rows_fp4(x, fmt)
+        between()
+        y = fp4_exec.fp4_gemm(q, wq, b, torch.bfloat16)
+        between()
+        z = fp4_exec.dequant_rows_fp4(q, torch.bfloat16)
+        between()
+        n = norm_exec.group_norm_quant_fp4(z[None], 32, gamma, beta, 1e-5, "silu", fmt)
+        between()
+        return y, z, fp4_exec.fp4_gemm(n, wq, b, torch.bfloat16)
+
+    want = [run(x, torch.cuda.synchronize) for x in xs]
+    for _ in range(10):
+        for x, w in zip(xs, want):
+            got = run(x, lambda: None)
+            assert all(torch.equal(a, e) for a, e in zip(got, w))
+            del got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [run(x, lambda: None) for x in xs]
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, w in zip(got, want):
+        assert all(torch.equal(u, e) for u, e in zip(a, w))
