@@ -530,9 +530,11 @@ def _fp4_code(fmt: str) -> int:
 
 
 def fp4_rows_aligned(x2: Tensor) -> Tensor:
-    """The 4-bit kernels load 32 bytes at a time: rows that start elsewhere are made contiguous."""
+    """The 4-bit kernels load 32 bytes at a time: rows that start elsewhere are made contiguous, and so are rows that overlap (one
+    row seen many times)."""
     assert x2.dim() == 2 and x2.is_cuda
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) % 16 != 0) or x2.data_ptr() % 32 != 0:
+    if (x2.stride(1) != 1 or (x2.shape[0] > 1 and (x2.stride(0) % 16 != 0 or x2.stride(0) < x2.shape[1]))
+            or x2.data_ptr() % 32 != 0):
         x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
 
@@ -572,7 +574,8 @@ def check_fp4_rows(codes: Tensor, scales: Tensor, row_scale: Optional[Tensor], w
 
 
 def _codes_aligned(codes: Tensor) -> Tensor:
-    if codes.stride(1) != 1 or (codes.shape[0] > 1 and codes.stride(0) % 16 != 0) or codes.data_ptr() % 16 != 0:
+    if (codes.stride(1) != 1 or (codes.shape[0] > 1 and (codes.stride(0) % 16 != 0 or codes.stride(0) < codes.shape[1]))
+            or codes.data_ptr() % 16 != 0):
         codes = codes.clone(memory_format=torch.contiguous_format)
     return codes
 

@@ -391,6 +391,20 @@ def test_streams_graphs_and_compile_wrappers(cuda_dev):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+def test_rows_that_overlap(cuda_dev, fmt):
+    """One row seen many times (a broadcast input) and windows that share elements are copied first, codes likewise."""
+    x = awkward_rows(40, 320, torch.bfloat16, 6).to(cuda_dev)
+    for view in (x[3:4].expand(70, 320), x.as_strided((20, 320), (64, 1)), x[:, :32][5:6].expand(3, 32)):
+        check_rows(fp4_exec.quant_rows_fp4(view, fmt), view, fmt)
+    q = fp4_exec.quant_rows_fp4(x[3:4].expand(70, 320), fmt)
+    wq = fp4_exec.quant_rows_fp4(x, fmt)
+    same = fp4_exec.Fp4Rows(q.codes[:1].expand(70, 160), q.scales, q.row_scale)
+    assert torch.equal(fp4_exec.fp4_gemm(same, wq, None, torch.bfloat16).view(torch.int16),
+                       fp4_exec.fp4_gemm(q, wq, None, torch.bfloat16).view(torch.int16))
+    assert torch.equal(fp4_exec.dequant_rows_fp4(same).view(torch.int16), fp4_exec.dequant_rows_fp4(q).view(torch.int16))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("M,N,K", [(1, 640, 640), (77, 1280, 640), (1000, 640, 2560), (4096, 1280, 640)])
 def test_kernels_in_a_row_wait_for_one_another(cuda_dev, fmt, M, N, K):
     """Quantisation, product, read-back, group norm and product again, eager and replayed, on memory that every call takes over from
