@@ -23,10 +23,11 @@ from .int8_exec import _eager, quant_rows
 def group_norm_rows(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                     eps: float = 1e-6, act: Optional[str] = None) -> torch.Tensor:
     """x [B, ..., C] bf16/fp16, channels last -> normed rows of the same shape and type.  ``act``: None or "silu".
-    weight / bias [C] in x's type or fp32, or None.  C % 8 == 0, C <= 8192, C % groups == 0."""
+    weight / bias [C] in x's type or fp32, or None.  C % 8 == 0, C <= 8192, C % groups == 0, B <= 65535."""
     assert x.is_cuda
     if _eager():
         return ops._group_norm_impl(x, groups, weight, bias, eps, act)
+    ops.check_group_norm_act(act)                     # the operator knows SiLU or nothing
     return torch.ops.pq_b200.group_norm_rows(x, groups, weight, bias, eps, act == "silu")
 
 

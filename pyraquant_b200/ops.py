@@ -243,13 +243,17 @@ def _affine_vector(v: Optional[Tensor]) -> Optional[Tensor]:
     return v.reshape(-1).clone(memory_format=torch.contiguous_format)
 
 
+def check_group_norm_act(act: Optional[str]) -> None:
+    if act not in GROUP_NORM_ACTS:
+        raise ValueError(f"unknown activation {act!r} (expected one of {tuple(GROUP_NORM_ACTS)})")
+
+
 def group_norm_args(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], act: Optional[str]):
     """Checks a group norm's operands; returns x as [B, T, C] with rows the kernels take, the affine vectors (both fp32 or both in
     x's type) and the activation's code."""
     assert x.is_cuda and x.dim() >= 2, "channels-last rows [B, ..., C] on a GPU"
     _dt(x.dtype)
-    if act not in GROUP_NORM_ACTS:
-        raise ValueError(f"unknown activation {act!r} (expected one of {tuple(GROUP_NORM_ACTS)})")
+    check_group_norm_act(act)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         raise RuntimeError("group norm has no gradient here: call it under torch.no_grad() or on detached tensors")
     C = x.shape[-1]

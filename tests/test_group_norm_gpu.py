@@ -274,6 +274,19 @@ def test_refusals_gpu(cuda_dev):
         norm_exec.group_norm_rows(x, 8, w)
 
 
+@pytest.mark.gpu
+def test_refusals_of_the_traced_form(cuda_dev, monkeypatch):
+    """Where a compiler traces the call, an unknown activation is refused too, and the known ones give the eager values."""
+    x = torch.randn(2, 5, 64, device=cuda_dev).to(torch.bfloat16)
+    want = {act: norm_exec.group_norm_rows(x, 8, act=act) for act in (None, "silu")}
+    monkeypatch.setattr(norm_exec, "_eager", lambda: False)
+    for act, z in want.items():
+        assert torch.equal(norm_exec.group_norm_rows(x, 8, act=act), z)
+    for f in (norm_exec.group_norm_rows, norm_exec.group_norm_quant_rows, norm_exec.group_norm_quant_fp4):
+        with pytest.raises(ValueError):
+            f(x, 8, act="gelu")
+
+
 def test_refusals_on_the_host():
     with pytest.raises(AssertionError):
         norm_exec.group_norm_rows(torch.randn(2, 4, 64, dtype=torch.bfloat16), 8)
