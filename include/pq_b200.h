@@ -349,6 +349,16 @@ int pq_fp4_gemm(const uint8_t* xq, int64_t ldx, const uint8_t* x_scales, const f
                 const uint8_t* w, int64_t ldw, const uint8_t* w_scales, const float* s_col, const float* bias, int fmt,
                 void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K,
                 void* workspace, size_t ws_bytes, void* stream);
+/* pq_fp4_gemm with a rank-32 term in the accumulator: out[m,n] = (sum_k x[m,k] w[n,k] + sum_r t[m,r] lb[n,r]) (s_row[m] s_col[n])
+ * (+ bias[n]), rounded once.  t [M,32] and lb [N,32] fp32, contiguous, 16-byte aligned, in units of the row scales: the activations
+ * that pq_fp4_lowrank_rows makes of 16-bit ones, and the 16-bit up-projection, transposed, over s_col.  Of each value the 11
+ * leading significant bits count (TF32), all that a 16-bit value has.  t and lb NULL: pq_fp4_gemm. */
+int pq_fp4_gemm_lowrank(const uint8_t* xq, int64_t ldx, const uint8_t* x_scales, const float* s_row,
+                        const uint8_t* w, int64_t ldw, const uint8_t* w_scales, const float* s_col, const float* bias,
+                        const float* t, const float* lb, int fmt, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N,
+                        int64_t K, void* workspace, size_t ws_bytes, void* stream);
+/* out [M,32] fp32 = t [M,32] 16-bit, contiguous, over row_scale [M] (NULL: 1); t 16-byte, out 32-byte aligned. */
+int pq_fp4_lowrank_rows(const void* t, int dtype, const float* row_scale, float* out, int64_t M, void* stream);
 
 /* Feathered scatter of routed rows back over the cached canvas, in place: the pull form of
  * fuse_patch_predictions (flux/routing.py:328-379).  For canvas token j with contributor list

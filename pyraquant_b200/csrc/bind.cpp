@@ -80,6 +80,10 @@ bool plain_rows(const Tensor* codes, const Tensor* scales, const Tensor* row) {
          scales->dim() == 3 && scales->size(0) == (M + 127) / 128 && scales->size(1) == (K2 + per - 1) / per && scales->size(2) == 512 &&
          (row == nullptr || (plain(*row, at::kFloat, codes->device()) && row->dim() == 1 && row->size(0) == M));
 }
+// a rank-32 factor of the product in fp32
+bool plain_low(const Tensor& t, int64_t rows, c10::Device device) {
+  return plain(t, at::kFloat, device) && t.dim() == 2 && t.size(0) == rows && t.size(1) == 32 && aligned(t, 16);
+}
 // an argument that is a tensor or None; false for anything else
 bool optional_tensor(PyObject* o, const Tensor** t) {
   *t = o == Py_None ? nullptr : tensor_of(o);
@@ -122,25 +126,29 @@ PyObject* dequant_rows_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// fp4_gemm(codes, scales, rows or None of x, the same of w, bias or None, bf16?, workspace, its bytes) -> [M,N], or None
+// fp4_gemm(codes, scales, rows or None of x, the same of w, bias or None, bf16?, workspace, its bytes, low-rank rows t and lb or
+// None) -> [M,N], or None
 PyObject* fp4_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    const Tensor *x_row, *w_row, *bias;
-    if (n != 10 || !optional_tensor(a[2], &x_row) || !optional_tensor(a[5], &w_row) || !optional_tensor(a[6], &bias)) return none();
+    const Tensor *x_row, *w_row, *bias, *t, *lb;
+    if (n != 12 || !optional_tensor(a[2], &x_row) || !optional_tensor(a[5], &w_row) || !optional_tensor(a[6], &bias) ||
+        !optional_tensor(a[10], &t) || !optional_tensor(a[11], &lb) || (t == nullptr) != (lb == nullptr))
+      return none();
     const Tensor *xq = tensor_of(a[0]), *xs = tensor_of(a[1]), *wq = tensor_of(a[3]), *ws = tensor_of(a[4]);
     if (!plain_rows(xq, xs, x_row) || !plain_rows(wq, ws, w_row) || (x_row == nullptr) != (w_row == nullptr) ||
         wq->device() != xq->device() || wq->size(1) != xq->size(1) || wq->size(0) == 0)
       return none();
     const int64_t M = xq->size(0), N = wq->size(0), K = xq->size(1) * 2;
     if (bias != nullptr && (!plain(*bias, at::kFloat, xq->device()) || bias->numel() != N)) return none();
+    if (t != nullptr && !(plain_low(*t, M, xq->device()) && plain_low(*lb, N, xq->device()))) return none();
     const bool bf16 = a[7] == Py_True;
     c10::cuda::CUDAGuard guard(xq->device());
     Tensor out = make({M, N}, bf16 ? at::kBFloat16 : at::kHalf, *xq);
-    const int rc = pq_fp4_gemm(xq->data_ptr<uint8_t>(), K / 2, xs->data_ptr<uint8_t>(), x_row != nullptr ? x_row->data_ptr<float>() : nullptr,
-                               wq->data_ptr<uint8_t>(), K / 2, ws->data_ptr<uint8_t>(), w_row != nullptr ? w_row->data_ptr<float>() : nullptr,
-                               bias != nullptr ? bias->data_ptr<float>() : nullptr, x_row != nullptr ? PQ_FP4_NV : PQ_FP4_MX, out.data_ptr(),
-                               bf16 ? PQ_DTYPE_BF16 : PQ_DTYPE_FP16, N, M, N, K, PyLong_AsVoidPtr(a[8]), static_cast<size_t>(PyLong_AsSize_t(a[9])),
-                               stream_of(*xq));
+    auto floats = [](const Tensor* v) { return v != nullptr ? v->data_ptr<float>() : nullptr; };
+    const int rc = pq_fp4_gemm_lowrank(xq->data_ptr<uint8_t>(), K / 2, xs->data_ptr<uint8_t>(), floats(x_row), wq->data_ptr<uint8_t>(), K / 2,
+                                       ws->data_ptr<uint8_t>(), floats(w_row), floats(bias), floats(t), floats(lb),
+                                       x_row != nullptr ? PQ_FP4_NV : PQ_FP4_MX, out.data_ptr(), bf16 ? PQ_DTYPE_BF16 : PQ_DTYPE_FP16, N, M, N, K,
+                                       PyLong_AsVoidPtr(a[8]), static_cast<size_t>(PyLong_AsSize_t(a[9])), stream_of(*xq));
     return rc == PQ_OK ? THPVariable_Wrap(out) : fail("pq_fp4_gemm", rc);
   });
 }

@@ -81,8 +81,8 @@ __device__ __forceinline__ void store_row64(unsigned short* o, int n, int lane, 
 
 template <int FMT, int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(kFp4Threads, STAGES == 3 ? 2 : 1)
-pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const Fp4GemmParams p,
-                   int split) {
+pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmLb, const Fp4GemmParams p, int split) {
   using L = Fp4Smem<FMT, STAGES>;
   using F = Fp4Fmt<FMT>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -101,6 +101,8 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const int num_kb = (p.K + kFp4StageK - 1) / kFp4StageK;
   const int kb0 = SPLIT ? static_cast<int>(static_cast<int64_t>(num_kb) * rank / split) : 0;
   const int kb1 = SPLIT ? static_cast<int>(static_cast<int64_t>(num_kb) * (rank + 1) / split) : num_kb;
+  // the low-rank term is a stage in front of the first CTA's
+  const int first = kb0 - (p.t != nullptr && rank == 0 ? 1 : 0);
   const bool aligned_ok = (smem_u32(smem) & 1023u) == 0;
 
   if (threadIdx.x == 0) {
@@ -127,13 +129,19 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const uint8_t* sfb = p.sfb + static_cast<int64_t>(n0 >> 7) * p.tiles_k * 512;
       bool ok = true;
 #pragma unroll 1
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, stage = i % STAGES;
+      for (int kb = first; kb < kb1; ++kb) {
+        const int i = kb - first, stage = i % STAGES;
         if (!wait_or_abort(&empty_bar[stage], ((i / STAGES) & 1) ^ 1u, abort_flag)) {
           report_timeout(p.status, 1, 1); *abort_flag = 1; ok = false;
           break;
         }
         uint8_t* a_s = smem + stage * L::kOperand;
+        if (kb < kb0) {
+          mbar_arrive_expect_tx(&full_bar[stage], static_cast<uint32_t>(p.a_rows * BK + L::kBBytes));
+          tma_load_2d(a_s, &tmT, &full_bar[stage], 0, row0);
+          tma_load_2d(a_s + L::kABytes, &tmLb, &full_bar[stage], 0, n0);
+          continue;
+        }
         uint8_t* s_s = smem + L::kScaleOff + stage * 2 * L::kScale;
         const int t0 = kb * F::kTilesPerStage;
         const uint32_t sbytes = static_cast<uint32_t>(p.tiles_k - t0 < F::kTilesPerStage ? p.tiles_k - t0 : F::kTilesPerStage) * 512u;
@@ -153,14 +161,30 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const uint32_t sfb_shift = static_cast<uint32_t>((n0 & 64) >> 5);
       bool ok = true;
 #pragma unroll 1
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, stage = i % STAGES;
+      for (int kb = first; kb < kb1; ++kb) {
+        const int i = kb - first, stage = i % STAGES;
         if (!wait_or_abort(&full_bar[stage], (i / STAGES) & 1, abort_flag)) {
           report_timeout(p.status, 2, 1); *abort_flag = 1; ok = false;
           break;
         }
         tc_fence_after();
         const uint32_t a_addr = smem_u32(smem + stage * L::kOperand);
+        const uint64_t a_desc = make_kmajor_sw128_desc(a_addr);
+        const uint64_t b_desc = make_kmajor_sw128_desc(a_addr + L::kABytes);
+        if (kb < kb0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tc_mma_tf32(tmem_base, a_desc + static_cast<uint64_t>(2 * j), b_desc + static_cast<uint64_t>(2 * j), make_idesc_tf32(BM, BN),
+                        j > 0 ? 1u : 0u);
+          tc_commit(&empty_bar[stage]);
+          // the accumulator is whole before the other kind of MMA adds to it; the first use of the first stage
+          if (!wait_or_abort(&empty_bar[stage], 0u, abort_flag)) {
+            report_timeout(p.status, 2, 4); *abort_flag = 1; ok = false;
+            break;
+          }
+          tc_fence_after();
+          continue;
+        }
         const uint32_t s_addr = smem_u32(smem + L::kScaleOff + stage * 2 * L::kScale);
         const uint32_t sfa_t = tmem_base + BN + stage * L::kSetCols;
         const uint32_t sfb_t = sfa_t + 4 * F::kTilesPerStage;
@@ -172,8 +196,6 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             tc_cp_scale_tile(sfb_t + 4 * j, scale_tile_desc(s_addr + L::kScale + j * 512));
           }
         }
-        const uint64_t a_desc = make_kmajor_sw128_desc(a_addr);
-        const uint64_t b_desc = make_kmajor_sw128_desc(a_addr + L::kABytes);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (j * 64 < left) {
@@ -290,7 +312,7 @@ pq_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 }
 
 template <int FMT, int STAGES, bool SPLIT>
-int launch_fp4(const CUtensorMap& tmA, const CUtensorMap& tmW, const Fp4GemmParams& p, int split, cudaStream_t st) {
+int launch_fp4(const CUtensorMap& tmA, const CUtensorMap& tmW, const CUtensorMap& tmT, const CUtensorMap& tmLb, const Fp4GemmParams& p, int split, cudaStream_t st) {
   using L = Fp4Smem<FMT, STAGES>;
   auto kern = pq_fp4_gemm_kernel<FMT, STAGES, SPLIT>;
   static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes
@@ -311,7 +333,7 @@ int launch_fp4(const CUtensorMap& tmA, const CUtensorMap& tmW, const Fp4GemmPara
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = SPLIT ? 2 : 1;
-  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmW, p, split));
+  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmW, tmT, tmLb, p, split));
   return PQ_OK;
 }
 
@@ -330,13 +352,15 @@ int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, 
   p.nt = (p.N + BN - 1) / BN;
   const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt;
   if (tiles > 0x0fffffff) return PQ_ERR_SHAPE;
-  CUtensorMap tmA, tmW;
+  CUtensorMap tmA, tmW, tmT = {}, tmLb = {};
   // a single tile of few rows loads only those: what the others hold ends up in rows that nobody stores
   p.a_rows = p.M < BM ? (p.M + 7) / 8 * 8 : BM;
   int rc = make_tile_map(&tmA, xq, p.M, p.K / 2, ldx, p.a_rows);
   if (rc != PQ_OK) return rc;
   rc = make_tile_map(&tmW, w, p.N, p.K / 2, ldw, BN);
   if (rc != PQ_OK) return rc;
+  if (p.t != nullptr && ((rc = make_tile_map(&tmT, p.t, p.M, BK, BK, p.a_rows)) != PQ_OK || (rc = make_tile_map(&tmLb, p.lb, p.N, BK, BK, BN)) != PQ_OK))
+    return rc;
   // Along K a stage takes 0.26 us; a cluster costs 1 to 2 us, the more the more rows the joined tiles have, and runs in rounds when
   // the clusters do not all find room at once (2560 -> 2560, 40 tiles: 6.0 us split in two, 10.2 in four).  Measured in us,
   // unsplit / in two / in four, by stages: 77 rows -> 640 (10 tiles) 8 stages 5.5 / 6.6 / 6.5 (-> 1280), 10: 6.2 / 6.9 / 6.5,
@@ -351,9 +375,9 @@ int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, 
     split = want;
     while (split > num_kb) split /= 2;
   }
-  if (split > 1) return launch_fp4<FMT, 7, true>(tmA, tmW, p, split, st);
-  if (tiles > sms) return launch_fp4<FMT, 3, false>(tmA, tmW, p, 1, st);
-  return launch_fp4<FMT, 7, false>(tmA, tmW, p, 1, st);
+  if (split > 1) return launch_fp4<FMT, 7, true>(tmA, tmW, tmT, tmLb, p, split, st);
+  if (tiles > sms) return launch_fp4<FMT, 3, false>(tmA, tmW, tmT, tmLb, p, 1, st);
+  return launch_fp4<FMT, 7, false>(tmA, tmW, tmT, tmLb, p, 1, st);
 }
 
 }  // namespace
@@ -361,24 +385,25 @@ int dispatch_fp4(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, 
 
 using namespace pq;
 
-extern "C" int pq_fp4_gemm(const uint8_t* xq, int64_t ldx, const uint8_t* x_scales, const float* s_row, const uint8_t* w,
-                           int64_t ldw, const uint8_t* w_scales, const float* s_col, const float* bias, int fmt, void* out,
-                           int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace, size_t ws_bytes,
-                           void* stream) {
+extern "C" int pq_fp4_gemm_lowrank(const uint8_t* xq, int64_t ldx, const uint8_t* x_scales, const float* s_row, const uint8_t* w,
+                                   int64_t ldw, const uint8_t* w_scales, const float* s_col, const float* bias, const float* t,
+                                   const float* lb, int fmt, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                                   void* workspace, size_t ws_bytes, void* stream) {
   if (M < 0 || N <= 0 || K <= 0 || M > 0x7fffff00LL || N > 0x7fffff00LL || K > 0x7fffff00LL) return PQ_ERR_SHAPE;
   if (out_dtype != PQ_DTYPE_BF16 && out_dtype != PQ_DTYPE_FP16) return PQ_ERR_DTYPE;
   if (fmt != PQ_FP4_MX && fmt != PQ_FP4_NV) return PQ_ERR_UNSUPPORTED;
   if (M == 0) return PQ_OK;
   if (xq == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr || out == nullptr) return PQ_ERR_NULL;
+  if ((t == nullptr) != (lb == nullptr)) return PQ_ERR_NULL;
   if (fmt == PQ_FP4_NV && (s_row == nullptr || s_col == nullptr)) return PQ_ERR_NULL;
   if (ldx < K / 2 || ldw < K / 2 || ldo < N) return PQ_ERR_SHAPE;
   if (K % 32 != 0 || ldx % 16 != 0 || ldw % 16 != 0) return PQ_ERR_ALIGN;
   if (!aligned_to(xq, 16) || !aligned_to(w, 16) || !aligned_to(x_scales, 16) || !aligned_to(w_scales, 16) || !aligned_to(out, 2) ||
-      !aligned_to(s_row, 4) || !aligned_to(s_col, 4) || !aligned_to(bias, 4))
+      !aligned_to(s_row, 4) || !aligned_to(s_col, 4) || !aligned_to(bias, 4) || !aligned_to(t, 16) || !aligned_to(lb, 16))
     return PQ_ERR_ALIGN;
   if (workspace != nullptr && ws_bytes < PQ_GEMM_WORKSPACE_BYTES) return PQ_ERR_WORKSPACE;
   Fp4GemmParams p{};
-  p.sfa = x_scales; p.sfb = w_scales; p.s_row = s_row; p.s_col = s_col; p.bias = bias; p.out = out;
+  p.sfa = x_scales; p.sfb = w_scales; p.s_row = s_row; p.s_col = s_col; p.bias = bias; p.t = t; p.lb = lb; p.out = out;
   p.status = static_cast<int32_t*>(workspace);
   p.ldo = ldo; p.M = static_cast<int>(M); p.N = static_cast<int>(N); p.K = static_cast<int>(K);
   p.tiles_k = static_cast<int>(fp4_scale_tiles(K, fmt));
@@ -387,4 +412,12 @@ extern "C" int pq_fp4_gemm(const uint8_t* xq, int64_t ldx, const uint8_t* x_scal
   p.vec = ldo % 8 == 0 && aligned_to(out, 16) ? 1 : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return fmt == PQ_FP4_MX ? dispatch_fp4<PQ_FP4_MX>(xq, ldx, w, ldw, p, st) : dispatch_fp4<PQ_FP4_NV>(xq, ldx, w, ldw, p, st);
+}
+
+extern "C" int pq_fp4_gemm(const uint8_t* xq, int64_t ldx, const uint8_t* x_scales, const float* s_row, const uint8_t* w,
+                           int64_t ldw, const uint8_t* w_scales, const float* s_col, const float* bias, int fmt, void* out,
+                           int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace, size_t ws_bytes,
+                           void* stream) {
+  return pq_fp4_gemm_lowrank(xq, ldx, x_scales, s_row, w, ldw, w_scales, s_col, bias, nullptr, nullptr, fmt, out, out_dtype, ldo, M, N, K,
+                             workspace, ws_bytes, stream);
 }

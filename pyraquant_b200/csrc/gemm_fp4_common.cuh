@@ -20,6 +20,8 @@ struct Fp4GemmParams {
   const float* s_row;      // [M] or NULL (1)
   const float* s_col;      // [N] or NULL (1)
   const float* bias;       // [N] or NULL
+  const float* t;          // [M, 32] low-rank activations over s_row, or NULL
+  const float* lb;         // [N, 32] low-rank up-projection over s_col
   void* out;
   int32_t* status;
   int64_t ldo;
@@ -54,6 +56,30 @@ __host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, bool mx, int
          | ((mx ? 1u : 0u) << 23)                                 // scale format: E8M0 (else E4M3)
          | (static_cast<uint32_t>(M >> 4) << 24)
          | (static_cast<uint32_t>(scale_id) << 29);               // A scale id
+}
+
+// The low-rank term t @ lb^T is one more stage of the product, in front of the others: 32 fp32 values are 128 bytes, so its tiles are
+// loaded, swizzled and addressed like those of 256 codes, and four kind::tf32 MMAs (K = 8) start the accumulator.  TF32 has the
+// significand of fp16 and the exponents of fp32: 16-bit values over powers of two are exact in it.  The MMAs of the other kind
+// are issued once these have completed.  Measured with the conversion of t, us, without the term / with it / with a library product
+// added to the output instead: mx 77 x 2048 -> 1280 4.8 / 6.2 / 7.6, 16384 x 1280 -> 10240 99 / 118 / 252, 8192^3 184 / 206 / 254;
+// nv 16384 x 1280 -> 1280 19.1 / 22.6 / 30.1.
+__host__ __device__ constexpr uint32_t make_idesc_tf32(int M, int N) {
+  return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_tf32(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_tf32_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
 }
 
 template <int FMT>

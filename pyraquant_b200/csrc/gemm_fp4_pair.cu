@@ -115,7 +115,8 @@ template <int FMT, bool SCALED, typename OutT>
 __global__ void __launch_bounds__(kPairThreads, 1)
 pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                         const __grid_constant__ CUtensorMap tmSa, const __grid_constant__ CUtensorMap tmSw,
-                        const __grid_constant__ CUtensorMap tmOut, const Fp4GemmParams p) {
+                        const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmT,
+                        const __grid_constant__ CUtensorMap tmLb, const Fp4GemmParams p) {
   using L = Fp4PairSmem<FMT>;
   using F = Fp4Fmt<FMT>;
   constexpr int S = kPairStages;
@@ -134,6 +135,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
   const int pair = static_cast<int>(blockIdx.x) >> 1, pairs = static_cast<int>(gridDim.x) >> 1;
   const int tiles = p.mt * p.nt;                                   // of 256 x 256
   const int num_kb = (p.K + kFp4StageK - 1) / kFp4StageK;
+  const bool low = p.t != nullptr;                                 // a stage of its own in front of each tile's
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmW); tma_prefetch_desc(&tmSa); tma_prefetch_desc(&tmSw);
@@ -167,18 +169,24 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const int n0 = w.nt * 256;
         const int nhalf0 = n0 + static_cast<int>(rank) * 128;
 #pragma unroll 1
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = low ? -1 : 0; kb < num_kb; ++kb) {
           if (!wait_or_abort(&empty_bar[stage], phase ^ 1u, abort_flag)) {
             report_timeout(p.status, 1, 1); *abort_flag = 1; ok = false; break;
           }
           uint8_t* a_s = smem + stage * L::kOperand;
           uint8_t* s_s = smem + L::kScaleOff + stage * (L::kSfa + L::kSfb);
           const uint32_t fb = leader_addr(&full_bar[stage]);
-          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kStageBytes);
-          tma_load_2d_pair(a_s, &tmA, fb, kb * BK, row0);
-          tma_load_2d_pair(a_s + L::kABytes, &tmW, fb, kb * BK, nhalf0);
-          tma_load_3d_pair(s_s, &tmSa, fb, 0, kb * F::kTilesPerStage, row0 >> 7);
-          tma_load_3d_pair(s_s + L::kSfa, &tmSw, fb, 0, kb * F::kTilesPerStage, n0 >> 7);
+          if (kb < 0) {
+            if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kOperand);
+            tma_load_2d_pair(a_s, &tmT, fb, 0, row0);
+            tma_load_2d_pair(a_s + L::kABytes, &tmLb, fb, 0, nhalf0);
+          } else {
+            if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kStageBytes);
+            tma_load_2d_pair(a_s, &tmA, fb, kb * BK, row0);
+            tma_load_2d_pair(a_s + L::kABytes, &tmW, fb, kb * BK, nhalf0);
+            tma_load_3d_pair(s_s, &tmSa, fb, 0, kb * F::kTilesPerStage, row0 >> 7);
+            tma_load_3d_pair(s_s + L::kSfa, &tmSw, fb, 0, kb * F::kTilesPerStage, n0 >> 7);
+          }
           if (issued < S) ++issued;
           if (++stage == S) { stage = 0; phase ^= 1u; }
         }
@@ -205,6 +213,33 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 #pragma unroll 1
       for (int t = pair; t < tiles && ok; t += pairs, ++it) {
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>((it & 1) * 128);
+        if (low) {
+          if (!full_ready && !wait_or_abort(&full_bar[stage], phase, abort_flag)) {
+            report_timeout(p.status, 2, 1); *abort_flag = 1; ok = false; break;
+          }
+          if (it > 0 && !wait_or_abort(shared_free, static_cast<uint32_t>(it - 1) & 1u, abort_flag)) {
+            report_timeout(p.status, 2, 2); *abort_flag = 1; ok = false; break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + stage * L::kOperand);
+          const uint64_t a_desc = make_kmajor_sw128_desc(a_addr), b_desc = make_kmajor_sw128_desc(a_addr + L::kABytes);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            tc_mma_tf32_pair(d_tmem, a_desc + static_cast<uint64_t>(2 * j), b_desc + static_cast<uint64_t>(2 * j),
+                             make_idesc_tf32(2 * BM, 256), j > 0 ? 1u : 0u);
+          // this stage has no scales; the hand-over of scale sets counts it all the same
+          if (L::kUnits > 1) tc_commit_pair(smem_u32(&half_bar[stage]));
+          if (issued < 2) ++issued;
+          commit_both(&empty_bar[stage]);
+          // the accumulator is whole before the other kind of MMA adds to it (the stage cannot be refilled and used again before
+          // this thread goes on, so its barrier keeps the parity waited for)
+          if (!wait_or_abort(&empty_bar[stage], phase, abort_flag)) {
+            report_timeout(p.status, 2, 4); *abort_flag = 1; ok = false; break;
+          }
+          tc_fence_after();
+          full_ready = false;
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
 #pragma unroll 1
         for (int kb = 0; kb < num_kb && ok; ++kb) {
           // nv: the scale columns of this stage were last read by MMAs up to the first half of the stage before last
@@ -238,7 +273,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
               tc_cp_scale_tile_pair(sfb_t + 8 * j + 4, scale_tile_desc(s_addr + L::kSfa + (F::kTilesPerStage + tile) * 512));
             }
             // the scales of a tile's first stage are under way before the accumulator is free
-            if (u == 0 && kb == 0 && it > 0) {
+            if (u == 0 && kb == 0 && it > 0 && !low) {
               if (!wait_or_abort(shared_free, static_cast<uint32_t>(it - 1) & 1u, abort_flag)) {
                 report_timeout(p.status, 2, 2); *abort_flag = 1; ok = false; break;
               }
@@ -251,7 +286,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 const int s = m * 64 / F::kTileK;
                 const uint32_t idesc = make_idesc_fp4(2 * BM, 256, FMT == PQ_FP4_MX, FMT == PQ_FP4_MX ? 2 * (j & 1) : 0);
                 tc_mma_fp4_pair<FMT>(d_tmem, a_desc + static_cast<uint64_t>(2 * j), b_desc + static_cast<uint64_t>(2 * j), idesc,
-                                     sfa_t + 4 * s, sfb_t + 8 * s, (kb > 0 || j > 0) ? 1u : 0u);
+                                     sfa_t + 4 * s, sfb_t + 8 * s, (kb > 0 || j > 0 || low) ? 1u : 0u);
               }
             }
             if (L::kUnits > 1 && u == 0) tc_commit_pair(smem_u32(&half_bar[stage]));
@@ -417,12 +452,13 @@ int launch_pair(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, F
   const int64_t tiles = static_cast<int64_t>(p.mt) * p.nt;
   if (tiles > 0x3fffffff) return PQ_ERR_SHAPE;
   p.vec = p.vec && p.N % 8 == 0;
-  CUtensorMap tmA, tmW, tmSa, tmSw, tmOut = {};
+  CUtensorMap tmA, tmW, tmSa, tmSw, tmOut = {}, tmT = {}, tmLb = {};
   int rc;
   if ((rc = make_tile_map(&tmA, xq, p.M, p.K / 2, ldx, BM)) != PQ_OK || (rc = make_tile_map(&tmW, w, p.N, p.K / 2, ldw, 128)) != PQ_OK ||
       (rc = make_scale_map(&tmSa, p.sfa, p.M, p.tiles_k, F::kTilesPerStage, 1)) != PQ_OK ||
       (rc = make_scale_map(&tmSw, p.sfb, p.N, p.tiles_k, F::kTilesPerStage, 2)) != PQ_OK ||
-      (p.vec && (rc = make_out_map(&tmOut, p.out, p.M, p.N, p.ldo)) != PQ_OK))
+      (p.vec && (rc = make_out_map(&tmOut, p.out, p.M, p.N, p.ldo)) != PQ_OK) ||
+      (p.t != nullptr && ((rc = make_tile_map(&tmT, p.t, p.M, BK, BK, BM)) != PQ_OK || (rc = make_tile_map(&tmLb, p.lb, p.N, BK, BK, 128)) != PQ_OK)))
     return rc;
   auto kern = pq_fp4_gemm_pair_kernel<FMT, SCALED, OutT>;
   static bool attr_set[64] = {false};     // per device; benign race: the attribute value never changes
@@ -444,7 +480,7 @@ int launch_pair(const uint8_t* xq, int64_t ldx, const uint8_t* w, int64_t ldw, F
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmW, tmSa, tmSw, tmOut, p));
+  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmW, tmSa, tmSw, tmOut, tmT, tmLb, p));
   return PQ_OK;
 }
 

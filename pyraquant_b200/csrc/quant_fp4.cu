@@ -188,6 +188,28 @@ pq_dequant_rows_fp4_kernel(const uint8_t* codes, int64_t ldc, const uint8_t* sca
   }
 }
 
+// Low-rank activations t [M, 32] for the product's accumulator, which stands in units of the row scale: eight elements per thread,
+// t / s_row in fp32 (exact: a 16-bit value over a power of two).
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+pq_fp4_lowrank_rows_kernel(const T* t, const float* row_scale, float* out, int64_t M) {
+  wait_for_previous_kernel();
+  allow_next_kernel();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= 4 * M) return;
+  const float inv = row_scale != nullptr ? 1.0f / row_scale[i >> 2] : 1.0f;
+  const uint4 v = *reinterpret_cast<const uint4*>(t + 8 * i);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  T tag{};
+  Chunk16 o;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    o.w[2 * k] = __float_as_uint(lo_f32(w[k], tag) * inv);
+    o.w[2 * k + 1] = __float_as_uint(hi_f32(w[k], tag) * inv);
+  }
+  st_chunk16(out + 8 * i, o);
+}
+
 struct Args {
   const void* x; int64_t ldx; uint8_t* codes; uint8_t* scales; float* row_scale; int64_t M; int K;
 };
@@ -287,4 +309,18 @@ extern "C" int pq_dequant_rows_fp4(const uint8_t* codes, int64_t ldc, const uint
                             : dispatch_dequant<__nv_bfloat16, PQ_FP4_NV>(codes, ldc, scales, row_scale, out, ldo, M, static_cast<int>(K), st);
   return fmt == PQ_FP4_MX ? dispatch_dequant<__half, PQ_FP4_MX>(codes, ldc, scales, row_scale, out, ldo, M, static_cast<int>(K), st)
                           : dispatch_dequant<__half, PQ_FP4_NV>(codes, ldc, scales, row_scale, out, ldo, M, static_cast<int>(K), st);
+}
+
+extern "C" int pq_fp4_lowrank_rows(const void* t, int dtype, const float* row_scale, float* out, int64_t M, void* stream) {
+  if (M < 0) return PQ_ERR_SHAPE;
+  if (dtype != PQ_DTYPE_BF16 && dtype != PQ_DTYPE_FP16) return PQ_ERR_DTYPE;
+  if (M == 0) return PQ_OK;
+  if (t == nullptr || out == nullptr) return PQ_ERR_NULL;
+  if (!aligned_to(t, 16) || !aligned_to(out, 32) || !aligned_to(row_scale, 4)) return PQ_ERR_ALIGN;
+  const int64_t blocks = (4 * M + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffffLL) return PQ_ERR_SHAPE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == PQ_DTYPE_BF16)
+    return launch_chained(pq_fp4_lowrank_rows_kernel<__nv_bfloat16>, blocks, st, static_cast<const __nv_bfloat16*>(t), row_scale, out, M);
+  return launch_chained(pq_fp4_lowrank_rows_kernel<__half>, blocks, st, static_cast<const __half*>(t), row_scale, out, M);
 }

@@ -55,13 +55,31 @@ def dequant_rows_fp4(q: Fp4Rows, dtype: torch.dtype = torch.bfloat16) -> torch.T
     return torch.ops.pq_b200.dequant_rows_fp4(q.codes, q.scales, q.row_scale, ops.dtype_code(dtype))
 
 
-def fp4_gemm(xq: Fp4Rows, w: Fp4Rows, bias: Optional[torch.Tensor] = None,
-             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """x [M,K] times the transpose of w [N,K] (+ fp32 bias [N]) in ``out_dtype``; both operands in the same format."""
+def fp4_gemm(xq: Fp4Rows, w: Fp4Rows, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16,
+             lowrank: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
+    """x [M,K] times the transpose of w [N,K] (+ fp32 bias [N]) in ``out_dtype``; both operands in the same format.
+    ``lowrank``: the factors of a rank-32 term that is added before the one rounding, as ``lowrank_rows`` and
+    ``lowrank_weight`` make them for these operands."""
+    t, lb = lowrank if lowrank is not None else (None, None)
     if _eager():
-        return ops._fp4_gemm_impl(xq.codes, xq.scales, xq.row_scale, w.codes, w.scales, w.row_scale, bias, out_dtype)
+        return ops._fp4_gemm_impl(xq.codes, xq.scales, xq.row_scale, w.codes, w.scales, w.row_scale, bias, out_dtype, t, lb)
     return torch.ops.pq_b200.fp4_gemm(xq.codes, xq.scales, xq.row_scale, w.codes, w.scales, w.row_scale, bias,
-                                      ops.dtype_code(out_dtype))
+                                      ops.dtype_code(out_dtype), t, lb)
+
+
+def lowrank_rows(t: torch.Tensor, xq: Fp4Rows) -> torch.Tensor:
+    """Low-rank activations t [M,32] bf16/fp16 in the units of the rows they go with: fp32, t over the row scale."""
+    if _eager():
+        return ops._fp4_lowrank_rows_impl(t, xq.row_scale)
+    return torch.ops.pq_b200.fp4_lowrank_rows(t, xq.row_scale)
+
+
+def lowrank_weight(B: torch.Tensor, w: Fp4Rows) -> torch.Tensor:
+    """The up-projection B [32,N] bf16/fp16 in the units of the weights it goes with: fp32 [N,32].  Plain tensor arithmetic, done
+    once per layer."""
+    assert B.dim() == 2 and B.shape == (32, w.codes.shape[0]) and B.dtype in ops._DT
+    b = B.t().float()
+    return (b if w.row_scale is None else b / w.row_scale[:, None]).contiguous()
 
 
 def fp4_linear_2d(x2: torch.Tensor, w: Fp4Rows, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -111,7 +129,8 @@ def quantize_weight_fp4(w: torch.Tensor, fmt: str = DEFAULT_FORMAT) -> Fp4Rows:
 class Fp4Linear(LowRankFactors, nn.Module):
     """4-bit stand-in for ``nn.Linear``: packed weights held as buffers, activations quantised per call in the same
     format.  A low-rank branch (``lowrank=(A, B)`` or the ``_lowrank_A`` / ``_lowrank_B`` attributes that
-    ``Int8Linear`` reads too) is added in the activation type after the product, ``y += (x @ A) @ B``.
+    ``Int8Linear`` reads too), ``y += (x @ A) @ B`` with x @ A rounded to the activation type, is added in the product's fp32
+    accumulator for rank 32 and factors in bf16 / fp16, in the activation type after the product otherwise.
     Needs in_features % 32 == 0."""
 
     def __init__(self, lin: nn.Linear, device: Optional[torch.device] = None, fmt: str = DEFAULT_FORMAT,
@@ -157,11 +176,32 @@ class Fp4Linear(LowRankFactors, nn.Module):
                 setattr(self, name, v.to(new.device))
         return self
 
+    def _lr_weight(self) -> torch.Tensor:
+        """``lowrank_weight`` of lr_B, remade whenever lr_B or the row scales are replaced, moved or written in place.  Kept only
+        when it is there for every stream: not while a graph is captured, and not of inference tensors, whose changes
+        nothing counts."""
+        src = [t for t in (self.lr_B, self.weight_row_scale) if t is not None]
+        if not _eager() or any(t.is_inference() for t in src):
+            return lowrank_weight(self.lr_B, self.weight_rows)
+        key = tuple((t.data_ptr(), t.dtype, t.device, tuple(t.shape), t._version) for t in src)
+        c = self.__dict__.get("_lr_weight_cache")
+        if c is None or c[0] != key:
+            c = (key, lowrank_weight(self.lr_B, self.weight_rows))
+            if self.lr_B.is_cuda:
+                if torch.cuda.is_current_stream_capturing():
+                    return c[1]
+                torch.cuda.current_stream(self.lr_B.device).synchronize()
+            self.__dict__["_lr_weight_cache"] = c
+        return c[1]
+
     def _product(self, xq: Fp4Rows, x2: torch.Tensor) -> torch.Tensor:
+        if self.lr_A is None:
+            return fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype)
+        t = self._down(x2).to(x2.dtype)
+        if t.shape[1] == 32 and self.lr_B.dtype in ops._DT:
+            return fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype, (lowrank_rows(t, xq), self._lr_weight()))
         y = fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype)
-        if self.lr_A is not None:
-            y.addmm_(self._down(x2).to(y.dtype), self.lr_B.to(y.dtype))
-        return y
+        return y.addmm_(t, self.lr_B.to(y.dtype))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape

@@ -601,11 +601,12 @@ def _dequant_rows_fp4_impl(codes: Tensor, scales: Tensor, row_scale: Optional[Te
 
 
 def _fp4_gemm_impl(xq: Tensor, xs: Tensor, x_row: Optional[Tensor], wq: Tensor, ws: Tensor, w_row: Optional[Tensor],
-                   bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+                   bias: Optional[Tensor], out_dtype: torch.dtype, t: Optional[Tensor] = None,
+                   lb: Optional[Tensor] = None) -> Tensor:
     dt = _dt(out_dtype)
     if xq.is_cuda:
         out = _BIND().fp4_gemm(xq, xs, x_row, wq, ws, w_row, bias, out_dtype is torch.bfloat16, status_word(xq.device).data_ptr(),
-                               _lib.GEMM_WORKSPACE_BYTES)
+                               _lib.GEMM_WORKSPACE_BYTES, t, lb)
         if out is not None:
             return out
     fmt, M, K = check_fp4_rows(xq, xs, x_row, "fp4_gemm, activations")
@@ -614,13 +615,17 @@ def _fp4_gemm_impl(xq: Tensor, xs: Tensor, x_row: Optional[Tensor], wq: Tensor, 
     assert N > 0 and wq.device == xq.device
     assert bias is None or (bias.dtype == torch.float32 and bias.numel() == N and bias.is_contiguous()
                             and bias.device == xq.device), "bias is an fp32 vector with one entry per output channel"
+    assert (t is None) == (lb is None), "a low-rank term has two factors"
+    for v, rows in ((t, M), (lb, N)):
+        assert v is None or (v.dtype == torch.float32 and tuple(v.shape) == (rows, 32) and v.is_contiguous() and v.device == xq.device
+                             and v.data_ptr() % 16 == 0), "low-rank factors are contiguous fp32 [M, 32] and [N, 32]"
     xq = _codes_aligned(xq); wq = _codes_aligned(wq)
     out = xq.new_empty((M, N), dtype=out_dtype)
     st = status_word(xq.device)
     with _on_device(xq):
-        rc = _LIB().pq_fp4_gemm(xq.data_ptr(), xq.stride(0) if M > 1 else K // 2, xs.data_ptr(), _ptr(x_row), wq.data_ptr(),
-                                wq.stride(0) if N > 1 else K // 2, ws.data_ptr(), _ptr(w_row), _ptr(bias), FP4_FORMATS[fmt],
-                                out.data_ptr(), dt, N, M, N, K, st.data_ptr(), st.numel() * 4, _stream(xq))
+        rc = _LIB().pq_fp4_gemm_lowrank(xq.data_ptr(), xq.stride(0) if M > 1 else K // 2, xs.data_ptr(), _ptr(x_row), wq.data_ptr(),
+                                        wq.stride(0) if N > 1 else K // 2, ws.data_ptr(), _ptr(w_row), _ptr(bias), _ptr(t), _ptr(lb),
+                                        FP4_FORMATS[fmt], out.data_ptr(), dt, N, M, N, K, st.data_ptr(), st.numel() * 4, _stream(xq))
     if rc:
         _lib.check(rc, f"pq_fp4_gemm(M={M}, N={N}, K={K}, {fmt})")
     return out
@@ -926,6 +931,22 @@ def _(xq, s_a, w_int8, s_w_gm, bias, out_dtype_code):
     return xq.new_empty((xq.shape[0], w_int8.shape[0]), dtype=_CODE2DT[out_dtype_code])
 
 
+def _fp4_lowrank_rows_impl(t: Tensor, row_scale: Optional[Tensor]) -> Tensor:
+    dt = _dt(t.dtype)
+    assert t.is_cuda and t.dim() == 2 and t.shape[1] == 32, "low-rank activations are [M, 32] on a GPU"
+    M = t.shape[0]
+    assert row_scale is None or (row_scale.dtype == torch.float32 and row_scale.numel() == M and row_scale.is_contiguous()
+                                 and row_scale.device == t.device), "one fp32 row scale per row"
+    if not t.is_contiguous() or t.data_ptr() % 16 != 0:
+        t = t.clone(memory_format=torch.contiguous_format)
+    out = t.new_empty((M, 32), dtype=torch.float32)
+    with _on_device(t):
+        rc = _LIB().pq_fp4_lowrank_rows(t.data_ptr(), dt, _ptr(row_scale), out.data_ptr(), M, _stream(t))
+    if rc:
+        _lib.check(rc, f"pq_fp4_lowrank_rows(M={M})")
+    return out
+
+
 @torch.library.custom_op("pq_b200::group_norm_rows", mutates_args=(), device_types="cuda")
 def group_norm_rows_op(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, silu: bool) -> Tensor:
     return _group_norm_impl(x, groups, weight, bias, eps, "silu" if silu else None)
@@ -963,13 +984,23 @@ def _(codes, scales, row_scale, dtype_code):
 
 @torch.library.custom_op("pq_b200::fp4_gemm", mutates_args=(), device_types="cuda")
 def fp4_gemm_op(xq: Tensor, xs: Tensor, x_row: Optional[Tensor], wq: Tensor, ws: Tensor, w_row: Optional[Tensor],
-                bias: Optional[Tensor], out_dtype_code: int) -> Tensor:
-    return _fp4_gemm_impl(xq, xs, x_row, wq, ws, w_row, bias, _CODE2DT[out_dtype_code])
+                bias: Optional[Tensor], out_dtype_code: int, t: Optional[Tensor] = None, lb: Optional[Tensor] = None) -> Tensor:
+    return _fp4_gemm_impl(xq, xs, x_row, wq, ws, w_row, bias, _CODE2DT[out_dtype_code], t, lb)
 
 
 @fp4_gemm_op.register_fake
-def _(xq, xs, x_row, wq, ws, w_row, bias, out_dtype_code):
+def _(xq, xs, x_row, wq, ws, w_row, bias, out_dtype_code, t=None, lb=None):
     return xq.new_empty((xq.shape[0], wq.shape[0]), dtype=_CODE2DT[out_dtype_code])
+
+
+@torch.library.custom_op("pq_b200::fp4_lowrank_rows", mutates_args=(), device_types="cuda")
+def fp4_lowrank_rows_op(t: Tensor, row_scale: Optional[Tensor]) -> Tensor:
+    return _fp4_lowrank_rows_impl(t, row_scale)
+
+
+@fp4_lowrank_rows_op.register_fake
+def _(t, row_scale):
+    return t.new_empty((t.shape[0], 32), dtype=torch.float32)
 
 
 @torch.library.custom_op("pq_b200::dequant_epilogue", mutates_args=(), device_types="cuda")

@@ -219,6 +219,128 @@ def test_product_on_cta_pairs(cuda_dev, fmt, M, N, K, bias):
     assert torch.equal(y, again)
 
 
+# ------------------------------------------------------------------------------------------------ product with a low-rank term
+def low_rank_case(M, N, K, fmt, dtype, dev):
+    """Packed operands, t = x A in ``dtype``, B and the fp32 factors that the product takes."""
+    x, xq = make_rows(M, K, fmt, dtype, 1, dev)
+    _, wq = make_rows(N, K, fmt, torch.bfloat16, 2, dev)
+    g = torch.Generator().manual_seed(K + N)
+    fi = torch.finfo(dtype)
+    t = (x.double() @ (torch.randn(K, 32, generator=g).double() / K ** 0.5).to(dev)).clamp(-fi.max, fi.max).to(dtype)
+    B = (torch.randn(32, N, generator=g) / 3).to(dtype).to(dev)
+    return xq, wq, t, B, (fp4_exec.lowrank_rows(t, xq), fp4_exec.lowrank_weight(B, wq))
+
+
+def check_low_rank(y, xq, wq, bias, fmt, t, B):
+    """As check_product with 32 terms more.  The factors are exact in TF32 (16-bit values over powers of two), their products in
+    fp32; each of the 32 additions is off by at most 2^-23 of the sum of magnitudes."""
+    X, W = (ofp4.packed_values(q.codes.cpu(), q.scales.cpu(), None if q.row_scale is None else q.row_scale.cpu(), fmt) for q in (xq, wq))
+    K = X.shape[1]
+    T, U = t.cpu().double(), B.cpu().double()
+    ref = X @ W.t() + T @ U
+    S = X.abs() @ W.abs().t() + T.abs() @ U.abs()
+    bound = (K / 16 + 36) * 2.0 ** -23 * S
+    if bias is not None:
+        ref = ref + bias.cpu().double()
+        bound = bound + 2.0 ** -24 * (S + bias.cpu().double().abs())
+    fi = torch.finfo(y.dtype)
+    bound = bound + (ref.abs() + bound) * fi.eps / 2 + fi.smallest_normal * fi.eps / 2
+    border = fi.max * (2 - fi.eps / 2) / (2 - fi.eps)
+    got = y.cpu().double()
+    inside = ref.abs() + bound < border
+    assert bool(torch.isfinite(got[inside]).all()) and torch.equal(got[ref.abs() - bound >= border].abs(), torch.full_like(got[ref.abs() - bound >= border], float("inf")))
+    worst = float((torch.where(inside, (got - ref).abs(), torch.zeros_like(ref)) / bound).max())
+    assert worst <= 1, f"error {worst:.3g} times the bound"
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K,options", [(1, 8, 32, {}), (5, 7, 96, {}), (128, 64, 256, {}), (77, 200, 640, {}), (129, 131, 288, {}),
+                                           (1, 1280, 5120, {}), (33, 650, 2592, {"fp4_pair": 0, "fp4_split": 8}),
+                                           (300, 200, 1280, {"fp4_pair": 0, "fp4_split": 2}), (2500, 587, 64, {"fp4_pair": 0}),
+                                           (1300, 2056, 2080, {"fp4_pair": 0}), (256, 256, 64, {"fp4_pair": 2}), (1, 8, 32, {"fp4_pair": 2}),
+                                           (300, 520, 288, {"fp4_pair": 2}), (2300, 2312, 96, {"fp4_pair": 2}),
+                                           (3000, 2560, 1600, {"fp4_pair": 2}), (700, 333, 160, {"fp4_pair": 2}), (4173, 640, 2560, {})])
+def test_product_with_a_low_rank_term(cuda_dev, fmt, dtype, M, N, K, options):
+    xq, wq, t, B, factors = low_rank_case(M, N, K, fmt, dtype, cuda_dev)
+    assert torch.equal(factors[0].double() * (1 if fmt == "mx" else xq.row_scale.double()[:, None]), t.double())
+    assert torch.equal(factors[1].double() * (1 if fmt == "mx" else wq.row_scale.double()[:, None]), B.t().double())
+    bias = torch.randn(N, device=cuda_dev) if N % 3 else None
+    for k, v in options.items():
+        _lib.set_option(k, v)
+    try:
+        y = fp4_exec.fp4_gemm(xq, wq, bias, dtype, factors)
+        again = fp4_exec.fp4_gemm(xq, wq, bias, dtype, factors)
+        nothing = fp4_exec.fp4_gemm(xq, wq, bias, dtype, (torch.zeros_like(factors[0]), factors[1]))
+        plain = fp4_exec.fp4_gemm(xq, wq, bias, dtype)
+    finally:
+        _lib.set_option("fp4_pair", 1)
+        _lib.set_option("fp4_split", 0)
+    check_low_rank(y, xq, wq, bias, fmt, t, B)
+    assert torch.equal(y, again) and torch.equal(nothing, plain)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_low_rank_refusals_and_layouts(cuda_dev, fmt):
+    xq, wq, t, B, (tl, lb) = low_rank_case(40, 72, 96, fmt, torch.bfloat16, cuda_dev)
+    want = fp4_exec.fp4_gemm(xq, wq, None, torch.bfloat16, (tl, lb))
+    wide = torch.zeros(40, 40, device=cuda_dev, dtype=torch.bfloat16)
+    wide[:, 3:35] = t
+    assert torch.equal(fp4_exec.lowrank_rows(wide[:, 3:35], xq), tl)             # rows that are not contiguous are copied
+    assert fp4_exec.lowrank_rows(t[:0], fp4_exec.Fp4Rows(xq.codes[:0], xq.scales[:0], None if fmt == "mx" else xq.row_scale[:0])).shape == (0, 32)
+    for bad in ((tl[:39], lb), (tl, lb[:, :31]), (tl.half(), lb), (tl.cpu(), lb), (tl, lb.t().contiguous().t()), (tl, None)):
+        with pytest.raises(AssertionError):
+            fp4_exec.fp4_gemm(xq, wq, None, torch.bfloat16, bad)
+    for bad in (t[:, :16], t.float().cpu(), t[None]):
+        with pytest.raises((AssertionError, TypeError)):
+            fp4_exec.lowrank_rows(bad, xq)
+    with pytest.raises(AssertionError):
+        fp4_exec.lowrank_weight(B[:, :71], wq)
+    assert torch.equal(torch.ops.pq_b200.fp4_gemm(xq.codes, xq.scales, xq.row_scale, wq.codes, wq.scales, wq.row_scale, None, 0, tl, lb), want)
+    assert torch.equal(torch.ops.pq_b200.fp4_lowrank_rows(t, xq.row_scale), tl)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_with_a_low_rank_branch(cuda_dev, fmt, dtype):
+    """Rank 32 goes through the product's accumulator, other ranks after it; the laid-out factor follows the buffers."""
+    torch.manual_seed(4)
+    lin = nn.Linear(640, 328).to(dtype)
+    x = torch.randn(75, 640, device=cuda_dev).to(dtype)
+    A, B = (torch.randn(640, 32) / 25).to(dtype), (torch.randn(32, 328) / 5).to(dtype)
+    m = fp4_exec.Fp4Linear(lin, device=cuda_dev, fmt=fmt, lowrank=(A, B))
+    xq = fp4_exec.quant_rows_fp4(x, fmt)
+
+    def want():
+        t = m._down(x)
+        return fp4_exec.fp4_gemm(xq, m.weight_rows, m.bias, dtype, (fp4_exec.lowrank_rows(t, xq), fp4_exec.lowrank_weight(m.lr_B, m.weight_rows)))
+    first = m(x)
+    assert torch.equal(first, want())
+    check_low_rank(first, xq, m.weight_rows, m.bias, fmt, m._down(x), m.lr_B)
+    m.lr_B.mul_(-2)                                               # written in place
+    assert torch.equal(m(x), want()) and not torch.equal(m(x), first)
+    m.lr_B = torch.ones_like(m.lr_B)                              # replaced
+    assert torch.equal(m(x), want())
+    if m.weight_row_scale is not None:
+        m.weight_row_scale.mul_(2)
+        assert torch.equal(m(x), want())
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    m.lr_B.mul_(0.5)                                              # laid out anew inside the capture
+    with torch.cuda.graph(graph):
+        y = m(x)
+    graph.replay()
+    assert torch.equal(y, want())
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        z = m(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(z, want())
+    assert m(x[:0]).shape == (0, 328) and torch.equal(m(x[0]), m(x[:1])[0])
+    other = fp4_exec.Fp4Linear(lin, device=cuda_dev, fmt=fmt, lowrank=(A[:, :16].contiguous(), B[:16].contiguous()))
+    ref = fp4_exec.fp4_gemm(xq, other.weight_rows, other.bias, dtype)
+    assert torch.equal(other(x), torch.addmm(ref, x @ other.lr_A, other.lr_B))
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("pair", [1, 2])
 def test_product_leaves_its_neighbourhood_alone(cuda_dev, fmt, pair):

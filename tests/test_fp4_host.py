@@ -101,6 +101,8 @@ def test_one_step_calls_leave_other_operands_to_the_general_path():
     assert bind.quant_rows_fp4(x, 1) is None and bind.quant_rows_fp4(None, 1) is None and bind.quant_rows_fp4(3, 1) is None
     assert bind.dequant_rows_fp4(*q, True) is None and bind.dequant_rows_fp4(q.codes, 5, None, True) is None
     assert bind.fp4_gemm(*q, *q, None, True, 0, 0) is None and bind.fp4_gemm(*q, *q, "bias", True, 0, 0) is None
+    assert bind.fp4_gemm(*q, *q, None, True, 0, 0, None, None) is None and bind.fp4_gemm(*q, *q, None, True, 0, 0, x, None) is None
+    assert bind.fp4_gemm(*q, *q, None, True, 0, 0, "t", 3) is None
     assert bind.group_norm(x[None], 4, None, None, 1e-6, 0, 0, True, 0) is None
     assert bind.group_norm(x[None], 4.0, "w", None, 1e-6, 0, 0, True, 0) is None
 
@@ -139,3 +141,13 @@ def test_argument_checks():
     assert gemm(N=0) == SHAPE and gemm(ldx=16) == SHAPE and gemm(ldw=16) == SHAPE and gemm(ldo=39) == SHAPE
     assert gemm(K=48, ldx=32, ldw=32) == ALIGN and gemm(ldx=40) == ALIGN and gemm(w=p + 8) == ALIGN and gemm(out=p + 1) == ALIGN
     assert gemm(dtype=2) == DTYPE and gemm(fmt=3) == UNSUPPORTED and gemm(ws=p, wsb=8) == WORKSPACE
+
+    def low(t=p, lb=p, M=4, K=64, fmt=1, sr=p):
+        return lib.pq_fp4_gemm_lowrank(p, 32, p, sr, p, 32, p, p, None, t, lb, fmt, p, 0, 40, M, 40, K, None, 0, None)
+    assert low(M=0) == 0 and low(t=None) == NULL and low(lb=None) == NULL and low(sr=None) == NULL
+    assert low(t=p + 8) == ALIGN and low(lb=p + 4) == ALIGN and low(K=0) == SHAPE and low(fmt=2) == UNSUPPORTED
+
+    def rows(t=p, dtype=0, row=p, out=p, M=4):
+        return lib.pq_fp4_lowrank_rows(t, dtype, row, out, M, None)
+    assert rows(M=0, t=None) == 0 and rows(t=None) == NULL and rows(out=None) == NULL and rows(M=-1) == SHAPE and rows(dtype=2) == DTYPE
+    assert rows(t=p + 8) == ALIGN and rows(out=p + 16) == ALIGN and rows(row=p + 2) == ALIGN
