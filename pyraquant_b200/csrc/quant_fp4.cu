@@ -142,7 +142,6 @@ pq_dequant_rows_fp4_kernel(const uint8_t* codes, int64_t ldc, const uint8_t* sca
   constexpr int RPB = kThreads / TPR;
   T tag{};
   wait_for_previous_kernel();
-  allow_next_kernel();
   const int lane = threadIdx.x % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
   if (row >= M) return;
