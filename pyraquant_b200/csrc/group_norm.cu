@@ -29,6 +29,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxC = 8192;
 constexpr int kSlots = 4;                         // segments in shared memory (1 x 262144 x 256: eight 75.5 us, four 73.6)
 constexpr int kSmemMax = 232448;
+// steps of R rows that one CTA takes alone, without cooperative launch and barrier: us, shared / alone, 12 x 640 (two steps)
+// 7.2 / 5.7, 18 x 640 (three) 7.2 / 6.3 and with nv codes 8.2 / 7.9; every further step adds 0.5
+constexpr int kAloneSteps = 3;
 constexpr int kPartsPerLane = 5;                  // chunks of a sample: at most 160
 
 enum Mode { kOut16 = 0, kInt8 = 1, kMx = 2, kNv = 3 };
@@ -596,6 +599,7 @@ int chunks_of(int B, int T, int C) {
   const Lanes l = lanes_of(C);
   int P = sm_count() / B;
   const int most = (T + l.R - 1) / l.R;
+  if (most <= kAloneSteps) return 1;
   if (P > most) P = most;
   if (P > 32 * kPartsPerLane) P = 32 * kPartsPerLane;
   return P < 1 ? 1 : P;
