@@ -153,6 +153,22 @@ PyObject* fp4_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// fp4_lowrank_rows(t [M,32], row scales or None) -> fp32 [M,32], or None
+PyObject* fp4_lowrank_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const Tensor *t = n == 2 ? tensor_of(a[0]) : nullptr, *row;
+    if (t == nullptr || !optional_tensor(a[1], &row) || !t->is_cuda() || t->dim() != 2 || t->size(1) != 32) return none();
+    const int code = dtype_code(t->scalar_type());
+    const int64_t M = t->size(0);
+    if (code < 0 || !plain(*t, t->scalar_type(), t->device()) || !aligned(*t, 16)) return none();
+    if (row != nullptr && !(plain(*row, at::kFloat, t->device()) && row->dim() == 1 && row->size(0) == M)) return none();
+    c10::cuda::CUDAGuard guard(t->device());
+    Tensor out = make({M, 32}, at::kFloat, *t);
+    const int rc = pq_fp4_lowrank_rows(t->data_ptr(), code, row != nullptr ? row->data_ptr<float>() : nullptr, out.data_ptr<float>(), M, stream_of(*t));
+    return rc == PQ_OK ? THPVariable_Wrap(out) : fail("pq_fp4_lowrank_rows", rc);
+  });
+}
+
 // group_norm(x [B,T,C], groups, weight or None, bias or None, eps, act, mode, z wanted?, status word) with mode 0: z, 1: INT8, 2: mx, 3: nv
 // -> z, (q, s, z or None), (codes, scales, row scales or None); None where the Python layer has to look; False for a size
 // that the quantising forms do not take
@@ -214,7 +230,7 @@ PyObject* group_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define PQ_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {PQ_FAST(quant_rows_fp4), PQ_FAST(dequant_rows_fp4), PQ_FAST(fp4_gemm), PQ_FAST(group_norm), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef kMethods[] = {PQ_FAST(quant_rows_fp4), PQ_FAST(dequant_rows_fp4), PQ_FAST(fp4_gemm), PQ_FAST(fp4_lowrank_rows), PQ_FAST(group_norm), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bind", "eager calls of the 4-bit and group-norm operators", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};
 

@@ -932,6 +932,9 @@ def _(xq, s_a, w_int8, s_w_gm, bias, out_dtype_code):
 
 
 def _fp4_lowrank_rows_impl(t: Tensor, row_scale: Optional[Tensor]) -> Tensor:
+    out = _BIND().fp4_lowrank_rows(t, row_scale)
+    if out is not None:
+        return out
     dt = _dt(t.dtype)
     assert t.is_cuda and t.dim() == 2 and t.shape[1] == 32, "low-rank activations are [M, 32] on a GPU"
     M = t.shape[0]

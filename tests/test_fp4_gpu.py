@@ -301,6 +301,27 @@ def test_low_rank_refusals_and_layouts(cuda_dev, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+def test_low_rank_general_path_agrees_with_the_one_step_calls(cuda_dev, fmt, monkeypatch):
+    xq, wq, t, B, (tl, lb) = low_rank_case(90, 136, 288, fmt, torch.bfloat16, cuda_dev)
+    bias = torch.randn(136, device=cuda_dev)
+    bind = ops._BIND()
+    status = ops.status_word(tl.device).data_ptr(), _lib.GEMM_WORKSPACE_BYTES
+    assert bind.fp4_lowrank_rows(t, xq.row_scale) is not None
+    assert bind.fp4_gemm(*xq, *wq, bias, True, *status, tl, lb) is not None
+    for bad in ((tl, None), (tl[:89], lb), (tl, lb.double()), (tl[:, ::2], lb), (tl, lb.t().contiguous().t())):
+        assert bind.fp4_gemm(*xq, *wq, bias, True, *status, *bad) is None
+    for bad in ((t.float(), xq.row_scale), (t[:, :16], xq.row_scale), (t, torch.ones(89, device=cuda_dev)), (t.t().contiguous().t(), None)):
+        assert bind.fp4_lowrank_rows(*bad) is None
+    one = fp4_exec.fp4_gemm(xq, wq, bias, torch.float16, (tl, lb))
+
+    class Refuses:
+        def __getattr__(self, name):
+            return lambda *a: None
+    monkeypatch.setattr(ops, "_bind_handle", Refuses())
+    assert torch.equal(fp4_exec.lowrank_rows(t, xq), tl) and torch.equal(fp4_exec.fp4_gemm(xq, wq, bias, torch.float16, (tl, lb)), one)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_with_a_low_rank_branch(cuda_dev, fmt, dtype):
     """Rank 32 goes through the product's accumulator, other ranks after it; the laid-out factor follows the buffers."""

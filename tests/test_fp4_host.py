@@ -103,6 +103,7 @@ def test_one_step_calls_leave_other_operands_to_the_general_path():
     assert bind.fp4_gemm(*q, *q, None, True, 0, 0) is None and bind.fp4_gemm(*q, *q, "bias", True, 0, 0) is None
     assert bind.fp4_gemm(*q, *q, None, True, 0, 0, None, None) is None and bind.fp4_gemm(*q, *q, None, True, 0, 0, x, None) is None
     assert bind.fp4_gemm(*q, *q, None, True, 0, 0, "t", 3) is None
+    assert bind.fp4_lowrank_rows(x[:, :32], None) is None and bind.fp4_lowrank_rows("t", None) is None and bind.fp4_lowrank_rows(x) is None
     assert bind.group_norm(x[None], 4, None, None, 1e-6, 0, 0, True, 0) is None
     assert bind.group_norm(x[None], 4.0, "w", None, 1e-6, 0, 0, True, 0) is None
 
