@@ -150,12 +150,14 @@ __device__ __forceinline__ BlockScale nv_block_scale(float amax, float s_row, bo
   return b;
 }
 
+// mx: x / div; nv: -x / div, since the correction of x / div itself would make a negative zero positive (x - q0 div = +0, and
+// +0 + -0 = +0) where that of the negative keeps both zeros' signs
 template <int FMT>
 __device__ __forceinline__ float2 e2m1_quotient(float2 x, const BlockScale& b) {
-  const float2 inv = make_float2(b.inv, b.inv);
-  const float2 q0 = __fmul2_rn(x, inv);
-  if constexpr (FMT == PQ_FP4_MX) return q0;
-  return __ffma2_rn(__ffma2_rn(q0, make_float2(-b.div, -b.div), x), inv, q0);
+  if constexpr (FMT == PQ_FP4_MX) return __fmul2_rn(x, make_float2(b.inv, b.inv));
+  const float2 ninv = make_float2(-b.inv, -b.inv);
+  const float2 q0 = __fmul2_rn(x, ninv);
+  return __ffma2_rn(__ffma2_rn(q0, make_float2(b.div, b.div), x), ninv, q0);
 }
 
 // 16 packed elements of one block (or half of an mx block) -> 8 bytes of codes
@@ -172,7 +174,7 @@ __device__ __forceinline__ uint2 quant_chunk16(const Chunk16& c, const BlockScal
       v[2 * i] = f.x;
       v[2 * i + 1] = f.y;
     }
-    (h == 0 ? r.x : r.y) = pack_e2m1x8(v);
+    (h == 0 ? r.x : r.y) = pack_e2m1x8(v) ^ (FMT == PQ_FP4_MX ? 0u : 0x88888888u);
   }
   return r;
 }

@@ -1,5 +1,5 @@
 // Pieces shared by the block-scaled 4-bit GEMM kernels: parameters, the tcgen05 wrappers and descriptors of
-// kind::mxf4 / kind::mxf4nvf4, and the output stores.
+// kind::mxf4 / kind::mxf4nvf4 and of the low-rank term.
 //
 // Operands.  A row of K E2M1 codes is K / 2 bytes, so a tile of 128-byte rows with the 128-byte swizzle holds 256
 // elements per row and one MMA (K = 64) takes 32 bytes of it: the same bytes as an INT8 MMA of K = 32.

@@ -99,6 +99,23 @@ def test_quant_every_significand_against_every_block_maximum(cuda_dev, fmt, dtyp
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_quant_keeps_the_sign_of_zeros(cuda_dev, dtype, fmt):
+    """Every byte is that of the plain arithmetic, the signs of zeros and of what rounds to zero among them."""
+    x = awkward_rows(64, 640, dtype, 9).float()
+    g = torch.Generator().manual_seed(10)
+    pick = torch.rand(x.shape, generator=g)
+    x = torch.where(pick < 0.2, torch.full_like(x, -0.0), torch.where(pick < 0.3, torch.zeros_like(x), torch.where(pick < 0.4, x * 1e-3, x)))
+    x[5] = -0.0
+    x = x.to(dtype).to(cuda_dev)
+    got, want = fp4_exec.quant_rows_fp4(x, fmt), fp4_exec.quantize_weight_fp4(x, fmt)
+    assert torch.equal(got.codes, want.codes)
+    kept = (got.codes & 8 != 0) == torch.signbit(x[:, 0::2])                          # wherever the block's scale is not zero
+    zero_scale = (fp4_exec.dequant_rows_fp4(want) == 0).reshape(64, -1, ops.FP4_BLOCK[fmt]).all(2).repeat_interleave(ops.FP4_BLOCK[fmt], 1)
+    assert bool((kept | zero_scale[:, 0::2]).all())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_quant_every_magnitude(cuda_dev, fmt, dtype):
     """Every positive finite value of the type as the maximum of a row: row scales, block scales and codes over the whole
     exponent range, subnormals among them."""
