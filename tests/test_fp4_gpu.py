@@ -601,3 +601,60 @@ def test_kernels_in_a_row_wait_for_one_another(cuda_dev, fmt, M, N, K):
     torch.cuda.synchronize()
     for a, w in zip(got, want):
         assert all(torch.equal(u, e) for u, e in zip(a, w))
+
+
+def test_several_threads_and_streams(cuda_dev):
+    """Group norm, quantisation and products with a low-rank term from three threads at once, each on a stream of its own."""
+    import threading
+
+    from pyraquant_b200 import norm_exec
+    torch.manual_seed(7)
+    shapes = [(2, 1024, 640, 640, "mx"), (1, 4096, 320, 1280, "nv"), (3, 77, 1280, 200, "nv")]
+
+    def make(B, T, C, N, fmt):
+        x = torch.randn(B, T, C, device=cuda_dev).bfloat16()
+        w = torch.randn(C, device=cuda_dev).bfloat16()
+        W = fp4_exec.quant_rows_fp4(torch.randn(N, C, device=cuda_dev).bfloat16(), fmt)
+        t = torch.randn(B * T, 32, device=cuda_dev).bfloat16()
+        lb = fp4_exec.lowrank_weight(torch.randn(32, N, device=cuda_dev).bfloat16(), W)
+
+        def run():
+            z = norm_exec.group_norm_rows(x, 32, w, w, 1e-5, "silu")
+            q = norm_exec.group_norm_quant_fp4(x, 32, w, w, 1e-5, "silu", fmt)
+            y = fp4_exec.fp4_gemm(q, W, None, torch.bfloat16, (fp4_exec.lowrank_rows(t, q), lb))
+            q2 = fp4_exec.quant_rows_fp4(z.reshape(-1, C), fmt)
+            return y, fp4_exec.fp4_gemm(q2, W, None, torch.bfloat16), fp4_exec.dequant_rows_fp4(q2)
+        return run
+    runs = [make(*s) for s in shapes]
+    want = [r() for r in runs]
+    torch.cuda.synchronize()
+    wrong = [None] * 3
+
+    def worker(i):
+        s = torch.cuda.Stream()
+        n = 0
+        with torch.cuda.stream(s):
+            for _ in range(40):
+                n += sum(not torch.equal(a, b) for a, b in zip(runs[i](), want[i]))
+        wrong[i] = n
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [0, 0, 0]
+
+
+def test_linear_in_inference_mode(cuda_dev):
+    """Weights made in inference mode and calls inside it give the values of ordinary ones."""
+    torch.manual_seed(8)
+    lin = nn.Linear(320, 96).to(torch.bfloat16)
+    low = (torch.randn(320, 32) / 18).bfloat16(), (torch.randn(32, 96) / 5).bfloat16()
+    x = torch.randn(9, 320, device=cuda_dev).bfloat16()
+    want = fp4_exec.Fp4Linear(lin, device=cuda_dev, lowrank=low)(x)
+    with torch.inference_mode():
+        m = fp4_exec.Fp4Linear(lin, device=cuda_dev, lowrank=low)
+        assert torch.equal(m(x), want)
+        m.lr_B.mul_(2)                                            # nothing counts this change
+        doubled = m(x)
+    assert not torch.equal(doubled, want) and torch.equal(m(x), doubled)
