@@ -1,4 +1,4 @@
-"""CPU restatement of the 4-bit floating-point formats in 64 bits (checker only; the package never imports it).
+"""CPU restatement of the 4-bit floating-point formats in 64 bits (for the tests only; the package never imports it).
 
 mx: one E8M0 scale per 32 elements, 2^(floor(log2 max) - 2).  nv: one E4M3 scale per 16 elements, e4m3(max / (6 s_row)), under
 a power of two per row, the smallest with row max <= 2688 s_row.  Codes are E2M1, nearest, ties to even.
