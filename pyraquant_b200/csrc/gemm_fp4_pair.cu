@@ -213,6 +213,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 #pragma unroll 1
       for (int t = pair; t < tiles && ok; t += pairs, ++it) {
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>((it & 1) * 128);
+        uint64_t* low_done = nullptr; uint32_t low_phase = 0;
         if (low) {
           if (!full_ready && !wait_or_abort(&full_bar[stage], phase, abort_flag)) {
             report_timeout(p.status, 2, 1); *abort_flag = 1; ok = false; break;
@@ -231,12 +232,7 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
           if (L::kUnits > 1) tc_commit_pair(smem_u32(&half_bar[stage]));
           if (issued < 2) ++issued;
           commit_both(&empty_bar[stage]);
-          // the accumulator is whole before the other kind of MMA adds to it (the stage cannot be refilled and used again before
-          // this thread goes on, so its barrier keeps the parity waited for)
-          if (!wait_or_abort(&empty_bar[stage], phase, abort_flag)) {
-            report_timeout(p.status, 2, 4); *abort_flag = 1; ok = false; break;
-          }
-          tc_fence_after();
+          low_done = &empty_bar[stage]; low_phase = phase;
           full_ready = false;
           if (++stage == S) { stage = 0; phase ^= 1u; }
         }
@@ -272,8 +268,15 @@ pq_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
               tc_cp_scale_tile_pair(sfb_t + 8 * j, scale_tile_desc(s_addr + L::kSfa + tile * 512));
               tc_cp_scale_tile_pair(sfb_t + 8 * j + 4, scale_tile_desc(s_addr + L::kSfa + (F::kTilesPerStage + tile) * 512));
             }
-            // the scales of a tile's first stage are under way before the accumulator is free
-            if (u == 0 && kb == 0 && it > 0 && !low) {
+            // The scales of a tile's first stage are under way before the accumulator is free, or before the low-rank term is whole
+            // and the other kind of MMA may add to it (its stage is not used again before this thread goes on, so the barrier
+            // keeps the parity waited for).
+            if (u == 0 && kb == 0 && low) {
+              if (!wait_or_abort(low_done, low_phase, abort_flag)) {
+                report_timeout(p.status, 2, 4); *abort_flag = 1; ok = false; break;
+              }
+              tc_fence_after();
+            } else if (u == 0 && kb == 0 && it > 0) {
               if (!wait_or_abort(shared_free, static_cast<uint32_t>(it - 1) & 1u, abort_flag)) {
                 report_timeout(p.status, 2, 2); *abort_flag = 1; ok = false; break;
               }
