@@ -62,8 +62,8 @@ __host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, bool mx, int
 // loaded, swizzled and addressed like those of 256 codes, and four kind::tf32 MMAs (K = 8) start the accumulator.  TF32 has the
 // significand of fp16 and the exponents of fp32: 16-bit values over powers of two are exact in it.  The MMAs of the other kind
 // are issued once these have completed.  Measured with the conversion of t, us, without the term / with it / with a library product
-// added to the output instead: mx 77 x 2048 -> 1280 4.8 / 6.2 / 7.6, 16384 x 1280 -> 10240 100 / 119 / 249, 8192^3 187 / 209 / 258;
-// nv 16384 x 1280 -> 1280 19.3 / 22.3 / 30.6.
+// added to the output instead: mx 77 x 2048 -> 1280 4.8 / 6.2 / 7.6, 16384 x 1280 -> 10240 100 / 119 / 249, 8192^3 186 / 195
+// in short runs (power decides in long ones), 187 / 209 / 258 in long ones; nv 16384 x 1280 -> 1280 19.3 / 22.3 / 30.6.
 __host__ __device__ constexpr uint32_t make_idesc_tf32(int M, int N) {
   return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
