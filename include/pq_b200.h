@@ -359,6 +359,10 @@ int pq_fp4_gemm_lowrank(const uint8_t* xq, int64_t ldx, const uint8_t* x_scales,
                         int64_t K, void* workspace, size_t ws_bytes, void* stream);
 /* out [M,32] fp32 = t [M,32] 16-bit, contiguous, over row_scale [M] (NULL: 1); t 16-byte, out 32-byte aligned. */
 int pq_fp4_lowrank_rows(const void* t, int dtype, const float* row_scale, float* out, int64_t M, void* stream);
+/* Both factors in one launch: t_out as pq_fp4_lowrank_rows makes it, and b_out [N,32] fp32 = the transpose of the up-projection
+ * b [32,N] (16-bit, row stride ldb elements, any alignment) over col_scale [N] (NULL: 1); b_out 32-byte aligned.  M or N may be 0. */
+int pq_fp4_lowrank_factors(const void* t, int t_dtype, const float* row_scale, float* t_out, int64_t M, const void* b, int b_dtype,
+                           int64_t ldb, const float* col_scale, float* b_out, int64_t N, void* stream);
 
 /* Feathered scatter of routed rows back over the cached canvas, in place: the pull form of
  * fuse_patch_predictions (flux/routing.py:328-379).  For canvas token j with contributor list

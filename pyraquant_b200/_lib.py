@@ -89,6 +89,8 @@ SIGNATURES = {
                                     c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_size_t,
                                     c_void_p]),
     "pq_fp4_lowrank_rows": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
+    "pq_fp4_lowrank_factors": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p, c_void_p,
+                                       c_int64, c_void_p]),
     "pq_fp4_gemm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int,
                             c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
     "pq_int8_gemm_g32": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,

@@ -169,6 +169,32 @@ PyObject* fp4_lowrank_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// fp4_lowrank_factors(t [M,32], row scales or None, B [32,N], column scales or None) -> (fp32 [M,32], fp32 [N,32]), or None
+PyObject* fp4_lowrank_factors(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const Tensor *t = n == 4 ? tensor_of(a[0]) : nullptr, *b = n == 4 ? tensor_of(a[2]) : nullptr, *row, *col;
+    if (t == nullptr || b == nullptr || !optional_tensor(a[1], &row) || !optional_tensor(a[3], &col) || !t->is_cuda() || t->dim() != 2 ||
+        t->size(1) != 32 || b->dim() != 2 || b->size(0) != 32)
+      return none();
+    const int tc = dtype_code(t->scalar_type()), bc = dtype_code(b->scalar_type());
+    const int64_t M = t->size(0), N = b->size(1);
+    if (tc < 0 || bc < 0 || !plain(*t, t->scalar_type(), t->device()) || !aligned(*t, 16) || !plain(*b, b->scalar_type(), t->device())) return none();
+    if (row != nullptr && !(plain(*row, at::kFloat, t->device()) && row->dim() == 1 && row->size(0) == M)) return none();
+    if (col != nullptr && !(plain(*col, at::kFloat, t->device()) && col->dim() == 1 && col->size(0) == N)) return none();
+    c10::cuda::CUDAGuard guard(t->device());
+    Tensor t_out = make({M, 32}, at::kFloat, *t), b_out = make({N, 32}, at::kFloat, *t);
+    const int rc = pq_fp4_lowrank_factors(t->data_ptr(), tc, row != nullptr ? row->data_ptr<float>() : nullptr, t_out.data_ptr<float>(), M, b->data_ptr(),
+                                          bc, N, col != nullptr ? col->data_ptr<float>() : nullptr, b_out.data_ptr<float>(), N, stream_of(*t));
+    if (rc != PQ_OK) return fail("pq_fp4_lowrank_factors", rc);
+    PyObject* r = PyTuple_New(2);
+    if (r == nullptr) return nullptr;
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(t_out));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(b_out));
+    if (PyTuple_GET_ITEM(r, 0) == nullptr || PyTuple_GET_ITEM(r, 1) == nullptr) { Py_DECREF(r); return nullptr; }
+    return r;
+  });
+}
+
 // group_norm(x [B,T,C], groups, weight or None, bias or None, eps, act, mode, z wanted?, status word) with mode 0: z, 1: INT8, 2: mx, 3: nv
 // -> z, (q, s, z or None), (codes, scales, row scales or None); None where the Python layer has to look; False for a size
 // that the quantising forms do not take
@@ -230,7 +256,8 @@ PyObject* group_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define PQ_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {PQ_FAST(quant_rows_fp4), PQ_FAST(dequant_rows_fp4), PQ_FAST(fp4_gemm), PQ_FAST(fp4_lowrank_rows), PQ_FAST(group_norm), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef kMethods[] = {PQ_FAST(quant_rows_fp4), PQ_FAST(dequant_rows_fp4), PQ_FAST(fp4_gemm), PQ_FAST(fp4_lowrank_rows), PQ_FAST(fp4_lowrank_factors),
+                           PQ_FAST(group_norm), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bind", "eager calls of the 4-bit and group-norm operators", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};
 

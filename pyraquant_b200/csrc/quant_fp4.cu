@@ -187,13 +187,29 @@ pq_dequant_rows_fp4_kernel(const uint8_t* codes, int64_t ldc, const uint8_t* sca
   }
 }
 
-// Low-rank activations t [M, 32] for the product's accumulator, which stands in units of the row scale: eight elements per thread,
-// t / s_row in fp32 (exact: a 16-bit value over a power of two).
-template <typename T>
+// The factors of a rank-32 term for the product's accumulator, which stands in units of the row scales.  The first `t_blocks` blocks:
+// activations t [M, 32], eight elements per thread, t / s_row in fp32 (exact: a 16-bit value over a power of two).  The others: the
+// up-projection B [32, N], transposed, over s_col; a block takes 64 columns, a thread eight elements of one of them, so that a warp
+// reads 64 contiguous bytes of a row of B and writes whole 32-byte sectors.  Laying B out costs a fraction of the launch that t needs
+// anyway, and nothing has to be kept from call to call: the term is always that of the factor as it is now.
+constexpr int kFactorCols = kThreads / 4;
+template <typename T, typename TB>
 __global__ void __launch_bounds__(kThreads)
-pq_fp4_lowrank_rows_kernel(const T* t, const float* row_scale, float* out, int64_t M) {
+pq_fp4_lowrank_factors_kernel(const T* t, const float* row_scale, float* out, int64_t M, unsigned t_blocks, const TB* b, int64_t ldb,
+                              const float* col_scale, float* b_out, int64_t N) {
   wait_for_previous_kernel();
   allow_next_kernel();
+  if (blockIdx.x >= t_blocks) {
+    const int64_t n = static_cast<int64_t>(blockIdx.x - t_blocks) * kFactorCols + threadIdx.x % kFactorCols;
+    const int r0 = static_cast<int>(threadIdx.x) / kFactorCols * 8;
+    if (n >= N) return;
+    const float s = col_scale != nullptr ? col_scale[n] : 1.0f;
+    Chunk16 o;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o.w[k] = __float_as_uint(__fdiv_rn(static_cast<float>(b[(r0 + k) * ldb + n]), s));
+    st_chunk16(b_out + n * 32 + r0, o);
+    return;
+  }
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (i >= 4 * M) return;
   const float inv = row_scale != nullptr ? 1.0f / row_scale[i >> 2] : 1.0f;
@@ -224,6 +240,18 @@ int launch_chained(void (*kern)(P...), int64_t blocks, cudaStream_t st, A... arg
   cfg.numAttrs = 1;
   PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
   return PQ_OK;
+}
+
+struct FactorArgs {
+  const void* t; const float* row_scale; float* t_out; int64_t M;
+  const void* b; int64_t ldb; const float* col_scale; float* b_out; int64_t N;
+};
+template <typename T, typename TB>
+int launch_factors(const FactorArgs& a, cudaStream_t st) {
+  const int64_t t_blocks = (4 * a.M + kThreads - 1) / kThreads, blocks = t_blocks + (a.N + kFactorCols - 1) / kFactorCols;
+  if (blocks > 0x7fffffffLL) return PQ_ERR_SHAPE;
+  return launch_chained(pq_fp4_lowrank_factors_kernel<T, TB>, blocks, st, static_cast<const T*>(a.t), a.row_scale, a.t_out, a.M,
+                        static_cast<unsigned>(t_blocks), static_cast<const TB*>(a.b), a.ldb, a.col_scale, a.b_out, a.N);
 }
 
 template <typename T, int FMT, int TPR, bool LONG>
@@ -310,16 +338,21 @@ extern "C" int pq_dequant_rows_fp4(const uint8_t* codes, int64_t ldc, const uint
                           : dispatch_dequant<__half, PQ_FP4_NV>(codes, ldc, scales, row_scale, out, ldo, M, static_cast<int>(K), st);
 }
 
-extern "C" int pq_fp4_lowrank_rows(const void* t, int dtype, const float* row_scale, float* out, int64_t M, void* stream) {
-  if (M < 0) return PQ_ERR_SHAPE;
-  if (dtype != PQ_DTYPE_BF16 && dtype != PQ_DTYPE_FP16) return PQ_ERR_DTYPE;
-  if (M == 0) return PQ_OK;
-  if (t == nullptr || out == nullptr) return PQ_ERR_NULL;
-  if (!aligned_to(t, 16) || !aligned_to(out, 32) || !aligned_to(row_scale, 4)) return PQ_ERR_ALIGN;
-  const int64_t blocks = (4 * M + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffffLL) return PQ_ERR_SHAPE;
+extern "C" int pq_fp4_lowrank_factors(const void* t, int t_dtype, const float* row_scale, float* t_out, int64_t M, const void* b,
+                                      int b_dtype, int64_t ldb, const float* col_scale, float* b_out, int64_t N, void* stream) {
+  if (M < 0 || N < 0 || M > 0x7fffffffffLL || N > 0x7fffffffffLL || (N > 0 && ldb < N)) return PQ_ERR_SHAPE;
+  if ((t_dtype != PQ_DTYPE_BF16 && t_dtype != PQ_DTYPE_FP16) || (b_dtype != PQ_DTYPE_BF16 && b_dtype != PQ_DTYPE_FP16)) return PQ_ERR_DTYPE;
+  if (M == 0 && N == 0) return PQ_OK;
+  if ((M > 0 && (t == nullptr || t_out == nullptr)) || (N > 0 && (b == nullptr || b_out == nullptr))) return PQ_ERR_NULL;
+  if (!aligned_to(t, 16) || !aligned_to(t_out, 32) || !aligned_to(row_scale, 4) || !aligned_to(b, 2) || !aligned_to(b_out, 32) || !aligned_to(col_scale, 4))
+    return PQ_ERR_ALIGN;
+  const FactorArgs a{t, row_scale, t_out, M, b, ldb, col_scale, b_out, N};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == PQ_DTYPE_BF16)
-    return launch_chained(pq_fp4_lowrank_rows_kernel<__nv_bfloat16>, blocks, st, static_cast<const __nv_bfloat16*>(t), row_scale, out, M);
-  return launch_chained(pq_fp4_lowrank_rows_kernel<__half>, blocks, st, static_cast<const __half*>(t), row_scale, out, M);
+  if (t_dtype == PQ_DTYPE_BF16)
+    return b_dtype == PQ_DTYPE_BF16 ? launch_factors<__nv_bfloat16, __nv_bfloat16>(a, st) : launch_factors<__nv_bfloat16, __half>(a, st);
+  return b_dtype == PQ_DTYPE_BF16 ? launch_factors<__half, __nv_bfloat16>(a, st) : launch_factors<__half, __half>(a, st);
+}
+
+extern "C" int pq_fp4_lowrank_rows(const void* t, int dtype, const float* row_scale, float* out, int64_t M, void* stream) {
+  return pq_fp4_lowrank_factors(t, dtype, row_scale, out, M, nullptr, dtype, 0, nullptr, nullptr, 0, stream);
 }

@@ -75,11 +75,19 @@ def lowrank_rows(t: torch.Tensor, xq: Fp4Rows) -> torch.Tensor:
 
 
 def lowrank_weight(B: torch.Tensor, w: Fp4Rows) -> torch.Tensor:
-    """The up-projection B [32,N] bf16/fp16 in the units of the weights it goes with: fp32 [N,32].  Plain tensor arithmetic, done
-    once per layer."""
+    """The up-projection B [32,N] bf16/fp16 in the units of the weights it goes with: fp32 [N,32].  Plain tensor arithmetic, for
+    factors that are laid out once; ``lowrank_factors`` lays B out on every call."""
     assert B.dim() == 2 and B.shape == (32, w.codes.shape[0]) and B.dtype in ops._DT
     b = B.t().float()
     return (b if w.row_scale is None else b / w.row_scale[:, None]).contiguous()
+
+
+def lowrank_factors(t: torch.Tensor, xq: Fp4Rows, B: torch.Tensor, w: Fp4Rows) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(lowrank_rows(t, xq), lowrank_weight(B, w))`` in one launch: what ``fp4_gemm`` takes as ``lowrank``."""
+    assert B.dim() == 2 and B.shape == (32, w.codes.shape[0]), (tuple(B.shape), w.codes.shape[0])
+    if _eager():
+        return ops._fp4_lowrank_factors_impl(t, xq.row_scale, B, w.row_scale)
+    return lowrank_rows(t, xq), lowrank_weight(B, w)
 
 
 def fp4_linear_2d(x2: torch.Tensor, w: Fp4Rows, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -176,30 +184,13 @@ class Fp4Linear(LowRankFactors, nn.Module):
                 setattr(self, name, v.to(new.device))
         return self
 
-    def _lr_weight(self) -> torch.Tensor:
-        """``lowrank_weight`` of lr_B, remade whenever lr_B or the row scales are replaced, moved or written in place.  Kept only
-        when it is there for every stream: not while a graph is captured, and not of inference tensors, whose changes
-        nothing counts."""
-        src = [t for t in (self.lr_B, self.weight_row_scale) if t is not None]
-        if not _eager() or any(t.is_inference() for t in src):
-            return lowrank_weight(self.lr_B, self.weight_rows)
-        key = tuple((t.data_ptr(), t.dtype, t.device, tuple(t.shape), t._version) for t in src)
-        c = self.__dict__.get("_lr_weight_cache")
-        if c is None or c[0] != key:
-            c = (key, lowrank_weight(self.lr_B, self.weight_rows))
-            if self.lr_B.is_cuda:
-                if torch.cuda.is_current_stream_capturing():
-                    return c[1]
-                torch.cuda.current_stream(self.lr_B.device).synchronize()
-            self.__dict__["_lr_weight_cache"] = c
-        return c[1]
-
     def _product(self, xq: Fp4Rows, x2: torch.Tensor) -> torch.Tensor:
         if self.lr_A is None:
             return fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype)
         t = self._down(x2).to(x2.dtype)
         if t.shape[1] == 32 and self.lr_B.dtype in ops._DT:
-            return fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype, (lowrank_rows(t, xq), self._lr_weight()))
+            w = self.weight_rows
+            return fp4_gemm(xq, w, self.bias, x2.dtype, lowrank_factors(t, xq, self.lr_B, w))
         y = fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype)
         return y.addmm_(t, self.lr_B.to(y.dtype))
 

@@ -950,6 +950,30 @@ def _fp4_lowrank_rows_impl(t: Tensor, row_scale: Optional[Tensor]) -> Tensor:
     return out
 
 
+def _fp4_lowrank_factors_impl(t: Tensor, row_scale: Optional[Tensor], B: Tensor, col_scale: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    out = _BIND().fp4_lowrank_factors(t, row_scale, B, col_scale)
+    if out is not None:
+        return out
+    dt, db = _dt(t.dtype), _dt(B.dtype)
+    assert t.is_cuda and t.dim() == 2 and t.shape[1] == 32, "low-rank activations are [M, 32] on a GPU"
+    assert B.dim() == 2 and B.shape[0] == 32 and B.device == t.device, "the up-projection is [32, N] on the activations' device"
+    M, N = t.shape[0], B.shape[1]
+    for s, n in ((row_scale, M), (col_scale, N)):
+        assert s is None or (s.dtype == torch.float32 and s.numel() == n and s.is_contiguous() and s.device == t.device), \
+            "one fp32 row scale per row"
+    if not t.is_contiguous() or t.data_ptr() % 16 != 0:
+        t = t.clone(memory_format=torch.contiguous_format)
+    if not B.is_contiguous():
+        B = B.contiguous()
+    t_out, b_out = t.new_empty((M, 32), dtype=torch.float32), t.new_empty((N, 32), dtype=torch.float32)
+    with _on_device(t):
+        rc = _LIB().pq_fp4_lowrank_factors(t.data_ptr(), dt, _ptr(row_scale), t_out.data_ptr(), M, B.data_ptr(), db, N, _ptr(col_scale),
+                                           b_out.data_ptr(), N, _stream(t))
+    if rc:
+        _lib.check(rc, f"pq_fp4_lowrank_factors(M={M}, N={N})")
+    return t_out, b_out
+
+
 @torch.library.custom_op("pq_b200::group_norm_rows", mutates_args=(), device_types="cuda")
 def group_norm_rows_op(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, silu: bool) -> Tensor:
     return _group_norm_impl(x, groups, weight, bias, eps, "silu" if silu else None)

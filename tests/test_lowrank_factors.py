@@ -1,0 +1,132 @@
+"""Low-rank branches follow their factors: replaced, moved or edited ones, in eager calls and in replayed graphs."""
+import ctypes
+
+import pytest
+import torch
+import torch.nn as nn
+
+from pyraquant_b200 import _lib, fp4_exec, ops
+
+FMTS = ["mx", "nv"]
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def layer(cls, dev, K=640, N=328, dtype=torch.bfloat16, seed=4, **kw):
+    g = torch.Generator().manual_seed(seed)
+    lin = nn.Linear(K, N).to(dtype)
+    with torch.no_grad():
+        lin.weight.copy_(torch.randn(N, K, generator=g) / K ** 0.5)
+        lin.bias.copy_(torch.randn(N, generator=g))
+    A, B = torch.randn(K, 32, generator=g) / K ** 0.5, torch.randn(32, N, generator=g) / 5
+    return cls(lin, device=dev, lowrank=(A.to(dtype), B.to(dtype)), **kw)
+
+
+def by_parts(m, x):
+    """The layer's steps one by one, the up-projection laid out on the spot."""
+    xq = fp4_exec.quant_rows_fp4(x, m.fmt)
+    factors = fp4_exec.lowrank_rows(m._down(x), xq), fp4_exec.lowrank_weight(m.lr_B, m.weight_rows)
+    return fp4_exec.fp4_gemm(xq, m.weight_rows, m.bias, x.dtype, factors)
+
+
+# ------------------------------------------------------------------------------------------------ the two factors in one launch
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("t_type", DTYPES)
+@pytest.mark.parametrize("b_type", DTYPES)
+def test_factors_are_laid_out_as_their_parts_are(cuda_dev, fmt, t_type, b_type, monkeypatch):
+    g = torch.Generator().manual_seed(3)
+    for M, N in ((1, 1), (63, 64), (64, 65), (300, 1280), (0, 40), (5, 10240)):
+        xq = fp4_exec.quant_rows_fp4((torch.randn(M, 32, generator=g) * 50).to(t_type).to(cuda_dev), fmt)
+        w = fp4_exec.quant_rows_fp4(torch.randn(N, 32, generator=g).bfloat16().to(cuda_dev), fmt)
+        t, B = torch.randn(M, 32, generator=g).to(t_type).to(cuda_dev), torch.randn(32, N, generator=g).to(b_type).to(cuda_dev)
+        want = fp4_exec.lowrank_rows(t, xq), fp4_exec.lowrank_weight(B, w)
+        got = fp4_exec.lowrank_factors(t, xq, B, w)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[1].is_contiguous()
+        wide = torch.zeros(32, N + 3, dtype=b_type, device=cuda_dev)
+        wide[:, 3:] = B
+        off = torch.zeros(M, 40, dtype=t_type, device=cuda_dev)
+        off[:, 3:35] = t
+        got = fp4_exec.lowrank_factors(off[:, 3:35], xq, wide[:, 3:], w)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    lib = _lib.load()                                             # rows of B that lie apart, nothing else written
+    out = torch.full((70 * 32 + 8,), 7.0, device=cuda_dev)
+    B = torch.randn(32, 91, generator=g).to(b_type).to(cuda_dev)
+    assert lib.pq_fp4_lowrank_factors(None, 0, None, None, 0, B.data_ptr() + 2 * 5, ops._DT[b_type], 91, None, out.data_ptr(), 70,
+                                      torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out[: 70 * 32].reshape(70, 32), B[:, 5:75].t().float()) and bool((out[70 * 32:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_factors_refusals(cuda_dev):
+    x = torch.randn(9, 96, device=cuda_dev).bfloat16()
+    xq, w = fp4_exec.quant_rows_fp4(x, "nv"), fp4_exec.quant_rows_fp4(torch.randn(40, 96, device=cuda_dev).bfloat16(), "nv")
+    t, B = torch.randn(9, 32, device=cuda_dev).bfloat16(), torch.randn(32, 40, device=cuda_dev).bfloat16()
+    for bad in ((t[:, :16], xq, B, w), (t, xq, B[:, :39], w), (t, xq, B[:16], w), (t[:8], xq, B, w), (t, xq, B.cpu(), w), (t.cpu(), xq, B, w),
+                (t[None], xq, B, w), (t, fp4_exec.Fp4Rows(xq.codes, xq.scales, xq.row_scale.double()), B, w)):
+        with pytest.raises(AssertionError):
+            fp4_exec.lowrank_factors(*bad)
+    for bad in ((t.float(), xq, B, w), (t, xq, B.float(), w)):
+        with pytest.raises(TypeError):
+            fp4_exec.lowrank_factors(*bad)
+
+
+def test_factors_argument_checks():
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 63) & ~63
+
+    def f(t=p, td=0, row=p, t_out=p, M=4, b=p, bd=0, ldb=8, col=p, b_out=p, N=8):
+        return lib.pq_fp4_lowrank_factors(t, td, row, t_out, M, b, bd, ldb, col, b_out, N, None)
+    assert f(M=0, N=0, t=None, b=None) == 0
+    assert f(M=-1) == 2 and f(N=-1) == 2 and f(ldb=7) == 2 and f(M=1 << 40) == 2 and f(N=1 << 40) == 2
+    assert f(td=2) == 4 and f(bd=2) == 4
+    assert f(t=None) == 1 and f(t_out=None) == 1 and f(b=None) == 1 and f(b_out=None) == 1
+    assert f(t=p + 8) == 3 and f(t_out=p + 16) == 3 and f(b=p + 1) == 3 and f(b_out=p + 16) == 3 and f(row=p + 2) == 3 and f(col=p + 2) == 3
+
+
+# ------------------------------------------------------------------------------------------------ Fp4Linear: the up-projection
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_fp4_follows_a_replaced_up_projection(cuda_dev, fmt):
+    """A factor taken off before its successor is made, which the allocator puts where the old one was; a round trip over the
+    CPU with an edit; a write that torch does not count."""
+    m = layer(fp4_exec.Fp4Linear, cuda_dev, fmt=fmt)
+    x = torch.randn(75, 640, device=cuda_dev).bfloat16()
+    m(x)
+    same = 0
+    for i in range(20):
+        before = m.lr_B.data_ptr()
+        m.lr_B = None
+        m.lr_B = torch.randn(32, 328, device=cuda_dev, dtype=torch.bfloat16)
+        same += m.lr_B.data_ptr() == before
+        assert torch.equal(m(x), by_parts(m, x)), i
+    assert same > 0                                               # or the test shows nothing
+    m.cpu()
+    m.lr_B.mul_(3)
+    m.cuda()
+    assert torch.equal(m(x), by_parts(m, x))
+    m.lr_B.data.mul_(-2)
+    assert torch.equal(m(x), by_parts(m, x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_fp4_graph_follows_the_up_projection(cuda_dev, fmt):
+    """A layer that ran before the capture: replays use the factor as it is then, whatever eager calls ran in between."""
+    m = layer(fp4_exec.Fp4Linear, cuda_dev, fmt=fmt)
+    x = torch.randn(75, 640, device=cuda_dev).bfloat16()
+    m(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = m(x)
+    graph.replay()
+    assert torch.equal(y, by_parts(m, x))
+    m.lr_B.mul_(-2)
+    graph.replay()
+    assert torch.equal(y, by_parts(m, x))
+    m(x)
+    filler = [torch.full((328, 32), 1e4, device=cuda_dev) for _ in range(8)]
+    graph.replay()
+    assert torch.equal(y, by_parts(m, x))
+    del filler
+    ops.check_device_status(cuda_dev)
