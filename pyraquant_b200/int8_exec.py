@@ -266,6 +266,21 @@ FLUX_SHARED_INPUT_GROUPS = (
 )
 
 
+class _Transposed:
+    """A factor's K-major copy and what it was made of: the tensor itself, its version, and an alias that keeps its memory from being
+    handed out again, so that a tensor at the same address is the same data."""
+    __slots__ = ("source", "alias", "version", "copy")
+
+    def __init__(self, src: torch.Tensor):
+        self.source, self.alias, self.version = src, src.detach(), ops.tensor_version(src)
+        self.copy = src.t().contiguous()
+
+    def holds(self, src: torch.Tensor) -> bool:
+        a = self.alias
+        return (self.source is src and self.version == ops.tensor_version(src) and a.data_ptr() == src.data_ptr()
+                and a.dtype is src.dtype and a.shape == src.shape and a.stride() == src.stride())
+
+
 class LowRankFactors:
     """What the Linears with a low-rank branch share: K-major copies of the factors, made once, and the down-projection."""
 
@@ -281,12 +296,11 @@ class LowRankFactors:
         """Contiguous transpose of a low-rank factor, remade whenever the buffer is replaced, converted (.to / .half),
         moved or written in place."""
         src = getattr(self, name)
-        key = (src.data_ptr(), src.dtype, src.device, tuple(src.shape), ops.tensor_version(src))
         c = self.__dict__.get("_t_cache_" + name)
-        if c is None or c[0] != key:
-            c = (key, src.t().contiguous())
+        if c is None or not c.holds(src):
+            c = _Transposed(src)
             self.__dict__["_t_cache_" + name] = c
-        return c[1]
+        return c.copy
 
     def _down(self, x2: torch.Tensor) -> torch.Tensor:
         """t = x2 @ lr_A rounded to the activation dtype (reference :390): the native streaming kernel for rank 32

@@ -5,7 +5,7 @@ import pytest
 import torch
 import torch.nn as nn
 
-from pyraquant_b200 import _lib, fp4_exec, ops
+from pyraquant_b200 import _lib, fp4_exec, int8_exec, ops
 
 FMTS = ["mx", "nv"]
 DTYPES = [torch.bfloat16, torch.float16]
@@ -130,3 +130,58 @@ def test_fp4_graph_follows_the_up_projection(cuda_dev, fmt):
     assert torch.equal(y, by_parts(m, x))
     del filler
     ops.check_device_status(cuda_dev)
+
+
+# ------------------------------------------------------------------------------------------------ both Linears: the kept copies
+LAYERS = [(int8_exec.Int8Linear, {}), (fp4_exec.Fp4Linear, {"fmt": "mx"}), (fp4_exec.Fp4Linear, {"fmt": "nv"})]
+layers = pytest.mark.parametrize("cls,kw", LAYERS, ids=["int8", "fp4_mx", "fp4_nv"])
+factors = pytest.mark.parametrize("name", ["lr_A", "lr_B"])
+
+
+def by_fresh_layer(m, x, **kw):
+    """What a layer with these factors that has never run gives."""
+    n = layer(type(m), x.device, **kw)
+    n.lr_A, n.lr_B = m.lr_A.clone(), m.lr_B.clone()
+    return n(x)
+
+
+def transposed(m, name):
+    return m._lr_At() if name == "lr_A" else m._lr_Bt()
+
+
+@factors
+def test_transposed_copies_follow_replacements(name):
+    m = layer(int8_exec.Int8Linear, torch.device("cpu"))
+    shape, dtype = getattr(m, name).shape, getattr(m, name).dtype
+    for i in range(100):                                          # the allocator often hands the same place out again
+        setattr(m, name, None)
+        setattr(m, name, torch.randn(shape).to(dtype))
+        assert torch.equal(transposed(m, name), getattr(m, name).t()), i
+    kept = transposed(m, name)
+    assert transposed(m, name) is kept                            # laid out once
+    getattr(m, name).mul_(2)
+    assert torch.equal(transposed(m, name), getattr(m, name).t())
+    m.half()
+    assert torch.equal(transposed(m, name), getattr(m, name).t()) and transposed(m, name).dtype == torch.float16
+    getattr(m, name).data = torch.randn(shape).half()
+    assert torch.equal(transposed(m, name), getattr(m, name).t())
+
+
+@pytest.mark.gpu
+@layers
+@factors
+def test_layers_follow_their_factors(cuda_dev, cls, kw, name):
+    m = layer(cls, cuda_dev, **kw)
+    x = torch.randn(75, 640, device=cuda_dev).bfloat16()
+    m(x)
+    shape = getattr(m, name).shape
+    for i in range(10):
+        setattr(m, name, None)
+        setattr(m, name, torch.randn(shape, device=cuda_dev, dtype=torch.bfloat16))
+        assert torch.equal(m(x), by_fresh_layer(m, x, **kw)), i
+    getattr(m, name).mul_(2)
+    assert torch.equal(m(x), by_fresh_layer(m, x, **kw))
+    m.cpu()
+    getattr(m, name).mul_(-2)
+    m.cuda()
+    assert torch.equal(m(x), by_fresh_layer(m, x, **kw))
