@@ -272,12 +272,12 @@ class _Transposed:
     __slots__ = ("source", "alias", "version", "copy")
 
     def __init__(self, src: torch.Tensor):
-        self.source, self.alias, self.version = src, src.detach(), ops.tensor_version(src)
+        self.source, self.alias, self.version = src, src.detach(), src._version
         self.copy = src.t().contiguous()
 
     def holds(self, src: torch.Tensor) -> bool:
         a = self.alias
-        return (self.source is src and self.version == ops.tensor_version(src) and a.data_ptr() == src.data_ptr()
+        return (self.source is src and self.version == src._version and a.data_ptr() == src.data_ptr()
                 and a.dtype is src.dtype and a.shape == src.shape and a.stride() == src.stride())
 
 
@@ -296,6 +296,8 @@ class LowRankFactors:
         """Contiguous transpose of a low-rank factor, remade whenever the buffer is replaced, converted (.to / .half),
         moved or written in place."""
         src = getattr(self, name)
+        if src.is_inference():                                 # nothing counts the writes to it
+            return src.t().contiguous()
         c = self.__dict__.get("_t_cache_" + name)
         if c is None or not c.holds(src):
             c = _Transposed(src)

@@ -167,6 +167,24 @@ def test_transposed_copies_follow_replacements(name):
     assert torch.equal(transposed(m, name), getattr(m, name).t())
 
 
+@factors
+def test_transposed_copies_in_inference_mode(name):
+    """Inference tensors count no writes: their copies are made anew.  Ordinary factors written inside inference mode are followed."""
+    with torch.inference_mode():
+        m = layer(int8_exec.Int8Linear, torch.device("cpu"))
+        transposed(m, name)
+        getattr(m, name).mul_(2)
+        assert torch.equal(transposed(m, name), getattr(m, name).t())
+    getattr(m, name)
+    assert torch.equal(transposed(m, name), getattr(m, name).t())
+    m = layer(int8_exec.Int8Linear, torch.device("cpu"))
+    transposed(m, name)
+    with torch.inference_mode():
+        getattr(m, name).mul_(2)
+        assert torch.equal(transposed(m, name), getattr(m, name).t())
+    assert torch.equal(transposed(m, name), getattr(m, name).t())
+
+
 @pytest.mark.gpu
 @layers
 @factors
@@ -185,3 +203,9 @@ def test_layers_follow_their_factors(cuda_dev, cls, kw, name):
     getattr(m, name).mul_(-2)
     m.cuda()
     assert torch.equal(m(x), by_fresh_layer(m, x, **kw))
+    with torch.inference_mode():
+        n = layer(cls, cuda_dev, **kw)
+        n(x)
+        getattr(n, name).mul_(2)
+        got = n(x)
+        assert torch.equal(got, by_fresh_layer(n, x, **kw))
