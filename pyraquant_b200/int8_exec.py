@@ -294,9 +294,11 @@ class LowRankFactors:
 
     def _transposed(self, name: str) -> torch.Tensor:
         """Contiguous transpose of a low-rank factor, remade whenever the buffer is replaced, converted (.to / .half),
-        moved or written in place."""
+        moved or written in place; under stream capture a part of the graph, so that replays follow the factor."""
         src = getattr(self, name)
-        if src.is_inference():                                 # nothing counts the writes to it
+        # Nothing counts the writes to an inference tensor.  What a graph reads has to be made inside it: a copy made before keeps
+        # out of the replays what happens to the factor later, one made during the capture holds nothing until the first replay.
+        if src.is_inference() or (src.is_cuda and ops.capturing()):
             return src.t().contiguous()
         c = self.__dict__.get("_t_cache_" + name)
         if c is None or not c.holds(src):

@@ -42,6 +42,10 @@ def _stream(t: Tensor) -> int:
         return torch.cuda.current_stream(t.device).cuda_stream
 
 
+# whether the current stream records a graph (without torch.cuda's check that CUDA is initialised)
+capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
+
+
 # torch.cuda.current_device() without its check that CUDA is initialised (a tensor of the device exists already)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 

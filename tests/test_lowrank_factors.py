@@ -209,3 +209,32 @@ def test_layers_follow_their_factors(cuda_dev, cls, kw, name):
         getattr(n, name).mul_(2)
         got = n(x)
         assert torch.equal(got, by_fresh_layer(n, x, **kw))
+
+
+@pytest.mark.gpu
+@layers
+@factors
+@pytest.mark.parametrize("warm", [True, False])
+def test_graphs_follow_the_factors(cuda_dev, cls, kw, name, warm):
+    """Replays use the factors as they are then, whether the layer ran before the capture or not, and whatever ran in between."""
+    layer(cls, cuda_dev, **kw)(torch.randn(75, 640, device=cuda_dev).bfloat16())           # libraries and kernels are loaded
+    m = layer(cls, cuda_dev, **kw)
+    x = torch.randn(75, 640, device=cuda_dev).bfloat16()
+    if warm:
+        m(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = m(x)
+    eager = m(x)                                                  # before anything of the capture has run
+    assert torch.equal(eager, by_fresh_layer(m, x, **kw))
+    graph.replay()
+    assert torch.equal(y, eager)
+    getattr(m, name).mul_(-2)
+    graph.replay()
+    assert torch.equal(y, by_fresh_layer(m, x, **kw))
+    m(x)
+    filler = [torch.full((640, 32), 1e4, device=cuda_dev, dtype=torch.bfloat16) for _ in range(8)]
+    graph.replay()
+    assert torch.equal(y, by_fresh_layer(m, x, **kw))
+    del filler
+    ops.check_device_status(cuda_dev)
