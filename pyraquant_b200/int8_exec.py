@@ -269,11 +269,28 @@ FLUX_SHARED_INPUT_GROUPS = (
 class _Transposed:
     """A factor's K-major copy and what it was made of: the tensor itself, its version, and an alias that keeps its memory from being
     handed out again, so that a tensor at the same address is the same data."""
-    __slots__ = ("source", "alias", "version", "copy")
+    __slots__ = ("source", "alias", "version", "copy", "stream", "made", "told")
 
     def __init__(self, src: torch.Tensor):
         self.source, self.alias, self.version = src, src.detach(), src._version
         self.copy = src.t().contiguous()
+        self.stream, self.made, self.told = None, None, set()
+        if src.is_cuda:
+            self.stream = ops._stream(src)
+            self.made = torch.cuda.Event()
+            self.made.record(torch.cuda.current_stream(src.device))
+
+    def on_current_stream(self) -> torch.Tensor:
+        """The copy, for work that the current stream is given next: a stream other than the one that made it waits for it, and
+        the allocator learns who reads it."""
+        if self.stream is not None:
+            stream = ops._stream(self.copy)
+            if stream != self.stream and stream not in self.told:
+                s = torch.cuda.current_stream(self.copy.device)
+                s.wait_event(self.made)
+                self.copy.record_stream(s)
+                self.told.add(stream)
+        return self.copy
 
     def holds(self, src: torch.Tensor) -> bool:
         a = self.alias
@@ -304,7 +321,7 @@ class LowRankFactors:
         if c is None or not c.holds(src):
             c = _Transposed(src)
             self.__dict__["_t_cache_" + name] = c
-        return c.copy
+        return c.on_current_stream()
 
     def _down(self, x2: torch.Tensor) -> torch.Tensor:
         """t = x2 @ lr_A rounded to the activation dtype (reference :390): the native streaming kernel for rank 32

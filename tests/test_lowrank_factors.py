@@ -238,3 +238,38 @@ def test_graphs_follow_the_factors(cuda_dev, cls, kw, name, warm):
     assert torch.equal(y, by_fresh_layer(m, x, **kw))
     del filler
     ops.check_device_status(cuda_dev)
+
+
+@pytest.mark.gpu
+@layers
+def test_first_call_on_another_stream(cuda_dev, cls, kw):
+    """A copy that one stream is still to make is waited for by a call on another one, and lives until that call has read it."""
+    layer(cls, cuda_dev, **kw)(torch.randn(75, 640, device=cuda_dev).bfloat16())
+    side = torch.cuda.Stream()
+    x = torch.randn(75, 640, device=cuda_dev).bfloat16()
+    for i in range(5):
+        m = layer(cls, cuda_dev, **kw, seed=10 + i)
+        want = by_fresh_layer(m, x, **kw, seed=10 + i)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)                         # some 10 ms
+            first = m(x)
+        here = m(x)
+        assert torch.equal(here, want)
+        torch.cuda.synchronize()
+        assert torch.equal(first, want)
+    torch.cuda.synchronize()
+    m = layer(cls, cuda_dev, **kw)
+    want = by_fresh_layer(m, x, **kw)
+    m(x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        late = m(x)
+    old = m.lr_A, m.lr_B                                          # the factors stay for the call that is still to read them
+    m.lr_A, m.lr_B = m.lr_A.clone(), m.lr_B.clone()               # here: the copies go, and their memory is written again
+    m(x)
+    filler = [torch.full((640 * 32,), 1e4, device=cuda_dev, dtype=torch.bfloat16) for _ in range(64)]
+    torch.cuda.synchronize()
+    assert torch.equal(late, want)
+    del filler, old
