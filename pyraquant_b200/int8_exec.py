@@ -301,6 +301,19 @@ class _Transposed:
 class LowRankFactors:
     """What the Linears with a low-rank branch share: K-major copies of the factors, made once, and the down-projection."""
 
+    # what forwards keep beside the buffers; none of it is part of the layer
+    _KEPT = ("_lean_cache", "_t_cache_lr_A", "_t_cache_lr_B")
+
+    def __getstate__(self):
+        """Copies and pickles leave what forwards keep behind (it is remade on the first forward)."""
+        return {k: v for k, v in self.__dict__.items() if k not in self._KEPT}
+
+    def _apply(self, fn, recurse=True):
+        """A layer that is moved or converted leaves nothing behind where it was."""
+        for k in self._KEPT:
+            self.__dict__.pop(k, None)
+        return super()._apply(fn, recurse)
+
     def _lr_Bt(self) -> torch.Tensor:
         """K-major copy of lr_B for the tensor-core low-rank path, made once per device/dtype (not part of the state)."""
         return self._transposed("lr_B")
@@ -366,10 +379,6 @@ class Int8Linear(LowRankFactors, nn.Module):
         else:
             self.lr_A = None
             self.lr_B = None
-
-    def __getstate__(self):
-        """Copies and pickles leave the address caches behind (they are remade on the first forward)."""
-        return {k: v for k, v in self.__dict__.items() if k != "_lean_cache"}
 
     def _one_launch_prologue(self, x2: torch.Tensor) -> bool:
         return (self.lr_A.shape[1] == 32 and self.lr_A.dtype == x2.dtype and ops.quant_lowrank_ok(x2)

@@ -273,3 +273,32 @@ def test_first_call_on_another_stream(cuda_dev, cls, kw):
     torch.cuda.synchronize()
     assert torch.equal(late, want)
     del filler, old
+
+
+@layers
+def test_kept_copies_stay_with_the_layer(cls, kw):
+    """Pickles and copies hold the buffers alone, a layer that is converted or moved drops what it kept."""
+    import copy
+    import pickle
+    m = layer(cls, torch.device("cpu"), **kw)
+    size = len(pickle.dumps(m))
+    before = set(m.__dict__)
+    m._lr_At(), m._lr_Bt()
+    assert len(pickle.dumps(m)) == size
+    for n in (pickle.loads(pickle.dumps(m)), copy.deepcopy(m), copy.copy(m)):
+        assert set(n.__dict__) == before and torch.equal(n.lr_A, m.lr_A) and torch.equal(n._lr_At(), m._lr_At())
+    assert set(m.half().__dict__) == before
+
+
+@pytest.mark.gpu
+@layers
+def test_a_layer_moved_off_leaves_no_memory(cuda_dev, cls, kw):
+    x = torch.randn(75, 640, device=cuda_dev).bfloat16()
+    layer(cls, cuda_dev, **kw)(x)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(cuda_dev)
+    m = layer(cls, cuda_dev, **kw)
+    m(x)
+    m.cpu()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated(cuda_dev) == before
