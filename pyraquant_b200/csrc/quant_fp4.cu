@@ -159,7 +159,7 @@ pq_dequant_rows_fp4_kernel(const uint8_t* codes, int64_t ldc, const uint8_t* sca
       if (c < nchunk) {
         const int blk = FMT == PQ_FP4_MX ? c >> 1 : c;
         w[j] = *reinterpret_cast<const uint2*>(crow + static_cast<int64_t>(c) * 8);
-        byte[j] = srow[(blk >> 2) * 512 + (blk & 3)];
+        byte[j] = srow[static_cast<int64_t>(blk >> 2) * 512 + (blk & 3)];      // 2^31 bytes at 2^28 elements (nv)
       }
     }
 #pragma unroll

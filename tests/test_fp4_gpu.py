@@ -658,3 +658,17 @@ def test_linear_in_inference_mode(cuda_dev):
         m.lr_B.mul_(2)                                            # nothing counts this change
         doubled = m(x)
     assert not torch.equal(doubled, want) and torch.equal(m(x), doubled)
+
+
+@pytest.mark.parametrize("fmt,K", [("nv", 2 ** 28 + 64), ("mx", 2 ** 29 + 128)])
+def test_rows_whose_scales_pass_two_gigabytes(cuda_dev, fmt, K):
+    """Offsets into the scale tiles of one row need more than 31 bits."""
+    x = torch.zeros(1, K, dtype=torch.bfloat16, device=cuda_dev)
+    ends = awkward_rows(1, 256, torch.bfloat16, 12).to(cuda_dev)
+    x[:, :128], x[:, -128:] = ends[:, :128], ends[:, 128:]
+    q = fp4_exec.quant_rows_fp4(x, fmt)
+    assert q.scales.numel() > 2 ** 31
+    v = fp4_exec.dequant_rows_fp4(q)
+    small = fp4_exec.dequant_rows_fp4(fp4_exec.quant_rows_fp4(ends, fmt))
+    assert torch.equal(v[:, :128], small[:, :128]) and torch.equal(v[:, -128:], small[:, 128:])
+    assert not v[:, 128:-128].any()
