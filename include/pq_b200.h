@@ -335,7 +335,7 @@ int64_t pq_fp4_scale_bytes(int64_t M, int64_t K, int fmt);
  * mx).  K % 32 == 0, ldx % 16 == 0, x 32-byte aligned, codes and scales 16-byte aligned. */
 int pq_quant_rows_fp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fmt, uint8_t* codes,
                       uint8_t* scales, float* row_scale, void* stream);
-/* The values that packed rows stand for, rounded to `dtype` (fp16: clipped to +-65504): codes with row stride ldc bytes
+/* The values that packed rows stand for, rounded to `dtype` and clipped to its largest finite value: codes with row stride ldc bytes
  * (% 16 == 0) -> out [M,K], row stride ldo (% 16 == 0), 32-byte aligned. */
 int pq_dequant_rows_fp4(const uint8_t* codes, int64_t ldc, const uint8_t* scales, const float* row_scale, int fmt,
                         void* out, int dtype, int64_t ldo, int64_t M, int64_t K, void* stream);

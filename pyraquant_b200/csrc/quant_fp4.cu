@@ -130,9 +130,11 @@ pq_quant_rows_fp4_kernel(const T* x, int64_t ldx, uint8_t* codes, uint8_t* scale
   }
 }
 
-// fp16 values stay finite: the largest code times a scale rounded up can pass 65504
-__device__ __forceinline__ float finite16(float v, __half) { return v > 65504.0f ? 65504.0f : (v < -65504.0f ? -65504.0f : v); }
-__device__ __forceinline__ float finite16(float v, __nv_bfloat16) { return v; }
+// Finite values stay finite: the largest code times a scale rounded up can pass 65504, and nv at the top of bf16's range the largest
+// fp32 value too (a row of bf16's largest gets 6 * 352 * 2^117).
+__device__ __forceinline__ float clip16(float v, float top) { return v > top ? top : (v < -top ? -top : v); }
+__device__ __forceinline__ float finite16(float v, __half) { return clip16(v, 65504.0f); }
+__device__ __forceinline__ float finite16(float v, __nv_bfloat16) { return clip16(v, __int_as_float(0x7F7F0000)); }
 
 // A thread turns units of 16 codes (8 bytes and a scale byte) into one 32-byte store each, five units at a time.
 template <typename T, int FMT, int TPR>

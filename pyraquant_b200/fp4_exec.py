@@ -49,7 +49,7 @@ def quant_rows_fp4(x2: torch.Tensor, fmt: str = DEFAULT_FORMAT) -> Fp4Rows:
 
 def dequant_rows_fp4(q: Fp4Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values packed rows stand for, [M,K] in ``dtype``.  bf16 holds them exactly; fp16 rounds what lies below its
-    normal range and clips to +-65504."""
+    normal range.  What passes the type's largest value, by a scale that was rounded up, is clipped to it."""
     if _eager():
         return ops._dequant_rows_fp4_impl(q.codes, q.scales, q.row_scale, dtype)
     return torch.ops.pq_b200.dequant_rows_fp4(q.codes, q.scales, q.row_scale, ops.dtype_code(dtype))

@@ -672,3 +672,18 @@ def test_rows_whose_scales_pass_two_gigabytes(cuda_dev, fmt, K):
     small = fp4_exec.dequant_rows_fp4(fp4_exec.quant_rows_fp4(ends, fmt))
     assert torch.equal(v[:, :128], small[:, :128]) and torch.equal(v[:, -128:], small[:, 128:])
     assert not v[:, 128:-128].any()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_read_back_of_every_magnitude(cuda_dev, fmt, dtype):
+    """Finite rows come back finite, the type's largest among them, and as the values of their codes."""
+    top = 0x7F80 if dtype == torch.bfloat16 else 0x7C00
+    v = torch.arange(1, top, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = torch.stack([v * f for f in (1.0, 0.75, -0.4, -1.0)], dim=1).repeat(1, 8)
+    q = fp4_exec.quant_rows_fp4(x.to(cuda_dev), fmt)
+    want = ofp4.packed_values(q.codes.cpu(), q.scales.cpu(), None if q.row_scale is None else q.row_scale.cpu(), fmt)
+    for t in DTYPES:
+        got, most = fp4_exec.dequant_rows_fp4(q, t).cpu(), torch.finfo(t).max
+        assert bool(torch.isfinite(got).all()) and torch.equal(got, want.clamp(-most, most).to(t))
+    assert dtype == torch.float16 or fmt == "mx" or bool((want.abs() > torch.finfo(dtype).max).any())
