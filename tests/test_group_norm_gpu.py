@@ -317,3 +317,46 @@ def test_argument_checks():
         return lib.pq_group_norm_quant_fp4(p, 0, 1, 4, C, C, 4 * C, 8, None, None, 0, 1e-6, 0, fmt, codes, scales, row, p, big, None, None)
     assert q4(fmt=2) == 7 and q4(codes=None) == 1 and q4(scales=None) == 1 and q4(row=None) == 1 and q4(C=80) == 3 and q4(scales=p + 4) == 3
     assert lib.pq_group_norm_workspace_bytes(1, 4, 64, 8) >= 64 and lib.pq_group_norm_workspace_bytes(0, 4, 64, 8) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("affine", ["as_x", "fp32"])
+def test_silu_of_every_value(cuda_dev, dtype, affine):
+    """A weight of zero leaves z = bias exactly: SiLU of every value of the type, tails, subnormals, infinities and NaN among them,
+    beside partners of every size.  The bound is that of the activation above, then the rounding to 16 bits.  Below z = -41.5, -infinity
+    included (its limit is 0), SiLU is between -41.5 / (1 + e^41.5) = -3.95e-17 and 0, and one such value may stand for all of them:
+    off by at most 4e-17."""
+    bits = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16)
+    v = bits.view(dtype)
+    order = torch.randperm(v.numel(), generator=torch.Generator().manual_seed(1))
+    x = torch.randn(2, 3, 8192, generator=torch.Generator().manual_seed(2)).to(dtype).to(cuda_dev)
+    t = dtype if affine == "as_x" else torch.float32
+    weight = torch.zeros(8192, dtype=t, device=cuda_dev)
+    fi = torch.finfo(dtype)
+    for values in (v, v[order]):
+        for b in values.to(t).reshape(8, 8192):
+            z = b.double()
+            want = torch.where(z == -float("inf"), 0.0, z / (1 + torch.exp(-z)))
+            got = norm_exec.group_norm_rows(x, 32, weight, b.to(cuda_dev), 1e-6, "silu").cpu().double()
+            assert torch.equal(torch.isnan(got), torch.isnan(want).expand_as(got)), "NaN where the formula has it, and nowhere else"
+            inf = torch.isinf(want)
+            assert bool((got[..., inf] == want[inf]).all())
+            ok = torch.isfinite(want)
+            err = torch.where(z < -41.5, 4e-17, (11 + z.abs()) * 2.0 ** -24 * want.abs())
+            bound = err + (want.abs() + err) * fi.eps / 2 + fi.smallest_normal * fi.eps / 2
+            off = ((got - want).abs() / bound)[..., ok]
+            assert float(off.max()) <= 1, (float(off.max()), z[ok][off.amax(dim=(0, 1)).argmax()])
+
+
+@pytest.mark.gpu
+def test_silu_far_below_zero(cuda_dev):
+    """fp32 biases outside the 16-bit types' ranges: SiLU stays within 4e-17 of zero."""
+    b = -torch.logspace(0, 38, 64)
+    x = torch.randn(1, 4, 64, generator=torch.Generator().manual_seed(3)).bfloat16().to(cuda_dev)
+    got = norm_exec.group_norm_rows(x, 8, torch.zeros(64, device=cuda_dev), b.to(cuda_dev), 1e-6, "silu")
+    z = b.double()
+    want = z / (1 + torch.exp(-z))
+    assert bool((got.cpu().double() - want).abs().le(want.abs() * ((11 + z.abs()) * 2.0 ** -24 + 2.0 ** -8) + 4e-17).all())
+    for rows in norm_exec.group_norm_quant_rows(x, 8, torch.zeros(64, device=cuda_dev), b.to(cuda_dev), 1e-6, "silu", want_normed=True)[2]:
+        assert torch.equal(rows, got[0])
