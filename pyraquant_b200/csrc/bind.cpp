@@ -68,6 +68,16 @@ PyObject* guarded(F&& f) {
   return nullptr;
 }
 
+// Allocation and launch run without the interpreter lock, like a call through ctypes: a launch waits while the queue is full, and
+// what it waits for may need another Python thread.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 Tensor scale_tensor(int64_t M, int64_t K, int fmt, const Tensor& like) {
   const int64_t per = fmt == PQ_FP4_MX ? 128 : 64;
   return make({(M + 127) / 128, (K + per - 1) / per, 512}, at::kByte, like);
@@ -99,11 +109,17 @@ PyObject* quant_rows_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int code = dtype_code(x.scalar_type()), fmt = static_cast<int>(PyLong_AsLong(a[1]));
     const int64_t M = x.size(0), K = x.size(1);
     if (code < 0 || K <= 0 || K % 32 != 0 || x.stride(1) != 1 || (M > 1 && (x.stride(0) % 16 != 0 || x.stride(0) < K)) || !aligned(x, 32)) return none();
-    c10::cuda::CUDAGuard guard(x.device());
-    Tensor codes = make({M, K / 2}, at::kByte, x), scales = scale_tensor(M, K, fmt, x), row;
-    if (fmt == PQ_FP4_NV) row = make({M}, at::kFloat, x);
-    const int rc = pq_quant_rows_fp4(x.data_ptr(), code, M, K, M > 1 ? x.stride(0) : K, fmt, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
-                                     row.defined() ? row.data_ptr<float>() : nullptr, stream_of(x));
+    Tensor codes, scales, row;
+    int rc;
+    {
+      Unlocked unlocked;
+      c10::cuda::CUDAGuard guard(x.device());
+      codes = make({M, K / 2}, at::kByte, x);
+      scales = scale_tensor(M, K, fmt, x);
+      if (fmt == PQ_FP4_NV) row = make({M}, at::kFloat, x);
+      rc = pq_quant_rows_fp4(x.data_ptr(), code, M, K, M > 1 ? x.stride(0) : K, fmt, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
+                             row.defined() ? row.data_ptr<float>() : nullptr, stream_of(x));
+    }
     return rc == PQ_OK ? tuple3(codes, scales, row) : fail("pq_quant_rows_fp4", rc);
   });
 }
@@ -116,12 +132,17 @@ PyObject* dequant_rows_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor *codes = tensor_of(a[0]), *scales = tensor_of(a[1]);
     if (!plain_rows(codes, scales, row)) return none();
     const bool bf16 = a[3] == Py_True;
-    c10::cuda::CUDAGuard guard(codes->device());
     const int64_t M = codes->size(0), K = codes->size(1) * 2;
-    Tensor out = make({M, K}, bf16 ? at::kBFloat16 : at::kHalf, *codes);
-    const int rc = pq_dequant_rows_fp4(codes->data_ptr<uint8_t>(), K / 2, scales->data_ptr<uint8_t>(), row != nullptr ? row->data_ptr<float>() : nullptr,
-                                       row != nullptr ? PQ_FP4_NV : PQ_FP4_MX, out.data_ptr(), bf16 ? PQ_DTYPE_BF16 : PQ_DTYPE_FP16, K, M, K,
-                                       stream_of(*codes));
+    Tensor out;
+    int rc;
+    {
+      Unlocked unlocked;
+      c10::cuda::CUDAGuard guard(codes->device());
+      out = make({M, K}, bf16 ? at::kBFloat16 : at::kHalf, *codes);
+      rc = pq_dequant_rows_fp4(codes->data_ptr<uint8_t>(), K / 2, scales->data_ptr<uint8_t>(), row != nullptr ? row->data_ptr<float>() : nullptr,
+                               row != nullptr ? PQ_FP4_NV : PQ_FP4_MX, out.data_ptr(), bf16 ? PQ_DTYPE_BF16 : PQ_DTYPE_FP16, K, M, K,
+                               stream_of(*codes));
+    }
     return rc == PQ_OK ? THPVariable_Wrap(out) : fail("pq_dequant_rows_fp4", rc);
   });
 }
@@ -142,13 +163,20 @@ PyObject* fp4_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (bias != nullptr && (!plain(*bias, at::kFloat, xq->device()) || bias->numel() != N)) return none();
     if (t != nullptr && !(plain_low(*t, M, xq->device()) && plain_low(*lb, N, xq->device()))) return none();
     const bool bf16 = a[7] == Py_True;
-    c10::cuda::CUDAGuard guard(xq->device());
-    Tensor out = make({M, N}, bf16 ? at::kBFloat16 : at::kHalf, *xq);
-    auto floats = [](const Tensor* v) { return v != nullptr ? v->data_ptr<float>() : nullptr; };
-    const int rc = pq_fp4_gemm_lowrank(xq->data_ptr<uint8_t>(), K / 2, xs->data_ptr<uint8_t>(), floats(x_row), wq->data_ptr<uint8_t>(), K / 2,
-                                       ws->data_ptr<uint8_t>(), floats(w_row), floats(bias), floats(t), floats(lb),
-                                       x_row != nullptr ? PQ_FP4_NV : PQ_FP4_MX, out.data_ptr(), bf16 ? PQ_DTYPE_BF16 : PQ_DTYPE_FP16, N, M, N, K,
-                                       PyLong_AsVoidPtr(a[8]), static_cast<size_t>(PyLong_AsSize_t(a[9])), stream_of(*xq));
+    void* const workspace = PyLong_AsVoidPtr(a[8]);
+    const size_t ws_bytes = PyLong_AsSize_t(a[9]);
+    Tensor out;
+    int rc;
+    {
+      Unlocked unlocked;
+      c10::cuda::CUDAGuard guard(xq->device());
+      out = make({M, N}, bf16 ? at::kBFloat16 : at::kHalf, *xq);
+      auto floats = [](const Tensor* v) { return v != nullptr ? v->data_ptr<float>() : nullptr; };
+      rc = pq_fp4_gemm_lowrank(xq->data_ptr<uint8_t>(), K / 2, xs->data_ptr<uint8_t>(), floats(x_row), wq->data_ptr<uint8_t>(), K / 2,
+                               ws->data_ptr<uint8_t>(), floats(w_row), floats(bias), floats(t), floats(lb),
+                               x_row != nullptr ? PQ_FP4_NV : PQ_FP4_MX, out.data_ptr(), bf16 ? PQ_DTYPE_BF16 : PQ_DTYPE_FP16, N, M, N, K,
+                               workspace, ws_bytes, stream_of(*xq));
+    }
     return rc == PQ_OK ? THPVariable_Wrap(out) : fail("pq_fp4_gemm", rc);
   });
 }
@@ -162,9 +190,14 @@ PyObject* fp4_lowrank_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t M = t->size(0);
     if (code < 0 || !plain(*t, t->scalar_type(), t->device()) || !aligned(*t, 16)) return none();
     if (row != nullptr && !(plain(*row, at::kFloat, t->device()) && row->dim() == 1 && row->size(0) == M)) return none();
-    c10::cuda::CUDAGuard guard(t->device());
-    Tensor out = make({M, 32}, at::kFloat, *t);
-    const int rc = pq_fp4_lowrank_rows(t->data_ptr(), code, row != nullptr ? row->data_ptr<float>() : nullptr, out.data_ptr<float>(), M, stream_of(*t));
+    Tensor out;
+    int rc;
+    {
+      Unlocked unlocked;
+      c10::cuda::CUDAGuard guard(t->device());
+      out = make({M, 32}, at::kFloat, *t);
+      rc = pq_fp4_lowrank_rows(t->data_ptr(), code, row != nullptr ? row->data_ptr<float>() : nullptr, out.data_ptr<float>(), M, stream_of(*t));
+    }
     return rc == PQ_OK ? THPVariable_Wrap(out) : fail("pq_fp4_lowrank_rows", rc);
   });
 }
@@ -181,10 +214,16 @@ PyObject* fp4_lowrank_factors(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (tc < 0 || bc < 0 || !plain(*t, t->scalar_type(), t->device()) || !aligned(*t, 16) || !plain(*b, b->scalar_type(), t->device())) return none();
     if (row != nullptr && !(plain(*row, at::kFloat, t->device()) && row->dim() == 1 && row->size(0) == M)) return none();
     if (col != nullptr && !(plain(*col, at::kFloat, t->device()) && col->dim() == 1 && col->size(0) == N)) return none();
-    c10::cuda::CUDAGuard guard(t->device());
-    Tensor t_out = make({M, 32}, at::kFloat, *t), b_out = make({N, 32}, at::kFloat, *t);
-    const int rc = pq_fp4_lowrank_factors(t->data_ptr(), tc, row != nullptr ? row->data_ptr<float>() : nullptr, t_out.data_ptr<float>(), M, b->data_ptr(),
-                                          bc, N, col != nullptr ? col->data_ptr<float>() : nullptr, b_out.data_ptr<float>(), N, stream_of(*t));
+    Tensor t_out, b_out;
+    int rc;
+    {
+      Unlocked unlocked;
+      c10::cuda::CUDAGuard guard(t->device());
+      t_out = make({M, 32}, at::kFloat, *t);
+      b_out = make({N, 32}, at::kFloat, *t);
+      rc = pq_fp4_lowrank_factors(t->data_ptr(), tc, row != nullptr ? row->data_ptr<float>() : nullptr, t_out.data_ptr<float>(), M, b->data_ptr(),
+                                  bc, N, col != nullptr ? col->data_ptr<float>() : nullptr, b_out.data_ptr<float>(), N, stream_of(*t));
+    }
     if (rc != PQ_OK) return fail("pq_fp4_lowrank_factors", rc);
     PyObject* r = PyTuple_New(2);
     if (r == nullptr) return nullptr;
@@ -219,39 +258,44 @@ PyObject* group_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (const Tensor* v : {w, b})
       if (v != nullptr && (!plain(*v, x.scalar_type(), x.device()) || v->dim() != 1 || v->size(0) != C || !aligned(*v, 16) || (grad && v->requires_grad())))
         return none();
-    c10::cuda::CUDAGuard guard(x.device());
-    const void* wp = w != nullptr ? w->data_ptr() : nullptr;
-    const void* bp = b != nullptr ? b->data_ptr() : nullptr;
-    const int64_t bytes = pq_group_norm_workspace_bytes(B, T, C, static_cast<int>(groups));
-    Tensor ws = make({bytes}, at::kByte, x);
-    void* status = PyLong_AsVoidPtr(a[8]);
-    void* st = stream_of(x);
-    const float e = static_cast<float>(eps);
-    const int g = static_cast<int>(groups);
-    if (mode == 0) {
-      Tensor z = make({B, T, C}, x.scalar_type(), x);
-      const int rc = pq_group_norm(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, z.data_ptr(), C, T * C, ws.data_ptr(), bytes, status, st);
-      if (rc == PQ_ERR_UNSUPPORTED) return none();
-      return rc == PQ_OK ? THPVariable_Wrap(z) : fail("pq_group_norm", rc);
-    }
+    void* const status = PyLong_AsVoidPtr(a[8]);
+    const bool want_z = mode == 0 || a[7] == Py_True;
+    Tensor z, q, scales, row;
     int rc;
-    PyObject* result = nullptr;
-    if (mode == 1) {
-      Tensor z, q = make({B * T, C}, at::kChar, x), s = make({B * T}, at::kFloat, x);
-      if (a[7] == Py_True) z = make({B, T, C}, x.scalar_type(), x);
-      rc = pq_group_norm_quant_rows(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, z.defined() ? z.data_ptr() : nullptr, C, T * C,
-                                    q.data_ptr<int8_t>(), s.data_ptr<float>(), ws.data_ptr(), bytes, status, st);
-      if (rc == PQ_OK) result = tuple3(q, s, z);
-    } else {
-      const int fmt = mode == 2 ? PQ_FP4_MX : PQ_FP4_NV;
-      Tensor codes = make({B * T, C / 2}, at::kByte, x), scales = scale_tensor(B * T, C, fmt, x), row;
-      if (fmt == PQ_FP4_NV) row = make({B * T}, at::kFloat, x);
-      rc = pq_group_norm_quant_fp4(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, fmt, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
-                                   row.defined() ? row.data_ptr<float>() : nullptr, ws.data_ptr(), bytes, status, st);
-      if (rc == PQ_OK) result = tuple3(codes, scales, row);
+    {
+      Unlocked unlocked;
+      c10::cuda::CUDAGuard guard(x.device());
+      const void* wp = w != nullptr ? w->data_ptr() : nullptr;
+      const void* bp = b != nullptr ? b->data_ptr() : nullptr;
+      const int64_t bytes = pq_group_norm_workspace_bytes(B, T, C, static_cast<int>(groups));
+      Tensor ws = make({bytes}, at::kByte, x);
+      void* st = stream_of(x);
+      const float e = static_cast<float>(eps);
+      const int g = static_cast<int>(groups);
+      if (mode < 2 && want_z) z = make({B, T, C}, x.scalar_type(), x);
+      void* zp = z.defined() ? z.data_ptr() : nullptr;
+      if (mode == 0) {
+        rc = pq_group_norm(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, zp, C, T * C, ws.data_ptr(), bytes, status, st);
+      } else if (mode == 1) {
+        q = make({B * T, C}, at::kChar, x);
+        row = make({B * T}, at::kFloat, x);
+        rc = pq_group_norm_quant_rows(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, zp, C, T * C, q.data_ptr<int8_t>(),
+                                      row.data_ptr<float>(), ws.data_ptr(), bytes, status, st);
+      } else {
+        const int fmt = mode == 2 ? PQ_FP4_MX : PQ_FP4_NV;
+        q = make({B * T, C / 2}, at::kByte, x);
+        scales = scale_tensor(B * T, C, fmt, x);
+        if (fmt == PQ_FP4_NV) row = make({B * T}, at::kFloat, x);
+        rc = pq_group_norm_quant_fp4(x.data_ptr(), code, B, T, C, C, T * C, g, wp, bp, 0, e, act, fmt, q.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
+                                     row.defined() ? row.data_ptr<float>() : nullptr, ws.data_ptr(), bytes, status, st);
+      }
     }
-    if (rc == PQ_ERR_UNSUPPORTED) Py_RETURN_FALSE;
-    return rc == PQ_OK ? result : fail("pq_group_norm_quant", rc);
+    if (rc == PQ_ERR_UNSUPPORTED) {
+      if (mode == 0) return none();
+      Py_RETURN_FALSE;
+    }
+    if (rc != PQ_OK) return fail(mode == 0 ? "pq_group_norm" : "pq_group_norm_quant", rc);
+    return mode == 0 ? THPVariable_Wrap(z) : (mode == 1 ? tuple3(q, row, z) : tuple3(q, scales, row));
   });
 }
 

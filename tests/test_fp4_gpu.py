@@ -687,3 +687,45 @@ def test_read_back_of_every_magnitude(cuda_dev, fmt, dtype):
         got, most = fp4_exec.dequant_rows_fp4(q, t).cpu(), torch.finfo(t).max
         assert bool(torch.isfinite(got).all()) and torch.equal(got, want.clamp(-most, most).to(t))
     assert dtype == torch.float16 or fmt == "mx" or bool((want.abs() > torch.finfo(dtype).max).any())
+
+
+@pytest.mark.parametrize("op", ["quant", "dequant", "product", "factors", "norm", "norm_int8", "norm_fp4"])
+def test_calls_let_other_threads_run(cuda_dev, op):
+    """A launch waits while the queue is full.  Other Python threads run meanwhile."""
+    import threading
+    import time
+
+    from pyraquant_b200 import norm_exec
+    x = torch.randn(4, 64, device=cuda_dev).bfloat16()
+    q, t, B = fp4_exec.quant_rows_fp4(x, "nv"), torch.randn(4, 32, device=cuda_dev).bfloat16(), torch.randn(32, 4, device=cuda_dev).bfloat16()
+    call = {"quant": lambda: fp4_exec.quant_rows_fp4(x, "nv"), "dequant": lambda: fp4_exec.dequant_rows_fp4(q),
+            "product": lambda: fp4_exec.fp4_gemm(q, q), "factors": lambda: fp4_exec.lowrank_factors(t, q, B, q),
+            "norm": lambda: norm_exec.group_norm_rows(x[None], 4), "norm_int8": lambda: norm_exec.group_norm_quant_rows(x[None], 4),
+            "norm_fp4": lambda: norm_exec.group_norm_quant_fp4(x[None], 4)}[op]
+    call()
+    torch.cuda.synchronize()
+    longest, stop = [0.0], threading.Event()
+
+    def ticker():
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.002)
+            now = time.perf_counter()
+            longest[0], last = max(longest[0], now - last), now
+    other = threading.Thread(target=ticker)
+    other.start()
+    waited = 0.0
+    try:
+        torch.cuda._sleep(1_200_000_000)                          # some 0.6 s
+        for _ in range(4000):
+            t0 = time.perf_counter()
+            call()
+            waited = max(waited, time.perf_counter() - t0)
+            if waited > 0.1:
+                break
+    finally:
+        stop.set()
+        other.join()
+        torch.cuda.synchronize()
+    assert waited > 0.1, "no call had to wait"
+    assert longest[0] < waited / 2, (longest[0], waited)
