@@ -269,21 +269,26 @@ FLUX_SHARED_INPUT_GROUPS = (
 class _Transposed:
     """A factor's K-major copy and what it was made of: the tensor itself, its version, and an alias that keeps its memory from being
     handed out again, so that a tensor at the same address is the same data."""
-    __slots__ = ("source", "alias", "version", "copy", "stream", "made", "told")
+    __slots__ = ("source", "alias", "version", "ptr", "dtype", "shape", "strides", "copy", "index", "stream", "made", "told")
 
     def __init__(self, src: torch.Tensor):
         self.source, self.alias, self.version = src, src.detach(), src._version
-        self.copy = src.t().contiguous()
-        self.stream, self.made, self.told = None, None, set()
+        self.ptr, self.dtype, self.shape, self.strides = self.alias.data_ptr(), src.dtype, src.shape, src.stride()
+        self.copy = self.alias.t().contiguous()
+        self.index, self.told = src.get_device(), set()
         if src.is_cuda:
             self.stream = ops._stream(src)
             self.made = torch.cuda.Event()
             self.made.record(torch.cuda.current_stream(src.device))
 
+    def holds(self, src: torch.Tensor) -> bool:
+        return (self.source is src and self.version == src._version and self.ptr == src.data_ptr() and self.dtype is src.dtype
+                and self.shape == src.shape and self.strides == src.stride())
+
     def on_current_stream(self) -> torch.Tensor:
         """The copy, for work that the current stream is given next: a stream other than the one that made it waits for it, and
         the allocator learns who reads it."""
-        if self.stream is not None:
+        if self.index >= 0:
             stream = ops._stream(self.copy)
             if stream != self.stream and stream not in self.told:
                 s = torch.cuda.current_stream(self.copy.device)
@@ -291,11 +296,6 @@ class _Transposed:
                 self.copy.record_stream(s)
                 self.told.add(stream)
         return self.copy
-
-    def holds(self, src: torch.Tensor) -> bool:
-        a = self.alias
-        return (self.source is src and self.version == src._version and a.data_ptr() == src.data_ptr()
-                and a.dtype is src.dtype and a.shape == src.shape and a.stride() == src.stride())
 
 
 class LowRankFactors:
@@ -325,13 +325,17 @@ class LowRankFactors:
     def _transposed(self, name: str) -> torch.Tensor:
         """Contiguous transpose of a low-rank factor, remade whenever the buffer is replaced, converted (.to / .half),
         moved or written in place; under stream capture a part of the graph, so that replays follow the factor."""
-        src = getattr(self, name)
-        # Nothing counts the writes to an inference tensor.  What a graph reads has to be made inside it: a copy made before keeps
-        # out of the replays what happens to the factor later, one made during the capture holds nothing until the first replay.
-        if src.is_inference() or (src.is_cuda and ops.capturing()):
+        src = self._buffers.get(name)
+        if src is None:                                        # a Parameter, a plain attribute, a parametrised tensor
+            src = getattr(self, name)
+        # What a graph reads has to be made inside it: a copy made before keeps out of the replays what happens to the factor later,
+        # one made during the capture holds nothing until the first replay.  Nothing counts the writes to an inference tensor.
+        if src.is_cuda and ops.capturing():
             return src.t().contiguous()
         c = self.__dict__.get("_t_cache_" + name)
         if c is None or not c.holds(src):
+            if src.is_inference():
+                return src.t().contiguous()
             c = _Transposed(src)
             self.__dict__["_t_cache_" + name] = c
         return c.on_current_stream()
