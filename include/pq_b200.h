@@ -257,6 +257,11 @@ int pq_int8_gemm_g32(const int8_t* xq, int64_t ldx, const float* s_a,
                      int64_t M, int64_t N, int64_t K,
                      void* workspace, size_t ws_bytes, void* stream);
 
+/* K-major copies of the factors of a rank-32 branch, 16-bit values: a_t [32,K] contiguous of a [K,32] (row stride lda elements,
+ * % 8 == 0, 16-byte aligned) and b_t [N,32] contiguous, 16-byte aligned, of b [32,N] (row stride ldb).  K or N may be 0: that factor
+ * is left out.  One launch; what pq_lowrank_down, pq_quant_rows_lowrank (a_t) and the GEMMs (lb_t) take. */
+int pq_lowrank_layout(const void* a, int64_t lda, void* a_t, int64_t K, const void* b, int64_t ldb, void* b_t, int64_t N, void* stream);
+
 /* Down-projection of the rank-32 branch: t[m, 0:R] = round(sum_k x[m,k] * A[k, 0:R]), fp32 accumulation on the
  * tensor cores, result rounded to `dtype`.  Replaces `x2.to(lr_A.dtype) @ lr_A` (deploy/int8_exec.py:390), a torch
  * matmul in the reference; same value up to fp32 summation order.  R = 32 for one layer; 64, 96 or 128 when the

@@ -80,6 +80,7 @@ SIGNATURES = {
                                      c_void_p, c_size_t, c_void_p]),
     "pq_lowrank_down": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_int64,
                                 c_void_p, c_size_t, c_void_p]),
+    "pq_lowrank_layout": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
     "pq_unpack_int4": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
     "pq_fp4_scale_bytes": (c_int64, [c_int64, c_int64, c_int]),
     "pq_quant_rows_fp4": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),

@@ -10,6 +10,7 @@
 // slices added in order by the epilogue, so that a row's t is the same bits whichever kernel computes it.
 #include <type_traits>
 
+#include "fp4_common.cuh"
 #include "gemm_common.cuh"
 
 namespace pq {
@@ -253,10 +254,60 @@ int launch_low_cols(int R, const CUtensorMap& tmX, const CUtensorMap& tmX1, int 
   }
 }
 
+// K-major copies of both factors of a rank-32 branch, 16-bit values moved as they are: a_t [32, K] of A [K, 32] by the first `a_blocks`
+// blocks, b_t [N, 32] of B [32, N] by the others.  A block takes 64 indices of the long axis, a thread one of them and eight of the
+// 32: one 16-byte access on the side where those are neighbours, eight 2-byte ones on the other, where a warp's 32 threads are.
+// For graphs, which lay the factors out themselves: latency, so one launch for both, chained to the kernel before (fp4_common.cuh).
+constexpr int kLayoutThreads = 256, kLayoutRows = kLayoutThreads / 4;
+__global__ void __launch_bounds__(kLayoutThreads)
+pq_lowrank_layout_kernel(const uint16_t* a, int64_t lda, uint16_t* a_t, int64_t K, unsigned a_blocks, const uint16_t* b, int64_t ldb,
+                         uint16_t* b_t, int64_t N) {
+  wait_for_previous_kernel();
+  allow_next_kernel();
+  const int r0 = static_cast<int>(threadIdx.x) / kLayoutRows * 8;
+  const int in_block = static_cast<int>(threadIdx.x) % kLayoutRows;
+  if (blockIdx.x < a_blocks) {
+    const int64_t k = static_cast<int64_t>(blockIdx.x) * kLayoutRows + in_block;
+    if (k >= K) return;
+    const uint4 v = *reinterpret_cast<const uint4*>(a + k * lda + r0);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a_t[(r0 + i) * K + k] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+  } else {
+    const int64_t n = static_cast<int64_t>(blockIdx.x - a_blocks) * kLayoutRows + in_block;
+    if (n >= N) return;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = static_cast<uint32_t>(b[(r0 + 2 * i) * ldb + n]) | (static_cast<uint32_t>(b[(r0 + 2 * i + 1) * ldb + n]) << 16);
+    st_v4(b_t + n * 32 + r0, make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+
 }  // namespace
 }  // namespace pq
 
 using namespace pq;
+
+extern "C" int pq_lowrank_layout(const void* a, int64_t lda, void* a_t, int64_t K, const void* b, int64_t ldb, void* b_t, int64_t N,
+                                 void* stream) {
+  if (K < 0 || N < 0 || K > 0x7fffffffLL || N > 0x7fffffffLL || (K > 0 && lda < 32) || (N > 0 && ldb < N)) return PQ_ERR_SHAPE;
+  if (K == 0 && N == 0) return PQ_OK;
+  if ((K > 0 && (a == nullptr || a_t == nullptr)) || (N > 0 && (b == nullptr || b_t == nullptr))) return PQ_ERR_NULL;
+  if (K > 0 && (lda % 8 != 0 || !aligned_to(a, 16) || !aligned_to(a_t, 2))) return PQ_ERR_ALIGN;
+  if (N > 0 && (!aligned_to(b, 2) || !aligned_to(b_t, 16))) return PQ_ERR_ALIGN;
+  const int64_t a_blocks = (K + kLayoutRows - 1) / kLayoutRows, blocks = a_blocks + (N + kLayoutRows - 1) / kLayoutRows;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at = chained_launch();
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(kLayoutThreads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  PQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, pq_lowrank_layout_kernel, static_cast<const uint16_t*>(a), lda, static_cast<uint16_t*>(a_t), K,
+                                 static_cast<unsigned>(a_blocks), static_cast<const uint16_t*>(b), ldb, static_cast<uint16_t*>(b_t), N));
+  return PQ_OK;
+}
 
 namespace {
 int lowrank_down_impl(const void* x, int64_t K0, int64_t ldx, const void* x1, int64_t K1, int64_t ldx1, int dtype,

@@ -325,16 +325,27 @@ class LowRankFactors:
     def _transposed(self, name: str) -> torch.Tensor:
         """Contiguous transpose of a low-rank factor, remade whenever the buffer is replaced, converted (.to / .half),
         moved or written in place; under stream capture a part of the graph, so that replays follow the factor."""
+        if self._in_graph():
+            src = getattr(self, name)
+            return ops.lowrank_layout(src, None)[0] if name == "lr_A" else ops.lowrank_layout(None, src)[1]
+        return self._kept(name)
+
+    def _lr_At_Bt(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Both, in a graph by one launch."""
+        return ops.lowrank_layout(self.lr_A, self.lr_B) if self._in_graph() else (self._kept("lr_A"), self._kept("lr_B"))
+
+    def _in_graph(self) -> bool:
+        """What a graph reads has to be made inside it: a copy made before keeps out of the replays what happens to the factor later,
+        one made during the capture holds nothing until the first replay."""
+        return self.lr_A.is_cuda and ops.capturing()
+
+    def _kept(self, name: str) -> torch.Tensor:
         src = self._buffers.get(name)
         if src is None:                                        # a Parameter, a plain attribute, a parametrised tensor
             src = getattr(self, name)
-        # What a graph reads has to be made inside it: a copy made before keeps out of the replays what happens to the factor later,
-        # one made during the capture holds nothing until the first replay.  Nothing counts the writes to an inference tensor.
-        if src.is_cuda and ops.capturing():
-            return src.t().contiguous()
         c = self.__dict__.get("_t_cache_" + name)
         if c is None or not c.holds(src):
-            if src.is_inference():
+            if src.is_inference():                             # nothing counts the writes to it
                 return src.t().contiguous()
             c = _Transposed(src)
             self.__dict__["_t_cache_" + name] = c
@@ -431,7 +442,8 @@ class Int8Linear(LowRankFactors, nn.Module):
                 return None
             rank = 32
             one_launch = ops.quant_lowrank_ok(x2)              # else: rows too short or too long for the shared launch
-            lr_b, lbt, at = self.lr_B, self._lr_Bt(), self._lr_At() if one_launch else None
+            lr_b = self.lr_B
+            at, lbt = self._lr_At_Bt() if one_launch else (None, self._lr_Bt())
             # the library sees bare pointers: factors that do not fit the layer must not get there
             assert at is None or (at.numel() == 32 * K and at.get_device() == x2.get_device()), (tuple(at.shape), at.device)
             if lr_b.stride(1) != 1:

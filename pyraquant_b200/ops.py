@@ -422,6 +422,24 @@ def lowrank_down(x2: Tensor, a_t: Tensor) -> Tensor:
     return t
 
 
+def lowrank_layout(A: Optional[Tensor], B: Optional[Tensor]) -> Tuple[Optional[Tensor], Optional[Tensor]]:
+    """(A.t(), B.t()), contiguous, of a branch's factors A [K, R] and B [R, N] (each may be left out): one launch for CUDA factors of rank 32
+    in a 16-bit type (pq_lowrank_layout), torch's copies otherwise."""
+    a_ok = A is None or (A.is_cuda and A.dim() == 2 and A.dtype in _DT and A.shape[1] == 32 and A.is_contiguous() and A.data_ptr() % 16 == 0)
+    b_ok = B is None or (B.is_cuda and B.dim() == 2 and B.dtype in _DT and B.shape[0] == 32 and B.is_contiguous())
+    if not (a_ok and b_ok) or (A is not None and B is not None and A.device != B.device):
+        return (None if A is None else A.t().contiguous()), (None if B is None else B.t().contiguous())
+    K, N = 0 if A is None else A.shape[0], 0 if B is None else B.shape[1]
+    a_t = None if A is None else A.new_empty((32, K))
+    b_t = None if B is None else B.new_empty((N, 32))
+    like = A if A is not None else B
+    with _on_device(like):
+        rc = _LIB().pq_lowrank_layout(_ptr(A), 32, _ptr(a_t), K, _ptr(B), N, _ptr(b_t), N, _stream(like))
+    if rc:
+        _lib.check(rc, f"pq_lowrank_layout(K={K}, N={N})")
+    return a_t, b_t
+
+
 def lowrank_down_ok(x2: Tensor) -> bool:
     """Shapes pq_lowrank_down takes without a copy and is the faster choice for."""
     return (LOWRANK_DOWN_NATIVE and x2.is_cuda and x2.dtype in _DT and x2.dim() == 2 and x2.stride(1) == 1

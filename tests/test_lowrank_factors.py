@@ -302,3 +302,37 @@ def test_a_layer_moved_off_leaves_no_memory(cuda_dev, cls, kw):
     m.cpu()
     torch.cuda.synchronize()
     assert torch.cuda.memory_allocated(cuda_dev) == before
+
+
+# ------------------------------------------------------------------------------------------------ the copies of a graph
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layout_of_both_factors(cuda_dev, dtype):
+    g = torch.Generator().manual_seed(5)
+    for K, N in ((1, 1), (63, 64), (65, 129), (640, 328), (10240, 7), (7, 10240)):
+        A, B = torch.randn(K, 32, generator=g).to(dtype).to(cuda_dev), torch.randn(32, N, generator=g).to(dtype).to(cuda_dev)
+        for a, b in ((A, B), (A, None), (None, B)):
+            at, bt = ops.lowrank_layout(a, b)
+            assert at is None if a is None else (torch.equal(at, A.t()) and at.is_contiguous())
+            assert bt is None if b is None else (torch.equal(bt, B.t()) and bt.is_contiguous())
+    wide = torch.randn(70, 40, generator=g).to(dtype).to(cuda_dev)
+    for a, b in ((wide[:, 1:33], wide[:32, 3:]), (wide[:, :32].t().contiguous().t(), wide[:32]), (wide, wide[:16]), (wide.float()[:, :32].contiguous(), None)):
+        at, bt = ops.lowrank_layout(a, b)                         # what the kernel does not take as it is
+        assert torch.equal(at, a.t()) and at.is_contiguous() and (b is None or (torch.equal(bt, b.t()) and bt.is_contiguous()))
+    lib, A = _lib.load(), torch.randn(9, 48, generator=g).to(dtype).to(cuda_dev)
+    out = torch.full((32 * 9 + 8,), 7.0, dtype=dtype, device=cuda_dev)            # rows apart, nothing else written
+    assert lib.pq_lowrank_layout(A.data_ptr() + 16, 48, out.data_ptr() + 2, 9, None, 0, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out[1: 289].reshape(32, 9), A[:, 8:40].t()) and bool((out[289:] == 7).all()) and float(out[0]) == 7
+
+
+def test_layout_argument_checks():
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 63) & ~63
+
+    def f(a=p, lda=32, a_t=p, K=4, b=p, ldb=8, b_t=p, N=8):
+        return lib.pq_lowrank_layout(a, lda, a_t, K, b, ldb, b_t, N, None)
+    assert f(K=0, N=0, a=None, b=None) == 0
+    assert f(K=-1) == 2 and f(N=-1) == 2 and f(lda=24) == 2 and f(ldb=7) == 2 and f(K=1 << 31) == 2
+    assert f(a=None) == 1 and f(a_t=None) == 1 and f(b=None) == 1 and f(b_t=None) == 1
+    assert f(lda=36) == 3 and f(a=p + 8) == 3 and f(a_t=p + 1) == 3 and f(b=p + 1) == 3 and f(b_t=p + 8) == 3
