@@ -336,3 +336,38 @@ def test_layout_argument_checks():
     assert f(K=-1) == 2 and f(N=-1) == 2 and f(lda=24) == 2 and f(ldb=7) == 2 and f(K=1 << 31) == 2
     assert f(a=None) == 1 and f(a_t=None) == 1 and f(b=None) == 1 and f(b_t=None) == 1
     assert f(lda=36) == 3 and f(a=p + 8) == 3 and f(a_t=p + 1) == 3 and f(b=p + 1) == 3 and f(b_t=p + 8) == 3
+
+
+# ------------------------------------------------------------------------------------------------ torch.compile
+@pytest.mark.gpu
+@layers
+@pytest.mark.parametrize("norm", [False, True])
+def test_compiled_layers_give_the_eager_values(cuda_dev, cls, kw, norm):
+    """``torch.compile`` of a layer's forward and of its group-norm form, with a branch and without: the eager values, also after the
+    factors were written in place and replaced."""
+    torch._dynamo.reset()
+    m = layer(cls, cuda_dev, **kw)
+    plain = cls(nn.Linear(640, 328).bfloat16(), device=cuda_dev, **kw)
+    x = torch.randn(2, 75, 640, device=cuda_dev).bfloat16()
+    w = torch.randn(640, device=cuda_dev).bfloat16()
+
+    def call(n, x):
+        return n.forward_group_norm(x, 32, w, w, 1e-6, "silu") if norm else n(x)
+    compiled = torch.compile(call, backend="aot_eager")
+    with torch.no_grad():
+        assert torch.equal(compiled(plain, x), call(plain, x))
+        for i in range(6):
+            # the compiled call may sum x @ A in another kernel: a rounding of t, then of y
+            want = call(m, x)
+            got = compiled(m, x)
+            tol = 4 * torch.finfo(x.dtype).eps * float(want.abs().max())
+            assert float((got.float() - want.float()).abs().max()) <= tol, i
+            name = ("lr_A", "lr_B")[i % 2]
+            if i < 2:
+                getattr(m, name).mul_(-2)
+            elif i < 4:
+                setattr(m, name, torch.randn_like(getattr(m, name)) / 8)
+            else:
+                m.cpu()
+                getattr(m, name).mul_(2)
+                m.cuda()
