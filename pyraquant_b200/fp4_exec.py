@@ -184,21 +184,20 @@ class Fp4Linear(LowRankFactors, nn.Module):
                 setattr(self, name, v.to(new.device))
         return self
 
-    def _product(self, xq: Fp4Rows, x2: torch.Tensor) -> torch.Tensor:
-        if self.lr_A is None:
-            return fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype)
+    def _with_branch(self, x2: torch.Tensor) -> torch.Tensor:
+        xq, w = quant_rows_fp4(x2, self.fmt), self.weight_rows
         t = self._down(x2).to(x2.dtype)
         if t.shape[1] == 32 and self.lr_B.dtype in ops._DT:
-            w = self.weight_rows
             return fp4_gemm(xq, w, self.bias, x2.dtype, lowrank_factors(t, xq, self.lr_B, w))
-        y = fp4_gemm(xq, self.weight_rows, self.bias, x2.dtype)
+        y = fp4_gemm(xq, w, self.bias, x2.dtype)
         return y.addmm_(t, self.lr_B.to(y.dtype))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape
         assert shape[-1] == self.in_features, (tuple(shape), self.in_features)
         x2 = x.detach().reshape(-1, shape[-1])                 # no gradient, not even through the low-rank branch alone
-        return self._product(quant_rows_fp4(x2, self.fmt), x2).reshape(*shape[:-1], self.out_features)
+        y2 = fp4_linear_2d(x2, self.weight_rows, self.bias) if self.lr_A is None else self._with_branch(x2)
+        return y2.reshape(*shape[:-1], self.out_features)
 
     def forward_group_norm(self, h: torch.Tensor, groups: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
                            eps: float = 1e-6, act: Optional[str] = None) -> torch.Tensor:

@@ -729,3 +729,50 @@ def test_calls_let_other_threads_run(cuda_dev, op):
         torch.cuda.synchronize()
     assert waited > 0.1, "no call had to wait"
     assert longest[0] < waited / 2, (longest[0], waited)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_2d(cuda_dev, fmt, dtype):
+    x = awkward_rows(77, 640, dtype, 3).to(cuda_dev)
+    w = fp4_exec.quant_rows_fp4(awkward_rows(200, 640, torch.bfloat16, 4).to(cuda_dev), fmt)
+    b = torch.randn(200, device=cuda_dev)
+    y = fp4_exec.fp4_linear_2d(x, w, b)
+    assert y.dtype == dtype and torch.equal(y, fp4_exec.fp4_gemm(fp4_exec.quant_rows_fp4(x, fmt), w, b, dtype))
+    check_product(y, fp4_exec.quant_rows_fp4(x, fmt), w, b, fmt)
+    m = fp4_exec.Fp4Linear(nn.Linear(640, 200).to(dtype), device=cuda_dev, fmt=fmt)
+    assert torch.equal(m(x), fp4_exec.fp4_linear_2d(x, m.weight_rows, m.bias))
+
+
+def test_graph_of_two_branches(cuda_dev):
+    """Capture over two streams that part and meet again: the chained launches behind the meeting wait for both."""
+    g = torch.Generator().manual_seed(4)
+    x, u = (torch.randn(300, 640, generator=g).bfloat16().to(cuda_dev) for _ in range(2))
+    w = fp4_exec.quant_rows_fp4(torch.randn(640, 640, generator=g).bfloat16().to(cuda_dev), "nv")
+    side = torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        a = fp4_exec.quant_rows_fp4(x, "nv")
+        with torch.cuda.stream(side):
+            b = fp4_exec.quant_rows_fp4(u * 2, "nv")
+            y1 = fp4_exec.fp4_gemm(b, w, None, torch.bfloat16)
+        y0 = fp4_exec.fp4_gemm(a, w, None, torch.bfloat16)
+        main.wait_stream(side)
+        q = fp4_exec.quant_rows_fp4(y1, "nv")
+        z = fp4_exec.fp4_gemm(q, w, None, torch.bfloat16)
+        keep.append((a, b, q))
+        return y0, y1, z
+    keep = []
+    want = run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for k in range(3):
+        x.mul_(-1); u.mul_(-1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, run() if k < 2 else [-t for t in want]):
+            assert torch.equal(a, b)
