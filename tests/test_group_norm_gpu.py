@@ -360,3 +360,32 @@ def test_silu_far_below_zero(cuda_dev):
     assert bool((got.cpu().double() - want).abs().le(want.abs() * ((11 + z.abs()) * 2.0 ** -24 + 2.0 ** -8) + 4e-17).all())
     for rows in norm_exec.group_norm_quant_rows(x, 8, torch.zeros(64, device=cuda_dev), b.to(cuda_dev), 1e-6, "silu", want_normed=True)[2]:
         assert torch.equal(rows, got[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("C,groups", [(32, 4), (96, 4), (224, 4), (320, 32), (672, 32)])
+def test_scale_bytes_past_the_row(cuda_dev, fmt, C, groups):
+    """The fused form writes every scale byte of its rows, the zeros behind a row's last scale among them, into memory that held
+    others; products at those widths take its rows as they take the quantiser's."""
+    x, w, b = (t.to(cuda_dev) for t in rows(2, 77, C, torch.bfloat16, C))
+    z = norm_exec.group_norm_rows(x, groups, w, b, 1e-6, "silu").reshape(-1, C)
+    shape = ops.fp4_scale_shape(154, C, fmt)
+    assert ops.group_norm_quant_fp4_fused(x, groups, w, b, 1e-6, "silu", fmt) is not None
+
+    def poisoned(call):
+        del_me = [torch.full(shape, 255, dtype=torch.uint8, device=cuda_dev) for _ in range(8)]
+        del del_me
+        return call()
+    f0 = poisoned(lambda: fp4_exec.quant_rows_fp4(z, fmt))
+    f = poisoned(lambda: norm_exec.group_norm_quant_fp4(x, groups, w, b, 1e-6, "silu", fmt))
+    r = torch.arange(154, device=cuda_dev)
+    for tile in range(shape[1]):
+        for k in range(4):
+            at = (r % 32) * 16 + (r // 32 % 4) * 4 + k
+            assert torch.equal(f.scales[r // 128, tile, at], f0.scales[r // 128, tile, at])
+            if tile * 4 + k >= C // ops.FP4_BLOCK[fmt]:
+                assert not f.scales[r // 128, tile, at].any()
+    wq = fp4_exec.quant_rows_fp4(torch.randn(72, C, generator=torch.Generator().manual_seed(1)).bfloat16().to(cuda_dev), fmt)
+    y = fp4_exec.fp4_gemm(f, wq)
+    assert bool(torch.isfinite(y).all()) and torch.equal(y, fp4_exec.fp4_gemm(f0, wq))
