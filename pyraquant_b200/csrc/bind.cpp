@@ -37,17 +37,19 @@ PyObject* fail(const char* what, int rc) {
   return nullptr;
 }
 // a tuple of new references; an undefined tensor becomes None
-PyObject* tuple3(const Tensor& a, const Tensor& b, const Tensor& c) {
-  PyObject* t = PyTuple_New(3);
+PyObject* tuple_of(std::initializer_list<const Tensor*> v) {
+  PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(v.size()));
   if (t == nullptr) return nullptr;
-  const Tensor* v[3] = {&a, &b, &c};
-  for (int i = 0; i < 3; ++i) {
-    PyObject* o = v[i]->defined() ? THPVariable_Wrap(*v[i]) : Py_NewRef(Py_None);
+  Py_ssize_t i = 0;
+  for (const Tensor* e : v) {
+    PyObject* o = e->defined() ? THPVariable_Wrap(*e) : Py_NewRef(Py_None);
     if (o == nullptr) { Py_DECREF(t); return nullptr; }
-    PyTuple_SET_ITEM(t, i, o);
+    PyTuple_SET_ITEM(t, i++, o);
   }
   return t;
 }
+PyObject* tuple2(const Tensor& a, const Tensor& b) { return tuple_of({&a, &b}); }
+PyObject* tuple3(const Tensor& a, const Tensor& b, const Tensor& c) { return tuple_of({&a, &b, &c}); }
 
 // C++ exceptions (allocation failures, a bad device) become Python's
 template <typename F>
@@ -224,13 +226,31 @@ PyObject* fp4_lowrank_factors(PyObject*, PyObject* const* a, Py_ssize_t n) {
       rc = pq_fp4_lowrank_factors(t->data_ptr(), tc, row != nullptr ? row->data_ptr<float>() : nullptr, t_out.data_ptr<float>(), M, b->data_ptr(),
                                   bc, N, col != nullptr ? col->data_ptr<float>() : nullptr, b_out.data_ptr<float>(), N, stream_of(*t));
     }
-    if (rc != PQ_OK) return fail("pq_fp4_lowrank_factors", rc);
-    PyObject* r = PyTuple_New(2);
-    if (r == nullptr) return nullptr;
-    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(t_out));
-    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(b_out));
-    if (PyTuple_GET_ITEM(r, 0) == nullptr || PyTuple_GET_ITEM(r, 1) == nullptr) { Py_DECREF(r); return nullptr; }
-    return r;
+    return rc == PQ_OK ? tuple2(t_out, b_out) : fail("pq_fp4_lowrank_factors", rc);
+  });
+}
+
+// lowrank_layout(A [K,32] or None, B [32,N] or None) -> (A^T or None, B^T or None), contiguous; or None
+PyObject* lowrank_layout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const Tensor *A, *B;
+    if (n != 2 || !optional_tensor(a[0], &A) || !optional_tensor(a[1], &B) || (A == nullptr && B == nullptr)) return none();
+    const Tensor& like = A != nullptr ? *A : *B;
+    for (const Tensor* v : {A, B})
+      if (v != nullptr && (!v->is_cuda() || v->dim() != 2 || dtype_code(v->scalar_type()) < 0 || !plain(*v, v->scalar_type(), like.device()))) return none();
+    if ((A != nullptr && (A->size(1) != 32 || !aligned(*A, 16))) || (B != nullptr && B->size(0) != 32)) return none();
+    const int64_t K = A != nullptr ? A->size(0) : 0, N = B != nullptr ? B->size(1) : 0;
+    Tensor at, bt;
+    int rc;
+    {
+      Unlocked unlocked;
+      c10::cuda::CUDAGuard guard(like.device());
+      if (A != nullptr) at = make({32, K}, A->scalar_type(), *A);
+      if (B != nullptr) bt = make({N, 32}, B->scalar_type(), *B);
+      rc = pq_lowrank_layout(A != nullptr ? A->data_ptr() : nullptr, 32, at.defined() ? at.data_ptr() : nullptr, K, B != nullptr ? B->data_ptr() : nullptr,
+                             N, bt.defined() ? bt.data_ptr() : nullptr, N, stream_of(like));
+    }
+    return rc == PQ_OK ? tuple2(at, bt) : fail("pq_lowrank_layout", rc);
   });
 }
 
@@ -300,7 +320,7 @@ PyObject* group_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define PQ_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {PQ_FAST(quant_rows_fp4), PQ_FAST(dequant_rows_fp4), PQ_FAST(fp4_gemm), PQ_FAST(fp4_lowrank_rows), PQ_FAST(fp4_lowrank_factors),
+PyMethodDef kMethods[] = {PQ_FAST(quant_rows_fp4), PQ_FAST(dequant_rows_fp4), PQ_FAST(fp4_gemm), PQ_FAST(fp4_lowrank_rows), PQ_FAST(fp4_lowrank_factors), PQ_FAST(lowrank_layout),
                            PQ_FAST(group_norm), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bind", "eager calls of the 4-bit and group-norm operators", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

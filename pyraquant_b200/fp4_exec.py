@@ -184,6 +184,10 @@ class Fp4Linear(LowRankFactors, nn.Module):
                 setattr(self, name, v.to(new.device))
         return self
 
+    def _lr_At(self) -> torch.Tensor:
+        """lr_A transposed, on every call like lr_B: this layer keeps nothing that a write to its buffers could leave behind."""
+        return ops.lowrank_layout(self.lr_A, None)[0] if _eager() else self.lr_A.t().contiguous()
+
     def _with_branch(self, x2: torch.Tensor) -> torch.Tensor:
         xq, w = quant_rows_fp4(x2, self.fmt), self.weight_rows
         t = self._down(x2).to(x2.dtype)

@@ -299,7 +299,9 @@ class _Transposed:
 
 
 class LowRankFactors:
-    """What the Linears with a low-rank branch share: K-major copies of the factors, made once, and the down-projection."""
+    """What the Linears with a low-rank branch share: K-major copies of the factors and the down-projection.  A copy that is kept
+    follows its factor as far as torch counts the changes: replacing, moving, converting and writing in place are seen, a write through
+    ``.data`` is not (assign the factor anew after one)."""
 
     # what forwards keep beside the buffers; none of it is part of the layer
     _KEPT = ("_lean_cache", "_t_cache_lr_A", "_t_cache_lr_B")

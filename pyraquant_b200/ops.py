@@ -425,6 +425,9 @@ def lowrank_down(x2: Tensor, a_t: Tensor) -> Tensor:
 def lowrank_layout(A: Optional[Tensor], B: Optional[Tensor]) -> Tuple[Optional[Tensor], Optional[Tensor]]:
     """(A.t(), B.t()), contiguous, of a branch's factors A [K, R] and B [R, N] (each may be left out): one launch for CUDA factors of rank 32
     in a 16-bit type (pq_lowrank_layout), torch's copies otherwise."""
+    r = _BIND().lowrank_layout(A, B) if (A if A is not None else B).is_cuda else None
+    if r is not None:
+        return r
     a_ok = A is None or (A.is_cuda and A.dim() == 2 and A.dtype in _DT and A.shape[1] == 32 and A.is_contiguous() and A.data_ptr() % 16 == 0)
     b_ok = B is None or (B.is_cuda and B.dim() == 2 and B.dtype in _DT and B.shape[0] == 32 and B.is_contiguous())
     if not (a_ok and b_ok) or (A is not None and B is not None and A.device != B.device):

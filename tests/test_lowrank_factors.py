@@ -70,6 +70,28 @@ def test_factors_refusals(cuda_dev):
             fp4_exec.lowrank_factors(*bad)
 
 
+@pytest.mark.gpu
+def test_layout_general_path_agrees_with_the_one_step_call(cuda_dev, monkeypatch):
+    A, B = torch.randn(90, 32, device=cuda_dev).half(), torch.randn(32, 70, device=cuda_dev).bfloat16()
+    t, x = torch.randn(9, 32, device=cuda_dev).half(), fp4_exec.quant_rows_fp4(torch.randn(9, 32, device=cuda_dev).half(), "nv")
+    w = fp4_exec.quant_rows_fp4(torch.randn(70, 32, device=cuda_dev).half(), "nv")
+    bind = ops._BIND()
+    for good in ((A, B), (A, None), (None, B)):
+        assert bind.lowrank_layout(*good) is not None
+    for bad in ((A.float(), B), (A[:, :16], None), (A.cpu(), B), (None, B[:31]), (None, None), ("A", B), (A.t().contiguous().t(), B)):
+        assert bind.lowrank_layout(*bad) is None
+    assert bind.fp4_lowrank_factors(t, x.row_scale, B, w.row_scale) is not None
+    for bad in ((t, None, B[:, ::2], None), (t, w.row_scale, B, None), (t, None, B, x.row_scale), (t.float(), None, B, None), (t, None, B, "c"), (t, None, None, None)):
+        assert bind.fp4_lowrank_factors(*bad) is None
+    one = (*ops.lowrank_layout(A, B), *fp4_exec.lowrank_factors(t, x, B, w))
+
+    class Refuses:
+        def __getattr__(self, name):
+            return lambda *a: None
+    monkeypatch.setattr(ops, "_bind_handle", Refuses())
+    assert all(torch.equal(a, b) for a, b in zip(one, (*ops.lowrank_layout(A, B), *fp4_exec.lowrank_factors(t, x, B, w))))
+
+
 def test_factors_argument_checks():
     lib = _lib.load()
     buf = ctypes.create_string_buffer(4096)
@@ -203,6 +225,10 @@ def test_layers_follow_their_factors(cuda_dev, cls, kw, name):
     getattr(m, name).mul_(-2)
     m.cuda()
     assert torch.equal(m(x), by_fresh_layer(m, x, **kw))
+    if cls is fp4_exec.Fp4Linear:                                 # keeps nothing: not even a write that torch does not count is missed
+        getattr(m, name).data.mul_(-2)
+        assert torch.equal(m(x), by_fresh_layer(m, x, **kw))
+        assert not [k for k, v in m.__dict__.items() if k.startswith("_t_cache")]
     with torch.inference_mode():
         n = layer(cls, cuda_dev, **kw)
         n(x)
