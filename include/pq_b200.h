@@ -65,8 +65,8 @@ int pq_last_cuda_error(void);
  *                       schedule (the rows of a panel stay in L2 across the rounds); 0 = one panel over all rows;
  *   "gemm_l2_hints"     CTA-pair kernel, L2 eviction priorities: bit 0 weights evict-last, bit 1 activations evict-first,
  *                       bit 2 activations evict-last, bit 3 streaming output stores;
- *   "fp4_pair"          4-bit GEMM: 0 = never use the CTA-pair kernel, 1 = where its tiles fill the SM pairs (default), 2 =
- *                       always;
+ *   "fp4_pair"          4-bit GEMM: 0 = never use the CTA-pair kernel, 1 = from a quarter as many of its 256 x 256 tiles as SMs on
+ *                       (default; half as many up to 128 rows, as many for 65 to 128 columns, never below), 2 = always;
  *   "fp4_split"         4-bit GEMM outside the CTA-pair kernel: CTAs that share a tile's K (1, 2, 4 or 8);
  *   "g32_variant"       group-32 GEMM: 0 = tile width by the size of the launch, 1 = 128 columns, 2 = 64 columns.
  * Unknown keys return PQ_ERR_UNSUPPORTED.  Not part of the reference API. */

@@ -48,7 +48,7 @@ struct Options {
   int gemm_tail_pairs = 1; // CTA-pair kernel: SM pairs that the pm x pn grid leaves over take a tail region of the tiles (0: they idle)
   int gemm_panel_mb = 0;   // CTA-pair kernel, several column rounds: megabytes of activation rows per row panel (0 = one panel)
   int gemm_l2_hints = 0;   // CTA-pair kernel: bit 0 weights evict-last, bit 1 activations evict-first, bit 2 activations evict-last, bit 3 streaming output stores
-  int fp4_pair = 1;        // 4-bit GEMM: CTA-pair kernel 0 never, 1 for launches that fill the SM pairs, 2 whenever it applies
+  int fp4_pair = 1;        // 4-bit GEMM: CTA-pair kernel 0 never, 1 by the number of its tiles (dispatch_fp4), 2 whenever it applies
   int fp4_split = 0;       // 4-bit GEMM, single-CTA tiles: CTAs that share a tile's K (0 automatic; 1, 2, 4, 8)
   int g32_variant = 0;     // group-32 GEMM tiles: 0 by the size of the launch, 1 128 columns, 2 64 columns
 };

@@ -2,8 +2,10 @@
 // the T rows and C / groups channels of a group, act nothing or SiLU (z * sigmoid(z)), one rounding to the 16-bit type;
 // with or without the per-row quantisation of z (INT8, mx, nv) in the same launch.
 //
-// HBM-bound: 2 bytes read and 2 (z), 1 (INT8) or 0.53 to 0.56 (4-bit) written per element, provided x is read once although the
-// statistics are needed before the first output.  So one cooperative launch of one CTA per SM: the T rows of a sample are
+// Cannot do without 2 bytes read and 2 (z), 1 (INT8) or 0.53 to 0.56 (4-bit) written per element, provided x is read once although
+// the statistics are needed before the first output.  What bounds it while the rows fit on the chip is latency: 5 of 16 us between
+// the sweeps, then chains of dependent operations (4 x 16384 x 320: issue slots 49 % used, no pipe above 31 %); beyond that HBM, with
+// the second reading.  One cooperative launch of one CTA per SM: the T rows of a sample are
 // cut into P consecutive chunks, one per CTA, which pass through a ring of four segments in shared memory (200 KB, 30 MB
 // over the GPU) by bulk copies, and what the ring holds at the end of the first pass is not read again for the second.
 //   1. First to last segment: a thread has a fixed column of eight channels and every R-th row and sums x - pivot and its
@@ -100,8 +102,8 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
 // reciprocal per value would keep the special-function pipe busy for 16 cycles a warp; this takes 12, next to about ten
 // instructions a value in all.  t is held at 60 so that the product stays finite and a NaN leaves its partner alone; the sigmoid then
 // ends at 2^-60, and the z beside it is held at -41.6 (t = 60.02): from there down the function lies between -4e-17 and 0 and comes out
-// as -41.6 * 2^-60 = -3.6e-17 however far down z is.  us without / with that hold: 1 x 1024 x 1280 8.8 / 8.9, 2 x 16384 x 320 17.0 /
-// 17.5, 1 x 262144 x 256 73.9 / 75.0; a select that ends at zero, or one test for several values, costs a little more.
+// as -41.6 * 2^-60 = -3.6e-17 however far down z is.  us without / with that hold: 1 x 1024 x 1280 9.0 / 9.1, 2 x 16384 x 320 15.5 /
+// 16.0, 1 x 262144 x 256 74.0 / 75.2; a select that ends at zero, or one test for several values, costs a little more.
 __device__ __forceinline__ float2 silu2(float2 z) {
   const float2 t = __fmul2_rn(z, make_float2(-1.4426950408889634f, -1.4426950408889634f));
   const float2 e = make_float2(ex2_approx(fminf(t.x, 60.0f)), ex2_approx(fminf(t.y, 60.0f)));
