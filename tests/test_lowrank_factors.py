@@ -397,3 +397,16 @@ def test_compiled_layers_give_the_eager_values(cuda_dev, cls, kw, norm):
                 m.cpu()
                 getattr(m, name).mul_(2)
                 m.cuda()
+
+
+def test_one_step_calls_leave_cpu_operands_alone():
+    bind = _lib.binding()
+    A, B = torch.randn(40, 32).bfloat16(), torch.randn(32, 24).bfloat16()
+    assert bind.lowrank_layout(A, B) is None and bind.lowrank_layout(None, None) is None and bind.lowrank_layout(A) is None and bind.lowrank_layout(3, B) is None
+    assert bind.fp4_lowrank_factors(A, None, B, None) is None and bind.fp4_lowrank_factors(A, None, "B", None) is None and bind.fp4_lowrank_factors() is None
+    at, bt = ops.lowrank_layout(A, B)
+    assert torch.equal(at, A.t()) and torch.equal(bt, B.t()) and at.is_contiguous() and bt.is_contiguous()
+    q = fp4_exec.quantize_weight_fp4(torch.randn(40, 32))
+    w = fp4_exec.quantize_weight_fp4(torch.randn(24, 32))
+    with pytest.raises(AssertionError):
+        fp4_exec.lowrank_factors(A, q, B, w)
